@@ -21,6 +21,10 @@ _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
 _F64 = ctypes.c_double
 
+_PAGED_ROWS = [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P]
+_PAGED_ATTENTION = [_P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32,
+                    _I32, _I32, _P, _P, _I64, _P, _P]
+
 # Argument types of every entry point, in the header's order.
 SIGNATURES = {
     "drift_abi_version": (_I32, []),
@@ -66,6 +70,13 @@ SIGNATURES = {
     "drift_attention_inputs_bf16": (_I32, [_P, _P, _P, _P, _P, _F32, _F32, _P, _I32, _I32, _I32, _I32, _I32, _F32,
                                            _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _I32,
                                            _I32, _P, _P]),
+    "drift_paged_write_f32": (_I32, _PAGED_ROWS),
+    "drift_paged_write_bf16": (_I32, _PAGED_ROWS),
+    "drift_paged_read_f32": (_I32, _PAGED_ROWS),
+    "drift_paged_read_bf16": (_I32, _PAGED_ROWS),
+    "drift_paged_attention_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
+    "drift_paged_attention_f32": (_I32, _PAGED_ATTENTION),
+    "drift_paged_attention_bf16": (_I32, _PAGED_ATTENTION),
     "drift_embedding_q8_0_f32": (_I32, [_P, _P, _P, _I64, _I64, _I32, _P, _P]),
     "drift_embedding_q8_0_bf16": (_I32, [_P, _P, _P, _I64, _I64, _I32, _P, _P]),
     "drift_embedding_f32": (_I32, [_P, _I32, _P, _P, _I64, _I64, _I32, _P, _P]),

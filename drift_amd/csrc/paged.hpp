@@ -1,0 +1,117 @@
+// The paged key and value cache as several sequences' calls see it: the page
+// tables, where each sequence's token rows lie and at which positions, and
+// the checks that the entry points over it share.
+//
+// The cache (ops/KvCache.scala:5-22): keys [pages, page_size, kv_heads,
+// head_dim], values [pages, kv_heads, head_dim, page_size] (transposed within
+// a page), in F16; or in 8 bits, the same two of int8 codes with F32 scales
+// [pages, kv_heads, page_size], one a position and key head: a value is its
+// code times its row's scale.
+#pragma once
+
+#include "common.hpp"
+
+namespace drift {
+
+// Several sequences' token rows, packed: sequence s has rows offsets[s] up to
+// offsets[s + 1] of the token tensors, at positions starts[s] and on, in the
+// pages of tables[s]. All three are read on the device, so a captured launch
+// serves as sequences grow. Without offsets there is one sequence of all
+// rows, or a row a sequence; without starts one sequence at `start`.
+struct Paging {
+  const int32_t* tables;   // [sequences, table_pages]
+  const int32_t* starts;   // nullable
+  const int32_t* offsets;  // nullable
+  int32_t sequences, table_pages, cache_pages, page_size, start, tokens;
+  int32_t* bad_page;  // nullable
+};
+
+struct Span {
+  int64_t first;         // its first token row
+  int32_t rows;          // 0 where the sequence is not described rightly
+  int64_t start;         // the first row's position
+  const int32_t* table;  // its pages
+};
+
+__device__ __forceinline__ void flag_bad(const Paging& p) {
+  if (p.bad_page) *p.bad_page = 1;
+}
+
+// Sequence s as the device's arrays describe it. Rows outside the token
+// tensors, a start below 0, or an end past the page table make it a sequence
+// of no rows and set the flag: nothing is read or written for it.
+__device__ __forceinline__ Span span_of(const Paging& p, int s) {
+  Span span;
+  int64_t from = p.sequences == 1 ? 0 : s, to = p.sequences == 1 ? p.tokens : s + 1;
+  if (p.offsets) {
+    from = p.offsets[s];
+    to = p.offsets[s + 1];
+  }
+  span.start = p.starts ? p.starts[s] : p.start;
+  span.first = from;
+  span.table = p.tables + (int64_t)s * p.table_pages;
+  const bool good = from >= 0 && to >= from && to <= p.tokens && span.start >= 0 &&
+                    (to == from || span.start + (to - from) <= (int64_t)p.table_pages * p.page_size);
+  if (!good) flag_bad(p);
+  span.rows = good ? (int32_t)(to - from) : 0;
+  return span;
+}
+
+// Work in units of `per` items, a row having `scale` of them: ceil(rows scale /
+// per) + extra units a sequence. The sequence that unit `unit` of the launch
+// belongs to (-1: none), and which of its units it is. Whole waves call, every
+// lane with the same unit.
+__device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, int extra, int64_t scale, int64_t& nth) {
+  if (!p.offsets) {
+    if (p.sequences == 1) {
+      nth = unit;
+      return 0;
+    }
+    const int64_t each = (scale + per - 1) / per + extra;
+    nth = unit % each;
+    const int64_t s = unit / each;
+    return s < p.sequences ? (int)s : -1;
+  }
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int base = 0; base < p.sequences; base += kWave) {
+    const int s = base + lane;
+    int64_t units = 0;
+    if (s < p.sequences) {
+      const int64_t from = p.offsets[s], to = p.offsets[s + 1];
+      const bool good = from >= 0 && to >= from && to <= p.tokens;
+      if (!good) flag_bad(p);  // and no units, so that the others' are all in the launch
+      units = good && to > from ? ((to - from) * scale + per - 1) / per + extra : 0;
+    }
+    int64_t end = units;  // units of this group of sequences, up to and with this lane's
+#pragma unroll
+    for (int step = 1; step < kWave; step <<= 1) {
+      const int64_t before = __shfl_up(end, step, kWave);
+      if (lane >= step) end += before;
+    }
+    const uint64_t past = __ballot(unit < end);
+    if (past) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      nth = unit - (__shfl(end, at, kWave) - __shfl(units, at, kWave));
+      return base + at;
+    }
+    unit -= __shfl(end, kWave - 1, kWave);
+  }
+  return -1;
+}
+
+// ---------------------------------------------------------------- host side
+
+// Units a launch needs for every sequence's (locate), whatever the offsets hold.
+inline int64_t units_of(const Paging& p, int64_t per, int64_t extra, int64_t scale) {
+  if (p.offsets) return (int64_t)p.tokens * scale / per + p.sequences * (1 + extra);
+  if (p.sequences == 1) return ceil_div((int64_t)p.tokens * scale, per) + extra;
+  return p.sequences * (ceil_div(scale, per) + extra);
+}
+
+// The checks of a call over the paged cache; nonzero (refused) if bad.
+int check_paging(const char* entry, const Paging& p, int32_t kv_heads, int32_t head_dim);
+// Its tensors: the cache's, and the page tables.
+int check_cache(const char* entry, const Paging& p, const void* keys, const void* values, const float* key_scales,
+                const float* value_scales);
+
+}  // namespace drift

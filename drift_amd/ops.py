@@ -18,6 +18,7 @@ stream given to the constructor); nothing synchronizes.
 
 from __future__ import annotations
 
+import ctypes
 import enum
 from dataclasses import dataclass, replace
 from typing import Optional, Sequence, Tuple
@@ -28,6 +29,7 @@ from . import _lib
 
 F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
 _FLOAT_TYPES = (F32, BF16)
+_MOST_POSITIONS = 2 ** 31 - 1  # the entry points take positions and counts of 32 bits
 
 
 class Activation(enum.IntEnum):
@@ -129,6 +131,81 @@ class KvCache:
         """HipOps.allocateCache: the cache's two tensors, uninitialised."""
         return KvCache(torch.empty((pages, pageSize, kvHeads, headDimension), dtype=F16, device=device),
                        torch.empty((pages, kvHeads, headDimension, pageSize), dtype=F16, device=device), pageSize)
+
+
+@dataclass
+class QuantizedKvCache:
+    """KvCache's pages in 8 bits: int8 codes keys [pages, pageSize, kvHeads,
+    headDimension] and values [pages, kvHeads, headDimension, pageSize], and
+    F32 scales [pages, kvHeads, pageSize], one a position and head of each: a
+    value is its code times its row's scale, max |x| / 127 of the row. Takes
+    (D + 4) / 2 D of the F16 cache's bytes. `cacheWrite` and
+    `cacheWriteSequences` quantise into it, `attention` and
+    `attentionSequences` read it, `cacheRead` and `cacheReadSequences` give
+    its positions back. The fused attention inputs write the F16 cache alone."""
+    keys: torch.Tensor
+    values: torch.Tensor
+    keyScales: torch.Tensor
+    valueScales: torch.Tensor
+    pageSize: int
+
+    def __post_init__(self):
+        if self.pageSize <= 0 or self.pageSize % 16 != 0:
+            raise ValueError(f"pages of {self.pageSize} tokens: not a multiple of 16")
+        if not (self.keys.dtype == torch.int8 and self.values.dtype == torch.int8):
+            raise ValueError("the 8-bit cache's codes are I8")
+        if not (self.keys.dim() == 4 and self.values.dim() == 4):
+            raise ValueError("the cache's keys and values are 4-dimensional")
+        self.pages, size, self.kvHeads, self.headDimension = (int(d) for d in self.keys.shape)
+        if size != self.pageSize or \
+                tuple(self.values.shape) != (self.pages, self.kvHeads, self.headDimension, self.pageSize):
+            raise ValueError(f"cache values {_shape(self.values)} for keys {_shape(self.keys)}")
+        for scales in (self.keyScales, self.valueScales):
+            requireF32("the 8-bit cache", scales)
+            if tuple(scales.shape) != (self.pages, self.kvHeads, self.pageSize):
+                raise ValueError(f"cache scales {_shape(scales)} for keys {_shape(self.keys)}")
+
+    @staticmethod
+    def allocate(pages: int, pageSize: int, kvHeads: int, headDimension: int, device="cuda") -> "QuantizedKvCache":
+        """The cache's four tensors, uninitialised."""
+        def scales():
+            return torch.empty((pages, kvHeads, pageSize), dtype=F32, device=device)
+        return QuantizedKvCache(
+            torch.empty((pages, pageSize, kvHeads, headDimension), dtype=torch.int8, device=device),
+            torch.empty((pages, kvHeads, headDimension, pageSize), dtype=torch.int8, device=device),
+            scales(), scales(), pageSize)
+
+
+@dataclass(frozen=True)
+class AttentionWindow:
+    """What a row at position P sees: the last `positions` positions up to its
+    own (j > P - positions), and the first `sinks` of the sequence."""
+    positions: int
+    sinks: int = 0
+
+    def __post_init__(self):
+        if not (0 < self.positions <= _MOST_POSITIONS and 0 <= self.sinks <= _MOST_POSITIONS):
+            raise ValueError(f"a window of {self.positions} positions with {self.sinks} sinks")
+
+
+@dataclass(frozen=True)
+class Sequences:
+    """Several sequences' token rows in one call, packed one after another:
+    sequence s has rows offsets[s] .. offsets[s + 1] - 1, at positions
+    starts[s] and on, in the pages pageTables[s]. All I32, in device memory,
+    and read there: a captured call serves as the sequences grow. Without
+    `offsets` each sequence has one row (a decode step). Rows outside every
+    sequence are left as they are. A sequence that the arrays describe wrongly
+    (rows outside the tensors, a negative start, an end past its page table)
+    gets nothing done and sets the call's `badPage`.
+
+    `longest`: a guess of the most positions that a sequence has, by which
+    attention splits its work (default: what its page table has room for); the
+    result does not depend on it beyond rounding."""
+    pageTables: torch.Tensor  # [sequences, table pages]
+    starts: torch.Tensor      # [sequences]: positions before the rows
+    offsets: Optional[torch.Tensor] = None  # [sequences + 1]
+    longest: int = 0
 
 
 @dataclass(frozen=True)
@@ -416,12 +493,60 @@ def checkPageTable(pageTable, cache: KvCache, positions: int) -> None:
 
 def checkCacheWrite(k, v, cache: KvCache, pageTable, start: int) -> int:
     """ops/AttentionOps.scala:225-241; returns the token count."""
+    if isinstance(cache, QuantizedKvCache):
+        raise ValueError("the fused attention inputs write the F16 cache: an 8-bit one takes cacheWrite")
     checkElementwise("cacheWrite", k, v)
     if not (k.dim() == 3 and tuple(k.shape[1:]) == (cache.kvHeads, cache.headDimension)):
         raise ValueError(f"cacheWrite: {_shape(k)} into a cache of {cache.kvHeads} heads of {cache.headDimension}")
     tokens = int(k.shape[0])
     checkPageTable(pageTable, cache, start + tokens)
     return tokens
+
+
+def checkSequences(operation: str, sequences: Sequences, tokens: int) -> int:
+    """The sequences of a call over `tokens` rows; returns their number."""
+    tables, starts, offsets = sequences.pageTables, sequences.starts, sequences.offsets
+    if not (tables.dtype == I32 and tables.dim() == 2):
+        raise ValueError(f"{operation}: page tables are I32 [sequences, pages], not {_name(tables.dtype)} "
+                         f"{_shape(tables)}")
+    count = tables.shape[0]
+    if not (starts.dtype == I32 and starts.dim() == 1 and starts.shape[0] == count):
+        raise ValueError(f"{operation}: starts {_name(starts.dtype)} {_shape(starts)} for {count} sequences")
+    if offsets is None:
+        if count != tokens:
+            raise ValueError(f"{operation}: {count} sequences for {tokens} rows (several rows a sequence need offsets)")
+    elif not (offsets.dtype == I32 and offsets.dim() == 1 and offsets.shape[0] == count + 1):
+        raise ValueError(f"{operation}: offsets {_name(offsets.dtype)} {_shape(offsets)} for {count} sequences")
+    if sequences.longest < 0:
+        raise ValueError(f"{operation}: a longest sequence of {sequences.longest} positions")
+    return count
+
+
+def checkCacheRows(operation: str, k, v, cache) -> int:
+    """Keys and values [tokens, kvHeads, D] to or from a cache; returns the
+    token count."""
+    checkElementwise(operation, k, v)
+    if not (k.dim() == 3 and tuple(k.shape[1:]) == (cache.kvHeads, cache.headDimension)):
+        raise ValueError(f"{operation}: {_shape(k)} for a cache of {cache.kvHeads} heads of {cache.headDimension}")
+    return k.shape[0]
+
+
+# paged_attention.hip's kMaxHead
+ATTENTION_HEAD_DIMENSION = 512
+
+
+def checkAttention(operation: str, queries, cache, out) -> tuple:
+    """Queries and out [tokens, heads, D] over a cache; returns (tokens, heads)."""
+    checkElementwise(operation, queries, out)
+    if queries.dim() != 3:
+        raise ValueError(f"{operation} takes [tokens, heads, headDimension], got {_shape(queries)}")
+    tokens, heads, dimension = queries.shape
+    if dimension != cache.headDimension or cache.kvHeads == 0 or heads == 0 or heads % cache.kvHeads != 0:
+        raise ValueError(f"{operation}: queries {_shape(queries)} over a cache of {cache.kvHeads} heads of "
+                         f"{cache.headDimension}")
+    if dimension > ATTENTION_HEAD_DIMENSION:
+        raise ValueError(f"{operation}: heads of {dimension} values (at most {ATTENTION_HEAD_DIMENSION})")
+    return tokens, heads
 
 
 def checkSplitHalves(x, first, second) -> None:
@@ -457,6 +582,11 @@ def _on_device(operation: str, *tensors) -> None:
             raise ValueError(f"{operation}: tensors are dense row-major")
 
 
+def checkBadPage(operation: str, badPage) -> None:
+    if badPage is not None and not (badPage.dtype == I32 and badPage.numel() >= 1):
+        raise ValueError(f"{operation}: badPage is I32 [1], not {_name(badPage.dtype)} {_shape(badPage)}")
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     """t's device address, as a c_void_p argument takes it."""
     return None if t is None else t.data_ptr()
@@ -490,6 +620,7 @@ class HipOps:
         self._quantizedValues: Optional[QuantizedValues] = None
         self._quantizedBuffer: Optional[torch.Tensor] = None
         self._scratch: Optional[torch.Tensor] = None
+        self._attentionBytes: dict = {}  # attention's workspace by its sizes
 
     def _stream(self) -> int:
         if self.stream is not None:
@@ -778,7 +909,11 @@ class HipOps:
         """Keys and values [tokens, kvHeads, D] into the cache at positions
         start .. start + tokens - 1 (ops/AttentionOps.scala:52-63). A page
         table entry outside the cache (which the reference fails on) writes
-        nothing and sets `badPage` (int32 [1], device) to 1 when given."""
+        nothing and sets `badPage` (int32 [1], device) to 1 when given. A
+        QuantizedKvCache gets them quantised."""
+        if isinstance(cache, QuantizedKvCache):
+            self._cacheRows("cacheWrite", "drift_paged_write", k, v, cache, pageTable, start, badPage)
+            return
         tokens = checkCacheWrite(k, v, cache, pageTable, start)
         _on_device("cacheWrite", k, v, cache.keys, cache.values, pageTable)
         self._launch(f"drift_cache_write_{_suffix(k.dtype)}", _ptr(k), _ptr(v), _ptr(cache.keys), _ptr(cache.values),
@@ -848,6 +983,132 @@ class HipOps:
                      tokens, heads, cache.kvHeads, d, r.rotaryDimensions, r.theta, int(r.layout), r.sections.code,
                      *r.sections.launch_sizes(), _ptr(rotatedQueries), _ptr(gate), _ptr(cache.keys),
                      _ptr(cache.values), _ptr(pageTable), pageTable.numel(), cache.pages, cache.pageSize, start,
+                     _ptr(badPage))
+
+    # ---------------------------------------------------------------- the paged cache, attention
+
+    def _onOneDevice(self, operation: str, tensors) -> None:
+        """_on_device, and all on the device that the launch goes to."""
+        for t in tensors:
+            if t is not None and not t.is_cuda:
+                raise ValueError(f"{operation}: tensors live in device memory")
+        device = torch.cuda.current_device() if self.stream is None else self.stream.device.index
+        for t in tensors:
+            if t is None:
+                continue
+            if t.get_device() != device:
+                raise ValueError(f"{operation}: a tensor on device {t.get_device()}, launched on device {device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{operation}: tensors are dense row-major")
+
+    def cacheWriteSequences(self, k, v, cache, sequences: Sequences, badPage: Optional[torch.Tensor] = None) -> None:
+        """Several sequences' keys and values [tokens, kvHeads, D] into the
+        cache (a KvCache, or a QuantizedKvCache that quantises them): one
+        launch where `cacheWrite` takes one a sequence. Two rows for one place
+        of the cache leave either."""
+        self._cacheRows("cacheWriteSequences", "drift_paged_write", k, v, cache, sequences, None, badPage)
+
+    def cacheRead(self, cache, pageTable, start: int, k, v, badPage: Optional[torch.Tensor] = None) -> None:
+        """Positions start .. start + tokens - 1 of the cache (a KvCache or a
+        QuantizedKvCache) into k and v [tokens, kvHeads, D], F32 or BF16. Rows
+        of a page outside the cache are left as they are, `badPage` set."""
+        self._cacheRows("cacheRead", "drift_paged_read", k, v, cache, pageTable, start, badPage)
+
+    def cacheReadSequences(self, cache, sequences: Sequences, k, v, badPage: Optional[torch.Tensor] = None) -> None:
+        """cacheRead of several sequences' positions: sequence s's from
+        starts[s] on, as many as it has rows."""
+        self._cacheRows("cacheReadSequences", "drift_paged_read", k, v, cache, sequences, None, badPage)
+
+    def _cacheRows(self, operation, entry, k, v, cache, pages, start, badPage) -> None:
+        tokens = checkCacheRows(operation, k, v, cache)
+        paging, tensors = self._paging(operation, cache, pages, start, tokens)
+        checkBadPage(operation, badPage)
+        self._onOneDevice(operation, (k, v, badPage, *tensors))
+        keys, values, keyScales, valueScales, *_ = tensors
+        self._launch(f"{entry}_{_suffix(k.dtype)}", _ptr(k), _ptr(v), _ptr(keys), _ptr(values), _ptr(keyScales),
+                     _ptr(valueScales), *paging, tokens, cache.kvHeads, cache.headDimension, cache.pageSize,
+                     _ptr(badPage))
+
+    @staticmethod
+    def _paging(operation, cache, pages, start, tokens) -> tuple:
+        """The entry points' paging arguments (page tables up to `start`), and
+        the tensors a call over the cache reads: keys, values, their scales,
+        page tables, starts, offsets (None where there is none)."""
+        quantized = isinstance(cache, QuantizedKvCache)
+        if cache.keys.shape[1] != cache.pageSize:
+            raise ValueError(f"{operation}: pages of {cache.pageSize} tokens in a cache {_shape(cache.keys)}")
+        scales = (cache.keyScales, cache.valueScales) if quantized else (None, None)
+        if start is None:
+            count = checkSequences(operation, pages, tokens)
+            tables, starts, offsets = pages.pageTables, pages.starts, pages.offsets
+            paging = (_ptr(tables), tables.shape[1], cache.pages, _ptr(starts), _ptr(offsets), count, 0)
+        else:
+            checkPageTable(pages, cache, start + tokens)
+            if not 0 <= start <= _MOST_POSITIONS - tokens:
+                raise ValueError(f"{operation}: {tokens} tokens from position {start}")
+            tables, starts, offsets = pages, None, None
+            paging = (_ptr(tables), tables.shape[0], cache.pages, None, None, 1, start)
+        return paging, (cache.keys, cache.values, *scales, tables, starts, offsets)
+
+    def attention(self, queries, cache, pageTable, start: int, scale: float, out,
+                  window: Optional[AttentionWindow] = None, badPage: Optional[torch.Tensor] = None) -> None:
+        """Attention of one sequence's new tokens over its paged cache (a
+        KvCache or a QuantizedKvCache), their own keys and values written to it
+        before: queries, out [tokens, heads, D] (F32 or BF16, out not queries),
+        token t at position start + t, which sees the positions up to its own,
+        or with `window` those of it; scores are `scale` q.k, query head h reads
+        key head h / (heads / kvHeads). What a token does not see has no part in
+        its row, whatever it holds. Positions on a page outside the cache are
+        not seen, `badPage` set; a row that sees nothing is zeros.
+
+        A capture holds `start` as it is: captured decode steps take
+        attentionSequences, whose starts are read on the device."""
+        tokens, heads = checkAttention("attention", queries, cache, out)
+        paging, tensors = self._paging("attention", cache, pageTable, start, tokens)
+        self._attention("attention", queries, cache, paging, tensors, tokens, heads, 1, start + tokens, scale, out,
+                        window, badPage)
+
+    def attentionSequences(self, queries, cache, sequences: Sequences, scale: float, out,
+                           window: Optional[AttentionWindow] = None,
+                           badPage: Optional[torch.Tensor] = None) -> None:
+        """`attention` of several sequences' rows in one call. Rows of out
+        outside every sequence are left as they are."""
+        tokens, heads = checkAttention("attentionSequences", queries, cache, out)
+        paging, tensors = self._paging("attentionSequences", cache, sequences, None, tokens)
+        room = sequences.pageTables.shape[1] * cache.pageSize
+        longest = min(sequences.longest, room) if sequences.longest else room
+        self._attention("attentionSequences", queries, cache, paging, tensors, tokens, heads, paging[5], longest,
+                        scale, out, window, badPage)
+
+    def _attention(self, operation, queries, cache, paging, tensors, tokens, heads, count, longest, scale, out,
+                   window, badPage) -> None:
+        checkBadPage(operation, badPage)
+        self._onOneDevice(operation, (queries, out, badPage, *tensors))
+        if queries.data_ptr() == out.data_ptr() and queries.numel():
+            raise ValueError(f"{operation}: out is queries")
+        positions, sinks = (window.positions, window.sinks) if window is not None else (0, 0)
+        longest = min(longest, _MOST_POSITIONS)
+        # scratch of this call's own, from torch's pool on the launch's stream: calls on several streams and
+        # captured graphs never share it
+        numbers = (count, tokens, heads, cache.kvHeads, cache.headDimension, positions, sinks, longest)
+        size = self._attentionBytes.get(numbers)
+        if size is None:
+            told = ctypes.c_int64()
+            _lib.call("drift_paged_attention_workspace", *numbers, ctypes.addressof(told))
+            size = self._attentionBytes[numbers] = told.value
+            if len(self._attentionBytes) > 4096:
+                self._attentionBytes.clear()
+        if size == 0:
+            workspace = None
+        elif self.stream is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=queries.device)
+        else:
+            with torch.cuda.stream(self.stream):
+                workspace = torch.empty(size, dtype=torch.uint8, device=queries.device)
+        keys, values, keyScales, valueScales, *_ = tensors
+        self._launch(f"drift_paged_attention_{_suffix(queries.dtype)}", _ptr(queries), _ptr(keys), _ptr(values),
+                     _ptr(keyScales), _ptr(valueScales), *paging, tokens, heads, cache.kvHeads, cache.headDimension,
+                     cache.pageSize, scale, positions, sinks, longest, _ptr(out), _ptr(workspace), size,
                      _ptr(badPage))
 
     # ---------------------------------------------------------------- embedding, convert

@@ -83,6 +83,30 @@ final class DriftKernels(path: Path) {
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, P, P, P,
     P, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, P)
 
+  // ------------------------------------------------------------ the paged cache, attention
+  // k, v, the cache's keys, values and their scales (NULL: the F16 cache),
+  // page tables and their widths, starts, offsets, ...
+  val pagedWrite = twins("drift_paged_write", P, P, P, P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, P)
+  val pagedRead = twins("drift_paged_read", P, P, P, P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, P)
+  val pagedAttention = twins("drift_paged_attention", P, P, P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, JAVA_INT, JAVA_INT, P, P, JAVA_LONG, P, P)
+  val pagedAttentionWorkspace = bind("drift_paged_attention_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P)
+
+  /** The bytes of scratch that a `pagedAttention` of these numbers takes. */
+  def attentionWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, window: Int,
+                         sinks: Int, longest: Int): Long = {
+    val arena = Arena.ofConfined()
+    try {
+      val bytes = arena.allocate(JAVA_LONG)
+      check("drift_paged_attention_workspace", (pagedAttentionWorkspace.invokeExact(sequences, tokens, heads, kvHeads,
+        headDimension, window, sinks, longest, bytes): Int))
+      bytes.get(JAVA_LONG, 0)
+    } finally arena.close()
+  }
+
   // ------------------------------------------------------------ tables
   val embeddingQ8_0 = twins("drift_embedding_q8_0", P, P, P, JAVA_LONG, JAVA_LONG, JAVA_INT, P, P)
   // any storage type the runner reads, by its GGUF type id

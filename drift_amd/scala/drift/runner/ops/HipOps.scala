@@ -6,7 +6,7 @@ import drift.runner.native.{DriftKernels, HipRuntime}
   * then the `Drift*` traits, whose overrides replace those traits' launches
   * with downcalls (the linearization puts them last, so theirs are the
   * members that run). The one change to the runner's `HipOps`
-  * (ops/HipOps.scala:8-20) is the `drift` library and the six traits.
+  * (ops/HipOps.scala:8-20) is the `drift` library and the seven traits.
   */
 final class HipOps(
     protected val hip: HipRuntime,
@@ -27,4 +27,5 @@ final class HipOps(
     with DriftElementwise
     with DriftLinear
     with DriftAttention
+    with DriftPagedAttention
     with DriftLayout

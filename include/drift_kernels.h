@@ -330,6 +330,89 @@ int drift_attention_inputs_bf16(const uint16_t* query_and_gate, const uint16_t* 
                                 int32_t cache_pages, int32_t page_size, int32_t start, int32_t* bad_page,
                                 void* stream);
 
+/* ---------------------------------------------------------------- the paged cache, several sequences a call
+ * Token rows packed sequence by sequence: sequence s (of `sequences`) has rows
+ * offsets[s] .. offsets[s + 1] - 1 of the token tensors, at positions starts[s]
+ * and on, in the pages page_tables[s] (int32 [sequences, table_pages]). The
+ * three arrays are read on the device, so a launch captured in a graph serves
+ * as its sequences grow; rows outside every sequence are left as they are. A
+ * sequence whose rows lie outside the `tokens` rows, whose start is negative or
+ * whose end is past its page table gets nothing done, and *bad_page = 1 (device
+ * int32, nullable).
+ * - offsets NULL: one sequence of all `tokens` rows, or (sequences == tokens) a
+ *   row a sequence, a decode step.
+ * - starts NULL: one sequence at position `start`, checked on the host against
+ *   the page table as drift_cache_write checks it; else `start` is not read.
+ * The cache is the F16 one above (key_scales and value_scales NULL), or the same
+ * two tensors of int8 codes with F32 scales [cache_pages, kv_heads, page_size]:
+ * a row x (one position's key or value of one head) is kept as codes
+ * round-half-away(x / d), at most 127 in size, d = F32 max |x| / 127 its scale,
+ * and read as code * d in F32. A row of zeros has scale 0; a row with a NaN or
+ * an infinity has scale NaN and codes 0.
+ * Replaces nothing of the reference, whose cache write takes one sequence
+ * (kernels/attention.hip:480-493) and whose cache is F16
+ * (src/drift/runner/ops/KvCache.scala:5-22).
+ *
+ * drift_paged_write_*: keys and values [tokens, kv_heads, head_dim] into the
+ * cache. Two rows for one place of the cache leave either.
+ * drift_paged_read_*: those positions out of the cache, as F32 or (rounded to
+ * nearest even) BF16. Rows on a page outside the cache are left as they are,
+ * and *bad_page = 1. */
+int drift_paged_write_f32(const float* k, const float* v, void* keys, void* values, float* key_scales,
+                          float* value_scales, const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                          const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,
+                          int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t* bad_page,
+                          void* stream);
+int drift_paged_write_bf16(const uint16_t* k, const uint16_t* v, void* keys, void* values, float* key_scales,
+                           float* value_scales, const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                           const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,
+                           int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t* bad_page,
+                           void* stream);
+int drift_paged_read_f32(float* k, float* v, const void* keys, const void* values, const float* key_scales,
+                         const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                         int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                         int32_t start, int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                         int32_t* bad_page, void* stream);
+int drift_paged_read_bf16(uint16_t* k, uint16_t* v, const void* keys, const void* values, const float* key_scales,
+                          const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                          int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                          int32_t start, int32_t tokens, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                          int32_t* bad_page, void* stream);
+
+/* Attention of the rows' queries [tokens, heads, head_dim] over the cache into
+ * out (like queries; may not be queries). The row at position P sees positions
+ * j <= P of its sequence; with window > 0 only j > P - window or j < sinks. Head
+ * h reads key head h / (heads / kv_heads). out = sum p_j v_j / sum p_j, p_j =
+ * exp(scale q.k_j - their maximum), statistics and sums in F32; BF16 outputs
+ * rounded once, and their weights p_j rounded to 11 bits. What a row does not
+ * see has no part in it, whatever it holds; positions on a page outside the
+ * cache are not seen, and *bad_page = 1. A row that sees nothing is zeros.
+ * head_dim is at most 512.
+ * `longest` is the caller's guess of the longest sequence's positions (at most
+ * the page table's; 0: the page table's): the work is split by it, and any guess
+ * gives the same result within rounding. `workspace` (device, 16-byte aligned)
+ * has at least the bytes that drift_paged_attention_workspace tells for the same
+ * numbers (0: it may be NULL); the launches write it before they read it, so it
+ * may hold anything before, and calls that may run at the same time need one
+ * each. The same call gives the same bits every time.
+ * The reference's attention (kernels/attention.hip:7-34,227-229,446-456) is one
+ * sequence's, without a window. */
+int drift_paged_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                    int32_t head_dim, int32_t window, int32_t sinks, int32_t longest, int64_t* bytes);
+int drift_paged_attention_f32(const float* queries, const void* keys, const void* values, const float* key_scales,
+                              const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                              int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                              int32_t start, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                              int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
+                              float* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page, void* stream);
+int drift_paged_attention_bf16(const uint16_t* queries, const void* keys, const void* values, const float* key_scales,
+                               const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                               int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                               int32_t start, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                               int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
+                               uint16_t* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page,
+                               void* stream);
+
 /* ---------------------------------------------------------------- embedding
  * Rows `ids` of a Q8_0 table ([vocab, cols], cols a multiple of 32: per 32
  * values a 34-byte block, fp16 scale d then 32 int8 codes), decoded as
