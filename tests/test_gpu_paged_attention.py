@@ -12,6 +12,14 @@ Bars, derived from the roundings on the way:
   relatively by that and 2^-20 (exponential, running rescales); weighted sums by
   a further (n + 8) 2^-24 in the worst case, sqrt(n) in earnest. Held to
   4 (2^-24 (sqrt(D) + 4) S' + 2^-20 + 2^-24 sqrt(n)) times the row's sum of p |v|.
+- and for both types, what a weight that is small next to its row's largest
+  loses: weights are F16 terms lifted so that the largest is 2^14 (its
+  first term exact), and F16's last step is 2^-24, half of it 2^-25, so the
+  last term of a weight is off by at most 2^-39 of the largest weight however
+  small the weight is. With the values that is 2^-39 max p sum |v| over the
+  visible positions; in 8 bits, where a weight is p times the value's scale w and
+  the values are codes up to 127, 2^-39 max(p w) 127 n. (It shows where a row's
+  one strong position has a value of 0.)
 - attention, BF16: besides those, the output's rounding, 2^-8 relative (half a
   step is eps / 2 = 2^-8), and the weights' to 11 bits: 2^-11 of the sum of p |v|.
 """
@@ -62,7 +70,7 @@ class Case:
         self.tokens = int(self.rows.sum())
         self.offsets = np.concatenate([[0], np.cumsum(self.rows)])
         # dense keys and values of each sequence, and the cache that holds them
-        self.dense = []
+        self.dense, self.scales = [], []
         if kind == "f16":
             keys = torch.full((pages, page, kv, dim), float("nan"), dtype=torch.float16)
             values = torch.full((pages, kv, dim, page), float("nan"), dtype=torch.float16)
@@ -89,6 +97,7 @@ class Case:
                 vs = (0.5 + torch.rand((n, kv), generator=gen)) * 2.5 / 127 * value_scale
                 keys[p, o], values[p, :, :, o] = k, v
                 key_scales[p, :, o], value_scales[p, :, o] = ks, vs
+                self.scales.append(vs.double())
                 self.dense.append((k.double() * ks.double()[..., None], v.double() * vs.double()[..., None]))
         if kind == "f16":
             self.cache = d.KvCache(keys.to(DEV), values.to(DEV), page)
@@ -107,6 +116,7 @@ def wanted(case, queries, scale, window=None, hidden=()):
     q = queries.double()
     out, mass = torch.zeros(tokens, heads, dim, dtype=torch.float64), torch.zeros(tokens, heads, dim, dtype=torch.float64)
     size, count = torch.zeros(tokens, heads, 1, dtype=torch.float64), torch.zeros(tokens, heads, 1, dtype=torch.float64)
+    small_weights = torch.zeros(tokens, heads, dim, dtype=torch.float64)
     group = heads // case.kv
     for s, (k, v) in enumerate(case.dense):
         rows = slice(int(case.offsets[s]), int(case.offsets[s + 1]))
@@ -138,11 +148,17 @@ def wanted(case, queries, scale, window=None, hidden=()):
                 sizes = torch.where(seen, abs(scale) * (q[rows, h].abs() @ kh.abs().T), torch.zeros(()).double())
                 size[rows, h] = sizes.amax(-1, keepdim=True)
             count[rows, h] = seen.sum(-1, keepdim=True).double()
-    return out, mass, size, count
+            if k.shape[0]:
+                if case.kind == "f16":
+                    lost = p.amax(-1, keepdim=True) * (seen.double() @ vh.abs().nan_to_num(0, 0, 0))
+                else:
+                    lost = (p * case.scales[s][:, h // group]).amax(-1, keepdim=True) * 127 * count[rows, h]
+                small_weights[rows, h] = 2.0 ** -39 * lost.nan_to_num(0)
+    return out, mass, size, count, small_weights
 
 
 def assert_rows(case, queries, scale, got, window=None, hidden=(), what=""):
-    out, mass, size, count = wanted(case, queries.cpu(), scale, window, hidden)
+    out, mass, size, count, small_weights = wanted(case, queries.cpu(), scale, window, hidden)
     got = got.cpu().double()
     same_nan = torch.isnan(out) == torch.isnan(got)
     assert bool(same_nan.all()), f"{what}: NaN in other places, {int((~same_nan).sum())}"
@@ -152,7 +168,7 @@ def assert_rows(case, queries, scale, got, window=None, hidden=(), what=""):
     bar = 4 * (2.0 ** -24 * (math.sqrt(case.dim) + 4) * size + 2.0 ** -20 + 2.0 ** -24 * count.sqrt()) * mass
     if queries.dtype == torch.bfloat16:
         bar = bar + 2.0 ** -11 * mass + 2.0 ** -8 * out.abs()
-    bar = bar + 1e-30
+    bar = bar + small_weights + 1e-30
     off = (got - out).abs()
     bad = fine & ~(off <= bar)
     worst = float((off / bar)[fine].max()) if bool(fine.any()) else 0.0
@@ -370,13 +386,13 @@ def test_queries_large_small_and_not_numbers(hip, dtype, kind, tokens):
     # head 0: scaled to scores of ordinary size; the others: weights near even
     for scale, heads in ((1e-30, [0]), (0.125, [1, 2, 3, 4, 5, 6, 7])):
         out = run(hip, case, q, scale, single=True)
-        want, mass, size, count = wanted(case, q.cpu(), scale)
+        want, mass, size, count, small_weights = wanted(case, q.cpu(), scale)
         got = out.cpu().double()
         for h in heads:
             if h in (3, 4):
                 assert bool(torch.isnan(got[0, h]).all())
                 got[0, h], want[0, h] = 0, 0
-            bar = (4 * (2.0 ** -24 * 12 * size + 2.0 ** -20 + 2.0 ** -24 * count.sqrt())) * mass
+            bar = (4 * (2.0 ** -24 * 12 * size + 2.0 ** -20 + 2.0 ** -24 * count.sqrt())) * mass + small_weights
             if dtype == "bf16":
                 bar = bar + 2.0 ** -11 * mass + 2.0 ** -8 * want.abs()
             assert bool(((got - want).abs()[:, h] <= bar[:, h].nan_to_num(0) + 1e-30).all()), f"head {h}"
@@ -399,6 +415,7 @@ def test_value_rows_of_unlike_sizes(hip, dtype, kind, tokens):
         else:
             case.cache.valueScales[p, :, off] *= factor
             case.dense[0][1][position] *= factor
+            case.scales[0][position] *= factor
     q = normal(14, (tokens, 4, 64), TYPES[dtype], 8.0).to(DEV)
     assert_rows(case, q, 0.125, run(hip, case, q, 0.125, single=True), what="unlike sizes")
 
