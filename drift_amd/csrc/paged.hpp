@@ -26,6 +26,22 @@ struct Paging {
   int32_t* bad_page;  // nullable
 };
 
+// A value that every lane of a wave holds alike, in scalar registers: what comes
+// from memory or across lanes the compiler takes for different otherwise, and
+// then masks every branch and loop on it.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+  } else {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)bits);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(bits >> 32));
+    return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
+  }
+}
+
 struct Span {
   int64_t first;         // its first token row
   int32_t rows;          // 0 where the sequence is not described rightly
@@ -39,15 +55,16 @@ __device__ __forceinline__ void flag_bad(const Paging& p) {
 
 // Sequence s as the device's arrays describe it. Rows outside the token
 // tensors, a start below 0, or an end past the page table make it a sequence
-// of no rows and set the flag: nothing is read or written for it.
+// of no rows and set the flag: nothing is read or written for it. Whole waves
+// call, every lane with the same s.
 __device__ __forceinline__ Span span_of(const Paging& p, int s) {
   Span span;
   int64_t from = p.sequences == 1 ? 0 : s, to = p.sequences == 1 ? p.tokens : s + 1;
   if (p.offsets) {
-    from = p.offsets[s];
-    to = p.offsets[s + 1];
+    from = uniform(p.offsets[s]);
+    to = uniform(p.offsets[s + 1]);
   }
-  span.start = p.starts ? p.starts[s] : p.start;
+  span.start = p.starts ? uniform(p.starts[s]) : p.start;
   span.first = from;
   span.table = p.tables + (int64_t)s * p.table_pages;
   const bool good = from >= 0 && to >= from && to <= p.tokens && span.start >= 0 &&
@@ -91,10 +108,10 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
     const uint64_t past = __ballot(unit < end);
     if (past) {
       const int at = __ffsll((unsigned long long)past) - 1;
-      nth = unit - (__shfl(end, at, kWave) - __shfl(units, at, kWave));
+      nth = unit - uniform(__shfl(end, at, kWave) - __shfl(units, at, kWave));
       return base + at;
     }
-    unit -= __shfl(end, kWave - 1, kWave);
+    unit -= uniform(__shfl(end, kWave - 1, kWave));
   }
   return -1;
 }

@@ -13,6 +13,7 @@
 #include "paged.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace drift {
 namespace {
@@ -28,10 +29,13 @@ struct AttentionArgs {
   const void *keys, *values;
   const float *key_scales, *value_scales;
   // the split over positions: at least `chunk` tiles a split, `splits` of them;
-  // their maxima and sums [splits, tokens, heads, 2] and unscaled results
-  // [splits, tokens, heads, dim] where there are several
+  // where there are several, their maxima and sums [splits, partial_rows, 3] and
+  // unscaled results [splits, partial_rows, dim]
   int32_t splits, chunk;
+  int64_t partial_rows;
   float *statistics, *partials;
+  int32_t few_most, few_units;  // attend_few's rows at most, and units, of a sequence and key head
+  int32_t few_rows;   // sequences of at most so many rows (tokens times group) are attend_few's, others attend_many's
   int32_t page_units, unit_shift;  // page_size / 16, and its logarithm where it is a power of two (else -1)
 };
 
@@ -54,8 +58,8 @@ struct RowScratch {
 // whatever the cache holds, and is slow: the vector unit and its narrow loads
 // bound it.
 template <typename T, bool I8>
-__device__ __noinline__ void attend_row(const T* queries, T* out, const AttentionArgs& a, const Span& span, int64_t nth,
-                                        int h, RowScratch& r) {
+__device__ __noinline__ void attend_row_of(const T* queries, T* out, const AttentionArgs& a, const Span& span,
+                                           int64_t nth, int h, RowScratch& r) {
   const int lane = threadIdx.x & (kWave - 1), kv = h / a.group;
   const int64_t position = span.start + nth, row = ((span.first + nth) * a.heads + h) * a.dim;
   wave_sync();
@@ -135,6 +139,16 @@ __device__ __noinline__ void attend_row(const T* queries, T* out, const Attentio
   }
 }
 
+// Copies of the arguments go by reference: the kernels' own then stay in scalar
+// registers (passed themselves, every use of theirs would read scratch memory).
+template <typename T, bool I8>
+__device__ __forceinline__ void attend_row(const T* queries, T* out, const AttentionArgs& a, const Span& span,
+                                           int64_t nth, int h, RowScratch& r) {
+  const AttentionArgs args = a;
+  const Span rows = span;
+  attend_row_of<T, I8>(queries, out, args, rows, nth, h, r);
+}
+
 template <typename T, bool I8>
 __global__ void __launch_bounds__(64) attend_rows(const T* queries, T* out, AttentionArgs a) {
   __shared__ RowScratch scratch;
@@ -152,6 +166,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 // 16 bytes at an address of 8-byte multiples
 typedef unsigned int u32x4_8 __attribute__((ext_vector_type(4), aligned(8)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -222,10 +237,14 @@ template <int TERMS>
 __device__ __forceinline__ Halves<TERMS> halves_of(const float (&v)[8]) {
   Halves<TERMS> h;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h.term[0][i] = (_Float16)v[i];
-  if constexpr (TERMS == 2)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h.term[1][i] = (_Float16)(v[i] - (float)h.term[0][i]);
+  for (int i = 0; i < 8; ++i) {
+    float x = v[i];
+    // one F32 value for both terms: left to itself the compiler rounds a product once, to F16, for the first and
+    // twice for the second, and at a tie the two then belong to different neighbours
+    if constexpr (TERMS == 2) asm volatile("" : "+v"(x));
+    h.term[0][i] = (_Float16)x;
+    if constexpr (TERMS == 2) h.term[1][i] = (_Float16)(x - (float)h.term[0][i]);
+  }
   return h;
 }
 
@@ -262,21 +281,20 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   __shared__ float stats[kWaves][C * 16][3];
   static_assert(sizeof(RowScratch) <= sizeof(merged) / kWaves, "a wave's part holds a row's scratch");
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
   const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
   const int split = rest % (unsigned)a.splits;
-  int64_t nth;
-  const int s = locate(a.p, rest / (unsigned)a.splits, C * 16, 0, a.group, nth);
-  if (s < 0) return;
+  const unsigned unit = rest / (unsigned)a.splits;
+  const int s = (int)(unit / (unsigned)a.few_units), nth = (int)(unit % (unsigned)a.few_units);
   const Span span = span_of(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
-  if (rows <= 0) return;
+  if (rows <= 0 || (int64_t)span.rows * a.group > a.few_rows) return;
   const uint32_t row0 = (uint32_t)nth * (C * 16), group = (uint32_t)a.group;
   const uint32_t p0 = (uint32_t)span.start + row0 / group, p1 = (uint32_t)span.start + (row0 + rows - 1) / group;
   const TileList list = tiles_of(a, p0, p1, TOK);
   const int each = split_tiles(a, list.count);
-  const int begin = split * each, end = min(begin + each, list.count);
+  const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
   if (begin >= end) return;
 
   // the rows' queries as B operands: column col, values 8 g .. of each 32 (8 bits: of each 64, 16 g ..)
@@ -466,8 +484,8 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t j = mine + 4 * t + e;
-            const bool seen = okay && j <= position[c] &&
-                              (a.window == 0 || j + (uint32_t)a.window > position[c] || j < (uint32_t)a.sinks);
+            const bool seen = okay & (j <= position[c]) &
+                              ((a.window == 0) | (j + (uint32_t)a.window > position[c]) | (j < (uint32_t)a.sinks));
             score[c][t][e] = seen ? score[c][t][e] : -kInfinity;
           }
 #pragma unroll
@@ -519,8 +537,8 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t j = mine + 2 * e + half;
-          const bool seen = okay && j <= p1 &&
-                            (a.window == 0 || j + (uint32_t)a.window > p0 || j < (uint32_t)a.sinks);
+          const bool seen = okay & (j <= p1) &
+                            ((a.window == 0) | (j + (uint32_t)a.window > p0) | (j < (uint32_t)a.sinks));
           keep[e] |= seen ? 0xffffu << (16 * half) : 0u;
         }
       }
@@ -592,6 +610,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
       const uint32_t row = row0 + c * 16 + r, token = row / group;
       const int h = kv * a.group + (int)(row - token * group);
       const int64_t place = (span.first + token) * a.heads + h;
+      const int64_t partial = ((int64_t)s * a.kv_heads + kv) * a.few_most + row;
       const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast(value_ref - ref) : 1.0f) / l;
       bool odd = false;
       for (int d = lane; d < a.dim; d += kWave) {
@@ -603,14 +622,14 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
           odd |= !(fabsf(x) < kInfinity);
           store_one(out + place * a.dim + d, x);
         } else {
-          a.partials[((int64_t)split * a.p.tokens * a.heads + place) * a.dim + d] = x;
+          a.partials[((int64_t)split * a.partial_rows + partial) * a.dim + d] = x;
         }
       }
       if (a.splits == 1) {
         // a row of -infinity alone, as one of NaN, is taken again
         if (__any(odd) || (l == 0.0f && m == -kInfinity)) again |= 1u << r;
       } else if (lane == 0) {
-        float* st = a.statistics + ((int64_t)split * a.p.tokens * a.heads + place) * 3;
+        float* st = a.statistics + ((int64_t)split * a.partial_rows + partial) * 3;
         st[0] = m, st[1] = l, st[2] = vm;
       }
     }
@@ -625,26 +644,497 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   }
 }
 
-// Joins the splits of attend_few (ROWS rows of TOK-position tiles a unit) row by row, a
-// wave a row.
+// The many-rows kernel: 64 rows of queries a wave (32 where heads are wider than
+// 128), four waves a block, positions in tiles of 64 that the block stages in LDS
+// once for all its rows, by 32 x 32 x 16 products. As in attend_few the scores are
+// taken transposed (the result's column, lane % 32, is a row of queries), with
+// the rows of K dealt out so that the 8 weights a lane brings to each product of
+// O^T = V^T P^T are those it holds (bits 2 and 3 of the row's number trade
+// places), and a wave's operand from LDS serves both its tiles of 32 rows: 1 KB
+// read for 64 cycles of matrix work a wave, half of what LDS gives.
+//
+// LDS: keys [64][DP], values [DP][64] in F16 (codes are made F16 numbers as they
+// are staged), 16-byte chunks moved by an exclusive or with the row's number so
+// that the rows of one operand lie on different banks; twice, so that a block needs
+// one barrier a tile. The next tile's chunks are in registers meanwhile.
+//
+// The maximum that weights are taken against is raised only when a score passes
+// it by more than kSlack (in powers of two), which keeps the rescaling of the
+// results out of most tiles: weights then reach 2^(kLift + kSlack) at most.
+template <typename T, bool I8, int DP>
+__global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, AttentionArgs a) {
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  constexpr int CT = DP > 128 ? 1 : 2;       // tiles of 32 rows a wave
+  constexpr int kRows = 4 * CT * 32;         // rows a block
+  constexpr int TOK = 64, KS = DP / 16, DT = DP / 32;
+  constexpr int kKeyChunks = DP / 8;         // of a position
+  constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
+  constexpr int kLoads = TOK * kKeyChunks / 256;  // chunks a thread stages, of keys and of values
+  // a tile in LDS: its keys, its values, and in 8 bits their scales and the exponents of the values'
+  constexpr int kValuesAt = TOK * DP * 2, kScalesAt = 2 * kValuesAt, kExponentsAt = kScalesAt + 2 * TOK * 4;
+  constexpr int kTileBytes = I8 ? kExponentsAt + 16 : kScalesAt;
+  __shared__ __attribute__((aligned(16))) char tiles[2 * kTileBytes];
+  static_assert(sizeof(RowScratch) * 4 <= sizeof(tiles), "");
+
+  const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
+  const int kv = blockIdx.x % (unsigned)a.kv_heads;
+  const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
+  const int split = rest % (unsigned)a.splits;
+  // the last rows first: they have the most positions
+  const int64_t unit = gridDim.x / (unsigned)(a.kv_heads * a.splits) - 1 - rest / (unsigned)a.splits;
+  int64_t nth;
+  const int s = locate(a.p, unit, kRows, 0, a.group, nth);
+  if (s < 0) return;
+  const Span span = span_of(a.p, s);
+  const int rows = (int)min((int64_t)span.rows * a.group - nth * kRows, (int64_t)kRows);
+  if (rows <= 0 || (int64_t)span.rows * a.group <= a.few_rows) return;
+  const uint32_t row0 = (uint32_t)nth * kRows, group = (uint32_t)a.group, start = (uint32_t)span.start;
+  const uint32_t p0 = start + row0 / group, p1 = start + (row0 + rows - 1) / group;
+  const TileList list = tiles_of(a, p0, p1, TOK);
+  const int each = split_tiles(a, list.count);
+  const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
+  if (begin >= end) return;
+
+  // ---- this wave's rows
+  const int wave_row = wave * CT * 32;
+  const bool idle = wave_row >= rows;
+  const uint32_t w0 = start + (row0 + min(wave_row, rows - 1)) / group;
+  const uint32_t w1 = start + (row0 + min(wave_row + CT * 32, rows) - 1) / group;
+  f16x8 query[CT][KS][TERMS];
+  float row_scale[CT];
+  uint32_t position[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const uint32_t row = row0 + min(wave_row + c * 32 + col, rows - 1), token = row / group;
+    position[c] = start + token;
+    const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
+    uint32_t most = 0;
+    float v[KS][8];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int d = k * 16 + h * 8;
+#pragma unroll
+      for (int e = 0; e < 8; e += Chunk<T>::N) {
+        float x[Chunk<T>::N];
+        Chunk<T>::unpack(cached_load(q + (d < a.dim ? d + e : e)), x);
+#pragma unroll
+        for (int i = 0; i < Chunk<T>::N; ++i) v[k][e + i] = d < a.dim ? x[i] : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[k][e]) & 0x7fffffffu);
+    }
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+    const bool finite = most < 0x7f800000u;
+    const int shift = finite && most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(most)) : 0;
+    // (above 0, so that the largest score is the largest product: a negative scale turns the query's sign. A scale
+    // of 0, or one that a tiny row makes it, is small enough to leave every weight even)
+    row_scale[c] = finite ? fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -shift), 0x1p-120f) : __builtin_nanf("");
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = finite ? ldexpf(v[k][e], shift) : 0.0f;
+        if (a.scale < 0.0f) x[e] = -x[e];
+      }
+      const Halves<TERMS> half = halves_of<TERMS>(x);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) query[c][k][t] = half.term[t];
+    }
+  }
+  f32x16 acc[CT][DT];
+  float ref[CT], total[CT];  // what weights are taken against, and their sum so far
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    ref[c] = -kInfinity;
+    total[c] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[c][d][e] = 0.0f;
+  }
+
+  // ---- staging: a thread's chunks of a tile
+  // Chunk n of a thread is of a unit that its whole wave shares, so that a load is
+  // a scalar base and an offset that stays. Where pages hold whole tiles, eight
+  // chunks of a value's row lie together; else two.
+  const uint32_t last_unit = p1 / 16;
+  const bool wide = a.page_units % 4 == 0;
+  constexpr int kUnitThreads = 2 * DP;  // threads that stage a unit's keys, or its values where pages are narrow
+  const int wave_unit = kUnitThreads < 256 ? uniform(thread) / kUnitThreads : 0;
+  auto unit_of = [&](int n) { return kUnitThreads <= 256 ? n * (256 / kUnitThreads) + wave_unit : n * 256 / kUnitThreads; };
+  struct Pages {
+    const char *key[4], *value[4];  // where the unit's keys and values of this head begin
+    int64_t scale[4];
+    uint32_t okay;  // bit u: unit u's page is one of the cache's
+  };
+  constexpr int kBytes = I8 ? 1 : 2;
+  typedef const int32_t __attribute__((address_space(4))) * Scalars;
+  auto pages_of = [&](int i) {
+    Pages w;
+    w.okay = 0;
+    const uint32_t first = (uint32_t)list.tile(i) * 4;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t at = min(first + u, last_unit);
+      const uint32_t column = a.unit_shift >= 0 ? at >> a.unit_shift : uniform(at / (uint32_t)a.page_units);
+      const uint32_t off = (at - column * (uint32_t)a.page_units) * 16;
+      const int32_t named = ((Scalars)(uintptr_t)span.table)[column];
+      const bool okay = (uint32_t)named < (uint32_t)a.p.cache_pages;
+      const int64_t page = okay ? named : 0;
+      w.okay |= okay ? 1u << u : 0u;
+      w.key[u] = (const char*)a.keys + ((page * a.p.page_size + off) * a.kv_heads + kv) * a.dim * kBytes;
+      w.scale[u] = (page * a.kv_heads + kv) * a.p.page_size + off;
+      w.value[u] = (const char*)a.values + ((w.scale[u] - off) * a.dim + off) * kBytes;
+    }
+    return w;
+  };
+  typedef typename std::conditional<I8, uint2, uint4>::type Raw;
+  Raw key_raw[kLoads], value_raw[kLoads];
+  float scale_raw = 0.0f;
+  auto key_chunk = [&](int n, int& token, int& chunk) {
+    const int q = thread + 256 * n;
+    token = q / kKeyChunks;
+    chunk = q % kKeyChunks;
+  };
+  auto value_chunk = [&](int n, int& d, int& chunk) {
+    const int q = thread + 256 * n;
+    d = wide ? q >> 3 : (q >> 1) % DP;
+    chunk = wide ? q & 7 : q / kUnitThreads * 2 + (q & 1);
+  };
+  uint32_t key_at[kLoads], value_at[kLoads];
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    int token, chunk, d;
+    key_chunk(n, token, chunk);
+    key_at[n] = ((uint32_t)(token % 16) * a.kv_heads * a.dim + (chunk * 8 < a.dim ? chunk * 8 : 0)) * kBytes;
+    value_chunk(n, d, chunk);
+    value_at[n] = ((uint32_t)min(d, a.dim - 1) * a.p.page_size + (wide ? chunk : chunk & 1) * 8) * kBytes;
+  }
+  auto load_tile = [&](const Pages& w) {
+    auto pick = [&](const char* const (&x)[4], int n) {
+      const int u = unit_of(n);
+      if constexpr (kUnitThreads >= 256) return x[u];
+      else return wave_unit ? x[(n * 2 + 1) & 3] : x[(n * 2) & 3];
+    };
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) key_raw[n] = *(const Raw*)(pick(w.key, n) + key_at[n]);
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const char* from = wide ? w.value[0] : pick(w.value, n);
+      value_raw[n] = *(const Raw*)(from + value_at[n]);
+    }
+    if constexpr (I8) {
+      // wave 0 brings the keys' scales, wave 1 the values'
+      if (wave < 2) {
+        const int u = lane / 16;
+        const int64_t at = u & 2 ? (u & 1 ? w.scale[3] : w.scale[2]) : (u & 1 ? w.scale[1] : w.scale[0]);
+        scale_raw = (wave == 0 ? a.key_scales : a.value_scales)[at + lane % 16];
+      }
+    }
+  };
+  // where a tile has chunk `chunk` of position `token`, or of value d
+  auto key_place = [](int token, int chunk) {
+    return (token * kKeyChunks + (chunk ^ (DP >= 128 ? token & 15 : (token >> 1) & 7))) * 16;
+  };
+  auto value_place = [](int d, int chunk) { return kValuesAt + (d * 8 + (chunk ^ ((d >> 1) & 7))) * 16; };
+  int key_to[kLoads], value_to[kLoads];
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    int token, chunk, d;
+    key_chunk(n, token, chunk);
+    key_to[n] = key_place(token, chunk);
+    value_chunk(n, d, chunk);
+    value_to[n] = value_place(d, chunk);
+  }
+  // operands: chunk 2 k + h of the lane's position (its low four bits are what the
+  // exclusive or moves), and chunk n of the lane's value
+  const int key_row = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
+  constexpr int kKeyPlaces = KS < 8 ? KS : 8;
+  int key_from[kKeyPlaces], value_from[4];
+#pragma unroll
+  for (int k = 0; k < kKeyPlaces; ++k) key_from[k] = key_place(key_row, 2 * k + h);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) value_from[n] = value_place(col, 2 * n + h);
+  auto staged = [](const Raw& raw) {
+    if constexpr (I8) return __builtin_bit_cast(uint4, codes_f16(raw.x, raw.y));
+    else return raw;
+  };
+  constexpr int kNone = -1000;  // no scale above 0
+  auto store_tile = [&](char* tile, int i, uint32_t okay) {
+    const uint32_t base = (uint32_t)list.tile(i) * TOK;
+    // positions that no row of the block sees count as zeros: they may hold anything
+    const bool whole = okay == 15u && base + TOK - 1 <= p1 &&
+                       (a.window == 0 || base + (uint32_t)a.window > p0 || base + TOK - 1 < (uint32_t)a.sinks);
+    auto seen = [&](int token) {
+      const uint32_t j = base + token;
+      return (bool)(okay >> (token / 16) & 1) & (j <= p1) &
+             ((a.window == 0) | (j + (uint32_t)a.window > p0) | (j < (uint32_t)a.sinks));
+    };
+    if (okay != 15u && thread < TOK && !(okay >> (thread / 16) & 1)) {
+      const uint32_t j = base + thread;
+      if (j <= p1 && (a.window == 0 || j + (uint32_t)a.window > p0 || j < (uint32_t)a.sinks)) flag_bad(a.p);
+    }
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) *(uint4*)(tile + key_to[n]) = staged(key_raw[n]);
+    if (I8 || whole) {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) *(uint4*)(tile + value_to[n]) = staged(value_raw[n]);
+    } else {
+#pragma unroll 1
+      for (int n = 0; n < kLoads; ++n) {
+        int d, chunk, to = value_to[0];
+        value_chunk(n, d, chunk);
+        uint4 x = staged(value_raw[0]);
+#pragma unroll
+        for (int o = 1; o < kLoads; ++o)
+          if (n == o) x = staged(value_raw[o]), to = value_to[o];
+        uint32_t keep[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          keep[e] = (seen(chunk * 8 + 2 * e) ? 0xffffu : 0u) | (seen(chunk * 8 + 2 * e + 1) ? 0xffff0000u : 0u);
+        x.x &= keep[0], x.y &= keep[1], x.z &= keep[2], x.w &= keep[3];
+        *(uint4*)(tile + to) = x;
+      }
+    }
+    if constexpr (I8) {
+      float* scales = (float*)(tile + kScalesAt);
+      if (wave == 0) scales[lane] = scale_raw;
+      else if (wave == 1) {
+        const float x = whole || seen(lane) ? scale_raw : 0.0f;
+        scales[TOK + lane] = x;
+        const bool counts = x > 0.0f && x < kInfinity;
+        const float exponent = (float)__builtin_amdgcn_frexp_expf(x);
+        const float most = group_max<64>(counts ? exponent : (float)kNone);
+        const float least = -group_max<64>(counts ? -exponent : (float)kNone);
+        if (lane == 0) *(int2*)(tile + kExponentsAt) = make_int2((int)most, (int)least);
+      }
+    }
+  };
+
+  int value_exponent = kNone, least_exponent = -kNone;  // of the values' scales so far
+  Pages pages = pages_of(begin);
+  load_tile(pages);
+  uint32_t okay = pages.okay;
+  pages = pages_of(min(begin + 1, end - 1));
+  for (int i = begin; i < end; ++i) {
+    int now = uniform(((i - begin) & 1) * kTileBytes);
+    asm volatile("" : "+s"(now));  // (or both buffers' every address is kept in registers)
+    char* tile = tiles + now;
+    store_tile(tile, i, okay);
+    const uint32_t okay_now = okay;
+    if (i + 1 < end) {
+      load_tile(pages);
+      okay = pages.okay;
+      pages = pages_of(min(i + 2, end - 1));
+    }
+    __syncthreads();
+    const uint32_t base = (uint32_t)list.tile(i) * TOK;
+    // whether any, and whether every row of the wave sees the tile
+    if (idle || base > w1) continue;
+    if (a.window && base + TOK - 1 + (uint32_t)a.window <= w0 && base >= (uint32_t)a.sinks) continue;
+    const bool whole = okay_now == 15u && base + TOK - 1 <= w0 &&
+                       (a.window == 0 || base + (uint32_t)a.window > w1 || base + TOK - 1 < (uint32_t)a.sinks);
+    float lower = 1.0f;  // 2^-value_exponent
+    if constexpr (I8) {
+      const int2 exponents = *(const int2*)(tile + kExponentsAt);
+      const int most = max(uniform(exponents.x), -126);
+      if (most > value_exponent) {
+        const float keep = value_exponent == kNone ? 0.0f : exp2_fast((float)(value_exponent - most));
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c][d][e] *= keep;
+        value_exponent = most;
+      }
+      least_exponent = min(least_exponent, uniform(exponents.y));
+      lower = exp2_fast((float)-value_exponent);
+    }
+    // scores: score[half][c][e] is row 32 c + col, position base + 32 half + 16 (e / 8) + 8 h + e % 8
+    f32x16 score[2][CT];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) score[half][c][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const f16x8 key = *(const f16x8*)(tile + key_from[k % 8] + half * 32 * DP * 2 + k / 8 * 256);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int m = 0; m < TERMS; ++m)
+            score[half][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, query[c][k][m], score[half][c], 0, 0, 0);
+      }
+    }
+    if constexpr (I8) {
+      const float* scales = (const float*)(tile + kScalesAt) + h * 8;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 x = *(const float4*)(scales + half * 32 + e / 8 * 16 + e % 8);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            score[half][c][e] *= x.x, score[half][c][e + 1] *= x.y;
+            score[half][c][e + 2] *= x.z, score[half][c][e + 3] *= x.w;
+          }
+        }
+    }
+    if (!whole) {
+      uint32_t mine = base + h * 8;
+      asm volatile("" : "+v"(mine));
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int n = 0; n < 32; ++n) {
+          const uint32_t j = mine + n / 8 * 16 + n % 8;
+          const bool seen = (bool)(okay_now >> (n / 8) & 1) & (j <= position[c]) &
+                            ((a.window == 0) | (j + (uint32_t)a.window > position[c]) | (j < (uint32_t)a.sinks));
+          score[n / 16][c][n % 16] = seen ? score[n / 16][c][n % 16] : -kInfinity;
+        }
+    }
+    float high[CT];
+    bool raise = false;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      high[c] = fmaxf(score[0][c][0], score[1][c][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) high[c] = fmaxf(high[c], fmaxf(score[0][c][e], score[1][c][e]));
+      raise |= high[c] * row_scale[c] > ref[c] + kSlack;
+    }
+    if (__any(raise))
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const float next = fmaxf(ref[c], fmaxf(high[c], __shfl_xor(high[c], 32, kWave)) * row_scale[c]);
+        const float keep = exp2_fast(ref[c] - (next == -kInfinity ? 0.0f : next));
+        ref[c] = next;
+        total[c] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c][d][e] *= keep;
+      }
+    float lift[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) lift[c] = kManyLift - (ref[c] == -kInfinity ? 0.0f : ref[c]);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {  // 16 positions
+      float value_scale[I8 ? 8 : 1];
+      if constexpr (I8) {
+        const float* scales = (const float*)(tile + kScalesAt) + TOK + h * 8 + n * 16;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) value_scale[e] = scales[e] * lower;
+      }
+      Halves<TERMS> weights[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = exp2_fast(fmaf(score[n / 2][c][n % 2 * 8 + e], row_scale[c], lift[c]));
+          total[c] += p;
+          w[e] = I8 ? p * value_scale[e] : p;
+        }
+        weights[c] = halves_of<TERMS>(w);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const f16x8 value = *(const f16x8*)(tile + value_from[n] + d * 4096);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int m = 0; m < TERMS; ++m)
+            acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, weights[c].term[m], acc[c][d], 0, 0, 0);
+      }
+    }
+  }
+
+  // scales so far apart that the smaller ones' weights lost bits: the rows are taken again, one by one
+  const bool apart = I8 && value_exponent - least_exponent > 16;
+  if (value_exponent == kNone) value_exponent = 0;
+  uint64_t again[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int r = wave_row + c * 32 + col;
+    const bool there = r < rows;
+    const uint32_t row = row0 + min(r, rows - 1), token = row / group;
+    const int64_t place = (span.first + token) * a.heads + kv * a.group + (row - token * group);
+    const float sum = total[c] + __shfl_xor(total[c], 32, kWave);
+    bool odd = apart || (sum == 0.0f && ref[c] == -kInfinity);
+    if (a.splits == 1) {
+      const float inverse = sum == 0.0f ? 0.0f : (I8 ? exp2_fast((float)value_exponent) : 1.0f) / sum;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int at = d * 32 + 2 * e + 4 * h;
+          float x[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            x[n] = acc[c][d][e + n] * inverse;
+            odd |= !(fabsf(x[n]) < kInfinity);
+          }
+          if (there && at < a.dim) {
+            if constexpr (TERMS == 2) *(float4*)(out + place * a.dim + at) = make_float4(x[0], x[1], x[2], x[3]);
+            else *(uint2*)(out + place * a.dim + at) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+          }
+        }
+      again[c] = __ballot(odd && there);
+    } else {
+      const int64_t at = (int64_t)split * a.partial_rows + place;
+      if (there) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (d * 32 + 2 * e + 4 * h < a.dim)
+              *(f32x4*)(a.partials + at * a.dim + d * 32 + 2 * e + 4 * h) =
+                  f32x4{acc[c][d][e], acc[c][d][e + 1], acc[c][d][e + 2], acc[c][d][e + 3]};
+        if (h == 0) {
+          a.statistics[at * 3] = ref[c];
+          a.statistics[at * 3 + 1] = apart ? __builtin_nanf("") : sum;
+          a.statistics[at * 3 + 2] = ref[c] + (float)value_exponent;
+        }
+      }
+      again[c] = 0;
+    }
+  }
+  __syncthreads();  // the tiles are free, and hold the scratch
+  RowScratch& scratch = reinterpret_cast<RowScratch*>(tiles)[wave];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+    for (uint32_t rest_rows = (uint32_t)again[c] | (uint32_t)(again[c] >> 32); rest_rows; rest_rows &= rest_rows - 1) {
+      const uint32_t row = row0 + wave_row + c * 32 + __ffs(rest_rows) - 1;
+      attend_row<T, I8>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
+    }
+}
+
+// Joins the splits of the kernels above (units of `rows` rows, tiles of `tile`
+// positions) row by row, a wave a row.
 template <typename T, bool I8>
-__global__ void __launch_bounds__(64) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
+__global__ void __launch_bounds__(64) attend_join(const T* queries, T* out, AttentionArgs a, bool few, int rows, int tile) {
   __shared__ RowScratch scratch;
   const int lane = threadIdx.x, h = blockIdx.x % (unsigned)a.heads;
   int64_t nth;
   const int s = locate(a.p, blockIdx.x / (unsigned)a.heads, 1, 0, 1, nth);
   if (s < 0) return;
   const Span span = span_of(a.p, s);
-  if (nth >= span.rows) return;
+  if (nth >= span.rows || ((int64_t)span.rows * a.group <= a.few_rows) != few) return;
   // the unit the row was in, its tiles and so its splits
   const int64_t row0 = (nth * a.group + h % a.group) / rows * rows;
   const int64_t last = min(row0 + rows, (int64_t)span.rows * a.group) - 1;
   const TileList list = tiles_of(a, span.start + row0 / a.group, span.start + last / a.group, tile);
   const int each = split_tiles(a, list.count), splits = (list.count + each - 1) / each;
-  const int64_t place = (span.first + nth) * a.heads + h, stride = (int64_t)a.p.tokens * a.heads;
+  const int64_t place = (span.first + nth) * a.heads + h, stride = a.partial_rows;
+  const int64_t partial =
+      few ? ((int64_t)s * a.kv_heads + h / a.group) * a.few_most + nth * a.group + h % a.group : place;
   float m = -kInfinity, vm = -kInfinity;
   for (int i = lane; i < splits; i += kWave) {
-    const float* st = a.statistics + (i * stride + place) * 3;
+    const float* st = a.statistics + (i * stride + partial) * 3;
     m = fmaxf(m, st[0]);
     vm = fmaxf(vm, st[2]);
   }
@@ -655,10 +1145,10 @@ __global__ void __launch_bounds__(64) attend_join(const T* queries, T* out, Atte
   constexpr int kEach = kMaxHead / kWave;
   float x[kEach] = {};
   for (int i = 0; i < splits; ++i) {
-    const float* st = a.statistics + (i * stride + place) * 3;
+    const float* st = a.statistics + (i * stride + partial) * 3;
     l = fmaf(st[1], exp2_fast(st[0] - ref), l);
     const float factor = exp2_fast(st[2] - value_ref);
-    const float* part = a.partials + (i * stride + place) * a.dim;
+    const float* part = a.partials + (i * stride + partial) * a.dim;
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
       if (lane + e * kWave < a.dim) x[e] = fmaf(part[lane + e * kWave], factor, x[e]);
@@ -691,27 +1181,49 @@ int check_attention(const char* entry, int32_t heads, int32_t kv_heads, int32_t 
 
 // How a call's work is laid out, by its numbers alone (the workspace's size
 // follows from it before there are tensors).
+struct Split {
+  int splits;  // over positions; 0: nothing is to be done this way
+  int chunk;   // tiles of 64 positions that a split has at least
+};
 struct Plan {
-  bool few;    // at most 16 rows of queries a sequence and key head
-  int splits;  // over positions
-  int chunk;   // tiles of 32 positions that a split has at least
+  bool few16;       // attend_few's sequences have at most 16 rows
+  Split few, many;  // attend_few, attend_many
+  int64_t few_most, few_partials, many_partials;  // AttentionArgs::few_most, partial_rows
   int64_t bytes;
 };
 
+// Rows of queries of a sequence and key head up to which it is attend_few's.
+constexpr int kFewRows = 64;
+constexpr int many_rows(int64_t dim) { return dim > 128 ? 128 : 256; }
+
+// `blocks` blocks before the split, over `positions` positions, towards `wanted`
+// of them.
+Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least, int64_t most) {
+  const int64_t tiles = std::max<int64_t>(ceil_div(positions, 64), 1);
+  const int64_t chunk = std::min(std::max(tiles * blocks / wanted, least), most);
+  return {(int)std::min<int64_t>(ceil_div(tiles, chunk), 1024), (int)std::min<int64_t>(chunk, INT32_MAX)};
+}
+
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
-             int64_t sinks, int64_t longest) {
-  Plan p{true, 1, 1, 0};
+             int64_t sinks, int64_t longest, bool by_offsets) {
+  Plan p{true, {0, 1}, {0, 1}, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
-  const int64_t group = heads / kv_heads, each = ceil_div(tokens, sequences);
-  p.few = each * group <= 16;
-  const int64_t seen = window ? std::min(longest, window + sinks + each) : longest;
-  const int64_t tiles = std::max<int64_t>(ceil_div(seen, 32), 1);
-  const int64_t blocks = (sequences + tokens * group / (p.few ? 16 : 64)) * kv_heads;
-  int64_t chunk = tiles * blocks / 1024;
-  chunk = std::min<int64_t>(std::max<int64_t>(chunk, 8), 64);
-  p.chunk = (int)chunk;
-  p.splits = (int)std::min<int64_t>(ceil_div(tiles, chunk), 1024);
-  if (p.splits > 1) p.bytes = (int64_t)p.splits * tokens * heads * (dim + 3) * 4;
+  const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
+  const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
+  // (mixed batches are single tokens for the most part: 16 rows a unit while a sequence has 24 on average)
+  p.few16 = by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
+  if (by_offsets || each * group <= kFewRows) p.few = split_of(sequences * kv_heads, seen, 1024, 4, 32);
+  if (each * group > kFewRows) {
+    const int64_t blocks = ceil_div(tokens * group, many_rows(dim)) * kv_heads;
+    p.many = split_of(blocks, seen, 512, 8, blocks >= 256 ? INT64_MAX / 2 : 1 << 20);
+    if (blocks >= 384) p.many.splits = 1;
+  }
+  p.few_most = std::min(each * group, (int64_t)kFewRows);
+  p.few_partials = sequences * kv_heads * p.few_most;
+  p.many_partials = tokens * heads;
+  // the one's launches are done with it before the other's begin
+  if (p.few.splits > 1) p.bytes = p.few.splits * p.few_partials * (dim + 3) * 4;
+  if (p.many.splits > 1) p.bytes = std::max(p.bytes, p.many.splits * p.many_partials * (dim + 3) * 4);
   return p;
 }
 
@@ -720,34 +1232,61 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
 template <typename T, bool I8, int DP>
 constexpr int kManyTiles = DP > 128 ? 1 : DP <= 64 || (sizeof(T) == 2 && !I8) ? 4 : 2;
 
-template <typename T, bool I8, int DP>
-int launch_few(const char* entry, const T* queries, T* out, const AttentionArgs& a, bool few, hipStream_t st) {
-  constexpr int kMany = kManyTiles<T, I8, DP>;
-  const int rows = 16 * (few ? 1 : kMany);
-  const dim3 grid((unsigned)(units_of(a.p, rows, 0, a.group) * a.splits * a.kv_heads)), block(256);
-  if (few) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), grid, block, 0, st, queries, out, a);
-  else hipLaunchKernelGGL((attend_few<T, I8, DP, kMany>), grid, block, 0, st, queries, out, a);
+template <typename T, bool I8>
+int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, bool few, int rows, int tile,
+         hipStream_t st) {
   const int bad = launched(entry);
   if (bad || a.splits == 1) return bad;
   hipLaunchKernelGGL((attend_join<T, I8>), dim3((unsigned)(units_of(a.p, 1, 0, 1) * a.heads)), dim3(kWave), 0, st,
-                     queries, out, a, rows, I8 ? 64 : 32);
+                     queries, out, a, few, rows, tile);
   return launched(entry);
+}
+
+template <typename T, bool I8, int DP>
+int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, hipStream_t st) {
+  if (plan.few.splits > 0) {
+    a.splits = plan.few.splits;
+    a.chunk = I8 ? plan.few.chunk : plan.few.chunk * 2;
+    constexpr int kMany = kManyTiles<T, I8, DP>;
+    const int rows = 16 * (plan.few16 ? 1 : kMany);
+    a.few_most = (int)plan.few_most;
+    a.few_units = (int)ceil_div(plan.few_most, rows);
+    a.partial_rows = plan.few_partials;
+    a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
+    const dim3 grid((unsigned)((int64_t)a.p.sequences * a.few_units * a.splits * a.kv_heads)), block(256);
+    if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), grid, block, 0, st, queries, out, a);
+    else hipLaunchKernelGGL((attend_few<T, I8, DP, kMany>), grid, block, 0, st, queries, out, a);
+    if (const int bad = join<T, I8>(entry, queries, out, a, true, rows, I8 ? 64 : 32, st)) return bad;
+  }
+  if (plan.many.splits > 0) {
+    a.splits = plan.many.splits;
+    a.chunk = plan.many.chunk;
+    a.partial_rows = plan.many_partials;
+    a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
+    constexpr int kRows = many_rows(DP);
+    const dim3 grid((unsigned)(units_of(a.p, kRows, 0, a.group) * a.splits * a.kv_heads)), block(256);
+    hipLaunchKernelGGL((attend_many<T, I8, DP>), grid, block, 0, st, queries, out, a);
+    return join<T, I8>(entry, queries, out, a, false, kRows, 64, st);
+  }
+  return 0;
 }
 
 template <typename T, bool I8>
 int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, bool aligned, hipStream_t st) {
   const int64_t row_blocks = units_of(a.p, 1, 0, 1) * a.heads;
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
-  const int64_t blocks = units_of(a.p, 16, 0, a.group) * plan.splits * a.kv_heads;  // at most
-  if (!aligned || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
+  const int64_t blocks = std::max((int64_t)a.p.sequences * 4 * plan.few.splits,
+                                  units_of(a.p, 128, 0, a.group) * plan.many.splits) * a.kv_heads;
+  // (the tile kernels' offsets within a page's unit and a head's values have 32 bits)
+  const bool small = (int64_t)a.kv_heads * a.dim * 32 < (int64_t)1 << 31 && (int64_t)a.p.page_size * a.dim * 2 < (int64_t)1 << 31;
+  if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
     hipLaunchKernelGGL((attend_rows<T, I8>), dim3((unsigned)row_blocks), dim3(kWave), 0, st, queries, out, a);
     return launched(entry);
   }
-  a.splits = plan.splits;
-  a.chunk = I8 ? plan.chunk / 2 : plan.chunk;
-  if (a.dim <= 64) return launch_few<T, I8, 64>(entry, queries, out, a, plan.few, st);
-  if (a.dim <= 128) return launch_few<T, I8, 128>(entry, queries, out, a, plan.few, st);
-  return launch_few<T, I8, 256>(entry, queries, out, a, plan.few, st);
+  a.few_rows = plan.few.splits == 0 ? 0 : plan.many.splits == 0 ? INT32_MAX : kFewRows;
+  if (a.dim <= 64) return launch_tiles<T, I8, 64>(entry, queries, out, a, plan, st);
+  if (a.dim <= 128) return launch_tiles<T, I8, 128>(entry, queries, out, a, plan, st);
+  return launch_tiles<T, I8, 256>(entry, queries, out, a, plan, st);
 }
 
 template <typename T>
@@ -765,12 +1304,12 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   a.group = a.heads / a.kv_heads;
   a.page_units = a.p.page_size / 16;
   a.unit_shift = (a.page_units & (a.page_units - 1)) == 0 ? __builtin_ctz((unsigned)a.page_units) : -1;
-  const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest);
+  const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
+                            a.p.offsets != nullptr);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,
                   (long long)plan.bytes);
   a.partials = (float*)workspace;
-  a.statistics = a.partials + (int64_t)plan.splits * a.p.tokens * a.heads * a.dim;
   const bool aligned = a.dim % 8 == 0 && aligned16(queries) && aligned16(a.keys) && aligned16(a.values) &&
                        (!a.key_scales || (aligned16(a.key_scales) && aligned16(a.value_scales)));
   const hipStream_t st = (hipStream_t)stream;
@@ -792,14 +1331,16 @@ extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens
   if (const int bad = check_attention("drift_paged_attention_workspace", heads, kv_heads, head_dim, window, sinks,
                                       longest))
     return bad;
-  *bytes = plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest).bytes;
+  // with offsets or without
+  for (const bool by_offsets : {false, true})
+    *bytes = std::max(*bytes, plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest, by_offsets).bytes);
   return 0;
 }
 
 #define DRIFT_ATTENTION_ARGS                                                                                        \
   AttentionArgs {                                                                                                   \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, nullptr, nullptr, 0, 0 \
+        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, 0, 0 \
   }
 
 extern "C" int drift_paged_attention_f32(const float* queries, const void* keys, const void* values,

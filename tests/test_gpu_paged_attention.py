@@ -17,11 +17,11 @@ Bars, derived from the roundings on the way:
   first term exact), and F16's last step is 2^-24, half of it 2^-25, so the
   last term of a weight is off by at most 2^-39 of the largest weight however
   small the weight is. With the values that is 2^-39 max p sum |v| over the
-  visible positions; in 8 bits, where a weight is p times the value's scale w and
-  the values are codes up to 127, 2^-39 max(p w) 127 n. (It shows where a row's
-  one strong position has a value of 0.)
-- attention, BF16: besides those, the output's rounding, 2^-8 relative (half a
-  step is eps / 2 = 2^-8), and the weights' to 11 bits: 2^-11 of the sum of p |v|.
+  visible positions; in 8 bits, where a weight is p times the value's scale w over
+  a power of two above every scale so far (less than twice the largest), and the
+  values are codes up to 127, 2^-39 max p 2 max w 127 n. BF16's one term is lifted
+  by 2^7 at least, which makes it 2^-32. (It shows where a row's one strong
+  position has a value of 0.)
 """
 
 import math
@@ -152,8 +152,9 @@ def wanted(case, queries, scale, window=None, hidden=()):
                 if case.kind == "f16":
                     lost = p.amax(-1, keepdim=True) * (seen.double() @ vh.abs().nan_to_num(0, 0, 0))
                 else:
-                    lost = (p * case.scales[s][:, h // group]).amax(-1, keepdim=True) * 127 * count[rows, h]
-                small_weights[rows, h] = 2.0 ** -39 * lost.nan_to_num(0)
+                    lost = p.amax(-1, keepdim=True) * 2 * case.scales[s][:, h // group].max() * 127 * count[rows, h]
+                small_weights[rows, h] = (2.0 ** -39 if queries.dtype == torch.float32 else 2.0 ** -32) * \
+                    lost.nan_to_num(0)
     return out, mass, size, count, small_weights
 
 
