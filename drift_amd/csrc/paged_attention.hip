@@ -1113,57 +1113,89 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
     }
 }
 
-// Joins the splits of the kernels above (units of `rows` rows, tiles of `tile`
-// positions) row by row, a wave a row.
-template <typename T, bool I8>
-__global__ void __launch_bounds__(64) attend_join(const T* queries, T* out, AttentionArgs a, bool few, int rows, int tile) {
-  __shared__ RowScratch scratch;
-  const int lane = threadIdx.x, h = blockIdx.x % (unsigned)a.heads;
+// Joins the splits of attend_few (FEW) or attend_many: a block takes up to
+// kJoinRows rows of one unit (`rows` of them, tiles of `tile` positions, which say
+// how many splits it had), a row by as many lanes as hold its values in fours.
+constexpr int kJoinRows = 16;
+
+template <typename T, bool I8, bool FEW, int DP>
+__global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
+  constexpr int L = DP / 4;  // lanes a row
+  __shared__ RowScratch scratch[4];
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), in = lane % L;
+  const int parts = rows / kJoinRows;
+  const int kv = blockIdx.x % (unsigned)a.kv_heads, part = blockIdx.x / (unsigned)a.kv_heads % (unsigned)parts;
+  const unsigned unit = blockIdx.x / (unsigned)a.kv_heads / (unsigned)parts;
+  int s;
   int64_t nth;
-  const int s = locate(a.p, blockIdx.x / (unsigned)a.heads, 1, 0, 1, nth);
+  if constexpr (FEW) s = (int)(unit / (unsigned)a.few_units), nth = unit % (unsigned)a.few_units;
+  else s = locate(a.p, unit, rows, 0, a.group, nth);
   if (s < 0) return;
   const Span span = span_of(a.p, s);
-  if (nth >= span.rows || ((int64_t)span.rows * a.group <= a.few_rows) != few) return;
-  // the unit the row was in, its tiles and so its splits
-  const int64_t row0 = (nth * a.group + h % a.group) / rows * rows;
-  const int64_t last = min(row0 + rows, (int64_t)span.rows * a.group) - 1;
-  const TileList list = tiles_of(a, span.start + row0 / a.group, span.start + last / a.group, tile);
+  const uint32_t all = (uint32_t)span.rows * (uint32_t)a.group, group = (uint32_t)a.group;
+  const uint32_t row0 = (uint32_t)nth * rows;
+  if (row0 + part * kJoinRows >= all || (all <= (uint32_t)a.few_rows) != FEW) return;
+  const uint32_t last = min(row0 + rows, all) - 1, end = min(row0 + (part + 1) * kJoinRows, last + 1);
+  const TileList list = tiles_of(a, span.start + row0 / group, span.start + last / group, tile);
   const int each = split_tiles(a, list.count), splits = (list.count + each - 1) / each;
-  const int64_t place = (span.first + nth) * a.heads + h, stride = a.partial_rows;
-  const int64_t partial =
-      few ? ((int64_t)s * a.kv_heads + h / a.group) * a.few_most + nth * a.group + h % a.group : place;
-  float m = -kInfinity, vm = -kInfinity;
-  for (int i = lane; i < splits; i += kWave) {
-    const float* st = a.statistics + (i * stride + partial) * 3;
-    m = fmaxf(m, st[0]);
-    vm = fmaxf(vm, st[2]);
-  }
-  m = group_max<64>(m);
-  vm = group_max<64>(vm);
-  const float ref = m == -kInfinity ? 0.0f : m, value_ref = vm == -kInfinity ? 0.0f : vm;
-  float l = 0.0f;
-  constexpr int kEach = kMaxHead / kWave;
-  float x[kEach] = {};
-  for (int i = 0; i < splits; ++i) {
-    const float* st = a.statistics + (i * stride + partial) * 3;
-    l = fmaf(st[1], exp2_fast(st[0] - ref), l);
-    const float factor = exp2_fast(st[2] - value_ref);
-    const float* part = a.partials + (i * stride + partial) * a.dim;
+  for (uint32_t first = row0 + part * kJoinRows + wave * (64 / L); first < end; first += 4 * (64 / L)) {
+    const uint32_t mine = first + lane / L, row = min(mine, end - 1), token = row / group;
+    const int h = kv * a.group + (int)(row - token * group);
+    const int64_t place = (span.first + token) * a.heads + h;
+    const int64_t partial = FEW ? ((int64_t)s * a.kv_heads + kv) * a.few_most + row : place;
+    const float* st = a.statistics + partial * 3;
+    const float* from = a.partials + partial * a.dim + min(in * 4, a.dim - 4);
+    const int64_t st_step = a.partial_rows * 3, step = a.partial_rows * a.dim;
+    float m = -kInfinity, vm = -kInfinity, l = 0.0f;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    // eight splits at a time, their loads on the way together
+    for (int i = 0; i < splits; i += 8) {
+      float sm[8], sl[8], sv[8];
+      f32x4 v[8];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (lane + e * kWave < a.dim) x[e] = fmaf(part[lane + e * kWave], factor, x[e]);
-  }
-  const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast(value_ref - ref) : 1.0f) / l;
-  bool odd = l == 0.0f && m == -kInfinity;
+      for (int n = 0; n < 8; ++n) {
+        const int64_t at = min(i + n, splits - 1);
+        sm[n] = st[at * st_step], sl[n] = st[at * st_step + 1], sv[n] = st[at * st_step + 2];
+        v[n] = *(const f32x4*)(from + at * step);
+      }
+      float next = m, value_next = vm;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int d = lane + e * kWave;
-    if (d >= a.dim) break;
-    x[e] *= inverse;
-    odd |= !(fabsf(x[e]) < kInfinity);
-    store_one(out + place * a.dim + d, x[e]);
+      for (int n = 0; n < 8; ++n) {
+        if (i + n >= splits) sm[n] = sv[n] = -kInfinity, sl[n] = 0.0f, v[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        next = fmaxf(next, sm[n]), value_next = fmaxf(value_next, sv[n]);
+      }
+      const float ref = next == -kInfinity ? 0.0f : next, value_ref = value_next == -kInfinity ? 0.0f : value_next;
+      l *= exp2_fast(m - ref);
+      x *= exp2_fast(vm - value_ref);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        l = fmaf(sl[n], exp2_fast(sm[n] - ref), l);
+        const float factor = exp2_fast(sv[n] - value_ref);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(v[n][e], factor, x[e]);
+      }
+      m = next, vm = value_next;
+    }
+    const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast((vm == -kInfinity ? 0.0f : vm) - (m == -kInfinity ? 0.0f : m)) : 1.0f) / l;
+    bool odd = l == 0.0f && m == -kInfinity;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] *= inverse;
+      odd |= !(fabsf(x[e]) < kInfinity);
+    }
+    const bool there = mine < end && in * 4 < a.dim;
+    if (there) {
+      if constexpr (sizeof(T) == 4) *(f32x4*)(out + place * a.dim + in * 4) = x;
+      else *(uint2*)(out + place * a.dim + in * 4) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    }
+    // rows that came out as no numbers are taken again
+    for (uint64_t again = __ballot(there && odd); again;) {
+      const int which = (__ffsll((unsigned long long)again) - 1) / L;
+      const uint32_t r = first + which, t = r / group;
+      attend_row<T, I8>(queries, out, a, span, t, kv * a.group + (int)(r - t * group), scratch[wave]);
+      again &= L == 64 ? 0 : ~(((1ull << (L % 64)) - 1) << (which * L));
+    }
   }
-  if (__any(odd)) attend_row<T, I8>(queries, out, a, span, nth, h, scratch);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1232,13 +1264,13 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
 template <typename T, bool I8, int DP>
 constexpr int kManyTiles = DP > 128 ? 1 : DP <= 64 || (sizeof(T) == 2 && !I8) ? 4 : 2;
 
-template <typename T, bool I8>
-int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, bool few, int rows, int tile,
+template <typename T, bool I8, bool FEW, int DP>
+int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, int64_t units, int rows, int tile,
          hipStream_t st) {
   const int bad = launched(entry);
   if (bad || a.splits == 1) return bad;
-  hipLaunchKernelGGL((attend_join<T, I8>), dim3((unsigned)(units_of(a.p, 1, 0, 1) * a.heads)), dim3(kWave), 0, st,
-                     queries, out, a, few, rows, tile);
+  hipLaunchKernelGGL((attend_join<T, I8, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows))), dim3(256),
+                     0, st, queries, out, a, rows, tile);
   return launched(entry);
 }
 
@@ -1253,10 +1285,11 @@ int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, c
     a.few_units = (int)ceil_div(plan.few_most, rows);
     a.partial_rows = plan.few_partials;
     a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
-    const dim3 grid((unsigned)((int64_t)a.p.sequences * a.few_units * a.splits * a.kv_heads)), block(256);
+    const int64_t units = (int64_t)a.p.sequences * a.few_units;
+    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(256);
     if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), grid, block, 0, st, queries, out, a);
     else hipLaunchKernelGGL((attend_few<T, I8, DP, kMany>), grid, block, 0, st, queries, out, a);
-    if (const int bad = join<T, I8>(entry, queries, out, a, true, rows, I8 ? 64 : 32, st)) return bad;
+    if (const int bad = join<T, I8, true, DP>(entry, queries, out, a, units, rows, I8 ? 64 : 32, st)) return bad;
   }
   if (plan.many.splits > 0) {
     a.splits = plan.many.splits;
@@ -1264,9 +1297,10 @@ int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, c
     a.partial_rows = plan.many_partials;
     a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
     constexpr int kRows = many_rows(DP);
-    const dim3 grid((unsigned)(units_of(a.p, kRows, 0, a.group) * a.splits * a.kv_heads)), block(256);
+    const int64_t units = units_of(a.p, kRows, 0, a.group);
+    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(256);
     hipLaunchKernelGGL((attend_many<T, I8, DP>), grid, block, 0, st, queries, out, a);
-    return join<T, I8>(entry, queries, out, a, false, kRows, 64, st);
+    return join<T, I8, false, DP>(entry, queries, out, a, units, kRows, 64, st);
   }
   return 0;
 }
@@ -1275,8 +1309,8 @@ template <typename T, bool I8>
 int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, bool aligned, hipStream_t st) {
   const int64_t row_blocks = units_of(a.p, 1, 0, 1) * a.heads;
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
-  const int64_t blocks = std::max((int64_t)a.p.sequences * 4 * plan.few.splits,
-                                  units_of(a.p, 128, 0, a.group) * plan.many.splits) * a.kv_heads;
+  const int64_t blocks = std::max((int64_t)a.p.sequences * 4 * std::max(plan.few.splits, 4),
+                                  units_of(a.p, 128, 0, a.group) * std::max(plan.many.splits, 16)) * a.kv_heads;
   // (the tile kernels' offsets within a page's unit and a head's values have 32 bits)
   const bool small = (int64_t)a.kv_heads * a.dim * 32 < (int64_t)1 << 31 && (int64_t)a.p.page_size * a.dim * 2 < (int64_t)1 << 31;
   if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
