@@ -29,6 +29,8 @@ int check_paging(const char* entry, const Paging& p, int32_t kv_heads, int32_t h
     if (p.sequences == 1 && (int64_t)p.table_pages * p.page_size < (int64_t)p.start + p.tokens)
       return refuse("%s: a page table of %d pages for %lld positions", entry, p.table_pages,
                     (long long)p.start + p.tokens);
+    if (p.sequences == 1 && (int64_t)p.start + p.tokens > kMostPositions)
+      return refuse("%s: %lld positions (at most %lld)", entry, (long long)p.start + p.tokens, (long long)kMostPositions);
   }
   if (!p.offsets && p.sequences > 1 && p.sequences != p.tokens)
     return refuse("%s: %d sequences of %d tokens without offsets", entry, p.sequences, p.tokens);

@@ -42,6 +42,9 @@ __device__ __forceinline__ T uniform(T v) {
   }
 }
 
+// Positions a sequence can have: a tile past its last still counts in 32 bits.
+constexpr int64_t kMostPositions = INT32_MAX - 127;
+
 struct Span {
   int64_t first;         // its first token row
   int32_t rows;          // 0 where the sequence is not described rightly
@@ -68,7 +71,7 @@ __device__ __forceinline__ Span span_of(const Paging& p, int s) {
   span.first = from;
   span.table = p.tables + (int64_t)s * p.table_pages;
   const bool good = from >= 0 && to >= from && to <= p.tokens && span.start >= 0 &&
-                    (to == from || span.start + (to - from) <= (int64_t)p.table_pages * p.page_size);
+                    (to == from || span.start + (to - from) <= min((int64_t)p.table_pages * p.page_size, kMostPositions));
   if (!good) flag_bad(p);
   span.rows = good ? (int32_t)(to - from) : 0;
   return span;

@@ -36,8 +36,16 @@ struct AttentionArgs {
   float *statistics, *partials;
   int32_t few_most, few_units;  // attend_few's rows at most, and units, of a sequence and key head
   int32_t few_rows;   // sequences of at most so many rows (tokens times group) are attend_few's, others attend_many's
-  int32_t page_units, unit_shift;  // page_size / 16, and its logarithm where it is a power of two (else -1)
+  // page_size / 16, and what divides a unit's number (below 2^27) by it exactly
+  uint32_t page_units, page_magic, page_shift;
 };
+
+// The column of a page table that unit `unit` of 16 positions is in: with L = ceil(log2
+// page_units) and M = ceil(2^(27 + L) / page_units), unit M / 2^(27 + L) is above the quotient by
+// less than unit / (2^27 page_units), so its whole part is the quotient's.
+__device__ __forceinline__ uint32_t column_of(const AttentionArgs& a, uint32_t unit) {
+  return (uint32_t)(((uint64_t)unit * a.page_magic) >> a.page_shift);
+}
 
 __device__ __forceinline__ float f16_value(uint32_t bits) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
@@ -227,6 +235,9 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t w0, uint32_t w1) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Instructions as __builtin_amdgcn_sched_group_barrier counts them.
+constexpr int kVectors = 0x2, kProducts = 0x8, kReads = 0x100;
+
 // A lane's eight weights as the product takes them: F16, and for F32 results the
 // F16 remainder too.
 template <int TERMS>
@@ -355,8 +366,8 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   // the page of unit u (-1: nothing of it is seen, or it names no page), and the unit's place in it
   auto page_of = [&](uint32_t u, uint32_t& off) -> int32_t {
     const uint32_t in = u > units ? units : u;
-    const uint32_t column = a.unit_shift >= 0 ? in >> a.unit_shift : in / (uint32_t)a.page_units;
-    off = (in - column * (uint32_t)a.page_units) * 16;
+    const uint32_t column = column_of(a, in);
+    off = (in - column * a.page_units) * 16;
     const int32_t page = span.table[column];
     return page;
   };
@@ -644,14 +655,13 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   }
 }
 
-// The many-rows kernel: 64 rows of queries a wave (32 where heads are wider than
-// 128), four waves a block, positions in tiles of 64 that the block stages in LDS
-// once for all its rows, by 32 x 32 x 16 products. As in attend_few the scores are
-// taken transposed (the result's column, lane % 32, is a row of queries), with
-// the rows of K dealt out so that the 8 weights a lane brings to each product of
-// O^T = V^T P^T are those it holds (bits 2 and 3 of the row's number trade
-// places), and a wave's operand from LDS serves both its tiles of 32 rows: 1 KB
-// read for 64 cycles of matrix work a wave, half of what LDS gives.
+// The many-rows kernel: 32 rows of queries a wave, eight waves a block (four
+// where heads are wider than 128), positions in tiles of 64 that the block
+// stages in LDS once for all its rows, by 32 x 32 x 16 products. As in attend_few
+// the scores are taken transposed (the result's column, lane % 32, is a row of
+// queries), with the rows of K dealt out so that the 8 weights a lane brings to
+// each product of O^T = V^T P^T are those it holds (bits 2 and 3 of the row's
+// number trade places).
 //
 // LDS: keys [64][DP], values [DP][64] in F16 (codes are made F16 numbers as they
 // are staged), 16-byte chunks moved by an exclusive or with the row's number so
@@ -661,20 +671,25 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // The maximum that weights are taken against is raised only when a score passes
 // it by more than kSlack (in powers of two), which keeps the rescaling of the
 // results out of most tiles: weights then reach 2^(kLift + kSlack) at most.
+template <int DP>
+constexpr int kManyWaves = DP > 128 ? 4 : 8;
+
 template <typename T, bool I8, int DP>
-__global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, AttentionArgs a) {
+__global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
+    attend_many(const T* queries, T* out, AttentionArgs a) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-  constexpr int CT = DP > 128 ? 1 : 2;       // tiles of 32 rows a wave
-  constexpr int kRows = 4 * CT * 32;         // rows a block
+  constexpr int kThreads = 64 * kManyWaves<DP>;
+  constexpr int CT = 1;                      // tiles of 32 rows a wave
+  constexpr int kRows = kManyWaves<DP> * CT * 32;  // rows a block
   constexpr int TOK = 64, KS = DP / 16, DT = DP / 32;
   constexpr int kKeyChunks = DP / 8;         // of a position
   constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
-  constexpr int kLoads = TOK * kKeyChunks / 256;  // chunks a thread stages, of keys and of values
+  constexpr int kLoads = TOK * kKeyChunks / kThreads;  // chunks a thread stages, of keys and of values
   // a tile in LDS: its keys, its values, and in 8 bits their scales and the exponents of the values'
   constexpr int kValuesAt = TOK * DP * 2, kScalesAt = 2 * kValuesAt, kExponentsAt = kScalesAt + 2 * TOK * 4;
   constexpr int kTileBytes = I8 ? kExponentsAt + 16 : kScalesAt;
   __shared__ __attribute__((aligned(16))) char tiles[2 * kTileBytes];
-  static_assert(sizeof(RowScratch) * 4 <= sizeof(tiles), "");
+  static_assert(sizeof(RowScratch) * kManyWaves<DP> <= sizeof(tiles), "");
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
@@ -761,44 +776,44 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
   const uint32_t last_unit = p1 / 16;
   const bool wide = a.page_units % 4 == 0;
   constexpr int kUnitThreads = 2 * DP;  // threads that stage a unit's keys, or its values where pages are narrow
-  const int wave_unit = kUnitThreads < 256 ? uniform(thread) / kUnitThreads : 0;
-  auto unit_of = [&](int n) { return kUnitThreads <= 256 ? n * (256 / kUnitThreads) + wave_unit : n * 256 / kUnitThreads; };
+  constexpr int kUnits = kThreads >= kUnitThreads ? kThreads / kUnitThreads : 1;  // units that all threads stage at once
+  const int wave_unit = kUnits > 1 ? wave / (kUnitThreads / 64) : 0;
+  constexpr int kBytes = I8 ? 1 : 2;
+  // bytes of a page (the same for keys and values), of a position's keys, and where this head's lie in a page
+  const uint32_t page_bytes = (uint32_t)a.p.page_size * a.kv_heads * a.dim * kBytes;
+  const uint32_t position_bytes = (uint32_t)a.kv_heads * a.dim * kBytes, key_head = (uint32_t)kv * a.dim * kBytes;
+  const uint32_t value_head = (uint32_t)kv * a.dim * a.p.page_size * kBytes;
+  // A tile's four units, one a lane of four: the page table's entries, asked for
+  // two tiles ahead, and where they lie.
+  int32_t entry;
+  uint32_t entry_off;
+  auto load_entries = [&](int i) {
+    const uint32_t at = min((uint32_t)list.tile(min(i, end - 1)) * 4 + (lane & 3), last_unit);
+    const uint32_t column = column_of(a, at);
+    entry_off = (at - column * a.page_units) * 16;
+    entry = span.table[column];
+  };
   struct Pages {
-    const char *key[4], *value[4];  // where the unit's keys and values of this head begin
-    int64_t scale[4];
+    uint64_t from;  // the unit's page, in bytes from the first
+    uint32_t off;   // its first position in the page
+    uint32_t page;
     uint32_t okay;  // bit u: unit u's page is one of the cache's
   };
-  constexpr int kBytes = I8 ? 1 : 2;
-  typedef const int32_t __attribute__((address_space(4))) * Scalars;
-  auto pages_of = [&](int i) {
-    Pages w;
-    w.okay = 0;
-    const uint32_t first = (uint32_t)list.tile(i) * 4;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t at = min(first + u, last_unit);
-      const uint32_t column = a.unit_shift >= 0 ? at >> a.unit_shift : uniform(at / (uint32_t)a.page_units);
-      const uint32_t off = (at - column * (uint32_t)a.page_units) * 16;
-      const int32_t named = ((Scalars)(uintptr_t)span.table)[column];
-      const bool okay = (uint32_t)named < (uint32_t)a.p.cache_pages;
-      const int64_t page = okay ? named : 0;
-      w.okay |= okay ? 1u << u : 0u;
-      w.key[u] = (const char*)a.keys + ((page * a.p.page_size + off) * a.kv_heads + kv) * a.dim * kBytes;
-      w.scale[u] = (page * a.kv_heads + kv) * a.p.page_size + off;
-      w.value[u] = (const char*)a.values + ((w.scale[u] - off) * a.dim + off) * kBytes;
-    }
-    return w;
+  auto pages_of = [&]() {
+    const bool okay = (uint32_t)entry < (uint32_t)a.p.cache_pages;
+    const uint32_t page = okay ? entry : 0;
+    return Pages{(uint64_t)page * page_bytes, entry_off, page, (uint32_t)__ballot(okay) & 15u};
   };
   typedef typename std::conditional<I8, uint2, uint4>::type Raw;
   Raw key_raw[kLoads], value_raw[kLoads];
   float scale_raw = 0.0f;
   auto key_chunk = [&](int n, int& token, int& chunk) {
-    const int q = thread + 256 * n;
+    const int q = thread + kThreads * n;
     token = q / kKeyChunks;
     chunk = q % kKeyChunks;
   };
   auto value_chunk = [&](int n, int& d, int& chunk) {
-    const int q = thread + 256 * n;
+    const int q = thread + kThreads * n;
     d = wide ? q >> 3 : (q >> 1) % DP;
     chunk = wide ? q & 7 : q / kUnitThreads * 2 + (q & 1);
   };
@@ -812,24 +827,25 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
     value_at[n] = ((uint32_t)min(d, a.dim - 1) * a.p.page_size + (wide ? chunk : chunk & 1) * 8) * kBytes;
   }
   auto load_tile = [&](const Pages& w) {
-    auto pick = [&](const char* const (&x)[4], int n) {
-      const int u = unit_of(n);
-      if constexpr (kUnitThreads >= 256) return x[u];
-      else return wave_unit ? x[(n * 2 + 1) & 3] : x[(n * 2) & 3];
+    auto at_lane = [](uint64_t x, int u) {
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, u);
+      return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u) << 32) | lo;
     };
+    const uint64_t key_from = w.from + w.off * position_bytes, value_from = w.from + w.off * kBytes;
+    // the unit of a thread's chunk n
+    auto unit_of = [&](int n) { return kUnits == 1 ? n * kThreads / kUnitThreads : (n * kUnits & 3) + wave_unit; };
 #pragma unroll
-    for (int n = 0; n < kLoads; ++n) key_raw[n] = *(const Raw*)(pick(w.key, n) + key_at[n]);
+    for (int n = 0; n < kLoads; ++n)
+      key_raw[n] = *(const Raw*)((const char*)a.keys + at_lane(key_from, unit_of(n)) + key_head + key_at[n]);
 #pragma unroll
-    for (int n = 0; n < kLoads; ++n) {
-      const char* from = wide ? w.value[0] : pick(w.value, n);
-      value_raw[n] = *(const Raw*)(from + value_at[n]);
-    }
+    for (int n = 0; n < kLoads; ++n)
+      value_raw[n] = *(const Raw*)((const char*)a.values + at_lane(value_from, wide ? 0 : unit_of(n)) + value_head + value_at[n]);
     if constexpr (I8) {
       // wave 0 brings the keys' scales, wave 1 the values'
       if (wave < 2) {
-        const int u = lane / 16;
-        const int64_t at = u & 2 ? (u & 1 ? w.scale[3] : w.scale[2]) : (u & 1 ? w.scale[1] : w.scale[0]);
-        scale_raw = (wave == 0 ? a.key_scales : a.value_scales)[at + lane % 16];
+        const uint32_t row = (uint32_t)__shfl((int)(w.page * (uint32_t)a.kv_heads + kv), lane / 16, kWave);
+        const uint32_t off = (uint32_t)__shfl((int)w.off, lane / 16, kWave);
+        scale_raw = (wave == 0 ? a.key_scales : a.value_scales)[(uint64_t)row * a.p.page_size + off + lane % 16];
       }
     }
   };
@@ -881,20 +897,24 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
 #pragma unroll
       for (int n = 0; n < kLoads; ++n) *(uint4*)(tile + value_to[n]) = staged(value_raw[n]);
     } else {
-#pragma unroll 1
+      uint32_t from = base;
+      asm volatile("" : "+s"(from));
+#pragma unroll
       for (int n = 0; n < kLoads; ++n) {
-        int d, chunk, to = value_to[0];
+        int d, chunk;
         value_chunk(n, d, chunk);
-        uint4 x = staged(value_raw[0]);
+        // the chunk's first position, and whether its unit counts at all
+        const uint32_t j = from + chunk * 8;
+        const bool in = (bool)(okay >> (chunk / 2) & 1);
+        uint32_t keep[4] = {};
 #pragma unroll
-        for (int o = 1; o < kLoads; ++o)
-          if (n == o) x = staged(value_raw[o]), to = value_to[o];
-        uint32_t keep[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          keep[e] = (seen(chunk * 8 + 2 * e) ? 0xffffu : 0u) | (seen(chunk * 8 + 2 * e + 1) ? 0xffff0000u : 0u);
-        x.x &= keep[0], x.y &= keep[1], x.z &= keep[2], x.w &= keep[3];
-        *(uint4*)(tile + to) = x;
+        for (int e = 0; e < 8; ++e) {
+          const bool sees = in & (j + e <= p1) &
+                            ((a.window == 0) | (j + e + (uint32_t)a.window > p0) | (j + e < (uint32_t)a.sinks));
+          keep[e / 2] |= sees ? e % 2 ? 0xffff0000u : 0xffffu : 0u;
+        }
+        const uint4 x = staged(value_raw[n]);
+        *(uint4*)(tile + value_to[n]) = make_uint4(x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]);
       }
     }
     if constexpr (I8) {
@@ -913,10 +933,11 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
   };
 
   int value_exponent = kNone, least_exponent = -kNone;  // of the values' scales so far
-  Pages pages = pages_of(begin);
+  load_entries(begin);
+  Pages pages = pages_of();
   load_tile(pages);
   uint32_t okay = pages.okay;
-  pages = pages_of(min(begin + 1, end - 1));
+  load_entries(begin + 1);
   for (int i = begin; i < end; ++i) {
     int now = uniform(((i - begin) & 1) * kTileBytes);
     asm volatile("" : "+s"(now));  // (or both buffers' every address is kept in registers)
@@ -924,9 +945,10 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
     store_tile(tile, i, okay);
     const uint32_t okay_now = okay;
     if (i + 1 < end) {
+      pages = pages_of();
       load_tile(pages);
       okay = pages.okay;
-      pages = pages_of(min(i + 2, end - 1));
+      load_entries(i + 2);
     }
     __syncthreads();
     const uint32_t base = (uint32_t)list.tile(i) * TOK;
@@ -955,19 +977,36 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
     // scores: score[half][c][e] is row 32 c + col, position base + 32 half + 16 (e / 8) + 8 h + e % 8
     f32x16 score[2][CT];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) score[half][c][e] = 0.0f;
+    {
+      // operands four at a time, the next four on their way while these are multiplied
+      f16x8 keys[2][4];
+      auto load_keys = [&](int n, f16x8 (&to)[4]) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const f16x8 key = *(const f16x8*)(tile + key_from[k % 8] + half * 32 * DP * 2 + k / 8 * 256);
+        for (int e = 0; e < 4; ++e) {
+          const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
+          to[e] = *(const f16x8*)(tile + key_from[k % 8] + half * 32 * DP * 2 + k / 8 * 256);
+        }
+      };
+      load_keys(0, keys[0]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+      for (int n = 0; n < KS / 2; ++n) {
+        if (n + 1 < KS / 2) load_keys(n + 1, keys[(n + 1) % 2]);
 #pragma unroll
-          for (int m = 0; m < TERMS; ++m)
-            score[half][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, query[c][k][m], score[half][c], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) {
+          const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int m = 0; m < TERMS; ++m)
+              score[half][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[n % 2][e], query[c][k][m], score[half][c], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if constexpr (I8) {
@@ -985,17 +1024,22 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
         }
     }
     if (!whole) {
-      uint32_t mine = base + h * 8;
-      asm volatile("" : "+v"(mine));
+      int mine = (int)base + h * 8;
+      asm volatile("" : "+v"(mine));  // (or what depends on it alone is kept for every tile)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+      for (int c = 0; c < CT; ++c) {
+        const int last = (int)position[c], low = a.window ? last - a.window + 1 : INT32_MIN;
 #pragma unroll
         for (int n = 0; n < 32; ++n) {
-          const uint32_t j = mine + n / 8 * 16 + n % 8;
-          const bool seen = (bool)(okay_now >> (n / 8) & 1) & (j <= position[c]) &
-                            ((a.window == 0) | (j + (uint32_t)a.window > position[c]) | (j < (uint32_t)a.sinks));
+          const int j = mine + n / 8 * 16 + n % 8;
+          const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
           score[n / 16][c][n % 16] = seen ? score[n / 16][c][n % 16] : -kInfinity;
         }
+        if (okay_now != 15u)
+#pragma unroll
+          for (int n = 0; n < 32; ++n)
+            if (!(okay_now >> (n / 8) & 1)) score[n / 16][c][n % 16] = -kInfinity;
+      }
     }
     float high[CT];
     bool raise = false;
@@ -1021,15 +1065,15 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
     float lift[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) lift[c] = kManyLift - (ref[c] == -kInfinity ? 0.0f : ref[c]);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {  // 16 positions
+    // 16 positions at a time, the next ones' weights made between the products of these
+    Halves<TERMS> weights[2][CT];
+    auto weigh = [&](int n, Halves<TERMS> (&to)[CT]) {
       float value_scale[I8 ? 8 : 1];
       if constexpr (I8) {
         const float* scales = (const float*)(tile + kScalesAt) + TOK + h * 8 + n * 16;
 #pragma unroll
         for (int e = 0; e < 8; ++e) value_scale[e] = scales[e] * lower;
       }
-      Halves<TERMS> weights[CT];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         float w[8];
@@ -1039,17 +1083,40 @@ __global__ void __launch_bounds__(256, 1) attend_many(const T* queries, T* out, 
           total[c] += p;
           w[e] = I8 ? p * value_scale[e] : p;
         }
-        weights[c] = halves_of<TERMS>(w);
+        to[c] = halves_of<TERMS>(w);
+      }
+    };
+    f16x8 values[2][DT];
+    auto load_values = [&](int n, f16x8 (&to)[DT]) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) to[d] = *(const f16x8*)(tile + value_from[n] + d * 4096);
+    };
+    load_values(0, values[0]);
+    weigh(0, weights[0]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n < 3) {
+        load_values(n + 1, values[(n + 1) % 2]);
+        weigh(n + 1, weights[(n + 1) % 2]);
       }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const f16x8 value = *(const f16x8*)(tile + value_from[n] + d * 4096);
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
           for (int m = 0; m < TERMS; ++m)
-            acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value, weights[c].term[m], acc[c][d], 0, 0, 0);
+            acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[n % 2][d], weights[n % 2][c].term[m], acc[c][d], 0, 0, 0);
+      if (n < 3) {
+        constexpr int kVector = (I8 ? 48 : 32) + (TERMS == 2 ? 24 : 0);  // about what the weights take
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          __builtin_amdgcn_sched_group_barrier(kProducts, CT * TERMS, 0);
+          __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kVectors, kVector / DT, 0);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -1298,7 +1365,7 @@ int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, c
     a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
     constexpr int kRows = many_rows(DP);
     const int64_t units = units_of(a.p, kRows, 0, a.group);
-    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(256);
+    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(64 * kManyWaves<DP>);
     hipLaunchKernelGGL((attend_many<T, I8, DP>), grid, block, 0, st, queries, out, a);
     return join<T, I8, false, DP>(entry, queries, out, a, units, kRows, 64, st);
   }
@@ -1311,8 +1378,9 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
   const int64_t blocks = std::max((int64_t)a.p.sequences * 4 * std::max(plan.few.splits, 4),
                                   units_of(a.p, 128, 0, a.group) * std::max(plan.many.splits, 16)) * a.kv_heads;
-  // (the tile kernels' offsets within a page's unit and a head's values have 32 bits)
-  const bool small = (int64_t)a.kv_heads * a.dim * 32 < (int64_t)1 << 31 && (int64_t)a.p.page_size * a.dim * 2 < (int64_t)1 << 31;
+  // (the tile kernels' offsets within a page, and rows of scales, have 32 bits)
+  const bool small = (int64_t)a.p.page_size * a.kv_heads * a.dim * 2 < (int64_t)1 << 31 &&
+                     (int64_t)a.p.cache_pages * a.kv_heads < (int64_t)1 << 31;
   if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
     hipLaunchKernelGGL((attend_rows<T, I8>), dim3((unsigned)row_blocks), dim3(kWave), 0, st, queries, out, a);
     return launched(entry);
@@ -1337,7 +1405,9 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   if (const int bad = check_cache(entry, a.p, a.keys, a.values, a.key_scales, a.value_scales)) return bad;
   a.group = a.heads / a.kv_heads;
   a.page_units = a.p.page_size / 16;
-  a.unit_shift = (a.page_units & (a.page_units - 1)) == 0 ? __builtin_ctz((unsigned)a.page_units) : -1;
+  a.page_shift = 27;
+  while (((uint64_t)a.page_units << 27) > ((uint64_t)1 << a.page_shift)) ++a.page_shift;
+  a.page_magic = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page_units - 1) / a.page_units);
   const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
                             a.p.offsets != nullptr);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
@@ -1374,7 +1444,7 @@ extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens
 #define DRIFT_ATTENTION_ARGS                                                                                        \
   AttentionArgs {                                                                                                   \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, 0, 0 \
+        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, 0, 0, 0 \
   }
 
 extern "C" int drift_paged_attention_f32(const float* queries, const void* keys, const void* values,

@@ -29,7 +29,7 @@ from . import _lib
 
 F32, BF16, F16, I32 = torch.float32, torch.bfloat16, torch.float16, torch.int32
 _FLOAT_TYPES = (F32, BF16)
-_MOST_POSITIONS = 2 ** 31 - 1  # the entry points take positions and counts of 32 bits
+_MOST_POSITIONS = 2 ** 31 - 128  # of a sequence in the paged cache (csrc/paged.hpp)
 
 
 class Activation(enum.IntEnum):

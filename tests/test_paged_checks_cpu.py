@@ -195,6 +195,7 @@ def test_rows_entry_points_refuse(entry):
     assert "start -1" in refusal(entry, *rows(start=-1))
     assert "a page table of 4 pages for 65 positions" in refusal(entry, *rows(start=62))
     assert "2147483650 positions" in refusal(entry, *rows(start=2 ** 31 - 1))
+    assert "2147483550 positions (at most 2147483520)" in refusal(entry, *rows(start=2147483547, table_pages=2 ** 27))
     assert "2 sequences without starts" in refusal(entry, *rows(sequences=2))
     assert "2 sequences of 3 tokens without offsets" in refusal(entry, *rows(sequences=2, starts=16))
     assert "null tensor" in refusal(entry, *rows(k=None))
@@ -203,7 +204,7 @@ def test_rows_entry_points_refuse(entry):
     assert "scales of keys or of values alone" in refusal(entry, *rows(key_scales=16))
     assert "not aligned to their elements" in refusal(entry, *rows(keys=17))
     assert "not aligned to their elements" in refusal(entry, *rows(key_scales=18, value_scales=16))
-    assert "in one call" in refusal(entry, *rows(tokens=2 ** 31 - 1, table_pages=2 ** 27, kv_heads=64, dim=7))
+    assert "in one call" in refusal(entry, *rows(tokens=2 ** 31 - 129, table_pages=2 ** 27, kv_heads=64, dim=7))
     assert refusal(entry, *rows(tokens=0)) == "code 0"
     assert refusal(entry, *rows(sequences=0, starts=None)) == "code 0"
 
