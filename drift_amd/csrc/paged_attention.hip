@@ -655,9 +655,9 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   }
 }
 
-// The many-rows kernel: 32 rows of queries a wave, eight waves a block (four
-// where heads are wider than 128), positions in tiles of 64 that the block
-// stages in LDS once for all its rows, by 32 x 32 x 16 products. As in attend_few
+// The many-rows kernel: 32 rows of queries a wave, four or eight waves a block
+// (plan_of says when), positions in tiles of 64 that the block stages in LDS once
+// for all its rows, by 32 x 32 x 16 products. As in attend_few
 // the scores are taken transposed (the result's column, lane % 32, is a row of
 // queries), with the rows of K dealt out so that the 8 weights a lane brings to
 // each product of O^T = V^T P^T are those it holds (bits 2 and 3 of the row's
@@ -671,25 +671,21 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // The maximum that weights are taken against is raised only when a score passes
 // it by more than kSlack (in powers of two), which keeps the rescaling of the
 // results out of most tiles: weights then reach 2^(kLift + kSlack) at most.
-template <int DP>
-constexpr int kManyWaves = DP > 128 ? 4 : 8;
-
-template <typename T, bool I8, int DP>
-__global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
-    attend_many(const T* queries, T* out, AttentionArgs a) {
+template <typename T, bool I8, int DP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
-  constexpr int kThreads = 64 * kManyWaves<DP>;
+  constexpr int kThreads = 64 * WAVES;
   constexpr int CT = 1;                      // tiles of 32 rows a wave
-  constexpr int kRows = kManyWaves<DP> * CT * 32;  // rows a block
+  constexpr int kRows = WAVES * CT * 32;  // rows a block
   constexpr int TOK = 64, KS = DP / 16, DT = DP / 32;
   constexpr int kKeyChunks = DP / 8;         // of a position
   constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
   constexpr int kLoads = TOK * kKeyChunks / kThreads;  // chunks a thread stages, of keys and of values
   // a tile in LDS: its keys, its values, and in 8 bits their scales and the exponents of the values'
   constexpr int kValuesAt = TOK * DP * 2, kScalesAt = 2 * kValuesAt, kExponentsAt = kScalesAt + 2 * TOK * 4;
-  constexpr int kTileBytes = I8 ? kExponentsAt + 16 : kScalesAt;
+  constexpr int kTileBytes = I8 ? (kExponentsAt + 16 + 255) / 256 * 256 : kScalesAt;
   __shared__ __attribute__((aligned(16))) char tiles[2 * kTileBytes];
-  static_assert(sizeof(RowScratch) * kManyWaves<DP> <= sizeof(tiles), "");
+  static_assert(sizeof(RowScratch) * WAVES <= sizeof(tiles), "");
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
@@ -758,6 +754,9 @@ __global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
     }
   }
   f32x16 acc[CT][DT];
+  float row_inverse[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) row_inverse[c] = 1.0f / row_scale[c];
   float ref[CT], total[CT];  // what weights are taken against, and their sum so far
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
@@ -804,158 +803,184 @@ __global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
     const uint32_t page = okay ? entry : 0;
     return Pages{(uint64_t)page * page_bytes, entry_off, page, (uint32_t)__ballot(okay) & 15u};
   };
-  typedef typename std::conditional<I8, uint2, uint4>::type Raw;
-  Raw key_raw[kLoads], value_raw[kLoads];
-  float scale_raw = 0.0f;
-  auto key_chunk = [&](int n, int& token, int& chunk) {
-    const int q = thread + kThreads * n;
-    token = q / kKeyChunks;
-    chunk = q % kKeyChunks;
+  auto at_lane = [](uint64_t x, int u) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, u);
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u) << 32) | lo;
   };
-  auto value_chunk = [&](int n, int& d, int& chunk) {
-    const int q = thread + kThreads * n;
-    d = wide ? q >> 3 : (q >> 1) % DP;
-    chunk = wide ? q & 7 : q / kUnitThreads * 2 + (q & 1);
-  };
-  uint32_t key_at[kLoads], value_at[kLoads];
-#pragma unroll
-  for (int n = 0; n < kLoads; ++n) {
-    int token, chunk, d;
-    key_chunk(n, token, chunk);
-    key_at[n] = ((uint32_t)(token % 16) * a.kv_heads * a.dim + (chunk * 8 < a.dim ? chunk * 8 : 0)) * kBytes;
-    value_chunk(n, d, chunk);
-    value_at[n] = ((uint32_t)min(d, a.dim - 1) * a.p.page_size + (wide ? chunk : chunk & 1) * 8) * kBytes;
-  }
-  auto load_tile = [&](const Pages& w) {
-    auto at_lane = [](uint64_t x, int u) {
-      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, u);
-      return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u) << 32) | lo;
-    };
-    const uint64_t key_from = w.from + w.off * position_bytes, value_from = w.from + w.off * kBytes;
-    // the unit of a thread's chunk n
-    auto unit_of = [&](int n) { return kUnits == 1 ? n * kThreads / kUnitThreads : (n * kUnits & 3) + wave_unit; };
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n)
-      key_raw[n] = *(const Raw*)((const char*)a.keys + at_lane(key_from, unit_of(n)) + key_head + key_at[n]);
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n)
-      value_raw[n] = *(const Raw*)((const char*)a.values + at_lane(value_from, wide ? 0 : unit_of(n)) + value_head + value_at[n]);
-    if constexpr (I8) {
-      // wave 0 brings the keys' scales, wave 1 the values'
-      if (wave < 2) {
-        const uint32_t row = (uint32_t)__shfl((int)(w.page * (uint32_t)a.kv_heads + kv), lane / 16, kWave);
-        const uint32_t off = (uint32_t)__shfl((int)w.off, lane / 16, kWave);
-        scale_raw = (wave == 0 ? a.key_scales : a.value_scales)[(uint64_t)row * a.p.page_size + off + lane % 16];
-      }
-    }
-  };
+  // the unit of a thread's chunk n of keys
+  auto unit_of = [&](int n) { return kUnits == 1 ? n * kThreads / kUnitThreads : (n * kUnits & 3) + wave_unit; };
   // where a tile has chunk `chunk` of position `token`, or of value d
   auto key_place = [](int token, int chunk) {
     return (token * kKeyChunks + (chunk ^ (DP >= 128 ? token & 15 : (token >> 1) & 7))) * 16;
   };
   auto value_place = [](int d, int chunk) { return kValuesAt + (d * 8 + (chunk ^ ((d >> 1) & 7))) * 16; };
-  int key_to[kLoads], value_to[kLoads];
+  // whether some row of the block sees position j
+  auto some_see = [&](uint32_t j) {
+    return (j <= p1) & ((a.window == 0) | (j + (uint32_t)a.window > p0) | (j < (uint32_t)a.sinks));
+  };
+  auto flag_units = [&](uint32_t base, uint32_t okay) {
+    if (okay != 15u && thread < TOK && !(okay >> (thread / 16) & 1) && some_see(base + thread)) flag_bad(a.p);
+  };
+
+  // F16: straight into LDS. A thread's chunk goes to the place of its number, so it asks for the chunk that belongs there.
+  typedef const __attribute__((address_space(1))) void* Global;
+  typedef __attribute__((address_space(3))) void* Local;
+  auto copy_tile = [&](const Pages& w, int to) {
+    const uint64_t key_from = w.from + w.off * position_bytes, value_from = w.from + w.off * kBytes;
+    int me = thread;
+    asm volatile("" : "+v"(me));  // (or every chunk's offset is kept in registers)
+    // the exclusive or is the same for all a thread's chunks, but for bit 3 where a step of n is 8 positions
+    constexpr int kStep = kThreads / kKeyChunks;
+    const int token = me / kKeyChunks, key_chunk = me % kKeyChunks ^ (DP >= 128 ? token & 15 : (token >> 1) & 7);
+    const uint32_t row = (uint32_t)(token % 16) * position_bytes;
 #pragma unroll
-  for (int n = 0; n < kLoads; ++n) {
-    int token, chunk, d;
-    key_chunk(n, token, chunk);
-    key_to[n] = key_place(token, chunk);
-    value_chunk(n, d, chunk);
-    value_to[n] = value_place(d, chunk);
-  }
-  // operands: chunk 2 k + h of the lane's position (its low four bits are what the
-  // exclusive or moves), and chunk n of the lane's value
-  const int key_row = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
-  constexpr int kKeyPlaces = KS < 8 ? KS : 8;
-  int key_from[kKeyPlaces], value_from[4];
+    for (int n = 0; n < kLoads; ++n) {
+      const int chunk = kStep % 16 ? key_chunk ^ (n * kStep & 8) : key_chunk;
+      const char* from = (const char*)a.keys + at_lane(key_from, unit_of(n)) + (key_head + n * kStep % 16 * position_bytes) +
+                         (row + (chunk * 8 < a.dim ? chunk * 16 : 0));
+      __builtin_amdgcn_global_load_lds((Global)from, (Local)(tiles + to + (wave * 64 + n * kThreads) * 16), 16, 0, 0);
+    }
+    const int d = me >> 3, value_chunk = (me & 7) ^ ((d >> 1) & 7);
+    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)value_from, value_chunk >> 1, kWave);
+    const uint64_t from = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(value_from >> 32), value_chunk >> 1, kWave) << 32) | lo;
+    const char* head = (const char*)a.values + from + (value_head + (value_chunk & 1) * 16);
 #pragma unroll
-  for (int k = 0; k < kKeyPlaces; ++k) key_from[k] = key_place(key_row, 2 * k + h);
+    for (int n = 0; n < kLoads; ++n) {
+      const uint32_t at = (uint32_t)min(d + n * (kThreads / 8), a.dim - 1) * a.p.page_size * 2;
+      __builtin_amdgcn_global_load_lds((Global)(head + at), (Local)(tiles + to + kValuesAt + (wave * 64 + n * kThreads) * 16), 16, 0, 0);
+    }
+  };
+  // Values that no row of the block sees count as zeros: they may hold anything. Each thread mends the chunks it asked
+  // for, once they have come.
+  auto mend_tile = [&](int at, int i, uint32_t okay) {
+    const uint32_t base = (uint32_t)list.tile(i) * TOK;
+    if (okay == 15u && base + TOK - 1 <= p1 &&
+        (a.window == 0 || base + (uint32_t)a.window > p0 || base + TOK - 1 < (uint32_t)a.sinks))
+      return;
+    flag_units(base, okay);
+    const int chunk = (thread & 7) ^ ((thread >> 4) & 7);
+    uint32_t keep[4] = {};
 #pragma unroll
-  for (int n = 0; n < 4; ++n) value_from[n] = value_place(col, 2 * n + h);
-  auto staged = [](const Raw& raw) {
-    if constexpr (I8) return __builtin_bit_cast(uint4, codes_f16(raw.x, raw.y));
-    else return raw;
+    for (int e = 0; e < 8; ++e)
+      keep[e / 2] |= (bool)(okay >> (chunk / 2) & 1) & some_see(base + chunk * 8 + e) ? e % 2 ? 0xffff0000u : 0xffffu : 0u;
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      uint4* place = (uint4*)(tiles + at + kValuesAt + (thread + n * kThreads) * 16);
+      const uint4 x = *place;
+      *place = make_uint4(x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]);
+    }
+  };
+
+  // 8 bits: by registers, made F16 numbers on the way.
+  uint2 key_raw[I8 ? kLoads : 1], value_raw[I8 ? kLoads : 1];
+  float scale_raw = 0.0f;
+  auto load_tile = [&](const Pages& w) {
+    const uint64_t key_from = w.from + w.off * position_bytes, value_from = w.from + w.off * kBytes;
+    int me = thread;
+    asm volatile("" : "+v"(me));
+    const int chunk0 = me % kKeyChunks * 8;
+    const uint32_t key_at = (uint32_t)(me / kKeyChunks % 16) * position_bytes + (chunk0 < a.dim ? chunk0 : 0);
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n)
+      key_raw[n] = *(const uint2*)((const char*)a.keys + at_lane(key_from, unit_of(n)) +
+                                   (key_head + n * kThreads / kKeyChunks % 16 * position_bytes) + key_at);
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int q = me + kThreads * n, d = min(wide ? q >> 3 : (q >> 1) % DP, a.dim - 1);
+      const uint32_t value_at = (uint32_t)d * a.p.page_size + (wide ? me & 7 : me & 1) * 8;
+      value_raw[n] = *(const uint2*)((const char*)a.values + at_lane(value_from, wide ? 0 : unit_of(n)) + value_head + value_at);
+    }
+    // wave 0 brings the keys' scales, wave 1 the values'
+    if (wave < 2) {
+      const uint32_t row = (uint32_t)__shfl((int)(w.page * (uint32_t)a.kv_heads + kv), lane / 16, kWave);
+      const uint32_t off = (uint32_t)__shfl((int)w.off, lane / 16, kWave);
+      scale_raw = (wave == 0 ? a.key_scales : a.value_scales)[(uint64_t)row * a.p.page_size + off + lane % 16];
+    }
   };
   constexpr int kNone = -1000;  // no scale above 0
   auto store_tile = [&](char* tile, int i, uint32_t okay) {
     const uint32_t base = (uint32_t)list.tile(i) * TOK;
-    // positions that no row of the block sees count as zeros: they may hold anything
-    const bool whole = okay == 15u && base + TOK - 1 <= p1 &&
-                       (a.window == 0 || base + (uint32_t)a.window > p0 || base + TOK - 1 < (uint32_t)a.sinks);
-    auto seen = [&](int token) {
-      const uint32_t j = base + token;
-      return (bool)(okay >> (token / 16) & 1) & (j <= p1) &
-             ((a.window == 0) | (j + (uint32_t)a.window > p0) | (j < (uint32_t)a.sinks));
-    };
-    if (okay != 15u && thread < TOK && !(okay >> (thread / 16) & 1)) {
-      const uint32_t j = base + thread;
-      if (j <= p1 && (a.window == 0 || j + (uint32_t)a.window > p0 || j < (uint32_t)a.sinks)) flag_bad(a.p);
+    flag_units(base, okay);
+    int me = thread;
+    asm volatile("" : "+v"(me));
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int q = me + kThreads * n;
+      *(uint4*)(tile + key_place(q / kKeyChunks, q % kKeyChunks)) =
+          __builtin_bit_cast(uint4, codes_f16(key_raw[n].x, key_raw[n].y));
     }
 #pragma unroll
-    for (int n = 0; n < kLoads; ++n) *(uint4*)(tile + key_to[n]) = staged(key_raw[n]);
-    if (I8 || whole) {
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n) *(uint4*)(tile + value_to[n]) = staged(value_raw[n]);
-    } else {
-      uint32_t from = base;
-      asm volatile("" : "+s"(from));
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n) {
-        int d, chunk;
-        value_chunk(n, d, chunk);
-        // the chunk's first position, and whether its unit counts at all
-        const uint32_t j = from + chunk * 8;
-        const bool in = (bool)(okay >> (chunk / 2) & 1);
-        uint32_t keep[4] = {};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const bool sees = in & (j + e <= p1) &
-                            ((a.window == 0) | (j + e + (uint32_t)a.window > p0) | (j + e < (uint32_t)a.sinks));
-          keep[e / 2] |= sees ? e % 2 ? 0xffff0000u : 0xffffu : 0u;
-        }
-        const uint4 x = staged(value_raw[n]);
-        *(uint4*)(tile + value_to[n]) = make_uint4(x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]);
-      }
+    for (int n = 0; n < kLoads; ++n) {
+      const int q = me + kThreads * n, d = wide ? q >> 3 : (q >> 1) % DP;
+      *(uint4*)(tile + value_place(d, wide ? q & 7 : q / kUnitThreads * 2 + (q & 1))) =
+          __builtin_bit_cast(uint4, codes_f16(value_raw[n].x, value_raw[n].y));
     }
-    if constexpr (I8) {
-      float* scales = (float*)(tile + kScalesAt);
-      if (wave == 0) scales[lane] = scale_raw;
-      else if (wave == 1) {
-        const float x = whole || seen(lane) ? scale_raw : 0.0f;
-        scales[TOK + lane] = x;
-        const bool counts = x > 0.0f && x < kInfinity;
-        const float exponent = (float)__builtin_amdgcn_frexp_expf(x);
-        const float most = group_max<64>(counts ? exponent : (float)kNone);
-        const float least = -group_max<64>(counts ? -exponent : (float)kNone);
-        if (lane == 0) *(int2*)(tile + kExponentsAt) = make_int2((int)most, (int)least);
-      }
+    // (every code is a number: what no row sees needs a scale of 0 alone)
+    float* scales = (float*)(tile + kScalesAt);
+    if (wave == 0) scales[lane] = scale_raw;
+    else if (wave == 1) {
+      const float x = (bool)(okay >> (lane / 16) & 1) & some_see(base + lane) ? scale_raw : 0.0f;
+      scales[TOK + lane] = x;
+      const bool counts = x > 0.0f && x < kInfinity;
+      const float exponent = (float)__builtin_amdgcn_frexp_expf(x);
+      const float most = group_max<64>(counts ? exponent : (float)kNone);
+      const float least = -group_max<64>(counts ? -exponent : (float)kNone);
+      if (lane == 0) *(int2*)(tile + kExponentsAt) = make_int2((int)most, (int)least);
     }
   };
-
+  // operands: chunk 2 k + h of the lane's position, and chunk 2 n + h of its value: the exclusive or with k and n
+  // (chunks of 16 bytes, in the low bits of places that are multiples of 128) gives them from one place each
+  const int key_row = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
+  const int key_from = key_place(key_row, h), value_from = value_place(col, h);
   int value_exponent = kNone, least_exponent = -kNone;  // of the values' scales so far
+  // A tile comes while the one before it is used (8 bits: is written then, and is in registers a tile before that).
   load_entries(begin);
   Pages pages = pages_of();
-  load_tile(pages);
-  uint32_t okay = pages.okay;
+  uint32_t okay = pages.okay, okay_now = okay;
+  if constexpr (I8) load_tile(pages);
+  else copy_tile(pages, 0);
   load_entries(begin + 1);
+  if constexpr (I8) {
+    store_tile(tiles, begin, okay);
+    if (begin + 1 < end) {
+      pages = pages_of();
+      load_tile(pages);
+      okay = pages.okay;
+      load_entries(begin + 2);
+    }
+  }
   for (int i = begin; i < end; ++i) {
     int now = uniform(((i - begin) & 1) * kTileBytes);
     asm volatile("" : "+s"(now));  // (or both buffers' every address is kept in registers)
     char* tile = tiles + now;
-    store_tile(tile, i, okay);
-    const uint32_t okay_now = okay;
-    if (i + 1 < end) {
-      pages = pages_of();
-      load_tile(pages);
-      okay = pages.okay;
-      load_entries(i + 2);
+    if constexpr (!I8) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the tile has come
+      mend_tile(now, i, okay_now);
     }
     __syncthreads();
+    const uint32_t okay_then = okay_now;
+    if (i + 1 < end) {
+      if constexpr (I8) {
+        store_tile(tiles + (kTileBytes - now), i + 1, okay);
+        okay_now = okay;
+        if (i + 2 < end) {
+          pages = pages_of();
+          load_tile(pages);
+          okay = pages.okay;
+          load_entries(i + 3);
+        }
+      } else {
+        pages = pages_of();
+        copy_tile(pages, kTileBytes - now);
+        okay_now = pages.okay;
+        load_entries(i + 2);
+      }
+    }
     const uint32_t base = (uint32_t)list.tile(i) * TOK;
     // whether any, and whether every row of the wave sees the tile
     if (idle || base > w1) continue;
     if (a.window && base + TOK - 1 + (uint32_t)a.window <= w0 && base >= (uint32_t)a.sinks) continue;
-    const bool whole = okay_now == 15u && base + TOK - 1 <= w0 &&
+    const bool whole = okay_then == 15u && base + TOK - 1 <= w0 &&
                        (a.window == 0 || base + (uint32_t)a.window > w1 || base + TOK - 1 < (uint32_t)a.sinks);
     float lower = 1.0f;  // 2^-value_exponent
     if constexpr (I8) {
@@ -989,7 +1014,7 @@ __global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
-          to[e] = *(const f16x8*)(tile + key_from[k % 8] + half * 32 * DP * 2 + k / 8 * 256);
+          to[e] = *(const f16x8*)(tiles + ((now + key_from) ^ (k % 8 * 32)) + half * 32 * DP * 2 + k / 8 * 256);
         }
       };
       load_keys(0, keys[0]);
@@ -1035,25 +1060,32 @@ __global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
           const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
           score[n / 16][c][n % 16] = seen ? score[n / 16][c][n % 16] : -kInfinity;
         }
-        if (okay_now != 15u)
+        if (okay_then != 15u)
 #pragma unroll
           for (int n = 0; n < 32; ++n)
-            if (!(okay_now >> (n / 8) & 1)) score[n / 16][c][n % 16] = -kInfinity;
+            if (!(okay_then >> (n / 8) & 1)) score[n / 16][c][n % 16] = -kInfinity;
       }
     }
-    float high[CT];
+    // Whether a score passes what weights are taken against by more than kSlack: while that bound is not below 0,
+    // the numbers' bits compare as whole numbers do (a NaN among them passes it), which takes half the
+    // instructions of a maximum that must quieten NaN. The maximum itself is taken only then.
     bool raise = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      high[c] = fmaxf(score[0][c][0], score[1][c][0]);
+      const float bound = (ref[c] + kSlack) * row_inverse[c];
+      int most = 0;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) high[c] = fmaxf(high[c], fmaxf(score[0][c][e], score[1][c][e]));
-      raise |= high[c] * row_scale[c] > ref[c] + kSlack;
+      for (int e = 0; e < 16; ++e)
+        most = max(most, max(__float_as_int(score[0][c][e]), __float_as_int(score[1][c][e])));
+      raise |= !(bound >= 0.0f) || most > __float_as_int(bound);
     }
     if (__any(raise))
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const float next = fmaxf(ref[c], fmaxf(high[c], __shfl_xor(high[c], 32, kWave)) * row_scale[c]);
+        float high = fmaxf(score[0][c][0], score[1][c][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) high = fmaxf(high, fmaxf(score[0][c][e], score[1][c][e]));
+        const float next = fmaxf(ref[c], fmaxf(high, __shfl_xor(high, 32, kWave)) * row_scale[c]);
         const float keep = exp2_fast(ref[c] - (next == -kInfinity ? 0.0f : next));
         ref[c] = next;
         total[c] *= keep;
@@ -1089,7 +1121,7 @@ __global__ void __launch_bounds__(64 * kManyWaves<DP>, kManyWaves<DP> / 4)
     f16x8 values[2][DT];
     auto load_values = [&](int n, f16x8 (&to)[DT]) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) to[d] = *(const f16x8*)(tile + value_from[n] + d * 4096);
+      for (int d = 0; d < DT; ++d) to[d] = *(const f16x8*)(tiles + ((now + value_from) ^ (n * 32)) + d * 4096);
     };
     load_values(0, values[0]);
     weigh(0, weights[0]);
@@ -1286,6 +1318,7 @@ struct Split {
 };
 struct Plan {
   bool few16;       // attend_few's sequences have at most 16 rows
+  int many_rows;    // rows a block of attend_many
   Split few, many;  // attend_few, attend_many
   int64_t few_most, few_partials, many_partials;  // AttentionArgs::few_most, partial_rows
   int64_t bytes;
@@ -1293,7 +1326,6 @@ struct Plan {
 
 // Rows of queries of a sequence and key head up to which it is attend_few's.
 constexpr int kFewRows = 64;
-constexpr int many_rows(int64_t dim) { return dim > 128 ? 128 : 256; }
 
 // `blocks` blocks before the split, over `positions` positions, towards `wanted`
 // of them.
@@ -1305,7 +1337,7 @@ Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least,
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
              int64_t sinks, int64_t longest, bool by_offsets) {
-  Plan p{true, {0, 1}, {0, 1}, 0, 0, 0, 0};
+  Plan p{true, 128, {0, 1}, {0, 1}, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
@@ -1313,9 +1345,12 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   p.few16 = by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
   if (by_offsets || each * group <= kFewRows) p.few = split_of(sequences * kv_heads, seen, 1024, 4, 32);
   if (each * group > kFewRows) {
-    const int64_t blocks = ceil_div(tokens * group, many_rows(dim)) * kv_heads;
-    p.many = split_of(blocks, seen, 512, 8, blocks >= 256 ? INT64_MAX / 2 : 1 << 20);
-    if (blocks >= 384) p.many.splits = 1;
+    // Blocks of 256 rows read keys and values half as often, blocks of 128 leave fewer rows idle and two of them
+    // on a compute unit wait at barriers of their own
+    const int64_t rows = tokens * group;
+    p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= 768 ? 256 : 128;
+    const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
+    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
   }
   p.few_most = std::min(each * group, (int64_t)kFewRows);
   p.few_partials = sequences * kv_heads * p.few_most;
@@ -1363,11 +1398,15 @@ int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, c
     a.chunk = plan.many.chunk;
     a.partial_rows = plan.many_partials;
     a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
-    constexpr int kRows = many_rows(DP);
-    const int64_t units = units_of(a.p, kRows, 0, a.group);
-    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(64 * kManyWaves<DP>);
-    hipLaunchKernelGGL((attend_many<T, I8, DP>), grid, block, 0, st, queries, out, a);
-    return join<T, I8, false, DP>(entry, queries, out, a, units, kRows, 64, st);
+    const int64_t units = units_of(a.p, plan.many_rows, 0, a.group);
+    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(plan.many_rows * 2);
+    if constexpr (DP == 128) {
+      if (plan.many_rows == 256) hipLaunchKernelGGL((attend_many<T, I8, DP, 8>), grid, block, 0, st, queries, out, a);
+      else hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), grid, block, 0, st, queries, out, a);
+    } else {
+      hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), grid, block, 0, st, queries, out, a);
+    }
+    return join<T, I8, false, DP>(entry, queries, out, a, units, plan.many_rows, 64, st);
   }
   return 0;
 }
