@@ -1018,6 +1018,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
         }
       };
       load_keys(0, keys[0]);
+      __builtin_amdgcn_s_setprio(1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < KS / 2; ++n) {
@@ -1066,9 +1067,11 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
             if (!(okay_then >> (n / 8) & 1)) score[n / 16][c][n % 16] = -kInfinity;
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     // Whether a score passes what weights are taken against by more than kSlack: while that bound is not below 0,
     // the numbers' bits compare as whole numbers do (a NaN among them passes it), which takes half the
-    // instructions of a maximum that must quieten NaN. The maximum itself is taken only then.
+    // instructions of a maximum that must quieten NaN. The maximum itself is taken only then, by whole numbers too (a
+    // row with a NaN is NaN whatever its weights are taken against).
     bool raise = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -1082,9 +1085,12 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
     if (__any(raise))
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        float high = fmaxf(score[0][c][0], score[1][c][0]);
+        // (the bits of numbers as whole numbers in order: those of negative ones turned)
+        auto ordered = [](float x) { const int b = __float_as_int(x); return b ^ (int)((uint32_t)(b >> 31) >> 1); };
+        int top = ordered(score[0][c][0]);
 #pragma unroll
-        for (int e = 1; e < 16; ++e) high = fmaxf(high, fmaxf(score[0][c][e], score[1][c][e]));
+        for (int e = 0; e < 16; ++e) top = max(top, max(ordered(score[0][c][e]), ordered(score[1][c][e])));
+        const float high = __int_as_float(top ^ (int)((uint32_t)(top >> 31) >> 1));
         const float next = fmaxf(ref[c], fmaxf(high, __shfl_xor(high, 32, kWave)) * row_scale[c]);
         const float keep = exp2_fast(ref[c] - (next == -kInfinity ? 0.0f : next));
         ref[c] = next;
@@ -1336,7 +1342,7 @@ Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least,
 }
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
-             int64_t sinks, int64_t longest, bool by_offsets) {
+             int64_t sinks, int64_t longest, bool by_offsets, bool quantized) {
   Plan p{true, 128, {0, 1}, {0, 1}, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
@@ -1345,10 +1351,11 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   p.few16 = by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
   if (by_offsets || each * group <= kFewRows) p.few = split_of(sequences * kv_heads, seen, 1024, 4, 32);
   if (each * group > kFewRows) {
-    // Blocks of 256 rows read keys and values half as often, blocks of 128 leave fewer rows idle and two of them
-    // on a compute unit wait at barriers of their own
+    // Blocks of 256 rows read keys and values (and make codes F16 numbers) half as often; blocks of 128 leave fewer
+    // rows idle, and two of them on a compute unit wait at barriers of their own. us, 128 / 256: a prompt of 8,192
+    // tokens, 32 heads over 8 733 / 702, a mixed batch of 1,811 tokens 257 / 273, 1,021 tokens over 8 bits 145 / 129.
     const int64_t rows = tokens * group;
-    p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= 768 ? 256 : 128;
+    p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= (quantized ? 64 : 768) ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
     p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
   }
@@ -1448,7 +1455,7 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   while (((uint64_t)a.page_units << 27) > ((uint64_t)1 << a.page_shift)) ++a.page_shift;
   a.page_magic = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page_units - 1) / a.page_units);
   const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
-                            a.p.offsets != nullptr);
+                            a.p.offsets != nullptr, a.key_scales != nullptr);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,
                   (long long)plan.bytes);
@@ -1474,9 +1481,10 @@ extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens
   if (const int bad = check_attention("drift_paged_attention_workspace", heads, kv_heads, head_dim, window, sinks,
                                       longest))
     return bad;
-  // with offsets or without
-  for (const bool by_offsets : {false, true})
-    *bytes = std::max(*bytes, plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest, by_offsets).bytes);
+  // with offsets or without, over either cache
+  for (const int kind : {0, 1, 2, 3})
+    *bytes = std::max(*bytes, plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest, kind & 1,
+                                      kind & 2).bytes);
   return 0;
 }
 
