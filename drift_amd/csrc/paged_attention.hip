@@ -410,30 +410,18 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
     }
   };
 
-  int i = begin + wave;
-  Places now = places_of(i), next = places_of(i + kWaves);
-  if (i < end) load_keys(now);
-  for (; i < end; i += kWaves) {
-    const uint32_t base = (uint32_t)list.tile(i) * TOK;
-    const uint32_t mine = base + g * (TOK / 4);  // the lane's first position
-    const bool okay = (uint32_t)now.value_page < (uint32_t)a.p.cache_pages;
-    const int32_t value_page = okay ? now.value_page : 0;
-    if (!okay && mine <= p1 &&
-        (a.window == 0 || mine + TOK / 4 - 1 + (uint32_t)a.window > p0 || mine < (uint32_t)a.sinks))
-      flag_bad(a.p);
-
-    // the values, and the scales in 8 bits
-    uint4 values[DT];
-    {
-      const char* from = (const char*)a.values + (((int64_t)value_page * a.kv_heads + kv) * a.dim * a.p.page_size +
-                                                  now.value_off + (g * (TOK / 4)) % 16) * (I8 ? 1 : 2);
-      const int64_t stride = (int64_t)a.p.page_size * (I8 ? 1 : 2);
+  // the values, and the scales in 8 bits
+  uint4 values[DT];
+  float key_scale[I8 ? 16 : 1], value_log[I8 ? 16 : 1];
+  auto load_values = [&](const Places& w) {
+    const int32_t page = (uint32_t)w.value_page < (uint32_t)a.p.cache_pages ? w.value_page : 0;
+    const char* from = (const char*)a.values + (((int64_t)page * a.kv_heads + kv) * a.dim * a.p.page_size +
+                                                w.value_off + (g * (TOK / 4)) % 16) * (I8 ? 1 : 2);
+    const int64_t stride = (int64_t)a.p.page_size * (I8 ? 1 : 2);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) values[d] = *(const uint4*)(from + min(d * 16 + col, a.dim - 1) * stride);
-    }
-    float key_scale[I8 ? 16 : 1], value_log[I8 ? 16 : 1];
+    for (int d = 0; d < DT; ++d) values[d] = *(const uint4*)(from + min(d * 16 + col, a.dim - 1) * stride);
     if constexpr (I8) {
-      const int64_t at = ((int64_t)value_page * a.kv_heads + kv) * a.p.page_size + now.value_off;
+      const int64_t at = ((int64_t)page * a.kv_heads + kv) * a.p.page_size + w.value_off;
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const float4 x = *(const float4*)(a.key_scales + at + e), y = *(const float4*)(a.value_scales + at + e);
@@ -441,6 +429,23 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
         value_log[e] = y.x, value_log[e + 1] = y.y, value_log[e + 2] = y.z, value_log[e + 3] = y.w;
       }
     }
+  };
+
+  // keys and values of a tile are asked for as soon as the one before it is done with their registers, so that
+  // both are on their way for a whole tile's time
+  int i = begin + wave;
+  Places now = places_of(i), next = places_of(i + kWaves);
+  if (i < end) {
+    load_keys(now);
+    load_values(now);
+  }
+  for (; i < end; i += kWaves) {
+    const uint32_t base = (uint32_t)list.tile(i) * TOK;
+    const uint32_t mine = base + g * (TOK / 4);  // the lane's first position
+    const bool okay = (uint32_t)now.value_page < (uint32_t)a.p.cache_pages;
+    if (!okay && mine <= p1 &&
+        (a.window == 0 || mine + TOK / 4 - 1 + (uint32_t)a.window > p0 || mine < (uint32_t)a.sinks))
+      flag_bad(a.p);
 
     // scores: score[c][t][i] is row c 16 + col, position mine + 4 t + i
     f32x4 score[C][NT];
@@ -583,6 +588,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
             acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weights[c].term[m], acc[c][d], 0, 0, 0);
       }
     }
+    if (i + kWaves < end) load_values(coming);
     now = coming;
   }
 
@@ -1349,7 +1355,10 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
   // (mixed batches are single tokens for the most part: 16 rows a unit while a sequence has 24 on average)
   p.few16 = by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
-  if (by_offsets || each * group <= kFewRows) p.few = split_of(sequences * kv_heads, seen, 1024, 4, 32);
+  // Up to 768 positions a second launch takes longer than it saves (one token at 517: 13.5 us, 15.6 in three splits);
+  // splits of 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000: 239 us, 264 by 2,048).
+  if (by_offsets || each * group <= kFewRows)
+    p.few = seen <= 768 ? Split{1, 1} : split_of(sequences * kv_heads, seen, 1024, 4, 16);
   if (each * group > kFewRows) {
     // Blocks of 256 rows read keys and values (and make codes F16 numbers) half as often; blocks of 128 leave fewer
     // rows idle, and two of them on a compute unit wait at barriers of their own. us, 128 / 256: a prompt of 8,192
