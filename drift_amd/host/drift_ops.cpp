@@ -91,6 +91,22 @@ KvCache KvCache::of(const Tensor& keys, const Tensor& values, int pageSize) {
   return KvCache{keys, values, pageSize};
 }
 
+QuantizedKvCache QuantizedKvCache::of(const Tensor& keys, const Tensor& values, const Tensor& keyScales,
+                                      const Tensor& valueScales, int pageSize) {
+  require(pageSize > 0 && pageSize % 16 == 0, text("pages of ", pageSize, " tokens: not a multiple of 16"));
+  require(keys.dtype == DType::I8 && values.dtype == DType::I8, "the 8-bit cache's codes are I8");
+  require(keys.shape.rank() == 4 && values.shape.rank() == 4, "the cache's keys and values are 4-dimensional");
+  const QuantizedKvCache cache{keys, values, keyScales, valueScales, pageSize};
+  require(keys.shape[1] == pageSize &&
+              values.shape == Shape{cache.pages(), cache.kvHeads(), cache.headDimension(), pageSize},
+          text("cache values ", values.shape.str(), " for keys ", keys.shape.str()));
+  checks::requireF32("the 8-bit cache", {&keyScales, &valueScales});
+  for (const Tensor* scales : {&keyScales, &valueScales})
+    require(scales->shape == Shape{cache.pages(), cache.kvHeads(), pageSize},
+            text("cache scales ", scales->shape.str(), " for keys ", keys.shape.str()));
+  return cache;
+}
+
 // tensor/DType.scala, GgmlQuants.scala:12-118, KQuants.scala:100-134,
 // IQuants.scala:40-80, RocmFp4.scala:75-84, with the GGUF type ids
 const std::vector<StorageType>& StorageType::all() {
@@ -264,6 +280,52 @@ int64_t checkCacheWrite(const Tensor& k, const Tensor& v, const KvCache& cache, 
   const int64_t tokens = k.shape[0];
   checkPageTable(pageTable, cache, start + tokens);
   return tokens;
+}
+
+void checkSequences(const char* operation, const Sequences& sequences, int64_t tokens) {
+  const Tensor& tables = sequences.pageTables;
+  require(tables.dtype == DType::I32 && tables.shape.rank() == 2,
+          text(operation, ": page tables are I32 [sequences, pages], not ", name(tables.dtype), " ",
+               tables.shape.str()));
+  const int64_t count = tables.shape[0];
+  const auto checkArray = [&](const char* what, const Tensor& array, int64_t values) {
+    require(array.dtype == DType::I32 && array.shape == Shape{values},
+            text(operation, ": ", what, " ", name(array.dtype), " ", array.shape.str(), " for ", count, " sequences"));
+  };
+  checkArray("starts", sequences.starts, count);
+  if (sequences.offsets)
+    checkArray("offsets", *sequences.offsets, count + 1);
+  else
+    require(count == tokens, text(operation, ": ", count, " sequences for ", tokens,
+                                  " rows (several rows a sequence need offsets)"));
+  require(sequences.longest >= 0, text(operation, ": a longest sequence of ", sequences.longest, " positions"));
+}
+
+// Keys and values to or from a cache: the token count.
+int64_t checkCacheRows(const char* operation, const Tensor& k, const Tensor& v, const PagedCache& cache) {
+  checkElementwise(operation, {&k, &v});
+  require(k.shape.rank() == 3 && k.shape[1] == cache.kvHeads() && k.shape[2] == cache.headDimension(),
+          text(operation, ": ", k.shape.str(), " for a cache of ", cache.kvHeads(), " heads of ",
+               cache.headDimension()));
+  return k.shape[0];
+}
+
+void checkAttention(const char* operation, const Tensor& queries, const PagedCache& cache, const Tensor& out,
+                    const std::optional<AttentionWindow>& window) {
+  checkElementwise(operation, {&queries, &out});
+  require(queries.shape.rank() == 3,
+          text(operation, " takes [tokens, heads, headDimension], got ", queries.shape.str()));
+  const int64_t heads = queries.shape[1];
+  require(queries.shape[2] == cache.headDimension() && cache.kvHeads() > 0 && heads > 0 &&
+              heads % cache.kvHeads() == 0,
+          text(operation, ": queries ", queries.shape.str(), " over a cache of ", cache.kvHeads(), " heads of ",
+               cache.headDimension()));
+  require(queries.shape[2] <= HipOps::AttentionHeadDimension,
+          text(operation, ": heads of ", queries.shape[2], " values (at most ", HipOps::AttentionHeadDimension, ")"));
+  if (window)
+    require(window->positions > 0 && window->positions <= HipOps::MostPositions && window->sinks >= 0 &&
+                window->sinks <= HipOps::MostPositions,
+            text("a window of ", window->positions, " positions with ", window->sinks, " sinks"));
 }
 
 // ops/LayoutOps.scala:73-80
@@ -766,6 +828,157 @@ void HipOps::fusedAttentionInputs(const Tensor& queryAndGate, const Tensor& keys
                  (int32_t)r.layout, r.sections.code, s[0], s[1], s[2], s[3], at<float>(rotatedQueries),
                  at<float>(gate), at<uint16_t>(cache.keys), at<uint16_t>(cache.values), at<int32_t>(pageTable), table,
                  (int32_t)cache.pages(), cache.pageSize, (int32_t)start, badPage, stream_));
+}
+
+// ---- the paged cache of several sequences, attention
+
+struct HipOps::Paging {
+  const int32_t *tables, *starts = nullptr, *offsets = nullptr;
+  int32_t tablePages, count = 1, start = 0, longest;
+};
+
+HipOps::Paging HipOps::pagingOf(const char* operation, const PagedCache& cache, const CacheRows& rows,
+                                int64_t tokens) {
+  require(tokens <= MostPositions, text(operation, ": ", tokens, " tokens"));
+  Paging p{};
+  if (!rows.sequences) {
+    const Tensor& table = *rows.pageTable;
+    require(table.dtype == DType::I32 && table.shape.rank() == 1,
+            text("a page table is I32 [pages], not ", name(table.dtype), " ", table.shape.str()));
+    require(rows.start >= 0 && rows.start <= MostPositions - tokens,
+            text(operation, ": ", tokens, " tokens from position ", rows.start));
+    require(table.elementCount() * cache.pageSize >= rows.start + tokens,
+            text("a page table of ", table.elementCount(), " pages for ", rows.start + tokens, " positions"));
+    p.tables = at<int32_t>(table);
+    p.tablePages = (int32_t)table.elementCount();
+    p.count = 1;
+    p.start = (int32_t)rows.start;
+    p.longest = (int32_t)(rows.start + tokens);
+    return p;
+  }
+  const Sequences& s = *rows.sequences;
+  checkSequences(operation, s, tokens);
+  const int64_t room = std::min<int64_t>(s.pageTables.shape[1] * cache.pageSize, MostPositions);
+  p.tables = at<int32_t>(s.pageTables);
+  p.starts = at<int32_t>(s.starts);
+  p.offsets = s.offsets ? at<int32_t>(*s.offsets) : nullptr;
+  p.tablePages = (int32_t)s.pageTables.shape[1];
+  p.count = (int32_t)s.pageTables.shape[0];
+  p.longest = (int32_t)(s.longest > 0 ? std::min(s.longest, room) : room);
+  return p;
+}
+
+namespace {
+float* scalesOf(const std::optional<Tensor>& scales) { return scales ? at<float>(*scales) : nullptr; }
+}  // namespace
+
+void HipOps::writeRows(const char* operation, const Tensor& k, const Tensor& v, const PagedCache& cache,
+                       const CacheRows& rows, int32_t* badPage) {
+  const auto tokens = (int32_t)checkCacheRows(operation, k, v, cache);
+  const Paging p = pagingOf(operation, cache, rows, k.shape[0]);
+  const auto heads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();
+  if (isBf16(k))
+    launched("drift_paged_write_bf16",
+             drift_paged_write_bf16(at<uint16_t>(k), at<uint16_t>(v), cache.keys.data, cache.values.data,
+                                    scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                    (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                    dimension, cache.pageSize, badPage, stream_));
+  else
+    launched("drift_paged_write_f32",
+             drift_paged_write_f32(at<float>(k), at<float>(v), cache.keys.data, cache.values.data,
+                                   scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                   (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                   dimension, cache.pageSize, badPage, stream_));
+}
+
+void HipOps::readRows(const char* operation, const PagedCache& cache, const CacheRows& rows, const Tensor& k,
+                      const Tensor& v, int32_t* badPage) {
+  const auto tokens = (int32_t)checkCacheRows(operation, k, v, cache);
+  const Paging p = pagingOf(operation, cache, rows, k.shape[0]);
+  const auto heads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();
+  if (isBf16(k))
+    launched("drift_paged_read_bf16",
+             drift_paged_read_bf16(at<uint16_t>(k), at<uint16_t>(v), cache.keys.data, cache.values.data,
+                                   scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                   (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                   dimension, cache.pageSize, badPage, stream_));
+  else
+    launched("drift_paged_read_f32",
+             drift_paged_read_f32(at<float>(k), at<float>(v), cache.keys.data, cache.values.data,
+                                  scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                  (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                  dimension, cache.pageSize, badPage, stream_));
+}
+
+void HipOps::cacheWrite(const Tensor& k, const Tensor& v, const QuantizedKvCache& cache, const Tensor& pageTable,
+                        int64_t start, int32_t* badPage) {
+  writeRows("cacheWrite", k, v, cache, CacheRows(pageTable, start), badPage);
+}
+
+void HipOps::cacheWriteSequences(const Tensor& k, const Tensor& v, const PagedCache& cache, const Sequences& sequences,
+                                 int32_t* badPage) {
+  writeRows("cacheWriteSequences", k, v, cache, sequences, badPage);
+}
+
+void HipOps::cacheRead(const PagedCache& cache, const Tensor& pageTable, int64_t start, const Tensor& k,
+                       const Tensor& v, int32_t* badPage) {
+  readRows("cacheRead", cache, CacheRows(pageTable, start), k, v, badPage);
+}
+
+void HipOps::cacheReadSequences(const PagedCache& cache, const Sequences& sequences, const Tensor& k, const Tensor& v,
+                                int32_t* badPage) {
+  readRows("cacheReadSequences", cache, sequences, k, v, badPage);
+}
+
+int64_t HipOps::attentionWorkspace(const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
+                                   const std::optional<AttentionWindow>& window) {
+  checkAttention("attentionWorkspace", queries, cache, queries, window);
+  const Paging p = pagingOf("attentionWorkspace", cache, rows, queries.shape[0]);
+  int64_t bytes = 0;
+  const int code = drift_paged_attention_workspace(
+      p.count, (int32_t)queries.shape[0], (int32_t)queries.shape[1], (int32_t)cache.kvHeads(),
+      (int32_t)cache.headDimension(), window ? (int32_t)window->positions : 0, window ? (int32_t)window->sinks : 0,
+      p.longest, &bytes);
+  if (code != 0) throw HipException("drift_paged_attention_workspace", code, drift_last_error());
+  return bytes;
+}
+
+void HipOps::attend(const char* operation, const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
+                    float scale, const Tensor& out, const Tensor& workspace,
+                    const std::optional<AttentionWindow>& window, int32_t* badPage) {
+  checkAttention(operation, queries, cache, out, window);
+  require(queries.data != out.data || queries.elementCount() == 0, text(operation, ": out is queries"));
+  const Paging p = pagingOf(operation, cache, rows, queries.shape[0]);
+  const auto tokens = (int32_t)queries.shape[0], heads = (int32_t)queries.shape[1];
+  const auto kvHeads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();
+  const int32_t positions = window ? (int32_t)window->positions : 0, sinks = window ? (int32_t)window->sinks : 0;
+  const int64_t bytes = workspace.data ? workspace.byteSize() : 0;
+  if (isBf16(queries))
+    launched("drift_paged_attention_bf16",
+             drift_paged_attention_bf16(at<uint16_t>(queries), cache.keys.data, cache.values.data,
+                                        scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables,
+                                        p.tablePages, (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start,
+                                        tokens, heads, kvHeads, dimension, cache.pageSize, scale, positions, sinks,
+                                        p.longest, at<uint16_t>(out), workspace.data, bytes, badPage, stream_));
+  else
+    launched("drift_paged_attention_f32",
+             drift_paged_attention_f32(at<float>(queries), cache.keys.data, cache.values.data,
+                                       scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables,
+                                       p.tablePages, (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start,
+                                       tokens, heads, kvHeads, dimension, cache.pageSize, scale, positions, sinks,
+                                       p.longest, at<float>(out), workspace.data, bytes, badPage, stream_));
+}
+
+void HipOps::attention(const Tensor& queries, const PagedCache& cache, const Tensor& pageTable, int64_t start,
+                       float scale, const Tensor& out, const Tensor& workspace,
+                       const std::optional<AttentionWindow>& window, int32_t* badPage) {
+  attend("attention", queries, cache, CacheRows(pageTable, start), scale, out, workspace, window, badPage);
+}
+
+void HipOps::attentionSequences(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, float scale,
+                                const Tensor& out, const Tensor& workspace,
+                                const std::optional<AttentionWindow>& window, int32_t* badPage) {
+  attend("attentionSequences", queries, cache, sequences, scale, out, workspace, window, badPage);
 }
 
 // ---- tables

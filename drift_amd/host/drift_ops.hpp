@@ -123,6 +123,63 @@ struct KvCache {
   int64_t headDimension() const { return keys.shape[3]; }
 };
 
+// KvCache's pages in 8 bits: I8 codes keys [pages, pageSize, kvHeads, D] and
+// values [pages, kvHeads, D, pageSize], F32 scales [pages, kvHeads, pageSize],
+// one a position and head of each: a value is its code times its row's scale,
+// max |x| / 127 of the row. `of` checks that the four agree.
+struct QuantizedKvCache {
+  Tensor keys, values, keyScales, valueScales;
+  int pageSize = 16;
+
+  static QuantizedKvCache of(const Tensor& keys, const Tensor& values, const Tensor& keyScales,
+                             const Tensor& valueScales, int pageSize);
+  int64_t pages() const { return keys.shape[0]; }
+  int64_t kvHeads() const { return keys.shape[2]; }
+  int64_t headDimension() const { return keys.shape[3]; }
+};
+
+// Either cache, as the calls that take both see it.
+struct PagedCache {
+  Tensor keys, values;
+  std::optional<Tensor> keyScales, valueScales;
+  int pageSize;
+
+  PagedCache(const KvCache& c) : keys(c.keys), values(c.values), pageSize(c.pageSize) {}
+  PagedCache(const QuantizedKvCache& c)
+      : keys(c.keys), values(c.values), keyScales(c.keyScales), valueScales(c.valueScales), pageSize(c.pageSize) {}
+  int64_t pages() const { return keys.shape[0]; }
+  int64_t kvHeads() const { return keys.shape[2]; }
+  int64_t headDimension() const { return keys.shape[3]; }
+};
+
+// What a row at position P sees: j > P - positions, and j < sinks.
+struct AttentionWindow {
+  int64_t positions;
+  int64_t sinks = 0;
+};
+
+// Several sequences' token rows in one call: sequence s has rows offsets[s] to
+// offsets[s + 1], at positions starts[s] and on, in the pages pageTables[s]
+// ([sequences, pages]), all I32 and read on the device; without `offsets` each
+// has one row. `longest`: a guess of the most positions of one, by which
+// attention splits its work (0: what the page tables have room for).
+struct Sequences {
+  Tensor pageTables, starts;
+  std::optional<Tensor> offsets;
+  int64_t longest = 0;
+};
+
+// Where a call's rows lie: one sequence's from `start` on in the pages
+// `pageTable`, or several sequences'.
+struct CacheRows {
+  std::optional<Tensor> pageTable;
+  int64_t start = 0;
+  std::optional<Sequences> sequences;
+
+  CacheRows(const Tensor& pageTable, int64_t start) : pageTable(pageTable), start(start) {}
+  CacheRows(const Sequences& sequences) : sequences(sequences) {}
+};
+
 // A table's storage type (tensor/DType.scala:14-66): values per block of
 // bytes, its GGUF type id (the kernels' `format`) and the alignment its
 // blocks' fields need.
@@ -208,6 +265,10 @@ RotatedTable checkRotated(const Tensor& codes, const ConvRotParts& parts);
 void checkPageTable(const Tensor& pageTable, const KvCache& cache, int64_t positions);
 int64_t checkCacheWrite(const Tensor& k, const Tensor& v, const KvCache& cache, const Tensor& pageTable,
                         int64_t start);
+void checkSequences(const char* operation, const Sequences& sequences, int64_t tokens);
+int64_t checkCacheRows(const char* operation, const Tensor& k, const Tensor& v, const PagedCache& cache);
+void checkAttention(const char* operation, const Tensor& queries, const PagedCache& cache, const Tensor& out,
+                    const std::optional<AttentionWindow>& window);
 void checkSplitHalves(const Tensor& x, const Tensor& first, const Tensor& second);
 int checkConvert(const Tensor& x, const Tensor& out);  // the reference's conversion code
 }  // namespace checks
@@ -217,6 +278,11 @@ class HipOps {
  public:
   // attention.hip's ATTENTION_INPUT_DIMENSION (ops/HipAttention.scala:217-218)
   static constexpr int64_t AttentionInputDimension = 512;
+
+  // paged_attention.hip's widest head, and the most positions of a sequence in
+  // the calls over several sequences and in attention
+  static constexpr int64_t AttentionHeadDimension = 512;
+  static constexpr int64_t MostPositions = INT32_MAX - 127;
 
   // `stream`: a hipStream_t, null for the default stream.
   explicit HipOps(void* stream = nullptr);
@@ -294,6 +360,34 @@ class HipOps {
                              const Tensor& positions, const KvCache& cache, const Tensor& pageTable, int64_t start,
                              const Tensor& rotatedQueries, int32_t* badPage = nullptr);
 
+  // ---- the paged cache of several sequences a call, in F16 and in 8 bits,
+  // and attention over it. *badPage (device int32) is set where a page lies
+  // outside the cache or the arrays describe a sequence wrongly.
+  // one sequence's rows quantised into the 8-bit cache
+  void cacheWrite(const Tensor& k, const Tensor& v, const QuantizedKvCache& cache, const Tensor& pageTable,
+                  int64_t start, int32_t* badPage = nullptr);
+  void cacheWriteSequences(const Tensor& k, const Tensor& v, const PagedCache& cache, const Sequences& sequences,
+                           int32_t* badPage = nullptr);
+  // the cache's positions into k and v [tokens, kvHeads, D]
+  void cacheRead(const PagedCache& cache, const Tensor& pageTable, int64_t start, const Tensor& k, const Tensor& v,
+                 int32_t* badPage = nullptr);
+  void cacheReadSequences(const PagedCache& cache, const Sequences& sequences, const Tensor& k, const Tensor& v,
+                          int32_t* badPage = nullptr);
+  // bytes of scratch that an attention call over these needs; the caller owns
+  // it, one for each of the calls that may run at the same time
+  int64_t attentionWorkspace(const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
+                             const std::optional<AttentionWindow>& window = {});
+  // queries, out [tokens, heads, D]: a sequence's row at position P over its
+  // positions up to P, or with `window` those of it, its own keys and values
+  // written before; scores are scale q.k, head h reads key head h / (heads /
+  // kvHeads). `workspace`: dense memory of attentionWorkspace's bytes.
+  void attention(const Tensor& queries, const PagedCache& cache, const Tensor& pageTable, int64_t start, float scale,
+                 const Tensor& out, const Tensor& workspace, const std::optional<AttentionWindow>& window = {},
+                 int32_t* badPage = nullptr);
+  void attentionSequences(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, float scale,
+                          const Tensor& out, const Tensor& workspace,
+                          const std::optional<AttentionWindow>& window = {}, int32_t* badPage = nullptr);
+
   // ---- tables (ops/LinearOps.scala:16-33, ops/MemoryOps.scala:46)
   // An id outside the table (which the reference refuses) gets a zero row
   // and sets *badId (device int32) when given.
@@ -336,6 +430,15 @@ class HipOps {
                             const QueryKeyNorms& norms, const Tensor& positions, const KvCache& cache,
                             const Tensor& pageTable, int64_t start, const Tensor* gate, const Tensor& rotatedQueries,
                             int32_t* badPage);
+  struct Paging;  // a call's page tables, starts and offsets, and the sizes with them
+  static Paging pagingOf(const char* operation, const PagedCache& cache, const CacheRows& rows, int64_t tokens);
+  void writeRows(const char* operation, const Tensor& k, const Tensor& v, const PagedCache& cache,
+                 const CacheRows& rows, int32_t* badPage);
+  void readRows(const char* operation, const PagedCache& cache, const CacheRows& rows, const Tensor& k,
+                const Tensor& v, int32_t* badPage);
+  void attend(const char* operation, const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
+              float scale, const Tensor& out, const Tensor& workspace, const std::optional<AttentionWindow>& window,
+              int32_t* badPage);
   void decodeRotated(const RotatedTable& table, const Tensor& out, const Tensor* ids, int32_t* badId);
 };
 

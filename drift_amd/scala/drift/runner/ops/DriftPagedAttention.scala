@@ -58,6 +58,9 @@ final case class Sequences(pageTables: Tensor, starts: Tensor, offsets: Option[T
   */
 private[ops] trait DriftPagedAttention extends DriftAttention {
 
+  /** The most positions of a sequence (csrc/paged.hpp). */
+  private val MostPositions: Long = Int.MaxValue - 127L
+
   /** A cache as the entry points take it: its tensors and sizes. */
   private final case class Paged(keys: Tensor, values: Tensor, keyScales: Option[Tensor], valueScales: Option[Tensor],
                                  pages: Int, kvHeads: Int, headDimension: Int, pageSize: Int)
@@ -113,14 +116,14 @@ private[ops] trait DriftPagedAttention extends DriftAttention {
         require(table.dtype == DType.I32 && table.shape.rank == 1,
           s"a page table is I32 [pages], not ${table.dtype} ${table.shape}")
         val count = table.shape.elementCount
-        require(start >= 0 && start.toLong + tokens <= Int.MaxValue, s"$operation: $tokens tokens from position $start")
+        require(start >= 0 && start.toLong + tokens <= MostPositions, s"$operation: $tokens tokens from position $start")
         require(count * cache.pageSize >= start.toLong + tokens,
           s"a page table of $count pages for ${start.toLong + tokens} positions")
         Rows(table, count.toInt, None, None, 1, start, start + tokens)
       case Right(sequences) =>
         checkSequences(operation, sequences, tokens)
         val tablePages = sequences.pageTables.shape.last.toInt
-        val room = (tablePages.toLong * cache.pageSize).min(Int.MaxValue).toInt
+        val room = (tablePages.toLong * cache.pageSize).min(MostPositions).toInt
         Rows(sequences.pageTables, tablePages, Some(sequences.starts), sequences.offsets, sequences.count, 0,
           if (sequences.longest > 0) sequences.longest.min(room) else room)
     }
@@ -176,7 +179,7 @@ private[ops] trait DriftPagedAttention extends DriftAttention {
     Ops.checkElementwise(operation, queries, out)
     require(queries.shape.rank == 3, s"$operation takes [tokens, heads, headDimension], got ${queries.shape}")
     val (tokens, heads) = (queries.shape.dimensions(0).toInt, queries.shape.dimensions(1).toInt)
-    require(queries.shape.last == cache.headDimension && heads > 0 && heads % cache.kvHeads == 0,
+    require(queries.shape.last == cache.headDimension && cache.kvHeads > 0 && heads > 0 && heads % cache.kvHeads == 0,
       s"$operation: queries ${queries.shape} over a cache of ${cache.kvHeads} heads of ${cache.headDimension}")
     val rows = rowsOf(operation, cache, tokens, where)
     val (tablePages: Int, pages: Int, count: Int, start: Int) = (rows.tablePages, cache.pages, rows.count, rows.start)

@@ -155,6 +155,47 @@ CHECK_TEST(cache_and_attention_inputs_are_checked) {
   }, "queryKeyNormRopeCache: queries [20×4×1024]");
 }
 
+CHECK_TEST(paged_calls_are_checked) {
+  HipOps hip;
+  const Tensor codes = fake(DType::I8, {2, 16, 2, 64}), codesV = fake(DType::I8, {2, 2, 64, 16});
+  const Tensor scales = fake(DType::F32, {2, 2, 16});
+  refused([&] { QuantizedKvCache::of(codes, codesV, scales, scales, 24); }, "pages of 24 tokens: not a multiple of 16");
+  refused([&] { QuantizedKvCache::of(fake(DType::F16, {2, 16, 2, 64}), codesV, scales, scales, 16); },
+          "the 8-bit cache's codes are I8");
+  refused([&] { QuantizedKvCache::of(codes, codes, scales, scales, 16); },
+          "cache values [2×16×2×64] for keys [2×16×2×64]");
+  refused([&] { QuantizedKvCache::of(codes, codesV, scales, fake(DType::F32, {2, 16, 2}), 16); },
+          "cache scales [2×16×2] for keys [2×16×2×64]");
+  const QuantizedKvCache eight = QuantizedKvCache::of(codes, codesV, scales, scales, 16);
+  const KvCache cache = KvCache::of(fake(DType::F16, {2, 16, 2, 64}), fake(DType::F16, {2, 2, 64, 16}), 16);
+  const Tensor k = fake(DType::BF16, {20, 2, 64}), table = fake(DType::I32, {2});
+  refused([&] { hip.cacheWrite(k, k, eight, fake(DType::I32, {1}), 0); }, "a page table of 1 pages for 20 positions");
+  refused([&] { hip.cacheWrite(k, k, eight, table, -1); }, "cacheWrite: 20 tokens from position -1");
+  refused([&] { hip.cacheRead(cache, table, 0, fake(DType::F32, {20, 3, 64}), fake(DType::F32, {20, 3, 64})); },
+          "cacheRead: [20×3×64] for a cache of 2 heads of 64");
+  const Sequences s{fake(DType::I32, {3, 2}), fake(DType::I32, {3}), {}, 0};
+  refused([&] { hip.cacheWriteSequences(k, k, cache, s); },
+          "cacheWriteSequences: 3 sequences for 20 rows (several rows a sequence need offsets)");
+  refused([&] { hip.cacheReadSequences(eight, Sequences{table, s.starts, {}, 0}, k, k); },
+          "cacheReadSequences: page tables are I32 [sequences, pages], not I32 [2]");
+  refused([&] { hip.cacheWriteSequences(k, k, eight, Sequences{s.pageTables, fake(DType::I32, {2}), {}, 0}); },
+          "cacheWriteSequences: starts I32 [2] for 3 sequences");
+  const Tensor q = fake(DType::F32, {3, 4, 64}), out = fake(DType::F32, {3, 4, 64}, 8192);
+  const Tensor none{DType::U8, {0}, nullptr};
+  refused([&] { hip.attentionSequences(q, eight, Sequences{s.pageTables, s.starts, fake(DType::I32, {3}), 0}, 1.0f, out,
+                                       none); }, "attentionSequences: offsets I32 [3] for 3 sequences");
+  refused([&] { hip.attentionSequences(q, cache, s, 1.0f, q, none); }, "attentionSequences: out is queries");
+  refused([&] { hip.attention(fake(DType::F32, {3, 3, 64}), cache, table, 0, 1.0f, fake(DType::F32, {3, 3, 64}, 8192),
+                              none); }, "attention: queries [3×3×64] over a cache of 2 heads of 64");
+  refused([&] { hip.attention(q, cache, table, 30, 1.0f, out, none); }, "a page table of 2 pages for 33 positions");
+  refused([&] { hip.attention(q, cache, table, 0, 1.0f, out, none, AttentionWindow{0, 0}); },
+          "a window of 0 positions with 0 sinks");
+  // a long sequence is split, so it needs scratch
+  const Sequences wide{fake(DType::I32, {3, 4096}), fake(DType::I32, {3}), {}, 0};
+  expect(hip.attentionWorkspace(q, cache, wide) > 0, "scratch of a long sequence");
+  refused<HipException>([&] { hip.attentionSequences(q, cache, wide, 1.0f, out, none); }, "workspace");
+}
+
 CHECK_TEST(tables_are_checked) {
   HipOps hip;
   const StorageType& q4k = StorageType::named("Q4_K");
@@ -658,6 +699,92 @@ GPU_TEST(attention_inputs_equal_their_steps) {
   hip.queryKeyNormRopeCache(q2, kd, vd, norms, pos, nogate_cache, pt, start, rq3);
   exact(dev.download<float>(rq2), dev.download<float>(rq3), "queryKeyNormRopeCache queries");
   exact(dev.download<uint16_t>(steps_cache.keys), dev.download<uint16_t>(nogate_cache.keys), "queryKeyNormRopeCache keys");
+}
+
+GPU_TEST(paged_attention_over_both_caches) {
+  // three sequences of unlike lengths: their positions written sequence by
+  // sequence and in one call, read back, and one decode step attended over
+  // either cache, held to the same sums in 64 bits over what the cache holds.
+  // F32 queries: a term of the score is off by at most 2^-22 of |q||k| and the
+  // weights by the exponential's 2^-21; with |s| below 16 and |v| below 5 all
+  // stays under 1e-4, which a wrong page, head or length passes by far.
+  HipOps hip;
+  Device dev;
+  const int kh = 2, heads = 6, dim = 64, page = 16, pages = 24, wide = 8, count = 3;
+  const std::vector<int32_t> lengths = {1, 37, 100};
+  std::vector<int32_t> table((size_t)count * wide), offsets = {0}, zeros(count, 0), starts;
+  for (size_t i = 0; i < table.size(); ++i) table[i] = (int32_t)((i * 7 + 3) % pages);
+  for (int n : lengths) {
+    offsets.push_back(offsets.back() + n);
+    starts.push_back(n - 1);
+  }
+  const int64_t tokens = offsets.back();
+  const std::vector<float> k = gaussian(60, (size_t)tokens * kh * dim), v = gaussian(61, (size_t)tokens * kh * dim);
+  const std::vector<float> q = gaussian(62, (size_t)count * heads * dim);
+  const Tensor kd = dev.upload(DType::F32, {tokens, kh, dim}, k), vd = dev.upload(DType::F32, {tokens, kh, dim}, v);
+  const Tensor qd = dev.upload(DType::F32, {count, heads, dim}, q), tables = dev.upload(DType::I32, {count, wide}, table);
+  const Sequences all{tables, dev.upload(DType::I32, {count}, zeros), dev.upload(DType::I32, {count + 1}, offsets), 0};
+  const Sequences step{tables, dev.upload(DType::I32, {count}, starts), {}, 100};
+  const std::vector<uint16_t> blank((size_t)pages * page * kh * dim, 0);
+  const std::vector<int8_t> blank8(blank.size(), 0);
+  const std::vector<float> blank_scales((size_t)pages * kh * page, 0.0f);
+  auto half = [&] {
+    return KvCache::of(dev.upload(DType::F16, {pages, page, kh, dim}, blank),
+                       dev.upload(DType::F16, {pages, kh, dim, page}, blank), page);
+  };
+  const KvCache one = half(), several = half();
+  const QuantizedKvCache eight = QuantizedKvCache::of(
+      dev.upload(DType::I8, {pages, page, kh, dim}, blank8), dev.upload(DType::I8, {pages, kh, dim, page}, blank8),
+      dev.upload(DType::F32, {pages, kh, page}, blank_scales), dev.upload(DType::F32, {pages, kh, page}, blank_scales),
+      page);
+  for (int s = 0; s < count; ++s) {
+    const auto rows = [&](const Tensor& t) {
+      return Tensor{DType::F32, {lengths[s], kh, dim}, static_cast<float*>(t.data) + (int64_t)offsets[s] * kh * dim};
+    };
+    hip.cacheWrite(rows(kd), rows(vd), one, Tensor{DType::I32, {wide}, static_cast<int32_t*>(tables.data) + s * wide}, 0);
+  }
+  hip.cacheWriteSequences(kd, vd, several, all);
+  exact(dev.download<uint16_t>(one.keys), dev.download<uint16_t>(several.keys), "keys of several sequences");
+  exact(dev.download<uint16_t>(one.values), dev.download<uint16_t>(several.values), "values of several sequences");
+  hip.cacheWriteSequences(kd, vd, eight, all);
+  for (const PagedCache& cache : {PagedCache(several), PagedCache(eight)}) {
+    const Tensor rk = dev.empty(DType::F32, {tokens, kh, dim}), rv = dev.empty(DType::F32, {tokens, kh, dim});
+    hip.cacheReadSequences(cache, all, rk, rv);
+    const std::vector<float> ck = dev.download<float>(rk), cv = dev.download<float>(rv);
+    for (size_t i = 0; i < ck.size(); ++i)  // |x| below 5: F16 2^-9, 8 bits 5 / 254
+      expect(std::fabs(ck[i] - k[i]) < 0.02f && std::fabs(cv[i] - v[i]) < 0.02f, "what the cache holds");
+    const Tensor out = dev.empty(DType::F32, {count, heads, dim});
+    const int64_t bytes = hip.attentionWorkspace(qd, cache, step);
+    hip.attentionSequences(qd, cache, step, 0.125f, out, dev.empty(DType::U8, {bytes}));
+    const std::vector<float> got = dev.download<float>(out);
+    for (int s = 0; s < count; ++s)
+      for (int h = 0; h < heads; ++h) {
+        const auto row = [&](int j) { return ((size_t)(offsets[s] + j) * kh + h / (heads / kh)) * dim; };
+        std::vector<double> p;
+        double top = -1e300, sum = 0;
+        for (int j = 0; j < lengths[s]; ++j) {
+          double dot = 0;
+          for (int d = 0; d < dim; ++d) dot += (double)q[(size_t)(s * heads + h) * dim + d] * ck[row(j) + d];
+          p.push_back(0.125 * dot);
+          top = std::max(top, p.back());
+        }
+        for (double& x : p) sum += x = std::exp(x - top);
+        for (int d = 0; d < dim; ++d) {
+          double want = 0;
+          for (int j = 0; j < lengths[s]; ++j) want += p[j] / sum * cv[row(j) + d];
+          expect(std::fabs(want - got[(size_t)(s * heads + h) * dim + d]) < 1e-4, "attention of a decode step");
+        }
+      }
+    // one sequence's call gives its row of the step
+    const Tensor single = dev.empty(DType::F32, {1, heads, dim});
+    const Tensor last{DType::F32, {1, heads, dim}, static_cast<float*>(qd.data) + 2 * heads * dim};
+    const Tensor its{DType::I32, {wide}, static_cast<int32_t*>(tables.data) + 2 * wide};
+    const int64_t its_bytes = hip.attentionWorkspace(last, cache, CacheRows(its, 99));
+    hip.attention(last, cache, its, 99, 0.125f, single, dev.empty(DType::U8, {its_bytes}));
+    const std::vector<float> alone = dev.download<float>(single);
+    for (int i = 0; i < heads * dim; ++i)
+      expect(std::fabs(alone[i] - got[(size_t)2 * heads * dim + i]) < 1e-4, "attention of one sequence");
+  }
 }
 
 GPU_TEST(stored_and_rotated_tables) {
