@@ -295,8 +295,11 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
   const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
-  const int split = rest % (unsigned)a.splits;
-  const unsigned unit = rest / (unsigned)a.splits;
+  // A unit's splits lie far apart: blocks go to the eight dies in turn, and where splits are neighbours those that have
+  // nothing to do are some dies' alone (64 sequences of 400 to 8,000 over 8 bits 158 us, 168 with neighbours).
+  const unsigned all_units = (unsigned)(a.p.sequences * a.few_units);
+  const int split = rest / all_units;
+  const unsigned unit = rest % all_units;
   const int s = (int)(unit / (unsigned)a.few_units), nth = (int)(unit % (unsigned)a.few_units);
   const Span span = span_of(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
@@ -307,6 +310,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   const int each = split_tiles(a, list.count);
   const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
   if (begin >= end) return;
+  const bool alone = each >= list.count;  // the rows' one split: no others to join
 
   // the rows' queries as B operands: column col, values 8 g .. of each 32 (8 bits: of each 64, 16 g ..)
   f16x8 query[C][KS][TERMS];
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
         float x = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) x = fmaf(merged[w][r][d], factor[w], x);
-        if (a.splits == 1) {
+        if (alone) {
           x *= inverse;
           odd |= !(fabsf(x) < kInfinity);
           store_one(out + place * a.dim + d, x);
@@ -642,7 +646,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
           a.partials[((int64_t)split * a.partial_rows + partial) * a.dim + d] = x;
         }
       }
-      if (a.splits == 1) {
+      if (alone) {
         // a row of -infinity alone, as one of NaN, is taken again
         if (__any(odd) || (l == 0.0f && m == -kInfinity)) again |= 1u << r;
       } else if (lane == 0) {
@@ -650,7 +654,7 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
         st[0] = m, st[1] = l, st[2] = vm;
       }
     }
-    if (a.splits == 1) {
+    if (alone) {
       __syncthreads();  // merged is free, and holds the scratch
       RowScratch& scratch = *reinterpret_cast<RowScratch*>(&merged[wave][0][0]);
       for (; again; again &= again - 1) {
@@ -696,9 +700,11 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
   const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
-  const int split = rest % (unsigned)a.splits;
-  // the last rows first: they have the most positions
-  const int64_t unit = gridDim.x / (unsigned)(a.kv_heads * a.splits) - 1 - rest / (unsigned)a.splits;
+  // A unit's splits lie far apart, as in attend_few (a mixed batch of 4 key heads in two splits 182 us, 315 with
+  // neighbours: half the dies idle); the last rows first: they have the most positions
+  const unsigned all_units = gridDim.x / (unsigned)(a.kv_heads * a.splits);
+  const int split = rest / all_units;
+  const int64_t unit = all_units - 1 - rest % all_units;
   int64_t nth;
   const int s = locate(a.p, unit, kRows, 0, a.group, nth);
   if (s < 0) return;
@@ -711,6 +717,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   const int each = split_tiles(a, list.count);
   const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
   if (begin >= end) return;
+  const bool alone = each >= list.count;  // the rows' one split: no others to join
 
   // ---- this wave's rows
   const int wave_row = wave * CT * 32;
@@ -1176,7 +1183,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
     const int64_t place = (span.first + token) * a.heads + kv * a.group + (row - token * group);
     const float sum = total[c] + __shfl_xor(total[c], 32, kWave);
     bool odd = apart || (sum == 0.0f && ref[c] == -kInfinity);
-    if (a.splits == 1) {
+    if (alone) {
       const float inverse = sum == 0.0f ? 0.0f : (I8 ? exp2_fast((float)value_exponent) : 1.0f) / sum;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -1227,14 +1234,18 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
 // Joins the splits of attend_few (FEW) or attend_many: a block takes up to
 // kJoinRows rows of one unit (`rows` of them, tiles of `tile` positions, which say
 // how many splits it had), a row by as many lanes as hold its values in fours.
-constexpr int kJoinRows = 16;
+template <bool FEW>
+constexpr int kJoinRows = FEW ? 16 : 32;
 
 template <typename T, bool I8, bool FEW, int DP>
 __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
-  constexpr int L = DP / 4;  // lanes a row
+  // (many rows have few splits: two fours a lane let each wave have twice the rows on the way; 2 splits of 32,672 rows
+  // of 128 values 9.5 us, 16.4 by one)
+  constexpr int V = FEW ? 1 : 2, N = FEW ? 8 : 4;  // fours of values a lane, splits at a time
+  constexpr int L = DP / 4 / V, kRows = kJoinRows<FEW>;  // lanes a row, rows a block
   __shared__ RowScratch scratch[4];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), in = lane % L;
-  const int parts = rows / kJoinRows;
+  const int parts = rows / kRows;
   const int kv = blockIdx.x % (unsigned)a.kv_heads, part = blockIdx.x / (unsigned)a.kv_heads % (unsigned)parts;
   const unsigned unit = blockIdx.x / (unsigned)a.kv_heads / (unsigned)parts;
   int s;
@@ -1245,59 +1256,73 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
   const Span span = span_of(a.p, s);
   const uint32_t all = (uint32_t)span.rows * (uint32_t)a.group, group = (uint32_t)a.group;
   const uint32_t row0 = (uint32_t)nth * rows;
-  if (row0 + part * kJoinRows >= all || (all <= (uint32_t)a.few_rows) != FEW) return;
-  const uint32_t last = min(row0 + rows, all) - 1, end = min(row0 + (part + 1) * kJoinRows, last + 1);
+  if (row0 + part * kRows >= all || (all <= (uint32_t)a.few_rows) != FEW) return;
+  const uint32_t last = min(row0 + rows, all) - 1, end = min(row0 + (part + 1) * kRows, last + 1);
   const TileList list = tiles_of(a, span.start + row0 / group, span.start + last / group, tile);
   const int each = split_tiles(a, list.count), splits = (list.count + each - 1) / each;
-  for (uint32_t first = row0 + part * kJoinRows + wave * (64 / L); first < end; first += 4 * (64 / L)) {
+  if (splits == 1) return;
+  for (uint32_t first = row0 + part * kRows + wave * (64 / L); first < end; first += 4 * (64 / L)) {
     const uint32_t mine = first + lane / L, row = min(mine, end - 1), token = row / group;
     const int h = kv * a.group + (int)(row - token * group);
     const int64_t place = (span.first + token) * a.heads + h;
     const int64_t partial = FEW ? ((int64_t)s * a.kv_heads + kv) * a.few_most + row : place;
     const float* st = a.statistics + partial * 3;
-    const float* from = a.partials + partial * a.dim + min(in * 4, a.dim - 4);
+    const float* from = a.partials + partial * a.dim;
     const int64_t st_step = a.partial_rows * 3, step = a.partial_rows * a.dim;
     float m = -kInfinity, vm = -kInfinity, l = 0.0f;
-    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    // eight splits at a time, their loads on the way together
-    for (int i = 0; i < splits; i += 8) {
-      float sm[8], sl[8], sv[8];
-      f32x4 v[8];
+    // a lane's values: fours in + k L of the row
+    int d[V];
+    f32x4 x[V];
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
+    for (int k = 0; k < V; ++k) d[k] = (in + k * L) * 4, x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // N splits at a time, their loads on the way together
+    for (int i = 0; i < splits; i += N) {
+      float sm[N], sl[N], sv[N];
+      f32x4 v[N][V];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
         const int64_t at = min(i + n, splits - 1);
         sm[n] = st[at * st_step], sl[n] = st[at * st_step + 1], sv[n] = st[at * st_step + 2];
-        v[n] = *(const f32x4*)(from + at * step);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[n][k] = *(const f32x4*)(from + at * step + min(d[k], a.dim - 4));
       }
       float next = m, value_next = vm;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        if (i + n >= splits) sm[n] = sv[n] = -kInfinity, sl[n] = 0.0f, v[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int n = 0; n < N; ++n) {
+        if (i + n >= splits) {
+          sm[n] = sv[n] = -kInfinity, sl[n] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[n][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         next = fmaxf(next, sm[n]), value_next = fmaxf(value_next, sv[n]);
       }
       const float ref = next == -kInfinity ? 0.0f : next, value_ref = value_next == -kInfinity ? 0.0f : value_next;
       l *= exp2_fast(m - ref);
-      x *= exp2_fast(vm - value_ref);
+      const float keep = exp2_fast(vm - value_ref);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) {
+      for (int k = 0; k < V; ++k) x[k] *= keep;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
         l = fmaf(sl[n], exp2_fast(sm[n] - ref), l);
         const float factor = exp2_fast(sv[n] - value_ref);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf(v[n][e], factor, x[e]);
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[k][e] = fmaf(v[n][k][e], factor, x[k][e]);
       }
       m = next, vm = value_next;
     }
     const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast((vm == -kInfinity ? 0.0f : vm) - (m == -kInfinity ? 0.0f : m)) : 1.0f) / l;
     bool odd = l == 0.0f && m == -kInfinity;
+    const bool there = mine < end;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] *= inverse;
-      odd |= !(fabsf(x[e]) < kInfinity);
-    }
-    const bool there = mine < end && in * 4 < a.dim;
-    if (there) {
-      if constexpr (sizeof(T) == 4) *(f32x4*)(out + place * a.dim + in * 4) = x;
-      else *(uint2*)(out + place * a.dim + in * 4) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    for (int k = 0; k < V; ++k) {
+      x[k] *= inverse;
+      if (!there || d[k] >= a.dim) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= !(fabsf(x[k][e]) < kInfinity);
+      if constexpr (sizeof(T) == 4) *(f32x4*)(out + place * a.dim + d[k]) = x[k];
+      else *(uint2*)(out + place * a.dim + d[k]) = make_uint2(pack_bf16(x[k][0], x[k][1]), pack_bf16(x[k][2], x[k][3]));
     }
     // rows that came out as no numbers are taken again
     for (uint64_t again = __ballot(there && odd); again;) {
@@ -1329,6 +1354,7 @@ struct Split {
   int chunk;   // tiles of 64 positions that a split has at least
 };
 struct Plan {
+  int few_rows;     // rows of a sequence and key head up to which it is attend_few's, where both run
   bool few16;       // attend_few's sequences have at most 16 rows
   int many_rows;    // rows a block of attend_many
   Split few, many;  // attend_few, attend_many
@@ -1336,25 +1362,29 @@ struct Plan {
   int64_t bytes;
 };
 
-// Rows of queries of a sequence and key head up to which it is attend_few's.
+// Rows of queries of a sequence and key head up to which attend_few takes it, at most.
 constexpr int kFewRows = 64;
 
 // `blocks` blocks before the split, over `positions` positions, towards `wanted`
 // of them.
 Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least, int64_t most) {
   const int64_t tiles = std::max<int64_t>(ceil_div(positions, 64), 1);
-  const int64_t chunk = std::min(std::max(tiles * blocks / wanted, least), most);
+  const int64_t chunk = std::min(std::max(ceil_div(tiles * blocks, wanted), least), most);
   return {(int)std::min<int64_t>(ceil_div(tiles, chunk), 1024), (int)std::min<int64_t>(chunk, INT32_MAX)};
 }
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
              int64_t sinks, int64_t longest, bool by_offsets, bool quantized) {
-  Plan p{true, 128, {0, 1}, {0, 1}, 0, 0, 0, 0};
+  Plan p{0, true, 128, {0, 1}, {0, 1}, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
-  // (mixed batches are single tokens for the most part: 16 rows a unit while a sequence has 24 on average)
-  p.few16 = by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
+  // (16 rows a unit while a sequence has 24 on average)
+  // Where sequences have more than kFewRows rows on average, those with few are single tokens for the most part, and a
+  // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 240 us, 270
+  // with units of 64 rows for all up to 64.
+  p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
+  p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
   // Up to 768 positions a second launch takes longer than it saves (one token at 517: 13.5 us, 15.6 in three splits);
   // splits of 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000: 239 us, 264 by 2,048).
   if (by_offsets || each * group <= kFewRows)
@@ -1366,9 +1396,13 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     const int64_t rows = tokens * group;
     p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= (quantized ? 64 : 768) ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
-    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
+    // Chunks of unlike sequences leave compute units idle behind the longest: splits of 40 tiles at most while there
+    // are few blocks (the mixed batch: 233 us, 245 unsplit).
+    const bool ragged = by_offsets && sequences > 1 && blocks < wanted * 2;
+    if (ragged) p.many = split_of(blocks, seen, wanted, 8, 40);
+    else p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
   }
-  p.few_most = std::min(each * group, (int64_t)kFewRows);
+  p.few_most = std::min(each * group, (int64_t)p.few_rows);
   p.few_partials = sequences * kv_heads * p.few_most;
   p.many_partials = tokens * heads;
   // the one's launches are done with it before the other's begin
@@ -1387,7 +1421,7 @@ int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, in
          hipStream_t st) {
   const int bad = launched(entry);
   if (bad || a.splits == 1) return bad;
-  hipLaunchKernelGGL((attend_join<T, I8, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows))), dim3(256),
+  hipLaunchKernelGGL((attend_join<T, I8, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows<FEW>))), dim3(256),
                      0, st, queries, out, a, rows, tile);
   return launched(entry);
 }
@@ -1440,7 +1474,7 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
     hipLaunchKernelGGL((attend_rows<T, I8>), dim3((unsigned)row_blocks), dim3(kWave), 0, st, queries, out, a);
     return launched(entry);
   }
-  a.few_rows = plan.few.splits == 0 ? 0 : plan.many.splits == 0 ? INT32_MAX : kFewRows;
+  a.few_rows = plan.few.splits == 0 ? 0 : plan.many.splits == 0 ? INT32_MAX : plan.few_rows;
   if (a.dim <= 64) return launch_tiles<T, I8, 64>(entry, queries, out, a, plan, st);
   if (a.dim <= 128) return launch_tiles<T, I8, 128>(entry, queries, out, a, plan, st);
   return launch_tiles<T, I8, 256>(entry, queries, out, a, plan, st);
