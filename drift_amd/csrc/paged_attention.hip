@@ -277,10 +277,16 @@ constexpr float kLift = 14.0f;
 // staged or shuffled, and each of a row's statistics sits in the lanes of its
 // column.
 //
-// Rows of queries are scaled by a power of two each to below 2^15 (exactly; F32
-// rows as two F16 terms, 22 bits), their scores scaled back in F32. In 8 bits the
+// Rows of queries are scaled by a power of two each to below 2^15 (BF16 exactly, down
+// to 2^-32 of the row's largest; F32 as two F16 terms, 22 bits), their scores scaled back in F32. In 8 bits the
 // codes are F16 numbers, a key's scale multiplies its score and a value's is part of
 // its weight, which has a running maximum of its own then.
+//
+// Memory bounds it where there is enough to do: one token of each of 64 sequences of
+// 400 to 8,000 positions, 32 heads over 8 of 128, 248 us (1,249 MB, 5.0 TB/s), in 8 bits
+// 151 us (645 MB; the codes' conversions add to it); one of 517 positions 11 us, a chain
+// of dependent loads. Tiles staged in LDS, as attend_many's, gain nothing here: no other
+// wave reads them.
 template <typename T, bool I8, int DP, int C>
 __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, AttentionArgs a) {
   constexpr int kWaves = 4;
@@ -676,17 +682,23 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // LDS: keys [64][DP], values [DP][64] in F16 (codes are made F16 numbers as they
 // are staged), 16-byte chunks moved by an exclusive or with the row's number so
 // that the rows of one operand lie on different banks; twice, so that a block needs
-// one barrier a tile. The next tile's chunks are in registers meanwhile.
+// one barrier a tile. The next tile comes meanwhile: F16 straight into LDS, 8 bits by
+// registers.
 //
 // The maximum that weights are taken against is raised only when a score passes
 // it by more than kSlack (in powers of two), which keeps the rescaling of the
-// results out of most tiles: weights then reach 2^(kLift + kSlack) at most.
+// results out of most tiles: weights then reach 2^(kManyLift + kSlack) at most.
+//
+// The vector unit bounds it, beside the products it feeds (two waves a SIMD, by
+// registers): BF16, 8,192 tokens of a prompt, 32 heads over 8 of 128, 596 us (550 GFLOP, 922
+// TFLOP/s); heads of 64, 4,096 tokens in windows of 1,024 40 us (426 TFLOP/s: an
+// exponential has half the products); F32, 509 tokens after 3,591, 16 heads over 2 of 256,
+// 96 us with the join (two terms of 32 GFLOP); 1,021 tokens after 2,500 over 8 bits 106 us.
 template <typename T, bool I8, int DP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   constexpr int kThreads = 64 * WAVES;
-  constexpr int CT = 1;                      // tiles of 32 rows a wave
-  constexpr int kRows = WAVES * CT * 32;  // rows a block
+  constexpr int kRows = WAVES * 32;  // rows a block
   constexpr int TOK = 64, KS = DP / 16, DT = DP / 32;
   constexpr int kKeyChunks = DP / 8;         // of a position
   constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
@@ -720,66 +732,55 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   const bool alone = each >= list.count;  // the rows' one split: no others to join
 
   // ---- this wave's rows
-  const int wave_row = wave * CT * 32;
+  const int wave_row = wave * 32;
   const bool idle = wave_row >= rows;
   const uint32_t w0 = start + (row0 + min(wave_row, rows - 1)) / group;
-  const uint32_t w1 = start + (row0 + min(wave_row + CT * 32, rows) - 1) / group;
-  f16x8 query[CT][KS][TERMS];
-  float row_scale[CT];
-  uint32_t position[CT];
+  const uint32_t w1 = start + (row0 + min(wave_row + 32, rows) - 1) / group;
+  f16x8 query[KS][TERMS];
+  const uint32_t row = row0 + min(wave_row + col, rows - 1), token = row / group;
+  const uint32_t position = start + token;
+  const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
+  uint32_t most = 0;
+  float v[KS][8];
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const uint32_t row = row0 + min(wave_row + c * 32 + col, rows - 1), token = row / group;
-    position[c] = start + token;
-    const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
-    uint32_t most = 0;
-    float v[KS][8];
+  for (int k = 0; k < KS; ++k) {
+    const int d = k * 16 + h * 8;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = k * 16 + h * 8;
+    for (int e = 0; e < 8; e += Chunk<T>::N) {
+      float x[Chunk<T>::N];
+      Chunk<T>::unpack(cached_load(q + (d < a.dim ? d + e : e)), x);
 #pragma unroll
-      for (int e = 0; e < 8; e += Chunk<T>::N) {
-        float x[Chunk<T>::N];
-        Chunk<T>::unpack(cached_load(q + (d < a.dim ? d + e : e)), x);
-#pragma unroll
-        for (int i = 0; i < Chunk<T>::N; ++i) v[k][e + i] = d < a.dim ? x[i] : 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[k][e]) & 0x7fffffffu);
+      for (int i = 0; i < Chunk<T>::N; ++i) v[k][e + i] = d < a.dim ? x[i] : 0.0f;
     }
-    most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
-    const bool finite = most < 0x7f800000u;
-    const int shift = finite && most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(most)) : 0;
-    // (above 0, so that the largest score is the largest product: a negative scale turns the query's sign. A scale
-    // of 0, or one that a tiny row makes it, is small enough to leave every weight even)
-    row_scale[c] = finite ? fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -shift), 0x1p-120f) : __builtin_nanf("");
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      float x[8];
+    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[k][e]) & 0x7fffffffu);
+  }
+  most = max(most, (uint32_t)__shfl_xor((int)most, 32, kWave));
+  const bool finite = most < 0x7f800000u;
+  const int shift = finite && most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(most)) : 0;
+  // (above 0, so that the largest score is the largest product: a negative scale turns the query's sign. A scale
+  // of 0, or one that a tiny row makes it, is small enough to leave every weight even)
+  const float row_scale =
+      finite ? fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -shift), 0x1p-120f) : __builtin_nanf("");
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = finite ? ldexpf(v[k][e], shift) : 0.0f;
-        if (a.scale < 0.0f) x[e] = -x[e];
-      }
-      const Halves<TERMS> half = halves_of<TERMS>(x);
+  for (int k = 0; k < KS; ++k) {
+    float x[8];
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) query[c][k][t] = half.term[t];
+    for (int e = 0; e < 8; ++e) {
+      x[e] = finite ? ldexpf(v[k][e], shift) : 0.0f;
+      if (a.scale < 0.0f) x[e] = -x[e];
     }
+    const Halves<TERMS> half = halves_of<TERMS>(x);
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) query[k][t] = half.term[t];
   }
-  f32x16 acc[CT][DT];
-  float row_inverse[CT];
+  f32x16 acc[DT];
+  const float row_inverse = 1.0f / row_scale;
+  float ref = -kInfinity, total = 0.0f;  // what weights are taken against, and their sum so far
 #pragma unroll
-  for (int c = 0; c < CT; ++c) row_inverse[c] = 1.0f / row_scale[c];
-  float ref[CT], total[CT];  // what weights are taken against, and their sum so far
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    ref[c] = -kInfinity;
-    total[c] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[c][d][e] = 0.0f;
-  }
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
 
   // ---- staging: a thread's chunks of a tile
   // Chunk n of a thread is of a unit that its whole wave shares, so that a load is
@@ -1002,24 +1003,20 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
       if (most > value_exponent) {
         const float keep = value_exponent == kNone ? 0.0f : exp2_fast((float)(value_exponent - most));
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[c][d][e] *= keep;
+          for (int e = 0; e < 16; ++e) acc[d][e] *= keep;
         value_exponent = most;
       }
       least_exponent = min(least_exponent, uniform(exponents.y));
       lower = exp2_fast((float)-value_exponent);
     }
-    // scores: score[half][c][e] is row 32 c + col, position base + 32 half + 16 (e / 8) + 8 h + e % 8
-    f32x16 score[2][CT];
+    // scores: score[half][e] is row col, position base + 32 half + 16 (e / 8) + 8 h + e % 8
+    f32x16 score[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) score[half][c][e] = 0.0f;
+      for (int e = 0; e < 16; ++e) score[half][e] = 0.0f;
     {
       // operands four at a time, the next four on their way while these are multiplied
       f16x8 keys[2][4];
@@ -1040,10 +1037,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
         for (int e = 0; e < 4; ++e) {
           const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
 #pragma unroll
-          for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int m = 0; m < TERMS; ++m)
-              score[half][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[n % 2][e], query[c][k][m], score[half][c], 0, 0, 0);
+          for (int m = 0; m < TERMS; ++m)
+            score[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[n % 2][e], query[k][m], score[half], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -1055,87 +1050,69 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 x = *(const float4*)(scales + half * 32 + e / 8 * 16 + e % 8);
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            score[half][c][e] *= x.x, score[half][c][e + 1] *= x.y;
-            score[half][c][e + 2] *= x.z, score[half][c][e + 3] *= x.w;
-          }
+          score[half][e] *= x.x, score[half][e + 1] *= x.y;
+          score[half][e + 2] *= x.z, score[half][e + 3] *= x.w;
         }
     }
     if (!whole) {
       int mine = (int)base + h * 8;
       asm volatile("" : "+v"(mine));  // (or what depends on it alone is kept for every tile)
+      const int last = (int)position, low = a.window ? last - a.window + 1 : INT32_MIN;
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const int last = (int)position[c], low = a.window ? last - a.window + 1 : INT32_MIN;
-#pragma unroll
-        for (int n = 0; n < 32; ++n) {
-          const int j = mine + n / 8 * 16 + n % 8;
-          const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
-          score[n / 16][c][n % 16] = seen ? score[n / 16][c][n % 16] : -kInfinity;
-        }
-        if (okay_then != 15u)
-#pragma unroll
-          for (int n = 0; n < 32; ++n)
-            if (!(okay_then >> (n / 8) & 1)) score[n / 16][c][n % 16] = -kInfinity;
+      for (int n = 0; n < 32; ++n) {
+        const int j = mine + n / 8 * 16 + n % 8;
+        const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
+        score[n / 16][n % 16] = seen ? score[n / 16][n % 16] : -kInfinity;
       }
+      if (okay_then != 15u)
+#pragma unroll
+        for (int n = 0; n < 32; ++n)
+          if (!(okay_then >> (n / 8) & 1)) score[n / 16][n % 16] = -kInfinity;
     }
     __builtin_amdgcn_s_setprio(0);
     // Whether a score passes what weights are taken against by more than kSlack: while that bound is not below 0,
     // the numbers' bits compare as whole numbers do (a NaN among them passes it), which takes half the
     // instructions of a maximum that must quieten NaN. The maximum itself is taken only then, by whole numbers too (a
     // row with a NaN is NaN whatever its weights are taken against).
-    bool raise = false;
+    const float bound = (ref + kSlack) * row_inverse;
+    int most = 0;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const float bound = (ref[c] + kSlack) * row_inverse[c];
-      int most = 0;
+    for (int e = 0; e < 16; ++e)
+      most = max(most, max(__float_as_int(score[0][e]), __float_as_int(score[1][e])));
+    if (__any(!(bound >= 0.0f) || most > __float_as_int(bound))) {
+      // (the bits of numbers as whole numbers in order: those of negative ones turned)
+      auto ordered = [](float x) { const int b = __float_as_int(x); return b ^ (int)((uint32_t)(b >> 31) >> 1); };
+      int top = ordered(score[0][0]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        most = max(most, max(__float_as_int(score[0][c][e]), __float_as_int(score[1][c][e])));
-      raise |= !(bound >= 0.0f) || most > __float_as_int(bound);
+      for (int e = 0; e < 16; ++e) top = max(top, max(ordered(score[0][e]), ordered(score[1][e])));
+      const float high = __int_as_float(top ^ (int)((uint32_t)(top >> 31) >> 1));
+      const float next = fmaxf(ref, fmaxf(high, __shfl_xor(high, 32, kWave)) * row_scale);
+      const float keep = exp2_fast(ref - (next == -kInfinity ? 0.0f : next));
+      ref = next;
+      total *= keep;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] *= keep;
     }
-    if (__any(raise))
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        // (the bits of numbers as whole numbers in order: those of negative ones turned)
-        auto ordered = [](float x) { const int b = __float_as_int(x); return b ^ (int)((uint32_t)(b >> 31) >> 1); };
-        int top = ordered(score[0][c][0]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = max(top, max(ordered(score[0][c][e]), ordered(score[1][c][e])));
-        const float high = __int_as_float(top ^ (int)((uint32_t)(top >> 31) >> 1));
-        const float next = fmaxf(ref[c], fmaxf(high, __shfl_xor(high, 32, kWave)) * row_scale[c]);
-        const float keep = exp2_fast(ref[c] - (next == -kInfinity ? 0.0f : next));
-        ref[c] = next;
-        total[c] *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[c][d][e] *= keep;
-      }
-    float lift[CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) lift[c] = kManyLift - (ref[c] == -kInfinity ? 0.0f : ref[c]);
+    const float lift = kManyLift - (ref == -kInfinity ? 0.0f : ref);
     // 16 positions at a time, the next ones' weights made between the products of these
-    Halves<TERMS> weights[2][CT];
-    auto weigh = [&](int n, Halves<TERMS> (&to)[CT]) {
+    Halves<TERMS> weights[2];
+    auto weigh = [&](int n, Halves<TERMS>& to) {
       float value_scale[I8 ? 8 : 1];
       if constexpr (I8) {
         const float* scales = (const float*)(tile + kScalesAt) + TOK + h * 8 + n * 16;
 #pragma unroll
         for (int e = 0; e < 8; ++e) value_scale[e] = scales[e] * lower;
       }
+      float w[8];
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = exp2_fast(fmaf(score[n / 2][c][n % 2 * 8 + e], row_scale[c], lift[c]));
-          total[c] += p;
-          w[e] = I8 ? p * value_scale[e] : p;
-        }
-        to[c] = halves_of<TERMS>(w);
+      for (int e = 0; e < 8; ++e) {
+        const float p = exp2_fast(fmaf(score[n / 2][n % 2 * 8 + e], row_scale, lift));
+        total += p;
+        w[e] = I8 ? p * value_scale[e] : p;
       }
+      to = halves_of<TERMS>(w);
     };
     f16x8 values[2][DT];
     auto load_values = [&](int n, f16x8 (&to)[DT]) {
@@ -1154,15 +1131,13 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int m = 0; m < TERMS; ++m)
-            acc[c][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[n % 2][d], weights[n % 2][c].term[m], acc[c][d], 0, 0, 0);
+        for (int m = 0; m < TERMS; ++m)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[n % 2][d], weights[n % 2].term[m], acc[d], 0, 0, 0);
       if (n < 3) {
         constexpr int kVector = (I8 ? 48 : 32) + (TERMS == 2 ? 24 : 0);  // about what the weights take
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          __builtin_amdgcn_sched_group_barrier(kProducts, CT * TERMS, 0);
+          __builtin_amdgcn_sched_group_barrier(kProducts, TERMS, 0);
           __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
           __builtin_amdgcn_sched_group_barrier(kVectors, kVector / DT, 0);
         }
@@ -1174,61 +1149,55 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   // scales so far apart that the smaller ones' weights lost bits: the rows are taken again, one by one
   const bool apart = I8 && value_exponent - least_exponent > 16;
   if (value_exponent == kNone) value_exponent = 0;
-  uint64_t again[CT];
+  uint64_t again;
+  const int r = wave_row + col;
+  const bool there = r < rows;
+  const int64_t place = (span.first + token) * a.heads + kv * a.group + (row - token * group);
+  const float sum = total + __shfl_xor(total, 32, kWave);
+  bool odd = apart || (sum == 0.0f && ref == -kInfinity);
+  if (alone) {
+    const float inverse = sum == 0.0f ? 0.0f : (I8 ? exp2_fast((float)value_exponent) : 1.0f) / sum;
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int r = wave_row + c * 32 + col;
-    const bool there = r < rows;
-    const uint32_t row = row0 + min(r, rows - 1), token = row / group;
-    const int64_t place = (span.first + token) * a.heads + kv * a.group + (row - token * group);
-    const float sum = total[c] + __shfl_xor(total[c], 32, kWave);
-    bool odd = apart || (sum == 0.0f && ref[c] == -kInfinity);
-    if (alone) {
-      const float inverse = sum == 0.0f ? 0.0f : (I8 ? exp2_fast((float)value_exponent) : 1.0f) / sum;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int at = d * 32 + 2 * e + 4 * h;
+        float x[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          x[n] = acc[d][e + n] * inverse;
+          odd |= !(fabsf(x[n]) < kInfinity);
+        }
+        if (there && at < a.dim) {
+          if constexpr (TERMS == 2) *(float4*)(out + place * a.dim + at) = make_float4(x[0], x[1], x[2], x[3]);
+          else *(uint2*)(out + place * a.dim + at) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+        }
+      }
+    again = __ballot(odd && there);
+  } else {
+    const int64_t at = (int64_t)split * a.partial_rows + place;
+    if (there) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int at = d * 32 + 2 * e + 4 * h;
-          float x[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            x[n] = acc[c][d][e + n] * inverse;
-            odd |= !(fabsf(x[n]) < kInfinity);
-          }
-          if (there && at < a.dim) {
-            if constexpr (TERMS == 2) *(float4*)(out + place * a.dim + at) = make_float4(x[0], x[1], x[2], x[3]);
-            else *(uint2*)(out + place * a.dim + at) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-          }
-        }
-      again[c] = __ballot(odd && there);
-    } else {
-      const int64_t at = (int64_t)split * a.partial_rows + place;
-      if (there) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (d * 32 + 2 * e + 4 * h < a.dim)
-              *(f32x4*)(a.partials + at * a.dim + d * 32 + 2 * e + 4 * h) =
-                  f32x4{acc[c][d][e], acc[c][d][e + 1], acc[c][d][e + 2], acc[c][d][e + 3]};
-        if (h == 0) {
-          a.statistics[at * 3] = ref[c];
-          a.statistics[at * 3 + 1] = apart ? __builtin_nanf("") : sum;
-          a.statistics[at * 3 + 2] = ref[c] + (float)value_exponent;
-        }
+        for (int e = 0; e < 16; e += 4)
+          if (d * 32 + 2 * e + 4 * h < a.dim)
+            *(f32x4*)(a.partials + at * a.dim + d * 32 + 2 * e + 4 * h) =
+                f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
+      if (h == 0) {
+        a.statistics[at * 3] = ref;
+        a.statistics[at * 3 + 1] = apart ? __builtin_nanf("") : sum;
+        a.statistics[at * 3 + 2] = ref + (float)value_exponent;
       }
-      again[c] = 0;
     }
+    again = 0;
   }
   __syncthreads();  // the tiles are free, and hold the scratch
   RowScratch& scratch = reinterpret_cast<RowScratch*>(tiles)[wave];
-#pragma unroll
-  for (int c = 0; c < CT; ++c)
-    for (uint32_t rest_rows = (uint32_t)again[c] | (uint32_t)(again[c] >> 32); rest_rows; rest_rows &= rest_rows - 1) {
-      const uint32_t row = row0 + wave_row + c * 32 + __ffs(rest_rows) - 1;
-      attend_row<T, I8>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
-    }
+  for (uint32_t rest_rows = (uint32_t)again | (uint32_t)(again >> 32); rest_rows; rest_rows &= rest_rows - 1) {
+    const uint32_t row = row0 + wave_row + __ffs(rest_rows) - 1;
+    attend_row<T, I8>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
+  }
 }
 
 // Joins the splits of attend_few (FEW) or attend_many: a block takes up to
@@ -1312,7 +1281,8 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
       }
       m = next, vm = value_next;
     }
-    const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast((vm == -kInfinity ? 0.0f : vm) - (m == -kInfinity ? 0.0f : m)) : 1.0f) / l;
+    const float apart = (vm == -kInfinity ? 0.0f : vm) - (m == -kInfinity ? 0.0f : m);
+    const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast(apart) : 1.0f) / l;
     bool odd = l == 0.0f && m == -kInfinity;
     const bool there = mine < end;
 #pragma unroll
