@@ -51,6 +51,26 @@ __device__ __forceinline__ float f16_value(uint32_t bits) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
+// A cache's number `at`, and eight from `at` on (a multiple of eight).
+template <bool I8>
+__device__ __forceinline__ float row_one(const void* cache, int64_t at) {
+  if constexpr (I8) return (float)((const int8_t*)cache)[at];
+  else return f16_value(((const uint16_t*)cache)[at]);
+}
+template <bool I8>
+__device__ __forceinline__ void row_eight(const void* cache, int64_t at, float (&v)[8]) {
+  if constexpr (I8) {
+    const uint2 raw = *(const uint2*)((const int8_t*)cache + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)(int8_t)((e < 4 ? raw.x : raw.y) >> (8 * (e % 4)));
+  } else {
+    const uint4 raw = *(const uint4*)((const uint16_t*)cache + at);
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f16_value(word[e / 2] >> (16 * (e % 2)));
+  }
+}
+
 // ------------------------------------------------------------------ rows one by one
 
 // LDS that one wave's attend_row takes.
@@ -60,14 +80,20 @@ struct RowScratch {
   int64_t place[kWave];  // a value's index at dimension 0, or -1: not visible
 };
 
-// One row (a token's query head) by one wave: 64 positions at a time, a lane a
-// position for the scores and then a lane a value for the sums, every product of
-// F32 values in F32 and one by one. It takes any head size and alignment and
-// whatever the cache holds, and is slow: the vector unit and its narrow loads
-// bound it.
-template <typename T, bool I8>
-__device__ __noinline__ void attend_row_of(const T* queries, T* out, const AttentionArgs& a, const Span& span,
-                                           int64_t nth, int h, RowScratch& r) {
+// A row's state over some of its positions: the sums of a lane's values, lane + 64 i.
+struct RowState {
+  float sums[kMaxHead / kWave], top, total;
+  bool any;  // some position is seen
+};
+
+// One row (a token's query head) by one wave over the tiles of 64 positions from,
+// from + step, ..: a lane a position for the scores and then a lane a value for the
+// sums, every product of F32 values in F32 and one by one. It takes any head size and
+// whatever the cache holds. WIDE: keys and values on 16-byte alignment, heads of a
+// multiple of 8 values, read in eights; else one by one, at any alignment.
+template <typename T, bool I8, bool WIDE>
+__device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& a, const Span& span, int64_t nth, int h,
+                                         int from, int step, RowScratch& r, RowState& state) {
   const int lane = threadIdx.x & (kWave - 1), kv = h / a.group;
   const int64_t position = span.start + nth, row = ((span.first + nth) * a.heads + h) * a.dim;
   wave_sync();
@@ -78,9 +104,12 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const Atten
   bool any = false;
   const int64_t low = a.window ? max(position - a.window + 1, (int64_t)0) : 0;
   const int64_t sink_end = a.window ? min((int64_t)a.sinks, low) : 0;
-  for (int64_t base = 0; base <= position; base += kWave) {
-    if (base >= sink_end && base + kWave <= low) base = low / kWave * kWave;  // what lies between is not seen
-    const int64_t j = base + lane;
+  for (int64_t tile = from; tile * kWave <= position; tile += step) {
+    if (tile * kWave >= sink_end && (tile + 1) * kWave <= low) {  // what lies between is not seen
+      tile += (low / kWave - tile + step - 1) / step * step;
+      if (tile * kWave > position) break;
+    }
+    const int64_t j = tile * kWave + lane;
     bool seen = j <= position && (j >= low || j < sink_end);
     int64_t page = 0, off = 0;
     if (seen) {
@@ -95,11 +124,16 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const Atten
     if (seen) {
       const int64_t key = ((page * a.p.page_size + off) * a.kv_heads + kv) * a.dim;
       float dot = 0.0f;
-      for (int d = 0; d < a.dim; ++d) {
-        float k;
-        if constexpr (I8) k = (float)((const int8_t*)a.keys)[key + d];
-        else k = f16_value(((const uint16_t*)a.keys)[key + d]);
-        dot = fmaf(r.query[d], k, dot);
+      if constexpr (WIDE) {
+#pragma unroll 4
+        for (int d = 0; d < a.dim; d += 8) {
+          float k[8];
+          row_eight<I8>(a.keys, key + d, k);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot = fmaf(r.query[d + e], k[e], dot);
+        }
+      } else {
+        for (int d = 0; d < a.dim; ++d) dot = fmaf(r.query[d], row_one<I8>(a.keys, key + d), dot);
       }
       if constexpr (I8) {
         const int64_t at = (page * a.kv_heads + kv) * (int64_t)a.p.page_size + off;
@@ -123,27 +157,61 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const Atten
     r.weight[lane] = p * value_scale;
     r.place[lane] = seen ? (page * a.kv_heads + kv) * (int64_t)a.dim * a.p.page_size + off : -1;
     wave_sync();
+    if constexpr (WIDE) {
+      // eight positions from a multiple of eight on lie together in a value's row
+      const uint64_t which = __ballot(seen);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int d = lane + i * kWave;
-      if (d >= a.dim) break;
-      float acc = sums[i] * keep;
-      for (int n = 0; n < kWave; ++n) {
-        const int64_t at = r.place[n];
-        if (at < 0) continue;
-        float v;
-        if constexpr (I8) v = (float)((const int8_t*)a.values)[at + (int64_t)d * a.p.page_size];
-        else v = f16_value(((const uint16_t*)a.values)[at + (int64_t)d * a.p.page_size]);
-        acc = fmaf(r.weight[n], v, acc);
+      for (int i = 0; i < kEach; ++i) sums[i] *= keep;
+      for (int n = 0; n < kWave; n += 8) {
+        const uint32_t some = (uint32_t)(which >> n) & 255u;
+        if (some == 0) continue;
+        const int first = __ffs(some) - 1;
+        const int64_t at = uniform(r.place[n + first]) - first;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int d = lane + i * kWave;
+          if (d >= a.dim) break;
+          float v[8];
+          row_eight<I8>(a.values, at + (int64_t)d * a.p.page_size, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            sums[i] = some >> e & 1 ? fmaf(r.weight[n + e], v[e], sums[i]) : sums[i];
+        }
       }
-      sums[i] = acc;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int d = lane + i * kWave;
+        if (d >= a.dim) break;
+        float acc = sums[i] * keep;
+        for (int n = 0; n < kWave; ++n) {
+          const int64_t at = r.place[n];
+          if (at < 0) continue;
+          acc = fmaf(r.weight[n], row_one<I8>(a.values, at + (int64_t)d * a.p.page_size), acc);
+        }
+        sums[i] = acc;
+      }
     }
   }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) state.sums[i] = sums[i];
+  state.top = top, state.total = total, state.any = any;
+}
+
+// One row by one wave, for the tile kernels' rows that came out as no numbers: slow,
+// and kept small, since its registers count in every kernel that calls it.
+template <typename T, bool I8>
+__device__ __noinline__ void attend_row_of(const T* queries, T* out, const AttentionArgs& a, const Span& span,
+                                           int64_t nth, int h, RowScratch& r) {
+  RowState state;
+  row_part<T, I8, false>(queries, a, span, nth, h, 0, 1, r, state);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t row = ((span.first + nth) * a.heads + h) * a.dim;
   // nothing seen: zeros; nothing but scores of -infinity seen: 0 / 0, as the formula has it
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
+  for (int i = 0; i < kMaxHead / kWave; ++i) {
     const int d = lane + i * kWave;
-    if (d < a.dim) store_one(out + row + d, any ? sums[i] / total : 0.0f);
+    if (d < a.dim) store_one(out + row + d, state.any ? state.sums[i] / state.total : 0.0f);
   }
 }
 
@@ -157,15 +225,54 @@ __device__ __forceinline__ void attend_row(const T* queries, T* out, const Atten
   attend_row_of<T, I8>(queries, out, args, rows, nth, h, r);
 }
 
-template <typename T, bool I8>
-__global__ void __launch_bounds__(64) attend_rows(const T* queries, T* out, AttentionArgs a) {
-  __shared__ RowScratch scratch;
+// Every row by itself, for what the tile kernels do not take: a block of four waves
+// (one, where the grid would not hold them) a row, each with every fourth tile, joined
+// in LDS. Loads of a position a lane, and a cache read once a query head, bound it:
+// one token of each of 64 sequences at 2,000 positions, 32 heads over 4 of 512 1.63 ms
+// (12.6 with a wave a row, value by value), over 8 of 100 1.12 ms (2.56).
+constexpr int kRowWaves = 4;
+
+template <typename T, bool I8, bool WIDE>
+__global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* queries, T* out, AttentionArgs a) {
+  __shared__ RowScratch scratch[kRowWaves];
+  __shared__ float tops[kRowWaves], totals[kRowWaves];
+  __shared__ int anys[kRowWaves];
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave);
+  const int waves = blockDim.x / kWave;
   int64_t nth;
   const int s = locate(a.p, blockIdx.x / (unsigned)a.heads, 1, 0, 1, nth);
   if (s < 0) return;
   const Span span = span_of(a.p, s);
   if (nth >= span.rows) return;
-  attend_row<T, I8>(queries, out, a, span, nth, blockIdx.x % (unsigned)a.heads, scratch);
+  const int h = blockIdx.x % (unsigned)a.heads;
+  RowState state;
+  row_part<T, I8, WIDE>(queries, a, span, nth, h, wave, waves, scratch[wave], state);
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < kMaxHead / kWave; ++i) scratch[wave].query[lane + i * kWave] = state.sums[i];
+  if (lane == 0) tops[wave] = state.top, totals[wave] = state.total, anys[wave] = state.any;
+  __syncthreads();
+  float top = -kInfinity, total = 0.0f, factor[kRowWaves];
+  bool any = false;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w)
+    if (w < waves) top = fmaxf(top, tops[w]), any |= anys[w] != 0;
+  const float ref = top == -kInfinity ? 0.0f : top;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w)
+    if (w < waves) {
+      factor[w] = expf(tops[w] - ref);
+      total = fmaf(totals[w], factor[w], total);
+    }
+  const int64_t row = ((span.first + nth) * a.heads + h) * a.dim;
+  // nothing seen: zeros; nothing but scores of -infinity seen: 0 / 0, as the formula has it
+  for (int d = threadIdx.x; d < a.dim; d += blockDim.x) {
+    float x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; ++w)
+      if (w < waves) x = fmaf(scratch[w].query[d], factor[w], x);
+    store_one(out + row + d, any ? x / total : 0.0f);
+  }
 }
 
 // ------------------------------------------------------------------ tiles by matrix instructions
@@ -1441,7 +1548,10 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
   const bool small = (int64_t)a.p.page_size * a.kv_heads * a.dim * 2 < (int64_t)1 << 31 &&
                      (int64_t)a.p.cache_pages * a.kv_heads < (int64_t)1 << 31;
   if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
-    hipLaunchKernelGGL((attend_rows<T, I8>), dim3((unsigned)row_blocks), dim3(kWave), 0, st, queries, out, a);
+    const dim3 grid((unsigned)row_blocks), block(kWave * (row_blocks * kRowWaves > kOneWaveBlocks ? 1 : kRowWaves));
+    const bool wide = a.dim % 8 == 0 && aligned16(a.keys) && aligned16(a.values);
+    if (wide) hipLaunchKernelGGL((attend_rows<T, I8, true>), grid, block, 0, st, queries, out, a);
+    else hipLaunchKernelGGL((attend_rows<T, I8, false>), grid, block, 0, st, queries, out, a);
     return launched(entry);
   }
   a.few_rows = plan.few.splits == 0 ? 0 : plan.many.splits == 0 ? INT32_MAX : plan.few_rows;

@@ -693,3 +693,153 @@ def test_two_captured_graphs_at_the_same_time(hip):
             assert torch.equal(out, alone)
             out.zero_()
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ more of what a program may do
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [None, d.AttentionWindow(2700, 4)])
+def test_unlike_sequences_in_splits(hip, kind, dtype, dim, window):
+    step(f"unlike sequences in splits {kind} {dtype} heads of {dim} {window}")
+    # long chunks split in several, short ones written at once; chunks of few rows among the chunks of many
+    case = Case(kind, [5000, 100, 2900, 2600, 0, 640], [40, 1, 30, 5, 3, 1], 2, dim, 16, seed=30)
+    q = normal(31, (case.tokens, 16, dim), TYPES[dtype], 2.0).to(DEV)
+    scale = 1 / math.sqrt(dim)
+    out = run(hip, case, q, scale, window)
+    assert_rows(case, q, scale, out, window, what="unlike sequences")
+    assert torch.equal(out, run(hip, case, q, scale, window))
+
+
+ROW_BY_ROW = [
+    # (start, tokens, heads, kv, dim, page, window, sinks): heads past 256 values, and off eights
+    (1500, 3, 4, 2, 320, 16, 100, 7), (1500, 3, 4, 2, 36, 48, 100, 70), (900, 70, 2, 1, 512, 64, 64, 0),
+    (257, 2, 6, 2, 264, 16, 1, 1), (255, 2, 3, 3, 13, 16, 200, 0), (300, 5, 2, 2, 300, 16, 63, 129),
+]
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,tokens,heads,kv,dim,page,positions,sinks", ROW_BY_ROW)
+def test_windows_of_rows_by_themselves(hip, kind, dtype, start, tokens, heads, kv, dim, page, positions, sinks):
+    step(f"row by row, window {positions} + {sinks} {kind} {dtype} {tokens} at {start}, {heads}/{kv} heads of {dim}")
+    case = Case(kind, [start], [tokens], kv, dim, page, seed=32)
+    q = normal(33, (tokens, heads, dim), TYPES[dtype], 2.0).to(DEV)
+    window, scale = d.AttentionWindow(positions, sinks), 1 / math.sqrt(dim)
+    assert_rows(case, q, scale, run(hip, case, q, scale, window, single=True), window, what="window")
+    assert_rows(case, q, scale, run(hip, case, q, scale, single=True), what="whole")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [320, 36])
+def test_masked_places_of_rows_by_themselves(hip, dtype, dim):
+    step(f"row by row, NaN and infinities in masked places {dtype} heads of {dim}")
+    window = d.AttentionWindow(60, 5)
+    case = Case("f16", [300], [3], 2, dim, 16, seed=34)
+    dense_k, dense_v = case.dense[0]
+    for position, k, v in ((6, float("nan"), float("nan")), (240, float("inf"), float("-inf")), (302, 1.0, float("inf"))):
+        page, off = int(case.tables[0, position // 16]), position % 16
+        case.cache.keys[page, off], case.cache.values[page, :, :, off] = k, v
+        dense_k[position], dense_v[position] = k, v
+    q = normal(35, (3, 4, dim), TYPES[dtype]).to(DEV)
+    assert_rows(case, q, 0.05, run(hip, case, q, 0.05, window, single=True), window, what="masked")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("tokens,dim", [(1, 128), (20, 128), (150, 128), (2, 320)])
+def test_pages_given_back_behind_the_window(hip, kind, tokens, dim):
+    step(f"pages given back behind the window {kind} {tokens} tokens, heads of {dim}")
+    # no row sees a position of them: nothing is read there and nothing flagged
+    case = Case(kind, [400], [tokens], 2, dim, 16, seed=36)
+    window = d.AttentionWindow(90, 5)
+    case.tables[0, 1:(400 - 90) // 16] = -1
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    q = normal(37, (tokens, 4, dim), torch.bfloat16, 2.0).to(DEV)
+    assert_rows(case, q, 0.09, run(hip, case, q, 0.09, window, single=True, bad=bad), window, what="pages given back")
+    assert int(bad.item()) == 0
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,dim", [(1, 128), (90, 128), (2, 300)])
+def test_scales_of_zero_and_below(hip, kind, dtype, tokens, dim):
+    step(f"scales of zero and below {kind} {dtype} {tokens} tokens, heads of {dim}")
+    case = Case(kind, [150], [tokens], 2, dim, 16, seed=38)
+    q = normal(39, (tokens, 4, dim), TYPES[dtype], 2.0).to(DEV)
+    for scale in (-0.1, 0.0):
+        assert_rows(case, q, scale, run(hip, case, q, scale, single=True), what=f"scale {scale}")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_sequences_that_share_pages(hip, kind):
+    step(f"sequences that share pages {kind}")
+    case = Case(kind, [200, 90, 400], [1, 50, 3], 2, 128, 16, seed=40)
+    for s, columns in ((1, 4), (2, 9)):  # the first sequence's pages as the others' prefix
+        case.tables[s, :columns] = case.tables[0, :columns]
+        for mine, first in zip(case.dense[s], case.dense[0]):
+            mine[:columns * 16] = first[:columns * 16]
+        if kind == "i8":
+            case.scales[s][:columns * 16] = case.scales[0][:columns * 16]
+    q = normal(41, (case.tokens, 8, 128), torch.bfloat16, 2.0).to(DEV)
+    assert_rows(case, q, 0.09, run(hip, case, q, 0.09), what="shared pages")
+
+
+@pytest.mark.parametrize("tokens", [1, 90])
+def test_subnormal_keys_and_values(hip, tokens):
+    step(f"subnormal keys and values {tokens}")
+    # numbers below F16's normal ones (2^-14) count as they are
+    case = Case("f16", [100], [tokens], 1, 64, 16, seed=42)
+    case.cache.keys.mul_(2.0 ** -15)
+    case.cache.values.mul_(2.0 ** -15)
+    k, v = (x.half().mul(2.0 ** -15).double() for x in case.dense[0])
+    assert bool((v != 0).float().mean() > 0.9)
+    case.dense[0] = (k, v)
+    q = normal(43, (tokens, 4, 64), torch.float32, 2.0).to(DEV)
+    scale = 2.0 ** 12
+    assert_rows(case, q, scale, run(hip, case, q, scale, single=True), what="subnormal")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_a_cache_past_2_31_values(hip, kind):
+    step(f"a cache past 2^31 values {kind}")
+    # the same rows in the last pages of a large cache and in a small one: the same bits written, read and attended
+    page, kv, dim, starts, rows = 16, 8, 128, [300, 40], [1, 100]
+    small_pages = 32
+    large_pages = (1 << 31) // (page * kv * dim) + small_pages
+
+    def cache(pages):
+        if kind == "i8":
+            return d.QuantizedKvCache.allocate(pages, page, kv, dim, DEV)
+        return d.KvCache(torch.empty((pages, page, kv, dim), dtype=torch.float16, device=DEV),
+                         torch.empty((pages, kv, dim, page), dtype=torch.float16, device=DEV), page)
+
+    lengths = [s + r for s, r in zip(starts, rows)]
+    offsets, all_offsets = np.cumsum([0] + rows), np.cumsum([0] + lengths)
+    tables = np.full((2, 20), -1, np.int32)
+    tables[0, :19], tables[1, :9] = np.arange(19), 19 + np.arange(9)
+    k, v = (normal(s, (int(all_offsets[-1]), kv, dim)).to(DEV) for s in (44, 45))
+    results = []
+    for pages, shift in ((small_pages, 0), (large_pages, large_pages - small_pages)):
+        c, where = cache(pages), dev_i32(np.where(tables >= 0, tables + shift, -1))
+        whole = d.Sequences(where, dev_i32(np.zeros(2)), dev_i32(all_offsets))
+        hip.cacheWriteSequences(k, v, c, whole)
+        rk, rv = torch.empty_like(k), torch.empty_like(v)
+        hip.cacheReadSequences(c, whole, rk, rv)
+        made = [rk, rv]
+        for dtype in (torch.float32, torch.bfloat16):
+            q = normal(46, (sum(rows), 16, dim), dtype, 2.0).to(DEV)
+            out = torch.empty_like(q)
+            hip.attentionSequences(q, c, d.Sequences(where, dev_i32(starts), dev_i32(offsets)), 0.09, out)
+            made.append(out)
+        off = torch.empty(1 + sum(rows) * 16 * dim, device=DEV)[1:].view(sum(rows), 16, dim)  # row by row
+        off.copy_(normal(46, (sum(rows), 16, dim), torch.float32, 2.0))
+        out = torch.empty_like(off)
+        hip.attentionSequences(off, c, d.Sequences(where, dev_i32(starts), dev_i32(offsets)), 0.09, out)
+        made.append(out)
+        results.append([x.cpu() for x in made])
+        del c
+        torch.cuda.empty_cache()
+    for one, other in zip(*results):
+        assert bool(torch.isfinite(one).all())
+        assert torch.equal(one, other)
