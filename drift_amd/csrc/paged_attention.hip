@@ -394,20 +394,26 @@ constexpr float kLift = 14.0f;
 // 151 us (645 MB; the codes' conversions add to it); one of 517 positions 11 us, a chain
 // of dependent loads. Tiles staged in LDS, as attend_many's, gain nothing here: no other
 // wave reads them.
+constexpr int kFewWaves = 4;
+template <int DP, int C>
+struct FewShared {
+  float merged[kFewWaves][16][DP + 4], stats[kFewWaves][C * 16][3];
+};
+
 template <typename T, bool I8, int DP, int C>
-__global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, AttentionArgs a) {
-  constexpr int kWaves = 4;
+__device__ __forceinline__ void few_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
+                                          FewShared<DP, C>& shared) {
+  constexpr int kWaves = kFewWaves;
   constexpr int TOK = I8 ? 64 : 32, NT = TOK / 16;  // positions a tile, and row tiles of its scores
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   constexpr int KS = DP / 32, DT = DP / 16;         // products along a head, value tiles
-  constexpr int kStride = DP + 4;
-  __shared__ float merged[kWaves][16][kStride];
-  __shared__ float stats[kWaves][C * 16][3];
+  auto& merged = shared.merged;
+  auto& stats = shared.stats;
   static_assert(sizeof(RowScratch) <= sizeof(merged) / kWaves, "a wave's part holds a row's scratch");
 
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int kv = blockIdx.x % (unsigned)a.kv_heads;
-  const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
+  const int kv = block % (unsigned)a.kv_heads;
+  const unsigned rest = block / (unsigned)a.kv_heads;
   // A unit's splits lie far apart: blocks go to the eight dies in turn, and where splits are neighbours those that have
   // nothing to do are some dies' alone (64 sequences of 400 to 8,000 over 8 bits 158 us, 168 with neighbours).
   const unsigned all_units = (unsigned)(a.p.sequences * a.few_units);
@@ -778,6 +784,12 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
   }
 }
 
+template <typename T, bool I8, int DP, int C>
+__global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, AttentionArgs a) {
+  __shared__ FewShared<DP, C> shared;
+  few_block<T, I8, DP, C>(queries, out, a, blockIdx.x, shared);
+}
+
 // The many-rows kernel: 32 rows of queries a wave, four or eight waves a block
 // (plan_of says when), positions in tiles of 64 that the block stages in LDS once
 // for all its rows, by 32 x 32 x 16 products. As in attend_few
@@ -801,8 +813,15 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // TFLOP/s); heads of 64, 4,096 tokens in windows of 1,024 40 us (426 TFLOP/s: an
 // exponential has half the products); F32, 509 tokens after 3,591, 16 heads over 2 of 256,
 // 96 us with the join (two terms of 32 GFLOP); 1,021 tokens after 2,500 over 8 bits 106 us.
+template <bool I8, int DP>
+struct ManyTile {
+  static constexpr int kValues = 64 * DP * 2, kScales = 2 * kValues, kExponents = kScales + 2 * 64 * 4;
+  static constexpr int kBytes = I8 ? (kExponents + 16 + 255) / 256 * 256 : kScales;
+};
+
 template <typename T, bool I8, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
+__device__ __forceinline__ void many_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
+                                           unsigned blocks, char (&tiles)[2 * ManyTile<I8, DP>::kBytes]) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   constexpr int kThreads = 64 * WAVES;
   constexpr int kRows = WAVES * 32;  // rows a block
@@ -811,17 +830,17 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
   constexpr int kLoads = TOK * kKeyChunks / kThreads;  // chunks a thread stages, of keys and of values
   // a tile in LDS: its keys, its values, and in 8 bits their scales and the exponents of the values'
-  constexpr int kValuesAt = TOK * DP * 2, kScalesAt = 2 * kValuesAt, kExponentsAt = kScalesAt + 2 * TOK * 4;
-  constexpr int kTileBytes = I8 ? (kExponentsAt + 16 + 255) / 256 * 256 : kScalesAt;
-  __shared__ __attribute__((aligned(16))) char tiles[2 * kTileBytes];
+  using Layout = ManyTile<I8, DP>;
+  constexpr int kValuesAt = Layout::kValues, kScalesAt = Layout::kScales, kExponentsAt = Layout::kExponents;
+  constexpr int kTileBytes = Layout::kBytes;
   static_assert(sizeof(RowScratch) * WAVES <= sizeof(tiles), "");
 
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
-  const int kv = blockIdx.x % (unsigned)a.kv_heads;
-  const unsigned rest = blockIdx.x / (unsigned)a.kv_heads;
+  const int kv = block % (unsigned)a.kv_heads;
+  const unsigned rest = block / (unsigned)a.kv_heads;
   // A unit's splits lie far apart, as in attend_few (a mixed batch of 4 key heads in two splits 182 us, 315 with
   // neighbours: half the dies idle); the last rows first: they have the most positions
-  const unsigned all_units = gridDim.x / (unsigned)(a.kv_heads * a.splits);
+  const unsigned all_units = blocks / (unsigned)(a.kv_heads * a.splits);
   const int split = rest / all_units;
   const int64_t unit = all_units - 1 - rest % all_units;
   int64_t nth;
@@ -1307,6 +1326,27 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
   }
 }
 
+template <typename T, bool I8, int DP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
+  __shared__ __attribute__((aligned(16))) char tiles[2 * ManyTile<I8, DP>::kBytes];
+  many_block<T, I8, DP, WAVES>(queries, out, a, blockIdx.x, gridDim.x, tiles);
+}
+
+// Both in one launch: the chunks' blocks, then the single tokens', whose reads fill the
+// time that the last chunks' products leave. 6 chunks (1,793 tokens) and 18 single tokens
+// over up to 6,000 positions, 28 heads over 4 of 128: 174 us, 172 and 49 in launches of
+// their own. The longest chunk's blocks bound it.
+template <typename T, bool I8, int DP>
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* queries, T* out, AttentionArgs few,
+                                                                     AttentionArgs many, unsigned many_blocks) {
+  constexpr size_t kMany = 2 * ManyTile<I8, DP>::kBytes, kFew = sizeof(FewShared<DP, 1>);
+  __shared__ __attribute__((aligned(16))) char shared[kMany > kFew ? kMany : kFew];
+  if (blockIdx.x < many_blocks)
+    many_block<T, I8, DP, 4>(queries, out, many, blockIdx.x, many_blocks, reinterpret_cast<char (&)[kMany]>(shared));
+  else
+    few_block<T, I8, DP, 1>(queries, out, few, blockIdx.x - many_blocks, reinterpret_cast<FewShared<DP, 1>&>(shared));
+}
+
 // Joins the splits of attend_few (FEW) or attend_many: a block takes up to
 // kJoinRows rows of one unit (`rows` of them, tiles of `tile` positions, which say
 // how many splits it had), a row by as many lanes as hold its values in fours.
@@ -1435,7 +1475,9 @@ struct Plan {
   bool few16;       // attend_few's sequences have at most 16 rows
   int many_rows;    // rows a block of attend_many
   Split few, many;  // attend_few, attend_many
+  bool both;                // in one launch
   int64_t few_most, few_partials, many_partials;  // AttentionArgs::few_most, partial_rows
+  int64_t few_at;  // where attend_few's partials begin
   int64_t bytes;
 };
 
@@ -1452,14 +1494,14 @@ Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least,
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
              int64_t sinks, int64_t longest, bool by_offsets, bool quantized) {
-  Plan p{0, true, 128, {0, 1}, {0, 1}, 0, 0, 0, 0};
+  Plan p{0, true, 128, {0, 1}, {0, 1}, false, 0, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
   // (16 rows a unit while a sequence has 24 on average)
   // Where sequences have more than kFewRows rows on average, those with few are single tokens for the most part, and a
   // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 240 us, 270
-  // with units of 64 rows for all up to 64.
+  // with units of 64 rows for all up to 64 (in launches of their own).
   p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
   p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
   // Up to 768 positions a second launch takes longer than it saves (one token at 517: 13.5 us, 15.6 in three splits);
@@ -1473,18 +1515,16 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     const int64_t rows = tokens * group;
     p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= (quantized ? 64 : 768) ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
-    // Chunks of unlike sequences leave compute units idle behind the longest: splits of 40 tiles at most while there
-    // are few blocks (the mixed batch: 233 us, 245 unsplit).
-    const bool ragged = by_offsets && sequences > 1 && blocks < wanted * 2;
-    if (ragged) p.many = split_of(blocks, seen, wanted, 8, 40);
-    else p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
+    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
   }
   p.few_most = std::min(each * group, (int64_t)p.few_rows);
   p.few_partials = sequences * kv_heads * p.few_most;
   p.many_partials = tokens * heads;
-  // the one's launches are done with it before the other's begin
-  if (p.few.splits > 1) p.bytes = p.few.splits * p.few_partials * (dim + 3) * 4;
-  if (p.many.splits > 1) p.bytes = std::max(p.bytes, p.many.splits * p.many_partials * (dim + 3) * 4);
+  // single tokens' blocks after the chunks' in one launch: the mixed batch 191 us, 239 in two, 213 the other way round
+  p.both = p.few.splits > 0 && p.many.splits > 0 && p.few16 && p.many_rows == 128;
+  if (p.many.splits > 1) p.bytes = p.many.splits * p.many_partials * (dim + 3) * 4;
+  p.few_at = ceil_div(p.bytes, 16) * 4;
+  if (p.few.splits > 1) p.bytes = p.few_at * 4 + p.few.splits * p.few_partials * (dim + 3) * 4;
   return p;
 }
 
@@ -1496,45 +1536,59 @@ constexpr int kManyTiles = DP > 128 ? 1 : DP <= 64 || (sizeof(T) == 2 && !I8) ? 
 template <typename T, bool I8, bool FEW, int DP>
 int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, int64_t units, int rows, int tile,
          hipStream_t st) {
-  const int bad = launched(entry);
-  if (bad || a.splits == 1) return bad;
   hipLaunchKernelGGL((attend_join<T, I8, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows<FEW>))), dim3(256),
                      0, st, queries, out, a, rows, tile);
   return launched(entry);
 }
 
 template <typename T, bool I8, int DP>
-int launch_tiles(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, hipStream_t st) {
+int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArgs& a, const Plan& plan, hipStream_t st) {
+  AttentionArgs few = a, many = a;
+  const int few_tiles = plan.few16 ? 1 : kManyTiles<T, I8, DP>, few_rows = 16 * few_tiles;
+  int64_t few_units = 0, many_units = 0;
   if (plan.few.splits > 0) {
-    a.splits = plan.few.splits;
-    a.chunk = I8 ? plan.few.chunk : plan.few.chunk * 2;
-    constexpr int kMany = kManyTiles<T, I8, DP>;
-    const int rows = 16 * (plan.few16 ? 1 : kMany);
-    a.few_most = (int)plan.few_most;
-    a.few_units = (int)ceil_div(plan.few_most, rows);
-    a.partial_rows = plan.few_partials;
-    a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
-    const int64_t units = (int64_t)a.p.sequences * a.few_units;
-    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(256);
-    if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), grid, block, 0, st, queries, out, a);
-    else hipLaunchKernelGGL((attend_few<T, I8, DP, kMany>), grid, block, 0, st, queries, out, a);
-    if (const int bad = join<T, I8, true, DP>(entry, queries, out, a, units, rows, I8 ? 64 : 32, st)) return bad;
+    few.splits = plan.few.splits;
+    few.chunk = I8 ? plan.few.chunk : plan.few.chunk * 2;
+    few.few_most = (int)plan.few_most;
+    few.few_units = (int)ceil_div(plan.few_most, few_rows);
+    few.partial_rows = plan.few_partials;
+    few.partials = a.partials + plan.few_at;
+    few.statistics = few.partials + few.splits * few.partial_rows * a.dim;
+    few_units = (int64_t)a.p.sequences * few.few_units;
   }
   if (plan.many.splits > 0) {
-    a.splits = plan.many.splits;
-    a.chunk = plan.many.chunk;
-    a.partial_rows = plan.many_partials;
-    a.statistics = a.partials + a.splits * a.partial_rows * a.dim;
-    const int64_t units = units_of(a.p, plan.many_rows, 0, a.group);
-    const dim3 grid((unsigned)(units * a.splits * a.kv_heads)), block(plan.many_rows * 2);
-    if constexpr (DP == 128) {
-      if (plan.many_rows == 256) hipLaunchKernelGGL((attend_many<T, I8, DP, 8>), grid, block, 0, st, queries, out, a);
-      else hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), grid, block, 0, st, queries, out, a);
-    } else {
-      hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), grid, block, 0, st, queries, out, a);
-    }
-    return join<T, I8, false, DP>(entry, queries, out, a, units, plan.many_rows, 64, st);
+    many.splits = plan.many.splits;
+    many.chunk = plan.many.chunk;
+    many.partial_rows = plan.many_partials;
+    many.statistics = many.partials + many.splits * many.partial_rows * a.dim;
+    many_units = units_of(a.p, plan.many_rows, 0, a.group);
   }
+  const unsigned few_blocks = (unsigned)(few_units * few.splits * a.kv_heads);
+  const unsigned many_blocks = (unsigned)(many_units * many.splits * a.kv_heads);
+  const dim3 block(256);
+  if (plan.both) {
+    hipLaunchKernelGGL((attend_both<T, I8, DP>), dim3(many_blocks + few_blocks), block, 0, st, queries, out, few, many,
+                       many_blocks);
+  } else {
+    if (few_blocks > 0) {
+      if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), dim3(few_blocks), block, 0, st, queries, out, few);
+      else hipLaunchKernelGGL((attend_few<T, I8, DP, kManyTiles<T, I8, DP>>), dim3(few_blocks), block, 0, st, queries, out, few);
+    }
+    if (many_blocks > 0) {
+      if constexpr (DP == 128) {
+        if (plan.many_rows == 256)
+          hipLaunchKernelGGL((attend_many<T, I8, DP, 8>), dim3(many_blocks), dim3(512), 0, st, queries, out, many);
+        else hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
+      } else {
+        hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
+      }
+    }
+  }
+  if (const int bad = launched(entry)) return bad;
+  if (few_blocks > 0 && few.splits > 1)
+    if (const int bad = join<T, I8, true, DP>(entry, queries, out, few, few_units, few_rows, I8 ? 64 : 32, st)) return bad;
+  if (many_blocks > 0 && many.splits > 1)
+    return join<T, I8, false, DP>(entry, queries, out, many, many_units, plan.many_rows, 64, st);
   return 0;
 }
 
@@ -1542,8 +1596,8 @@ template <typename T, bool I8>
 int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, bool aligned, hipStream_t st) {
   const int64_t row_blocks = units_of(a.p, 1, 0, 1) * a.heads;
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
-  const int64_t blocks = std::max((int64_t)a.p.sequences * 4 * std::max(plan.few.splits, 4),
-                                  units_of(a.p, 128, 0, a.group) * std::max(plan.many.splits, 16)) * a.kv_heads;
+  const int64_t blocks = ((int64_t)a.p.sequences * 4 * std::max(plan.few.splits, 4) +
+                          units_of(a.p, 128, 0, a.group) * std::max(plan.many.splits, 16)) * a.kv_heads;
   // (the tile kernels' offsets within a page, and rows of scales, have 32 bits)
   const bool small = (int64_t)a.p.page_size * a.kv_heads * a.dim * 2 < (int64_t)1 << 31 &&
                      (int64_t)a.p.cache_pages * a.kv_heads < (int64_t)1 << 31;

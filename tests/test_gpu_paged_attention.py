@@ -699,7 +699,7 @@ def test_two_captured_graphs_at_the_same_time(hip):
 
 @pytest.mark.parametrize("kind", CACHES)
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("window", [None, d.AttentionWindow(2700, 4)])
 def test_unlike_sequences_in_splits(hip, kind, dtype, dim, window):
     step(f"unlike sequences in splits {kind} {dtype} heads of {dim} {window}")
