@@ -390,8 +390,8 @@ constexpr float kLift = 14.0f;
 // its weight, which has a running maximum of its own then.
 //
 // Memory bounds it where there is enough to do: one token of each of 64 sequences of
-// 400 to 8,000 positions, 32 heads over 8 of 128, 248 us (1,249 MB, 5.0 TB/s), in 8 bits
-// 151 us (645 MB; the codes' conversions add to it); one of 517 positions 11 us, a chain
+// 400 to 8,000 positions, 32 heads over 8 of 128, 246 us (1,249 MB, 5.1 TB/s), in 8 bits
+// 150 us (645 MB; the codes' conversions add to it); one of 517 positions 11 us, a chain
 // of dependent loads. Tiles staged in LDS, as attend_many's, gain nothing here: no other
 // wave reads them.
 constexpr int kFewWaves = 4;
@@ -809,10 +809,10 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // results out of most tiles: weights then reach 2^(kManyLift + kSlack) at most.
 //
 // The vector unit bounds it, beside the products it feeds (two waves a SIMD, by
-// registers): BF16, 8,192 tokens of a prompt, 32 heads over 8 of 128, 596 us (550 GFLOP, 922
-// TFLOP/s); heads of 64, 4,096 tokens in windows of 1,024 40 us (426 TFLOP/s: an
+// registers): BF16, 8,192 tokens of a prompt, 32 heads over 8 of 128, 599 us (550 GFLOP, 918
+// TFLOP/s); heads of 64, 4,096 tokens in windows of 1,024 41 us (420 TFLOP/s: an
 // exponential has half the products); F32, 509 tokens after 3,591, 16 heads over 2 of 256,
-// 96 us with the join (two terms of 32 GFLOP); 1,021 tokens after 2,500 over 8 bits 106 us.
+// 99 us with the join (two terms of 32 GFLOP); 1,021 tokens after 2,500 over 8 bits 104 us.
 template <bool I8, int DP>
 struct ManyTile {
   static constexpr int kValues = 64 * DP * 2, kScales = 2 * kValues, kExponents = kScales + 2 * 64 * 4;
