@@ -388,9 +388,9 @@ int drift_paged_read_bf16(uint16_t* k, uint16_t* v, const void* keys, const void
  * see has no part in it, whatever it holds; positions on a page outside the
  * cache are not seen, and *bad_page = 1. A row that sees nothing is zeros.
  * head_dim is at most 512.
- * `longest` is the caller's guess of the longest sequence's positions (at most
- * the page table's; 0: the page table's): the work is split by it, and any guess
- * gives the same result within rounding. `workspace` (device, 16-byte aligned)
+ * `longest` is the caller's guess of the longest sequence's positions (the page
+ * table's room, where nothing better is known; 0: the work is not split): the work
+ * is split by it, and any guess gives the same result within rounding. `workspace` (device, 16-byte aligned)
  * has at least the bytes that drift_paged_attention_workspace tells for the same
  * numbers (0: it may be NULL); the launches write it before they read it, so it
  * may hold anything before, and calls that may run at the same time need one

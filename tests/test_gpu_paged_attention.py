@@ -843,3 +843,24 @@ def test_a_cache_past_2_31_values(hip, kind):
     for one, other in zip(*results):
         assert bool(torch.isfinite(one).all())
         assert torch.equal(one, other)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 264])
+@pytest.mark.parametrize("what", ["keys", "values"])
+def test_rows_that_see_a_quantised_nan(hip, dtype, dim, what):
+    step(f"rows that see a quantised NaN {dtype} heads of {dim} {what}")
+    # a row written with a NaN or an infinity reads as NaN throughout, and so do the rows that see it; no others
+    case = Case("i8", [60], [30], 2, dim, 16, seed=47)
+    k, v = normal(48, (1, 2, dim)), normal(49, (1, 2, dim))
+    (k if what == "keys" else v)[0, 1, 3] = float("inf")
+    hip.cacheWrite(k.to(DEV), v.to(DEV), case.cache, dev_i32(case.tables[0]), 70)
+    for mine, x in zip(case.dense[0], (k, v)):
+        codes, scales = quantised(x)
+        mine[70] = (codes.double() * scales.double()[..., None])[0]
+    case.scales[0][70] = quantised(v)[1][0].double().nan_to_num(0)
+    q = normal(50, (30, 4, dim), TYPES[dtype], 2.0).to(DEV)
+    out = run(hip, case, q, 0.09, single=True)
+    assert_rows(case, q, 0.09, out, what="a quantised NaN")
+    assert bool(torch.isnan(out[10:, 2:]).all()) and bool(torch.isfinite(out[:10]).all())
+    assert bool(torch.isfinite(out[:, :2]).all())
