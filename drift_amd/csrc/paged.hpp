@@ -11,6 +11,8 @@
 
 #include "common.hpp"
 
+#include <algorithm>
+
 namespace drift {
 
 // Several sequences' token rows, packed: sequence s has rows offsets[s] up to
@@ -78,10 +80,11 @@ __device__ __forceinline__ Span span_of(const Paging& p, int s) {
 }
 
 // Work in units of `per` items, a row having `scale` of them: ceil(rows scale /
-// per) + extra units a sequence. The sequence that unit `unit` of the launch
+// per) + extra units a sequence, by offsets none where there are `least` items or fewer. The sequence that unit `unit` of the launch
 // belongs to (-1: none), and which of its units it is. Whole waves call, every
 // lane with the same unit.
-__device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, int extra, int64_t scale, int64_t& nth) {
+__device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, int extra, int64_t scale, int64_t& nth,
+                                          int64_t least = 0) {
   if (!p.offsets) {
     if (p.sequences == 1) {
       nth = unit;
@@ -100,7 +103,7 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
       const int64_t from = p.offsets[s], to = p.offsets[s + 1];
       const bool good = from >= 0 && to >= from && to <= p.tokens;
       if (!good) flag_bad(p);  // and no units, so that the others' are all in the launch
-      units = good && to > from ? ((to - from) * scale + per - 1) / per + extra : 0;
+      units = good && (to - from) * scale > least ? ((to - from) * scale + per - 1) / per + extra : 0;
     }
     int64_t end = units;  // units of this group of sequences, up to and with this lane's
 #pragma unroll
@@ -121,9 +124,13 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
 
 // ---------------------------------------------------------------- host side
 
-// Units a launch needs for every sequence's (locate), whatever the offsets hold.
-inline int64_t units_of(const Paging& p, int64_t per, int64_t extra, int64_t scale) {
-  if (p.offsets) return (int64_t)p.tokens * scale / per + p.sequences * (1 + extra);
+// Units a launch needs for every sequence's (locate), whatever the offsets hold: a part of one is left over in as
+// many sequences as can have more than `least` items.
+inline int64_t units_of(const Paging& p, int64_t per, int64_t extra, int64_t scale, int64_t least = 0) {
+  if (p.offsets) {
+    const int64_t items = (int64_t)p.tokens * scale;
+    return items / per + std::min((int64_t)p.sequences, items / (least + 1)) * (1 + extra);
+  }
   if (p.sequences == 1) return ceil_div((int64_t)p.tokens * scale, per) + extra;
   return p.sequences * (ceil_div(scale, per) + extra);
 }

@@ -419,7 +419,9 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   const unsigned all_units = (unsigned)(a.p.sequences * a.few_units);
   const int split = rest / all_units;
   const unsigned unit = rest % all_units;
-  const int s = (int)(unit / (unsigned)a.few_units), nth = (int)(unit % (unsigned)a.few_units);
+  // (and its later units, of which most sequences have none: 64 single tokens in 4 units each, given by offsets, 235 us,
+  // 414 with a sequence's units as neighbours, whose first are all dealt to the same quarter of a die)
+  const int s = (int)(unit % (unsigned)a.p.sequences), nth = (int)(unit / (unsigned)a.p.sequences);
   const Span span = span_of(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
   if (rows <= 0 || (int64_t)span.rows * a.group > a.few_rows) return;
@@ -844,7 +846,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   const int split = rest / all_units;
   const int64_t unit = all_units - 1 - rest % all_units;
   int64_t nth;
-  const int s = locate(a.p, unit, kRows, 0, a.group, nth);
+  const int s = locate(a.p, unit, kRows, 0, a.group, nth, a.few_rows);
   if (s < 0) return;
   const Span span = span_of(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * kRows, (int64_t)kRows);
@@ -1366,8 +1368,8 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
   const unsigned unit = blockIdx.x / (unsigned)a.kv_heads / (unsigned)parts;
   int s;
   int64_t nth;
-  if constexpr (FEW) s = (int)(unit / (unsigned)a.few_units), nth = unit % (unsigned)a.few_units;
-  else s = locate(a.p, unit, rows, 0, a.group, nth);
+  if constexpr (FEW) s = (int)(unit % (unsigned)a.p.sequences), nth = unit / (unsigned)a.p.sequences;
+  else s = locate(a.p, unit, rows, 0, a.group, nth, a.few_rows);
   if (s < 0) return;
   const Span span = span_of(a.p, s);
   const uint32_t all = (uint32_t)span.rows * (uint32_t)a.group, group = (uint32_t)a.group;
@@ -1561,7 +1563,7 @@ int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArg
     many.chunk = plan.many.chunk;
     many.partial_rows = plan.many_partials;
     many.statistics = many.partials + many.splits * many.partial_rows * a.dim;
-    many_units = units_of(a.p, plan.many_rows, 0, a.group);
+    many_units = units_of(a.p, plan.many_rows, 0, a.group, a.few_rows);
   }
   const unsigned few_blocks = (unsigned)(few_units * few.splits * a.kv_heads);
   const unsigned many_blocks = (unsigned)(many_units * many.splits * a.kv_heads);
