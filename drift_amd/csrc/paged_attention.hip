@@ -1500,12 +1500,13 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
-  // (16 rows a unit while a sequence has 24 on average)
+  // (16 rows a unit while a sequence has no more on average: 64 sequences of 24 rows at 4,000 positions 307 us in
+  // units of 64, 413 in two of 16 each)
   // Where sequences have more than kFewRows rows on average, those with few are single tokens for the most part, and a
   // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 240 us, 270
   // with units of 64 rows for all up to 64 (in launches of their own).
   p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
-  p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 24 : each * group <= 16;
+  p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 16 : each * group <= 16;
   // Up to 768 positions a second launch takes longer than it saves (one token at 517: 13.5 us, 15.6 in three splits);
   // splits of 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000: 239 us, 264 by 2,048).
   if (by_offsets || each * group <= kFewRows)
