@@ -1640,7 +1640,8 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,
                   (long long)plan.bytes);
   a.partials = (float*)workspace;
-  const bool aligned = a.dim % 8 == 0 && aligned16(queries) && aligned16(a.keys) && aligned16(a.values) &&
+  // (the tile kernels load the one and store the other 8 or 16 bytes at a time)
+  const bool aligned = a.dim % 8 == 0 && aligned16(queries) && aligned16(out) && aligned16(a.keys) && aligned16(a.values) &&
                        (!a.key_scales || (aligned16(a.key_scales) && aligned16(a.value_scales)));
   const hipStream_t st = (hipStream_t)stream;
   return a.key_scales ? attend<T, true>(entry, queries, out, a, plan, aligned, st)

@@ -864,3 +864,29 @@ def test_rows_that_see_a_quantised_nan(hip, dtype, dim, what):
     assert_rows(case, q, 0.09, out, what="a quantised NaN")
     assert bool(torch.isnan(out[10:, 2:]).all()) and bool(torch.isfinite(out[:10]).all())
     assert bool(torch.isfinite(out[:, :2]).all())
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("off", ["out", "queries"])
+@pytest.mark.parametrize("start,tokens,heads", [
+    (90, 1, 4),      # few rows
+    (3000, 24, 4),   # few rows, in splits that are joined
+    (90, 200, 4),    # many rows
+    (3000, 90, 16),  # many rows, in splits that are joined
+])
+def test_queries_or_out_alone_off_16_bytes(hip, kind, dtype, off, start, tokens, heads):
+    step(f"{off} alone off 16 bytes {kind} {dtype} {tokens} tokens at {start}")
+    case = Case(kind, [start], [tokens], 2, 128, 16, seed=51)
+    t = TYPES[dtype]
+    q = normal(52, (tokens, heads, 128), t, 2.0).to(DEV)
+
+    def shifted():  # one value past a multiple of 16 bytes, a value to spare at either end
+        flat = torch.full((q.numel() + 2,), 7.0, dtype=t, device=DEV)
+        return flat, flat[1:-1].view(q.shape)
+
+    flat, moved = shifted()
+    queries, out = (q, moved) if off == "out" else (moved.copy_(q), torch.full_like(q, 7.0))
+    hip.attention(queries, case.cache, dev_i32(case.tables[0]), start, 0.09, out)
+    assert_rows(case, q, 0.09, out, what=f"{off} off 16 bytes")
+    assert float(flat[0]) == 7 and float(flat[-1]) == 7
