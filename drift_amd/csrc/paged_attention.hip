@@ -30,11 +30,12 @@ struct AttentionArgs {
   const float *key_scales, *value_scales;
   // the split over positions: at least `chunk` tiles a split, `splits` of them;
   // where there are several, their maxima and sums [splits, partial_rows, 3] and
-  // unscaled results [splits, partial_rows, dim]
+  // unscaled results [splits, partial_rows, dim], a row by its place among the
+  // call's rows [tokens, heads] or (attend_few's, few_slots) by few_partial
   int32_t splits, chunk;
   int64_t partial_rows;
   float *statistics, *partials;
-  int32_t few_most, few_units;  // attend_few's rows at most, and units, of a sequence and key head
+  int32_t few_slots, few_units;  // attend_few's rows of partials (0: by place), and units, of a sequence and key head
   int32_t few_rows;   // sequences of at most so many rows (tokens times group) are attend_few's, others attend_many's
   // page_size / 16, and what divides a unit's number (below 2^27) by it exactly
   uint32_t page_units, page_magic, page_shift;
@@ -49,6 +50,11 @@ __device__ __forceinline__ uint32_t column_of(const AttentionArgs& a, uint32_t u
 
 __device__ __forceinline__ float f16_value(uint32_t bits) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
+
+// Where attend_few's row `row` of a sequence and key head, at `place` among the call's, keeps its partials.
+__device__ __forceinline__ int64_t few_partial(const AttentionArgs& a, int s, int kv, uint32_t row, int64_t place) {
+  return a.few_slots ? ((int64_t)s * a.kv_heads + kv) * a.few_slots + row : place;
 }
 
 // A cache's number `at`, and eight from `at` on (a multiple of eight).
@@ -752,7 +758,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
       const uint32_t row = row0 + c * 16 + r, token = row / group;
       const int h = kv * a.group + (int)(row - token * group);
       const int64_t place = (span.first + token) * a.heads + h;
-      const int64_t partial = ((int64_t)s * a.kv_heads + kv) * a.few_most + row;
+      const int64_t partial = few_partial(a, s, kv, row, place);
       const float inverse = l == 0.0f ? 0.0f : (I8 ? exp2_fast(value_ref - ref) : 1.0f) / l;
       bool odd = false;
       for (int d = lane; d < a.dim; d += kWave) {
@@ -1383,7 +1389,7 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
     const uint32_t mine = first + lane / L, row = min(mine, end - 1), token = row / group;
     const int h = kv * a.group + (int)(row - token * group);
     const int64_t place = (span.first + token) * a.heads + h;
-    const int64_t partial = FEW ? ((int64_t)s * a.kv_heads + kv) * a.few_most + row : place;
+    const int64_t partial = FEW ? few_partial(a, s, kv, row, place) : place;
     const float* st = a.statistics + partial * 3;
     const float* from = a.partials + partial * a.dim;
     const int64_t st_step = a.partial_rows * 3, step = a.partial_rows * a.dim;
@@ -1478,25 +1484,33 @@ struct Plan {
   int many_rows;    // rows a block of attend_many
   Split few, many;  // attend_few, attend_many
   bool both;                // in one launch
-  int64_t few_most, few_partials, many_partials;  // AttentionArgs::few_most, partial_rows
-  int64_t few_at;  // where attend_few's partials begin
+  int64_t few_most;                               // rows of a sequence and key head that attend_few may have
+  int64_t few_slots, few_partials, many_partials;  // AttentionArgs::few_slots, partial_rows
+  // floats of the workspace before attend_few's partials, and before either's statistics
+  int64_t few_at, few_statistics, many_statistics;
   int64_t bytes;
 };
 
 // Rows of queries of a sequence and key head up to which attend_few takes it, at most.
 constexpr int kFewRows = 64;
 
+// Blocks with their splits, at most, where sequences are split evenly whatever the chip
+// has room for: 32 times 512 places even out any lengths, and what the splits leave in
+// the workspace stays within so many blocks' rows however wide the page tables are.
+constexpr int64_t kSplitBlocks = 16384;
+
 // `blocks` blocks before the split, over `positions` positions, towards `wanted`
 // of them.
 Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least, int64_t most) {
   const int64_t tiles = std::max<int64_t>(ceil_div(positions, 64), 1);
   const int64_t chunk = std::min(std::max(ceil_div(tiles * blocks, wanted), least), most);
-  return {(int)std::min<int64_t>(ceil_div(tiles, chunk), 1024), (int)std::min<int64_t>(chunk, INT32_MAX)};
+  const int64_t splits = std::min(ceil_div(tiles, chunk), std::min<int64_t>(std::max<int64_t>(kSplitBlocks / blocks, 1), 1024));
+  return {(int)splits, (int)std::min<int64_t>(chunk, INT32_MAX)};
 }
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
              int64_t sinks, int64_t longest, bool by_offsets, bool quantized) {
-  Plan p{0, true, 128, {0, 1}, {0, 1}, false, 0, 0, 0, 0, 0};
+  Plan p{0, true, 128, {0, 1}, {0, 1}, false, 0, 0, 0, 0, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
@@ -1518,16 +1532,24 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     const int64_t rows = tokens * group;
     p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= (quantized ? 64 : 768) ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
-    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 20);
+    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 25);
   }
   p.few_most = std::min(each * group, (int64_t)p.few_rows);
-  p.few_partials = sequences * kv_heads * p.few_most;
-  p.many_partials = tokens * heads;
   // single tokens' blocks after the chunks' in one launch: the mixed batch 191 us, 239 in two, 213 the other way round
   p.both = p.few.splits > 0 && p.many.splits > 0 && p.few16 && p.many_rows == 128;
-  if (p.many.splits > 1) p.bytes = p.many.splits * p.many_partials * (dim + 3) * 4;
-  p.few_at = ceil_div(p.bytes, 16) * 4;
-  if (p.few.splits > 1) p.bytes = p.few_at * 4 + p.few.splits * p.few_partials * (dim + 3) * 4;
+  // Partials by a row's place suit both kernels at once, since a row is one kernel's: attend_few has slots of its own
+  // only where those are fewer (a few sequences' few rows beside long chunks).
+  const int64_t rows = tokens * heads, slots = sequences * kv_heads * p.few_most;
+  p.few_slots = slots < rows ? p.few_most : 0;
+  p.few_partials = std::min(slots, rows);
+  p.many_partials = rows;
+  const int64_t few = p.few.splits > 1 ? p.few.splits * p.few_partials : 0;
+  const int64_t many = p.many.splits > 1 ? p.many.splits * p.many_partials : 0;
+  const int64_t by_place = p.few_slots ? many : std::max(few, many), by_slot = p.few_slots ? few : 0;
+  p.many_statistics = by_place * dim;
+  p.few_at = p.few_slots ? ceil_div(by_place * (dim + 3), 4) * 4 : 0;
+  p.few_statistics = p.few_at + (p.few_slots ? by_slot : by_place) * dim;
+  p.bytes = (p.few_slots ? p.few_at + by_slot * (dim + 3) : by_place * (dim + 3)) * 4;
   return p;
 }
 
@@ -1552,18 +1574,18 @@ int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArg
   if (plan.few.splits > 0) {
     few.splits = plan.few.splits;
     few.chunk = I8 ? plan.few.chunk : plan.few.chunk * 2;
-    few.few_most = (int)plan.few_most;
+    few.few_slots = (int)plan.few_slots;
     few.few_units = (int)ceil_div(plan.few_most, few_rows);
     few.partial_rows = plan.few_partials;
     few.partials = a.partials + plan.few_at;
-    few.statistics = few.partials + few.splits * few.partial_rows * a.dim;
+    few.statistics = a.partials + plan.few_statistics;
     few_units = (int64_t)a.p.sequences * few.few_units;
   }
   if (plan.many.splits > 0) {
     many.splits = plan.many.splits;
     many.chunk = plan.many.chunk;
     many.partial_rows = plan.many_partials;
-    many.statistics = many.partials + many.splits * many.partial_rows * a.dim;
+    many.statistics = a.partials + plan.many_statistics;
     many_units = units_of(a.p, plan.many_rows, 0, a.group, a.few_rows);
   }
   const unsigned few_blocks = (unsigned)(few_units * few.splits * a.kv_heads);

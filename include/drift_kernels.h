@@ -392,9 +392,11 @@ int drift_paged_read_bf16(uint16_t* k, uint16_t* v, const void* keys, const void
  * table's room, where nothing better is known; 0: the work is not split): the work
  * is split by it, and any guess gives the same result within rounding. `workspace` (device, 16-byte aligned)
  * has at least the bytes that drift_paged_attention_workspace tells for the same
- * numbers (0: it may be NULL); the launches write it before they read it, so it
- * may hold anything before, and calls that may run at the same time need one
- * each. The same call gives the same bits every time.
+ * numbers (0: it may be NULL): for a decode step splits * tokens * heads *
+ * (head_dim + 3) * 4, with no more splits than leave 16,384 blocks of a sequence,
+ * key head and split (64 sequences, 32 heads over 8 of 128: at most 34 MB, however
+ * wide the page tables are). The launches write it before they read it, so it may hold
+ * anything before, and calls that may run at the same time need one each. The same call gives the same bits every time.
  * The reference's attention (kernels/attention.hip:7-34,227-229,446-456) is one
  * sequence's, without a window. */
 int drift_paged_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,

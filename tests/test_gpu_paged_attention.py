@@ -890,3 +890,34 @@ def test_queries_or_out_alone_off_16_bytes(hip, kind, dtype, off, start, tokens,
     hip.attention(queries, case.cache, dev_i32(case.tables[0]), start, 0.09, out)
     assert_rows(case, q, 0.09, out, what=f"{off} off 16 bytes")
     assert float(flat[0]) == 7 and float(flat[-1]) == 7
+
+
+def repeated(case, times):
+    """The case's one sequence `times` over, on the same pages."""
+    case.starts, case.rows = np.tile(case.starts, times), np.tile(case.rows, times)
+    case.tables = np.tile(case.tables, (times, 1))
+    case.tokens, case.offsets = case.tokens * times, np.concatenate([[0], np.cumsum(case.rows)])
+    case.dense, case.scales = case.dense * times, case.scales * times
+    return case
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("sequences,offsets", [(340, False), (340, True), (1100, False)])
+def test_more_sequences_than_their_splits_have_blocks(hip, kind, sequences, offsets):
+    step(f"{sequences} sequences of 4,001 positions {kind} offsets {offsets}")
+    # three splits each, or one, where 4,001 positions alone would take four
+    case = repeated(Case(kind, [4000], [1], 16, 16, 16, seed=53), sequences)
+    q = normal(54, (sequences, 16, 16), torch.float32, 2.0).to(DEV)
+    assert_rows(case, q, 0.25, run(hip, case, q, 0.25, offsets=offsets), what="many sequences")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_and_many_rows_partials_by_place(hip, kind, dtype):
+    step(f"a chunk and single tokens in splits, partials by place {kind} {dtype}")
+    # the chunk's rows and the single tokens', both in splits, share one range of partials
+    case = Case(kind, [3000, 2500, 20, 4000, 1800, 900], [20, 1, 1, 1, 1, 1], 2, 128, 16, seed=55)
+    q = normal(56, (case.tokens, 16, 128), TYPES[dtype], 2.0).to(DEV)
+    out = run(hip, case, q, 0.09)
+    assert_rows(case, q, 0.09, out, what="by place")
+    assert torch.equal(out, run(hip, case, q, 0.09))

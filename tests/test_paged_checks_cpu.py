@@ -249,3 +249,27 @@ def test_the_workspace_is_told():
                     (0, 5, 8, 2, 64, 0, 0, 5), (3, 2 ** 20, 64, 8, 256, 0, 0, 2 ** 20)):
         code, size = workspace(*numbers)
         assert code == "code 0" and 0 <= size < 1 << 40
+
+
+@pytest.mark.parametrize("sequences", [1, 17, 64, 256])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (28, 4, 128), (16, 2, 256), (16, 16, 64)])
+def test_a_decode_steps_workspace_is_its_rows_splits(sequences, heads, kv_heads, dim):
+    """One token a sequence, by offsets or without: `splits` partial results
+    and statistics of each row there is, and no more splits than leave 16,384
+    blocks of a sequence, key head and split, however wide the page tables."""
+    sizes = []
+    for longest in (100, 8016, 32768, 131072, 2 ** 20, 2 ** 31 - 128):
+        code, size = workspace(sequences, sequences, heads, kv_heads, dim, 0, 0, longest)
+        assert code == "code 0"
+        splits = min(1024, max(1, 16384 // (sequences * kv_heads)), -(-longest // 256))
+        # (by offsets the rows may be one sequence's, of attend_many: its splits leave up to 512 blocks of 128 rows)
+        splits = max(splits, min(-(-longest // 512), -(-512 * 128 // (sequences * heads))))
+        assert size <= splits * sequences * heads * (dim + 3) * 4
+        sizes.append(size)
+    assert sizes == sorted(sizes)
+
+
+def test_a_mixed_batchs_workspace_has_slots_for_few_rows():
+    # 24 sequences, 1,811 tokens of 28 heads over 4: up to 16 rows of each sequence and key head may be split
+    code, size = workspace(24, 1811, 28, 4, 128, 0, 0, 131072)
+    assert code == "code 0" and 0 < size <= 170 * 24 * 4 * 16 * 131 * 4
