@@ -824,7 +824,8 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 template <bool I8, int DP>
 struct ManyTile {
   static constexpr int kValues = 64 * DP * 2, kScales = 2 * kValues, kExponents = kScales + 2 * 64 * 4;
-  static constexpr int kBytes = I8 ? (kExponents + 16 + 255) / 256 * 256 : kScales;
+  static constexpr int kRange = kExponents + 64 * 4;
+  static constexpr int kBytes = I8 ? (kRange + 16 + 255) / 256 * 256 : kScales;
 };
 
 template <typename T, bool I8, int DP, int WAVES>
@@ -837,9 +838,11 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   constexpr int kKeyChunks = DP / 8;         // of a position
   constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
   constexpr int kLoads = TOK * kKeyChunks / kThreads;  // chunks a thread stages, of keys and of values
-  // a tile in LDS: its keys, its values, and in 8 bits their scales and the exponents of the values'
+  // a tile in LDS: its keys, its values, and in 8 bits their scales, the exponents of the values' (-infinity: no scale
+  // above 0) and the most and the least of them
   using Layout = ManyTile<I8, DP>;
   constexpr int kValuesAt = Layout::kValues, kScalesAt = Layout::kScales, kExponentsAt = Layout::kExponents;
+  constexpr int kRangeAt = Layout::kRange;
   constexpr int kTileBytes = Layout::kBytes;
   static_assert(sizeof(RowScratch) * WAVES <= sizeof(tiles), "");
 
@@ -1071,16 +1074,24 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
       scales[TOK + lane] = x;
       const bool counts = x > 0.0f && x < kInfinity;
       const float exponent = (float)__builtin_amdgcn_frexp_expf(x);
+      ((float*)(tile + kExponentsAt))[lane] = counts ? exponent : -kInfinity;
       const float most = group_max<64>(counts ? exponent : (float)kNone);
       const float least = -group_max<64>(counts ? -exponent : (float)kNone);
-      if (lane == 0) *(int2*)(tile + kExponentsAt) = make_int2((int)most, (int)least);
+      if (lane == 0) *(int2*)(tile + kRangeAt) = make_int2((int)most, (int)least);
     }
   };
   // operands: chunk 2 k + h of the lane's position, and chunk 2 n + h of its value: the exclusive or with k and n
   // (chunks of 16 bytes, in the low bits of places that are multiples of 128) gives them from one place each
   const int key_row = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
   const int key_from = key_place(key_row, h), value_from = value_place(col, h);
-  int value_exponent = kNone, least_exponent = -kNone;  // of the values' scales so far
+  // In 8 bits weights are taken times the values' scales over 2^value_exponent: an F16 number keeps that for scales
+  // within 2^kNear of the largest so far, whose exponent it then is. Where scales lie further apart (a row of a value
+  // next to 0 among others) it is a row's own from there on: that of its largest weight times scale, so that a row keeps
+  // its bits whatever scales it hardly weighs (1,024 tokens after 6,000, 16 heads over 4 of 128, one value row 2^-30 of
+  // the others: 144 us, 132 without that row).
+  constexpr int kNear = 16, kLeastExponent = -100;  // (a scale below 2^28 over 2^kLeastExponent is a number)
+  int most_exponent = kNone, least_exponent = -kNone;  // of the values' scales so far
+  int value_exponent = kNone;
   // A tile comes while the one before it is used (8 bits: is written then, and is in registers a tile before that).
   load_entries(begin);
   Pages pages = pages_of();
@@ -1130,20 +1141,20 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
     if (a.window && base + TOK - 1 + (uint32_t)a.window <= w0 && base >= (uint32_t)a.sinks) continue;
     const bool whole = okay_then == 15u && base + TOK - 1 <= w0 &&
                        (a.window == 0 || base + (uint32_t)a.window > w1 || base + TOK - 1 < (uint32_t)a.sinks);
-    float lower = 1.0f;  // 2^-value_exponent
+    bool apart = false, change = false;
+    float factor = 1.0f;  // what the results so far are multiplied by, where there is a change
     if constexpr (I8) {
-      const int2 exponents = *(const int2*)(tile + kExponentsAt);
-      const int most = max(uniform(exponents.x), -126);
-      if (most > value_exponent) {
-        const float keep = value_exponent == kNone ? 0.0f : exp2_fast((float)(value_exponent - most));
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[d][e] *= keep;
+      const int2 range = *(const int2*)(tile + kRangeAt);
+      const int most = max(uniform(range.x), -126);
+      least_exponent = min(least_exponent, uniform(range.y));
+      const int before = most_exponent;
+      most_exponent = max(most_exponent, most);
+      apart = most_exponent - least_exponent > kNear;
+      if (!apart && most > before) {
+        factor = before == kNone ? 0.0f : exp2_fast((float)(before - most));
         value_exponent = most;
+        change = true;
       }
-      least_exponent = min(least_exponent, uniform(exponents.y));
-      lower = exp2_fast((float)-value_exponent);
     }
     // scores: score[half][e] is row col, position base + 32 half + 16 (e / 8) + 8 h + e % 8
     f32x16 score[2];
@@ -1221,15 +1232,44 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
       for (int e = 0; e < 16; ++e) top = max(top, max(ordered(score[0][e]), ordered(score[1][e])));
       const float high = __int_as_float(top ^ (int)((uint32_t)(top >> 31) >> 1));
       const float next = fmaxf(ref, fmaxf(high, __shfl_xor(high, 32, kWave)) * row_scale);
-      const float keep = exp2_fast(ref - (next == -kInfinity ? 0.0f : next));
+      const float to = next == -kInfinity ? 0.0f : next;
+      total *= exp2_fast(ref - to);
+      float down = 0.0f;
+      if constexpr (I8)
+        if (apart) {  // the results keep their size (up to doubled), and weights to come are taken times 2^down
+          const float room = (float)max(value_exponent - kLeastExponent, 0);
+          down = ceilf(fminf(fmaxf(next - ref, 0.0f), room));
+          value_exponent -= (int)down;
+        }
+      factor *= exp2_fast(ref + down - to);
       ref = next;
-      total *= keep;
+      change = true;
+    }
+    const float lift = kManyLift - (ref == -kInfinity ? 0.0f : ref);
+    if constexpr (I8)
+      if (apart) {
+        // a power of two that is no less than the row's largest weight times scale, over 2^kManyLift
+        float high = -kInfinity;
+#pragma unroll
+        for (int n = 0; n < 32; n += 4) {
+          const float4 x = *(const float4*)((const float*)(tile + kExponentsAt) + h * 8 + n / 8 * 16 + n % 8);
+          const float exponent[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            high = fmaxf(high, fmaf(score[n / 16][n % 16 + e], row_scale, lift - kManyLift) + exponent[e]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        high = fmaxf(high, __shfl_xor(high, 32, kWave));
+        const int next = max(value_exponent, (int)ceilf(fminf(fmaxf(high, (float)kLeastExponent), 126.0f)));
+        factor = ldexpf(factor, max(value_exponent - next, -200));
+        value_exponent = next;
+        change = true;
+      }
+    if (change)
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] *= keep;
-    }
-    const float lift = kManyLift - (ref == -kInfinity ? 0.0f : ref);
+        for (int e = 0; e < 16; ++e) acc[d][e] *= factor;
     // 16 positions at a time, the next ones' weights made between the products of these
     Halves<TERMS> weights[2];
     auto weigh = [&](int n, Halves<TERMS>& to) {
@@ -1237,7 +1277,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
       if constexpr (I8) {
         const float* scales = (const float*)(tile + kScalesAt) + TOK + h * 8 + n * 16;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) value_scale[e] = scales[e] * lower;
+        for (int e = 0; e < 8; ++e) value_scale[e] = ldexpf(scales[e], -value_exponent);
       }
       float w[8];
 #pragma unroll
@@ -1280,15 +1320,13 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
     }
   }
 
-  // scales so far apart that the smaller ones' weights lost bits: the rows are taken again, one by one
-  const bool apart = I8 && value_exponent - least_exponent > 16;
   if (value_exponent == kNone) value_exponent = 0;
   uint64_t again;
   const int r = wave_row + col;
   const bool there = r < rows;
   const int64_t place = (span.first + token) * a.heads + kv * a.group + (row - token * group);
   const float sum = total + __shfl_xor(total, 32, kWave);
-  bool odd = apart || (sum == 0.0f && ref == -kInfinity);
+  bool odd = sum == 0.0f && ref == -kInfinity;
   if (alone) {
     const float inverse = sum == 0.0f ? 0.0f : (I8 ? exp2_fast((float)value_exponent) : 1.0f) / sum;
 #pragma unroll
@@ -1320,7 +1358,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
                 f32x4{acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]};
       if (h == 0) {
         a.statistics[at * 3] = ref;
-        a.statistics[at * 3 + 1] = apart ? __builtin_nanf("") : sum;
+        a.statistics[at * 3 + 1] = sum;
         a.statistics[at * 3 + 2] = ref + (float)value_exponent;
       }
     }

@@ -921,3 +921,128 @@ def test_few_and_many_rows_partials_by_place(hip, kind, dtype):
     out = run(hip, case, q, 0.09)
     assert_rows(case, q, 0.09, out, what="by place")
     assert torch.equal(out, run(hip, case, q, 0.09))
+
+
+def scale_rows(case, sequence, position, factor):
+    """The 8-bit cache's value row at `position`, its scale times `factor`."""
+    p, off = int(case.tables[sequence, position // case.page]), position % case.page
+    case.cache.valueScales[p, :, off] *= factor
+    case.dense[sequence][1][position] *= factor
+    case.scales[sequence][position] *= factor
+
+
+def assert_rows_of_scales_apart(case, queries, scale, got, window=None, what=""):
+    """Value scales w any distance apart: a row's weights are p w in F16 terms
+    over a power of two such that the largest is 2^(lift - 17) at least (lift 14
+    for F32's two terms, 7 for BF16's one), their last step 2^-24. So with codes
+    up to 127 and n positions a row is off by 127 n 2^-25 / 2^(lift - 17) of its
+    own largest p w, not of the cache's largest w, beside the other roundings.
+    Few rows' weights are 2^(score + log2 w): the logarithm off by a step, its sums
+    with the score and the maximum by half of one, 2^-22 |log2 w| ln 2 together."""
+    out, mass, size, count, _ = wanted(case, queries.cpu(), scale, window)
+    logs = max(float(w.clamp(min=2.0 ** -126).log2().abs().max()) for w in case.scales)
+    bar = 4 * (2.0 ** -24 * (math.sqrt(case.dim) + 4) * size + 2.0 ** -20 + 2.0 ** -24 * count.sqrt()) * mass
+    bar = bar + math.log(2) * 2.0 ** -22 * logs * mass
+    if queries.dtype == torch.bfloat16:
+        bar = bar + 2.0 ** -11 * mass + 2.0 ** -8 * out.abs()
+    lift, group = 14 if queries.dtype == torch.float32 else 7, queries.shape[1] // case.kv
+    for s, (k, _) in enumerate(case.dense):
+        rows = slice(int(case.offsets[s]), int(case.offsets[s + 1]))
+        at = torch.arange(int(case.rows[s]))[:, None] + int(case.starts[s])
+        j = torch.arange(k.shape[0])[None, :]
+        seen = (j <= at) if window is None else (j <= at) & ((j > at - window.positions) | (j < window.sinks))
+        for h in range(queries.shape[1]):
+            logits = scale * (queries[rows, h].double().cpu() @ k[:, h // group].T)
+            p = torch.softmax(logits.masked_fill(~seen, -math.inf), -1)
+            most = (p * case.scales[s][:, h // group]).amax(-1, keepdim=True)
+            bar[rows, h] += 127 * count[rows, h] * 2.0 ** (-25 + 17 - lift) * most
+    off = (got.cpu().double() - out).abs()
+    print(f"[gpu]   worst {float((off / bar).max()):.3f} of the bar", flush=True)
+    assert bool((off <= bar).all()), f"{what}: {int((off > bar).sum())} beyond the bar, {float((off / bar).max()):.2f} of it"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("down", [20, 40, 90])
+@pytest.mark.parametrize("where", ["first", "thirds", "tiles", "last", "all but some", "none weighed"])
+@pytest.mark.parametrize("start,tokens,heads,dim", [(100, 1, 8, 128), (200, 80, 8, 64), (200, 80, 4, 128),
+                                                    (150, 70, 4, 256), (3000, 90, 16, 128)])
+def test_value_scales_far_apart(hip, dtype, down, where, start, tokens, heads, dim):
+    step(f"value scales 2^{down} apart, {where} {dtype} {tokens} tokens at {start}, heads of {dim}")
+    case = Case("i8", [start], [tokens], 2, dim, 16, seed=57, value_scale=4.0)
+    length = start + tokens
+    small = {"first": [0], "thirds": range(0, length, 3), "tiles": [j for j in range(length) if j // 64 % 2 == 0],
+             "last": range(start, length), "all but some": [j for j in range(length) if j % 50 != 49],
+             "none weighed": [0, 40]}[where]
+    for position in small:
+        scale_rows(case, 0, position, 2.0 ** -down)
+    q = normal(58, (tokens, heads, dim), torch.float32, 0.5)
+    # half of the heads weigh one small row so far above the others that these are e^-20 to e^-30 next to it
+    k = case.dense[0][0]
+    for h in range(0, heads, 2):
+        if where != "none weighed":
+            position = list(small)[len(small) // 2 if where != "last" else 0]
+            key = k[position, h // (heads // 2)].float()
+            q[:, h] += 25 / 0.09 / float(key @ key) * key
+    q = q.to(TYPES[dtype]).to(DEV)
+    assert_rows_of_scales_apart(case, q, 0.09, run(hip, case, q, 0.09, single=True), what="scales apart")
+    window = d.AttentionWindow(70, 3)
+    assert_rows_of_scales_apart(case, q, 0.09, run(hip, case, q, 0.09, window, single=True), window, "windowed")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rising", [True, False])
+def test_value_scales_far_apart_as_scores_rise(hip, dtype, rising):
+    step(f"value scales apart, scores {'rising' if rising else 'falling'} {dtype}")
+    # from tile to tile a row's scores go up (or down) by a few nats and its scales the other way, so that every
+    # tile's part of the result is of one size
+    case = Case("i8", [600], [70], 1, 128, 16, seed=59)
+    q = normal(60, (70, 4, 128), torch.float32, 0.25)
+    u = torch.sign(normal(61, (128,)))
+    case.cache.keyScales.fill_(2.0 / 127)
+    for position in range(670):
+        tile = position // 64 if rising else 10 - position // 64
+        page, off = int(case.tables[0, position // 16]), position % 16
+        case.cache.valueScales[page, :, off] *= math.exp(-3.0 * tile)
+        codes = (u * 12 * tile).to(torch.int8)  # q.k gains about 3 a tile
+        case.cache.keys[page, off, 0] = codes.to(DEV)
+        held = case.cache.valueScales[page, :, off].double().cpu()
+        case.dense[0][0][position, 0] = codes.double() * float(np.float32(2.0 / 127))
+        case.dense[0][1][position] = case.cache.values[page, :, :, off].double().cpu() * held[:, None]
+        case.scales[0][position] = held
+    q += u * (3.0 / 0.09 / (128 * 12 * 2.0 / 127))
+    q = q.to(TYPES[dtype]).to(DEV)
+    assert_rows_of_scales_apart(case, q, 0.09, run(hip, case, q, 0.09, single=True), what="scores that rise")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("context", [0, 6000])
+def test_a_value_row_next_to_zero_costs_no_more_than_its_tiles(hip, dtype, context):
+    step(f"a prompt over a value row next to zero {dtype} after {context}")
+    # one value row 2^-30 of the others must not send a prompt's rows to the kernel of single rows, which would take
+    # some hundred times as long
+    tokens, heads, kv, dim, page = 1024, 16, 4, 128, 16
+    pages = (context + tokens) // page
+    cache = d.QuantizedKvCache.allocate(pages, page, kv, dim)
+    cache.keys.random_(-127, 128)
+    cache.values.random_(-127, 128)
+    cache.keyScales.fill_(2.0 / 127)
+    cache.valueScales.fill_(2.0 / 127)
+    table, q = dev_i32(np.arange(pages)), normal(62, (tokens, heads, dim), TYPES[dtype]).to(DEV)
+    out = torch.empty_like(q)
+
+    def least():
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            hip.attention(q, cache, table, context, 0.09, out)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    even = least()
+    cache.valueScales[0, :, 5] *= 2.0 ** -30
+    apart = least()
+    print(f"[gpu]   {even * 1e3:.0f} us, {apart * 1e3:.0f} with scales apart", flush=True)
+    assert apart < 5 * even
