@@ -82,7 +82,7 @@ __device__ __forceinline__ bool tile_of(const CacheRows& c, Tile& t) {
   int64_t nth;
   const int s = locate(c.p, unit, kTile, c.extra, 1, nth);
   if (s < 0) return false;
-  const Span span = span_of(c.p, s);
+  const Span span = span_of<true>(c.p, s);
   t.first = (span.start / kTile + nth) * kTile;
   t.lo = max(t.first, span.start);
   t.hi = min(t.first + kTile, span.start + span.rows);
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(64) write_rows(const T* k, const T* v, CacheRo
   int64_t nth;
   const int s = locate(c.p, unit, 1, 0, 1, nth);
   if (s < 0) return;
-  const Span span = span_of(c.p, s);
+  const Span span = span_of<true>(c.p, s);
   if (nth >= span.rows) return;
   const int64_t position = span.start + nth, page = span.table[position / c.p.page_size];
   const int64_t off = position % c.p.page_size;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(64) read_rows(T* k, T* v, CacheRows c) {
   int64_t nth;
   const int s = locate(c.p, unit, 1, 0, 1, nth);
   if (s < 0) return;
-  const Span span = span_of(c.p, s);
+  const Span span = span_of<true>(c.p, s);
   if (nth >= span.rows) return;
   const int64_t position = span.start + nth, page = span.table[position / c.p.page_size];
   const int64_t off = position % c.p.page_size;

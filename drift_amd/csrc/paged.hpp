@@ -59,20 +59,34 @@ __device__ __forceinline__ void flag_bad(const Paging& p) {
 }
 
 // Sequence s as the device's arrays describe it. Rows outside the token
-// tensors, a start below 0, or an end past the page table make it a sequence
-// of no rows and set the flag: nothing is read or written for it. Whole waves
-// call, every lane with the same s.
+// tensors or before the end of an earlier sequence, a start below 0, or an end
+// past the page table make it a sequence of no rows and set the flag: nothing is
+// read or written for it. (Offsets that go back would else give rows to two
+// sequences, and more units than a launch has; LOCATED: locate has seen to that.)
+// Whole waves call, every lane with the same s.
+template <bool LOCATED>
 __device__ __forceinline__ Span span_of(const Paging& p, int s) {
   Span span;
+  bool behind = false;
   int64_t from = p.sequences == 1 ? 0 : s, to = p.sequences == 1 ? p.tokens : s + 1;
   if (p.offsets) {
-    from = uniform(p.offsets[s]);
-    to = uniform(p.offsets[s + 1]);
+    const int begin = p.offsets[s], end = p.offsets[s + 1];
+    if constexpr (!LOCATED) {
+      int l = threadIdx.x & (kWave - 1), before = p.offsets[min(l, s)];  // (asked for together with the others)
+      for (;;) {
+        behind |= before > begin && before <= p.tokens;
+        if ((l += kWave) >= s) break;
+        before = p.offsets[l];
+      }
+      behind = __any(behind);
+    }
+    from = uniform(begin);
+    to = uniform(end);
   }
   span.start = p.starts ? uniform(p.starts[s]) : p.start;
   span.first = from;
   span.table = p.tables + (int64_t)s * p.table_pages;
-  const bool good = from >= 0 && to >= from && to <= p.tokens && span.start >= 0 &&
+  const bool good = from >= 0 && to >= from && to <= p.tokens && !behind && span.start >= 0 &&
                     (to == from || span.start + (to - from) <= min((int64_t)p.table_pages * p.page_size, kMostPositions));
   if (!good) flag_bad(p);
   span.rows = good ? (int32_t)(to - from) : 0;
@@ -80,9 +94,9 @@ __device__ __forceinline__ Span span_of(const Paging& p, int s) {
 }
 
 // Work in units of `per` items, a row having `scale` of them: ceil(rows scale /
-// per) + extra units a sequence, by offsets none where there are `least` items or fewer. The sequence that unit `unit` of the launch
-// belongs to (-1: none), and which of its units it is. Whole waves call, every
-// lane with the same unit.
+// per) + extra units a sequence, by offsets none where there are `least` items or
+// fewer. The sequence that unit `unit` of the launch belongs to (-1: none), and
+// which of its units it is. Whole waves call, every lane with the same unit.
 __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, int extra, int64_t scale, int64_t& nth,
                                           int64_t least = 0) {
   if (!p.offsets) {
@@ -96,14 +110,26 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
     return s < p.sequences ? (int)s : -1;
   }
   const int lane = threadIdx.x & (kWave - 1);
+  int passed = INT32_MIN;  // the largest offset of the groups of sequences before, of those that name a row
   for (int base = 0; base < p.sequences; base += kWave) {
     const int s = base + lane;
     int64_t units = 0;
+    const int from = p.offsets[min(s, p.sequences)], to = p.offsets[min(s + 1, p.sequences)];
+    int most = from;  // of the offsets up to and with this lane's
+    if (__any(to < from || to > p.tokens)) {
+      most = from <= p.tokens ? from : INT32_MIN;
+#pragma unroll
+      for (int step = 1; step < kWave; step <<= 1) {
+        const int before = __shfl_up(most, step, kWave);
+        if (lane >= step) most = max(most, before);
+      }
+    }
+    most = max(most, passed);
     if (s < p.sequences) {
-      const int64_t from = p.offsets[s], to = p.offsets[s + 1];
-      const bool good = from >= 0 && to >= from && to <= p.tokens;
+      const bool good = from >= most && from >= 0 && to >= from && to <= p.tokens;
       if (!good) flag_bad(p);  // and no units, so that the others' are all in the launch
-      units = good && (to - from) * scale > least ? ((to - from) * scale + per - 1) / per + extra : 0;
+      const int64_t rows = (int64_t)to - from;
+      units = good && rows * scale > least ? (rows * scale + per - 1) / per + extra : 0;
     }
     int64_t end = units;  // units of this group of sequences, up to and with this lane's
 #pragma unroll
@@ -118,6 +144,7 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
       return base + at;
     }
     unit -= uniform(__shfl(end, kWave - 1, kWave));
+    passed = uniform(__shfl(most, kWave - 1, kWave));
   }
   return -1;
 }
@@ -125,11 +152,11 @@ __device__ __forceinline__ int locate(const Paging& p, int64_t unit, int per, in
 // ---------------------------------------------------------------- host side
 
 // Units a launch needs for every sequence's (locate), whatever the offsets hold: a part of one is left over in as
-// many sequences as can have more than `least` items.
+// many sequences as can have more than `least` items, and one unit more looks through every sequence's offsets.
 inline int64_t units_of(const Paging& p, int64_t per, int64_t extra, int64_t scale, int64_t least = 0) {
   if (p.offsets) {
     const int64_t items = (int64_t)p.tokens * scale;
-    return items / per + std::min((int64_t)p.sequences, items / (least + 1)) * (1 + extra);
+    return items / per + std::min((int64_t)p.sequences, items / (least + 1)) * (1 + extra) + (p.sequences > kWave);
   }
   if (p.sequences == 1) return ceil_div((int64_t)p.tokens * scale, per) + extra;
   return p.sequences * (ceil_div(scale, per) + extra);

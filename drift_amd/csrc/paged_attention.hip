@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* querie
   int64_t nth;
   const int s = locate(a.p, blockIdx.x / (unsigned)a.heads, 1, 0, 1, nth);
   if (s < 0) return;
-  const Span span = span_of(a.p, s);
+  const Span span = span_of<true>(a.p, s);
   if (nth >= span.rows) return;
   const int h = blockIdx.x % (unsigned)a.heads;
   RowState state;
@@ -428,7 +428,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   // (and its later units, of which most sequences have none: 64 single tokens in 4 units each, given by offsets, 235 us,
   // 414 with a sequence's units as neighbours, whose first are all dealt to the same quarter of a die)
   const int s = (int)(unit % (unsigned)a.p.sequences), nth = (int)(unit / (unsigned)a.p.sequences);
-  const Span span = span_of(a.p, s);
+  const Span span = span_of<false>(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
   if (rows <= 0 || (int64_t)span.rows * a.group > a.few_rows) return;
   const uint32_t row0 = (uint32_t)nth * (C * 16), group = (uint32_t)a.group;
@@ -857,7 +857,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   int64_t nth;
   const int s = locate(a.p, unit, kRows, 0, a.group, nth, a.few_rows);
   if (s < 0) return;
-  const Span span = span_of(a.p, s);
+  const Span span = span_of<true>(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * kRows, (int64_t)kRows);
   if (rows <= 0 || (int64_t)span.rows * a.group <= a.few_rows) return;
   const uint32_t row0 = (uint32_t)nth * kRows, group = (uint32_t)a.group, start = (uint32_t)span.start;
@@ -1415,7 +1415,7 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
   if constexpr (FEW) s = (int)(unit % (unsigned)a.p.sequences), nth = unit / (unsigned)a.p.sequences;
   else s = locate(a.p, unit, rows, 0, a.group, nth, a.few_rows);
   if (s < 0) return;
-  const Span span = span_of(a.p, s);
+  const Span span = span_of<!FEW>(a.p, s);
   const uint32_t all = (uint32_t)span.rows * (uint32_t)a.group, group = (uint32_t)a.group;
   const uint32_t row0 = (uint32_t)nth * rows;
   if (row0 + part * kRows >= all || (all <= (uint32_t)a.few_rows) != FEW) return;

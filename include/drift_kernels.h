@@ -336,9 +336,9 @@ int drift_attention_inputs_bf16(const uint16_t* query_and_gate, const uint16_t* 
  * and on, in the pages page_tables[s] (int32 [sequences, table_pages]). The
  * three arrays are read on the device, so a launch captured in a graph serves
  * as its sequences grow; rows outside every sequence are left as they are. A
- * sequence whose rows lie outside the `tokens` rows, whose start is negative or
- * whose end is past its page table gets nothing done, and *bad_page = 1 (device
- * int32, nullable).
+ * sequence whose rows lie outside the `tokens` rows or before the end of an
+ * earlier sequence's, whose start is negative or whose end is past its page table
+ * gets nothing done, and *bad_page = 1 (device int32, nullable).
  * - offsets NULL: one sequence of all `tokens` rows, or (sequences == tokens) a
  *   row a sequence, a decode step.
  * - starts NULL: one sequence at position `start`, checked on the host against

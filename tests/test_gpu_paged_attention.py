@@ -1046,3 +1046,61 @@ def test_a_value_row_next_to_zero_costs_no_more_than_its_tiles(hip, dtype, conte
     apart = least()
     print(f"[gpu]   {even * 1e3:.0f} us, {apart * 1e3:.0f} with scales apart", flush=True)
     assert apart < 5 * even
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dim", [128, 36])
+@pytest.mark.parametrize("each,before", [(3, 0), (90, 0), (90, 70)])
+def test_a_sequence_that_begins_before_an_earlier_ones_end(hip, kind, dim, each, before):
+    step(f"offsets that go back {kind} heads of {dim}, {each} rows after {before} sequences")
+    # `before` sequences of no rows, then rows 0 to n, back to n / 3, from there to n + n / 3, and n more: the one that
+    # begins inside the first's rows gets nothing done (its rows past them are left), the last is done
+    n, third = each, each // 3
+    case = Case(kind, [40] * 2, [n, n], 2, dim, 16, seed=63)
+    tables = np.full((before + 4, case.tables.shape[1]), -1, np.int32)
+    tables[before], tables[before + 3] = case.tables
+    tables[before + 1], tables[before + 2] = case.tables[0], case.tables[0]
+    starts = dev_i32([0] * before + [40, 40, 40, 40])
+    ends = [n, third, n + third, 2 * n + third]
+    offsets = dev_i32([0] * (before + 1) + ends)
+    tokens = ends[-1]
+    batch = d.Sequences(dev_i32(tables), starts, offsets)
+    q = normal(64, (tokens, 8, dim), torch.float32, 2.0).to(DEV)
+    out, bad = torch.full(q.shape, 7.0, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    hip.attentionSequences(q, case.cache, batch, 0.1, out, badPage=bad)
+    assert int(bad.item()) == 1
+    done = torch.tensor(list(range(n)) + list(range(n + third, tokens)))
+    assert_rows(case, q.cpu()[done], 0.1, out.cpu()[done], what="beside offsets that go back")
+    assert bool((out[n:n + third] == 7).all())
+    # reading: the same rows
+    k, v = (torch.full((tokens, 2, dim), 7.0, device=DEV) for _ in range(2))
+    bad.zero_()
+    hip.cacheReadSequences(case.cache, batch, k, v, bad)
+    assert int(bad.item()) == 1
+    assert bool((k[n:n + third] == 7).all()) and bool((v[n:n + third] == 7).all())
+    want = torch.cat([case.dense[s][0][40:40 + n] for s in (0, 1)])
+    assert float((k.cpu().double()[done] - want).abs().max()) < 1e-5
+    # an offset past the tokens spoils the two sequences that it bounds, and no other
+    offsets = dev_i32([0] * (before + 1) + [n, tokens + 5, n + third, 2 * n + third])
+    out.fill_(7.0), bad.zero_()
+    hip.attentionSequences(q, case.cache, d.Sequences(dev_i32(tables), starts, offsets), 0.1, out, badPage=bad)
+    assert int(bad.item()) == 1
+    assert_rows(case, q.cpu()[done], 0.1, out.cpu()[done], what="beside an offset past the tokens")
+    assert bool((out[n:n + third] == 7).all())
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_a_wrong_sequence_far_behind_the_rows_is_told(hip, kind):
+    step(f"a wrong sequence far behind the rows {kind}")
+    # one row, the first of 200 sequences'; the 150th ends past the tokens
+    case = Case(kind, [5], [1], 2, 64, 16, seed=65)
+    offsets = np.ones(201, np.int32)
+    offsets[0], offsets[150] = 0, 9
+    batch = d.Sequences(dev_i32(np.tile(case.tables, (200, 1))), dev_i32([5] * 200), dev_i32(offsets))
+    x, out = normal(66, (1, 2, 64)).to(DEV), torch.empty(1, 2, 64, device=DEV)
+    for call in (lambda bad: hip.cacheWriteSequences(x, x, case.cache, batch, bad),
+                 lambda bad: hip.cacheReadSequences(case.cache, batch, out, torch.empty_like(out), bad),
+                 lambda bad: hip.attentionSequences(x, case.cache, batch, 0.1, out, badPage=bad)):
+        bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+        call(bad)
+        assert int(bad.item()) == 1
