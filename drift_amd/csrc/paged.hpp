@@ -59,9 +59,9 @@ __device__ __forceinline__ void flag_bad(const Paging& p) {
 }
 
 // Sequence s as the device's arrays describe it. Rows outside the token
-// tensors or before the end of an earlier sequence, a start below 0, or an end
-// past the page table make it a sequence of no rows and set the flag: nothing is
-// read or written for it. (Offsets that go back would else give rows to two
+// tensors or before the end of an earlier sequence, or with rows a start below 0
+// or an end past the page table, make it a sequence of no rows and set the flag:
+// nothing is read or written for it. (Offsets that go back would else give rows to two
 // sequences, and more units than a launch has; LOCATED: locate has seen to that.)
 // Whole waves call, every lane with the same s.
 template <bool LOCATED>
@@ -86,8 +86,9 @@ __device__ __forceinline__ Span span_of(const Paging& p, int s) {
   span.start = p.starts ? uniform(p.starts[s]) : p.start;
   span.first = from;
   span.table = p.tables + (int64_t)s * p.table_pages;
-  const bool good = from >= 0 && to >= from && to <= p.tokens && !behind && span.start >= 0 &&
-                    (to == from || span.start + (to - from) <= min((int64_t)p.table_pages * p.page_size, kMostPositions));
+  const bool good = from >= 0 && to >= from && to <= p.tokens && !behind &&
+                    (to == from || (span.start >= 0 && span.start + (to - from) <=
+                                                           min((int64_t)p.table_pages * p.page_size, kMostPositions)));
   if (!good) flag_bad(p);
   span.rows = good ? (int32_t)(to - from) : 0;
   return span;

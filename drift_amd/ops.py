@@ -197,7 +197,8 @@ class Sequences:
     `offsets` each sequence has one row (a decode step). Rows outside every
     sequence are left as they are. A sequence that the arrays describe wrongly
     (rows outside the tensors or before an earlier one's end, a negative start,
-    an end past its page table) gets nothing done and sets the call's `badPage`.
+    an end past its page table) gets nothing done and sets the call's `badPage`;
+    one without rows (an empty place of a batch) may have any start.
 
     `longest`: a guess of the most positions that a sequence has, by which
     attention splits its work (default: what its page table has room for); the

@@ -337,8 +337,9 @@ int drift_attention_inputs_bf16(const uint16_t* query_and_gate, const uint16_t* 
  * three arrays are read on the device, so a launch captured in a graph serves
  * as its sequences grow; rows outside every sequence are left as they are. A
  * sequence whose rows lie outside the `tokens` rows or before the end of an
- * earlier sequence's, whose start is negative or whose end is past its page table
- * gets nothing done, and *bad_page = 1 (device int32, nullable).
+ * earlier sequence's, or that has rows and a negative start or an end past its page
+ * table, gets nothing done, and *bad_page = 1 (device int32, nullable). One without
+ * rows (an empty place of a batch) may have any start.
  * - offsets NULL: one sequence of all `tokens` rows, or (sequences == tokens) a
  *   row a sequence, a decode step.
  * - starts NULL: one sequence at position `start`, checked on the host against

@@ -1104,3 +1104,20 @@ def test_a_wrong_sequence_far_behind_the_rows_is_told(hip, kind):
         bad = torch.zeros(1, dtype=torch.int32, device=DEV)
         call(bad)
         assert int(bad.item()) == 1
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dim", [64, 36])
+def test_empty_places_of_a_batch_are_right_whatever_their_start(hip, kind, dim):
+    step(f"empty places of a batch {kind} heads of {dim}")
+    case = Case(kind, [40, 7], [5, 2], 2, dim, 16, seed=67)
+    tables = np.full((5, case.tables.shape[1]), -1, np.int32)
+    tables[[1, 3]] = case.tables
+    batch = d.Sequences(dev_i32(tables), dev_i32([-1, 40, 2 ** 31 - 1, 7, -(2 ** 31)]), dev_i32([0, 0, 5, 5, 7, 7]))
+    q, bad = normal(68, (7, 4, dim), torch.float32, 2.0).to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    out, k, v = torch.empty_like(q), torch.empty(7, 2, dim, device=DEV), torch.empty(7, 2, dim, device=DEV)
+    hip.attentionSequences(q, case.cache, batch, 0.1, out, badPage=bad)
+    hip.cacheReadSequences(case.cache, batch, k, v, bad)
+    hip.cacheWriteSequences(k, v, case.cache, batch, bad)
+    assert int(bad.item()) == 0
+    assert_rows(case, q, 0.1, out, what="beside empty places")
