@@ -1689,6 +1689,9 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   if ((reinterpret_cast<uintptr_t>(queries) | reinterpret_cast<uintptr_t>(out)) % sizeof(T) != 0)
     return refuse("%s: queries or out not aligned to their elements", entry);
   if (const int bad = check_cache(entry, a.p, a.keys, a.values, a.key_scales, a.value_scales)) return bad;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(queries), to = reinterpret_cast<uintptr_t>(out);
+  if ((from > to ? from - to : to - from) / sizeof(T) < (uint64_t)a.p.tokens * a.heads * a.dim)
+    return refuse("%s: out overlaps queries", entry);
   a.group = a.heads / a.kv_heads;
   a.page_units = a.p.page_size / 16;
   a.page_shift = 27;

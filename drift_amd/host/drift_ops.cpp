@@ -947,7 +947,9 @@ void HipOps::attend(const char* operation, const Tensor& queries, const PagedCac
                     float scale, const Tensor& out, const Tensor& workspace,
                     const std::optional<AttentionWindow>& window, int32_t* badPage) {
   checkAttention(operation, queries, cache, out, window);
-  require(queries.data != out.data || queries.elementCount() == 0, text(operation, ": out is queries"));
+  const auto from = reinterpret_cast<uintptr_t>(queries.data), to = reinterpret_cast<uintptr_t>(out.data);
+  require((from > to ? from - to : to - from) >= (uintptr_t)queries.byteSize(),
+          text(operation, from == to ? ": out is queries" : ": out overlaps queries"));
   const Paging p = pagingOf(operation, cache, rows, queries.shape[0]);
   const auto tokens = (int32_t)queries.shape[0], heads = (int32_t)queries.shape[1];
   const auto kvHeads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();

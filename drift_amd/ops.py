@@ -1055,7 +1055,7 @@ class HipOps:
                   window: Optional[AttentionWindow] = None, badPage: Optional[torch.Tensor] = None) -> None:
         """Attention of one sequence's new tokens over its paged cache (a
         KvCache or a QuantizedKvCache), their own keys and values written to it
-        before: queries, out [tokens, heads, D] (F32 or BF16, out not queries),
+        before: queries, out [tokens, heads, D] (F32 or BF16, no memory of both),
         token t at position start + t, which sees the positions up to its own,
         or with `window` those of it; scores are `scale` q.k, query head h reads
         key head h / (heads / kvHeads). What a token does not see has no part in
@@ -1085,8 +1085,9 @@ class HipOps:
                    window, badPage) -> None:
         checkBadPage(operation, badPage)
         self._onOneDevice(operation, (queries, out, badPage, *tensors))
-        if queries.data_ptr() == out.data_ptr() and queries.numel():
-            raise ValueError(f"{operation}: out is queries")
+        apart = abs(queries.data_ptr() - out.data_ptr())
+        if apart < queries.numel() * queries.element_size():
+            raise ValueError(f"{operation}: out {'is' if apart == 0 else 'overlaps'} queries")
         positions, sinks = (window.positions, window.sinks) if window is not None else (0, 0)
         longest = min(longest, _MOST_POSITIONS)
         # scratch of this call's own, from torch's pool on the launch's stream: calls on several streams and

@@ -381,7 +381,7 @@ int drift_paged_read_bf16(uint16_t* k, uint16_t* v, const void* keys, const void
                           int32_t* bad_page, void* stream);
 
 /* Attention of the rows' queries [tokens, heads, head_dim] over the cache into
- * out (like queries; may not be queries). The row at position P sees positions
+ * out (like queries; may not share memory with them). The row at position P sees positions
  * j <= P of its sequence; with window > 0 only j > P - window or j < sinks. Head
  * h reads key head h / (heads / kv_heads). out = sum p_j v_j / sum p_j, p_j =
  * exp(scale q.k_j - their maximum), statistics and sums in F32; BF16 outputs

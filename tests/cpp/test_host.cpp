@@ -185,6 +185,8 @@ CHECK_TEST(paged_calls_are_checked) {
   refused([&] { hip.attentionSequences(q, eight, Sequences{s.pageTables, s.starts, fake(DType::I32, {3}), 0}, 1.0f, out,
                                        none); }, "attentionSequences: offsets I32 [3] for 3 sequences");
   refused([&] { hip.attentionSequences(q, cache, s, 1.0f, q, none); }, "attentionSequences: out is queries");
+  refused([&] { hip.attentionSequences(q, cache, s, 1.0f, fake(DType::F32, {3, 4, 64}, 4096 + 3 * 4 * 64 * 4 - 16), none); },
+          "attentionSequences: out overlaps queries");
   refused([&] { hip.attention(fake(DType::F32, {3, 3, 64}), cache, table, 0, 1.0f, fake(DType::F32, {3, 3, 64}, 8192),
                               none); }, "attention: queries [3×3×64] over a cache of 2 heads of 64");
   refused([&] { hip.attention(q, cache, table, 30, 1.0f, out, none); }, "a page table of 2 pages for 33 positions");

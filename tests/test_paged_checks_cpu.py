@@ -273,3 +273,21 @@ def test_a_mixed_batchs_workspace_has_slots_for_few_rows():
     # 24 sequences, 1,811 tokens of 28 heads over 4: up to 16 rows of each sequence and key head may be split
     code, size = workspace(24, 1811, 28, 4, 128, 0, 0, 131072)
     assert code == "code 0" and 0 < size <= 170 * 24 * 4 * 16 * 131 * 4
+
+
+@pytest.mark.parametrize("entry,size", [("drift_paged_attention_f32", 4), ("drift_paged_attention_bf16", 2)])
+def test_out_that_overlaps_queries_is_refused(entry, size):
+    for apart in (16, 3 * 4 * 64 * size - 16):
+        assert "out overlaps queries" in refusal(entry, *attention(queries=1 << 20, out=(1 << 20) + apart))
+        assert "out overlaps queries" in refusal(entry, *attention(queries=(1 << 20) + apart, out=1 << 20))
+
+
+def test_out_that_overlaps_queries_is_refused_by_hip_ops(hip, monkeypatch):
+    monkeypatch.setattr(hip, "_onOneDevice", lambda *_: None)
+    flat, cache, table = zeros(4 * 4 * 64), f16_cache(), zeros(4, dtype=I32)
+    queries, over = flat[:768].view(3, 4, 64), flat[256:].view(3, 4, 64)
+    for out, what in ((queries, "is"), (over, "overlaps")):
+        with pytest.raises(ValueError, match=f"attention: out {what} queries"):
+            hip.attention(queries, cache, table, 0, 0.1, out)
+    with pytest.raises(ValueError, match="attentionSequences: out overlaps queries"):
+        hip.attentionSequences(over, cache, d.Sequences(zeros(3, 4, dtype=I32), zeros(3, dtype=I32)), 0.1, queries)
