@@ -896,9 +896,10 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   const bool finite = most < 0x7f800000u;
   const int shift = finite && most != 0 ? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(most)) : 0;
   // (above 0, so that the largest score is the largest product: a negative scale turns the query's sign. A scale
-  // of 0, or one that a tiny row makes it, is small enough to leave every weight even)
-  const float row_scale =
-      finite ? fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -shift), 0x1p-120f) : __builtin_nanf("");
+  // of 0, or one that a tiny row makes it, is small enough to leave every weight even; a NaN stays one)
+  const float row_scale = finite && a.scale == a.scale
+                              ? fmaxf(ldexpf(fabsf(a.scale) * 1.44269504088896340736f, -shift), 0x1p-120f)
+                              : __builtin_nanf("");
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
     float x[8];

@@ -1121,3 +1121,15 @@ def test_empty_places_of_a_batch_are_right_whatever_their_start(hip, kind, dim):
     hip.cacheWriteSequences(k, v, case.cache, batch, bad)
     assert int(bad.item()) == 0
     assert_rows(case, q, 0.1, out, what="beside empty places")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,tokens,heads,dim", [(150, 1, 4, 128), (150, 90, 4, 128), (3000, 90, 16, 64), (150, 2, 4, 300)])
+def test_scales_that_are_no_numbers(hip, kind, dtype, start, tokens, heads, dim):
+    step(f"scales that are no numbers {kind} {dtype} {tokens} tokens at {start}, heads of {dim}")
+    # every score is then a NaN or an infinity, and so is no row of weights a number
+    case = Case(kind, [start], [tokens], 2, dim, 16, seed=69)
+    q = normal(70, (tokens, heads, dim), TYPES[dtype], 2.0).to(DEV)
+    for scale in (math.nan, math.inf, -math.inf):
+        assert bool(torch.isnan(run(hip, case, q, scale, single=True)).all()), f"scale {scale}"
