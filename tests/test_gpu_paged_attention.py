@@ -1133,3 +1133,30 @@ def test_scales_that_are_no_numbers(hip, kind, dtype, start, tokens, heads, dim)
     q = normal(70, (tokens, heads, dim), TYPES[dtype], 2.0).to(DEV)
     for scale in (math.nan, math.inf, -math.inf):
         assert bool(torch.isnan(run(hip, case, q, scale, single=True)).all()), f"scale {scale}"
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,context", [(64, 130), (128, 400), (256, 3000), (36, 400)])
+def test_masked_content_leaves_a_decode_steps_bits_alone(hip, kind, dtype, dim, context):
+    step(f"masked content and a decode step's bits {kind} {dtype} heads of {dim}, {context} positions")
+    # one token a sequence: all its rows see the same positions, and what they do not see may be anything
+    case = Case(kind, [context, context // 3, 17], [1, 1, 1], 2, dim, 16, seed=71)
+    window = d.AttentionWindow(60, 5)
+    q = normal(72, (3, 8, dim), TYPES[dtype], 2.0).to(DEV)
+    first = run(hip, case, q, 0.09, window, offsets=False)
+    assert_rows(case, q, 0.09, first, window, what="before")
+    cache, held = case.cache, torch.zeros(case.cache.pages, 16, dtype=torch.bool)
+    for s, start in enumerate(case.starts):
+        for j in range(int(start) + 1):
+            if j > start - 60 or j < 5:
+                held[int(case.tables[s, j // 16]), j % 16] = True
+    page, off = [x.to(DEV) for x in (~held).nonzero(as_tuple=True)]
+    assert len(page) > 40
+    for junk in (0.0, 65504.0, math.inf, math.nan):
+        if kind == "f16":
+            cache.keys[page, off], cache.values[page, :, :, off] = junk, -junk
+        else:
+            cache.keys[page, off], cache.values[page, :, :, off] = -128, 127
+            cache.keyScales[page, :, off], cache.valueScales[page, :, off] = junk, junk
+        assert torch.equal(run(hip, case, q, 0.09, window, offsets=False), first), f"{junk} in masked places"
