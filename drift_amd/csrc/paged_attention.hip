@@ -1548,7 +1548,7 @@ Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least,
 }
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
-             int64_t sinks, int64_t longest, bool by_offsets, bool quantized) {
+             int64_t sinks, int64_t longest, bool by_offsets, bool quantized, bool f32) {
   Plan p{0, true, 128, {0, 1}, {0, 1}, false, 0, 0, 0, 0, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
@@ -1566,10 +1566,23 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     p.few = seen <= 768 ? Split{1, 1} : split_of(sequences * kv_heads, seen, 1024, 4, 16);
   if (each * group > kFewRows) {
     // Blocks of 256 rows read keys and values (and make codes F16 numbers) half as often; blocks of 128 leave fewer
-    // rows idle, and two of them on a compute unit wait at barriers of their own. us, 128 / 256: a prompt of 8,192
-    // tokens, 32 heads over 8 733 / 702, a mixed batch of 1,811 tokens 257 / 273, 1,021 tokens over 8 bits 145 / 129.
+    // rows idle, two of them on a compute unit wait at barriers of their own, and single tokens share their launch. So
+    // one sequence's go by blocks times positions; us, 128 / 256, 32 heads over 8 of 128, tokens after positions:
+    //   BF16: 64 after 500 27.8 / 29.8, 256 after 0 20.5 / 18.8, 1,021 after 0 48 / 38, 8,192 619 / 584
+    //   F32: 512 after 0 37.4 / 38.8, 512 after 500 53 / 47, 1,021 after 4,000 199 / 179
+    //   8 bits, BF16: 512 after 500 42.7 / 45.1, 256 after 1,000 39.7 / 42.7, 512 after 1,000 51 / 46, 1,021 after
+    //   2,500 122 / 107
+    // and several sequences' by blocks alone: BF16, 24 sequences of 1,811 tokens 198 / 267, 4 of 4,096 215 / 221,
+    // 8 of 8,192 515 / 522; in 8 bits 276 / 310, 302 / 269, 726 / 683.
     const int64_t rows = tokens * group;
-    p.many_rows = dim > 64 && dim <= 128 && rows / 256 * kv_heads >= (quantized ? 64 : 768) ? 256 : 128;
+    bool large;
+    if (!by_offsets && sequences == 1) {
+      const int64_t blocks = ceil_div(rows, 256) * kv_heads;
+      large = blocks * seen > (quantized ? 3 << 15 : f32 ? 1 << 15 : 1 << 13) && blocks >= (quantized ? 24 : 1);
+    } else {
+      large = rows / 256 * kv_heads >= (quantized ? 384 : 768);
+    }
+    p.many_rows = large && dim > 64 && dim <= 128 ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
     p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 25);
   }
@@ -1699,7 +1712,7 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   while (((uint64_t)a.page_units << 27) > ((uint64_t)1 << a.page_shift)) ++a.page_shift;
   a.page_magic = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page_units - 1) / a.page_units);
   const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
-                            a.p.offsets != nullptr, a.key_scales != nullptr);
+                            a.p.offsets != nullptr, a.key_scales != nullptr, sizeof(T) == 4);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,
                   (long long)plan.bytes);
@@ -1726,10 +1739,10 @@ extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens
   if (const int bad = check_attention("drift_paged_attention_workspace", heads, kv_heads, head_dim, window, sinks,
                                       longest))
     return bad;
-  // with offsets or without, over either cache
-  for (const int kind : {0, 1, 2, 3})
+  // with offsets or without, over either cache, in either type
+  for (int kind = 0; kind < 8; ++kind)
     *bytes = std::max(*bytes, plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest, kind & 1,
-                                      kind & 2).bytes);
+                                      kind & 2, kind & 4).bytes);
   return 0;
 }
 
