@@ -351,7 +351,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // Instructions as __builtin_amdgcn_sched_group_barrier counts them.
 constexpr int kVectors = 0x2, kProducts = 0x8, kReads = 0x100;
 
-// A lane's eight weights as the product takes them: F16, and for F32 results the
+// A lane's eight weights as the product takes them: F16, and with two terms the
 // F16 remainder too.
 template <int TERMS>
 struct Halves {
@@ -391,7 +391,8 @@ constexpr float kLift = 14.0f;
 // column.
 //
 // Rows of queries are scaled by a power of two each to below 2^15 (BF16 exactly, down
-// to 2^-32 of the row's largest; F32 as two F16 terms, 22 bits), their scores scaled back in F32. In 8 bits the
+// to 2^-32 of the row's largest; F32 as two F16 terms, 22 bits, since there are no F32
+// products near the F16 ones' rate), their scores scaled back in F32. In 8 bits the
 // codes are F16 numbers, a key's scale multiplies its score and a value's is part of
 // its weight, which has a running maximum of its own then.
 //
@@ -412,6 +413,10 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   constexpr int kWaves = kFewWaves;
   constexpr int TOK = I8 ? 64 : 32, NT = TOK / 16;  // positions a tile, and row tiles of its scores
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  // Over the F16 cache weights have 22 bits for BF16 results too, since memory hides the second term (decode batch 256 us,
+  // 259 with one): what is rounded to BF16 is the F32 result. In 8 bits, where the codes' conversions count and the
+  // cache's own rounding is 2^-8, they have 11 (heads of 64: 105 us, 117 with two; of 128 159 / 161).
+  constexpr int kWeightTerms = I8 ? TERMS : 2;
   constexpr int KS = DP / 32, DT = DP / 16;         // products along a head, value tiles
   auto& merged = shared.merged;
   auto& stats = shared.stats;
@@ -699,13 +704,13 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
     }
 #pragma unroll
     for (int n = 0; n < TOK / 32; ++n) {
-      Halves<TERMS> weights[C];
+      Halves<kWeightTerms> weights[C];
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = weight[c][2 * n + e / 4][e % 4];
-        weights[c] = halves_of<TERMS>(x);
+        weights[c] = halves_of<kWeightTerms>(x);
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -715,7 +720,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int m = 0; m < TERMS; ++m)
+          for (int m = 0; m < kWeightTerms; ++m)
             acc[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, weights[c].term[m], acc[c][d], 0, 0, 0);
       }
     }
@@ -831,6 +836,10 @@ struct ManyTile {
 template <typename T, bool I8, int DP, int WAVES>
 __device__ __forceinline__ void many_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
                                            unsigned blocks, char (&tiles)[2 * ManyTile<I8, DP>::kBytes]) {
+  // BF16's weights have one term, 11 bits: a row's result is then within 2^-11 of its values' sizes before it is rounded
+  // to 8 bits, and over many positions their roundings cancel (0.0017 off 64 bits either way, the rounding to BF16's
+  // own). A second term costs a fifth to a third: prefill 647 us, 851 with it, window chunk 47 / 56, mixed batch
+  // 177 / 225, chunk over 8 bits 120 / 141.
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   constexpr int kThreads = 64 * WAVES;
   constexpr int kRows = WAVES * 32;  // rows a block

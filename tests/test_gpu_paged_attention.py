@@ -1160,3 +1160,17 @@ def test_masked_content_leaves_a_decode_steps_bits_alone(hip, kind, dtype, dim, 
             cache.keys[page, off], cache.values[page, :, :, off] = -128, 127
             cache.keyScales[page, :, off], cache.valueScales[page, :, off] = junk, junk
         assert torch.equal(run(hip, case, q, 0.09, window, offsets=False), first), f"{junk} in masked places"
+
+
+@pytest.mark.parametrize("window", [None, d.AttentionWindow(300, 4)])
+@pytest.mark.parametrize("start,tokens,heads,kv,dim", [(517, 1, 32, 8, 128), (4000, 1, 32, 8, 128), (2000, 1, 16, 2, 256),
+                                                       (900, 3, 16, 4, 64), (700, 12, 8, 2, 128), (33, 5, 6, 2, 20)])
+def test_few_rows_results_in_bf16_are_the_f32_ones_rounded(hip, window, start, tokens, heads, kv, dim):
+    step(f"BF16 results of few rows {tokens} tokens at {start}, {heads}/{kv} heads of {dim} {window}")
+    # a BF16 query is an F32 one whose second F16 term is 0: over the F16 cache nothing else is rounded to fewer bits
+    # than for F32 results before the last step
+    case = Case("f16", [start], [tokens], kv, dim, 16, seed=73)
+    q = normal(74, (tokens, heads, dim), torch.bfloat16, 2.0).to(DEV)
+    scale = 1 / math.sqrt(dim)
+    one, other = (run(hip, case, x, scale, window, single=True) for x in (q, q.float()))
+    assert torch.equal(one, other.bfloat16())
