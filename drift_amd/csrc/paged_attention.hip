@@ -234,8 +234,8 @@ __device__ __forceinline__ void attend_row(const T* queries, T* out, const Atten
 // Every row by itself, for what the tile kernels do not take: a block of four waves
 // (one, where the grid would not hold them) a row, each with every fourth tile, joined
 // in LDS. Loads of a position a lane, and a cache read once a query head, bound it:
-// one token of each of 64 sequences at 2,000 positions, 32 heads over 4 of 512 1.63 ms
-// (12.6 with a wave a row, value by value), over 8 of 100 1.12 ms (2.56).
+// one token of each of 64 sequences at 2,000 positions, 32 heads over 4 of 512 1.65 ms
+// (12.6 with a wave a row, value by value), over 8 of 100 1.13 ms (2.56).
 constexpr int kRowWaves = 4;
 
 template <typename T, bool I8, bool WIDE>
@@ -397,10 +397,10 @@ constexpr float kLift = 14.0f;
 // its weight, which has a running maximum of its own then.
 //
 // Memory bounds it where there is enough to do: one token of each of 64 sequences of
-// 400 to 8,000 positions, 32 heads over 8 of 128, 246 us (1,249 MB, 5.1 TB/s), in 8 bits
-// 150 us (645 MB; the codes' conversions add to it); one of 517 positions 11 us, a chain
-// of dependent loads. Tiles staged in LDS, as attend_many's, gain nothing here: no other
-// wave reads them.
+// 400 to 8,000 positions, 32 heads over 8 of 128, 248 us (1,249 MB, 5.0 TB/s; vector
+// instructions issue 17% of the time), in 8 bits 151 us (645 MB; 37%, the codes'
+// conversions); one of 517 positions 11 us, a chain of dependent loads. Tiles staged in
+// LDS, as attend_many's, gain nothing here: no other wave reads them.
 constexpr int kFewWaves = 4;
 template <int DP, int C>
 struct FewShared {
@@ -426,12 +426,12 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   const int kv = block % (unsigned)a.kv_heads;
   const unsigned rest = block / (unsigned)a.kv_heads;
   // A unit's splits lie far apart: blocks go to the eight dies in turn, and where splits are neighbours those that have
-  // nothing to do are some dies' alone (64 sequences of 400 to 8,000 over 8 bits 158 us, 168 with neighbours).
+  // nothing to do are some dies' alone (64 sequences of 400 to 8,000 over 8 bits 155 us, 163 with neighbours).
   const unsigned all_units = (unsigned)(a.p.sequences * a.few_units);
   const int split = rest / all_units;
   const unsigned unit = rest % all_units;
-  // (and its later units, of which most sequences have none: 64 single tokens in 4 units each, given by offsets, 235 us,
-  // 414 with a sequence's units as neighbours, whose first are all dealt to the same quarter of a die)
+  // (and its later units, of which most sequences have none: 64 single tokens in 4 units each, given by offsets, 244 us,
+  // 457 with a sequence's units as neighbours, whose first are all dealt to the same quarter of a die)
   const int s = (int)(unit % (unsigned)a.p.sequences), nth = (int)(unit / (unsigned)a.p.sequences);
   const Span span = span_of<false>(a.p, s);
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
@@ -821,11 +821,13 @@ __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(c
 // it by more than kSlack (in powers of two), which keeps the rescaling of the
 // results out of most tiles: weights then reach 2^(kManyLift + kSlack) at most.
 //
-// The vector unit bounds it, beside the products it feeds (two waves a SIMD, by
-// registers): BF16, 8,192 tokens of a prompt, 32 heads over 8 of 128, 599 us (550 GFLOP, 918
-// TFLOP/s); heads of 64, 4,096 tokens in windows of 1,024 41 us (420 TFLOP/s: an
-// exponential has half the products); F32, 509 tokens after 3,591, 16 heads over 2 of 256,
-// 99 us with the join (two terms of 32 GFLOP); 1,021 tokens after 2,500 over 8 bits 104 us.
+// What bounds it are the waits between scores, weights and products, which two waves a
+// SIMD (by registers; one for heads of 256) cover in part: of the time of 8,192 BF16 tokens
+// of a prompt, 32 heads over 8 of 128, 605 us (550 GFLOP, 909 TFLOP/s), vector instructions
+// issue 47% and matrix products run 39%; of 4,096 tokens in windows of 1,024, heads of 64,
+// 42 us (410 TFLOP/s), 43 and 15%; of 509 F32 tokens after 3,591, 16 heads over 2 of 256, 97
+// us with the join (two terms of 32 GFLOP), 25 and 26%; of 1,021 after 2,500 over 8 bits, 106
+// us with the join, 44 and 19%.
 template <bool I8, int DP>
 struct ManyTile {
   static constexpr int kValues = 64 * DP * 2, kScales = 2 * kValues, kExponents = kScales + 2 * 64 * 4;
@@ -858,7 +860,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   const int thread = threadIdx.x, lane = thread & 63, wave = uniform(thread >> 6), col = lane & 31, h = lane >> 5;
   const int kv = block % (unsigned)a.kv_heads;
   const unsigned rest = block / (unsigned)a.kv_heads;
-  // A unit's splits lie far apart, as in attend_few (a mixed batch of 4 key heads in two splits 182 us, 315 with
+  // A unit's splits lie far apart, as in attend_few (a mixed batch of 4 key heads in two splits 171 us, 218 with
   // neighbours: half the dies idle); the last rows first: they have the most positions
   const unsigned all_units = blocks / (unsigned)(a.kv_heads * a.splits);
   const int split = rest / all_units;
@@ -1390,8 +1392,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
 
 // Both in one launch: the chunks' blocks, then the single tokens', whose reads fill the
 // time that the last chunks' products leave. 6 chunks (1,793 tokens) and 18 single tokens
-// over up to 6,000 positions, 28 heads over 4 of 128: 174 us, 172 and 49 in launches of
-// their own. The longest chunk's blocks bound it.
+// over up to 6,000 positions, 28 heads over 4 of 128: 162 us, 226 in launches of their
+// own. The longest chunk's blocks bound it.
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* queries, T* out, AttentionArgs few,
                                                                      AttentionArgs many, unsigned many_blocks) {
@@ -1412,7 +1414,7 @@ constexpr int kJoinRows = FEW ? 16 : 32;
 template <typename T, bool I8, bool FEW, int DP>
 __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
   // (many rows have few splits: two fours a lane let each wave have twice the rows on the way; 2 splits of 32,672 rows
-  // of 128 values 9.5 us, 16.4 by one)
+  // of 128 values 9.4 us, 11.5 by one)
   constexpr int V = FEW ? 1 : 2, N = FEW ? 8 : 4;  // fours of values a lane, splits at a time
   constexpr int L = DP / 4 / V, kRows = kJoinRows<FEW>;  // lanes a row, rows a block
   __shared__ RowScratch scratch[4];
@@ -1552,8 +1554,8 @@ constexpr int64_t kSplitBlocks = 16384;
 Split split_of(int64_t blocks, int64_t positions, int64_t wanted, int64_t least, int64_t most) {
   const int64_t tiles = std::max<int64_t>(ceil_div(positions, 64), 1);
   const int64_t chunk = std::min(std::max(ceil_div(tiles * blocks, wanted), least), most);
-  const int64_t splits = std::min(ceil_div(tiles, chunk), std::min<int64_t>(std::max<int64_t>(kSplitBlocks / blocks, 1), 1024));
-  return {(int)splits, (int)std::min<int64_t>(chunk, INT32_MAX)};
+  const int64_t room = std::min<int64_t>(std::max<int64_t>(kSplitBlocks / blocks, 1), 1024);
+  return {(int)std::min(ceil_div(tiles, chunk), room), (int)std::min<int64_t>(chunk, INT32_MAX)};
 }
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
@@ -1562,15 +1564,17 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
   const int64_t seen = window ? std::min(longest, window + sinks + std::min(each, (int64_t)kFewRows)) : longest;
-  // (16 rows a unit while a sequence has no more on average: 64 sequences of 24 rows at 4,000 positions 307 us in
-  // units of 64, 413 in two of 16 each)
+  // (16 rows a unit while a sequence has no more on average: 64 sequences of 24 rows at 4,000 positions 311 us in
+  // units of 64, 419 in two of 16 each)
   // Where sequences have more than kFewRows rows on average, those with few are single tokens for the most part, and a
-  // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 240 us, 270
-  // with units of 64 rows for all up to 64 (in launches of their own).
+  // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 162 us, 251
+  // with units of 64 rows for all up to 64 (in launches of their own; 226 with 16).
   p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
   p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 16 : each * group <= 16;
-  // Up to 768 positions a second launch takes longer than it saves (one token at 517: 13.5 us, 15.6 in three splits);
-  // splits of 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000: 239 us, 264 by 2,048).
+  // Up to 768 positions a second launch takes longer than it saves (one token at 517 12.5 us, 14.2 in splits, at 767 13.5
+  // and 13.8, at 1,023 15.9 and 14.3; heads of 256 over 8 bits at 500 16.4 and 17.7, at 760 20.1 and 17.7). Splits of
+  // 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000 251 us, in splits of 512 259, of 2,048
+  // 249, of 4,096 271; over 8 bits 155, 173, 154 and 160).
   if (by_offsets || each * group <= kFewRows)
     p.few = seen <= 768 ? Split{1, 1} : split_of(sequences * kv_heads, seen, 1024, 4, 16);
   if (each * group > kFewRows) {
@@ -1596,7 +1600,7 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 25);
   }
   p.few_most = std::min(each * group, (int64_t)p.few_rows);
-  // single tokens' blocks after the chunks' in one launch: the mixed batch 191 us, 239 in two, 213 the other way round
+  // single tokens' blocks after the chunks' in one launch: the mixed batch 162 us, 226 in two, 203 the other way round
   p.both = p.few.splits > 0 && p.many.splits > 0 && p.few16 && p.many_rows == 128;
   // Partials by a row's place suit both kernels at once, since a row is one kernel's: attend_few has slots of its own
   // only where those are fewer (a few sequences' few rows beside long chunks).

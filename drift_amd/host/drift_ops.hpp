@@ -152,7 +152,7 @@ struct PagedCache {
   int64_t headDimension() const { return keys.shape[3]; }
 };
 
-// What a row at position P sees: j > P - positions, and j < sinks.
+// What a row at position P sees of the positions j up to P: j > P - positions, or j < sinks.
 struct AttentionWindow {
   int64_t positions;
   int64_t sinks = 0;

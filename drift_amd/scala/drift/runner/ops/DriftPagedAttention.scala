@@ -26,7 +26,7 @@ final case class QuantizedKvCache(keys: Tensor, values: Tensor, keyScales: Tenso
   def headDimension: Int = dimension.toInt
 }
 
-/** What a row at position P sees: j > P - positions, and j < sinks. */
+/** What a row at position P sees of the positions j up to P: j > P - positions, or j < sinks. */
 final case class AttentionWindow(positions: Int, sinks: Int = 0) {
   require(positions > 0 && sinks >= 0, s"a window of $positions positions with $sinks sinks")
 }

@@ -381,23 +381,31 @@ int drift_paged_read_bf16(uint16_t* k, uint16_t* v, const void* keys, const void
                           int32_t* bad_page, void* stream);
 
 /* Attention of the rows' queries [tokens, heads, head_dim] over the cache into
- * out (like queries; may not share memory with them). The row at position P sees positions
- * j <= P of its sequence; with window > 0 only j > P - window or j < sinks. Head
- * h reads key head h / (heads / kv_heads). out = sum p_j v_j / sum p_j, p_j =
- * exp(scale q.k_j - their maximum), statistics and sums in F32; BF16 outputs
- * rounded once, and their weights p_j rounded to 11 bits. What a row does not
- * see has no part in it, whatever it holds; positions on a page outside the
- * cache are not seen, and *bad_page = 1. A row that sees nothing is zeros.
+ * out (like queries; may not share memory with them). The row at position P sees
+ * positions j <= P of its sequence; with window > 0 only j > P - window or j <
+ * sinks. Head h reads key head h / (heads / kv_heads). out = sum p_j v_j / sum p_j,
+ * p_j = exp(scale q.k_j - their maximum), statistics and sums in F32. Products are
+ * of F16 numbers with sums in F32: F32 queries and the weights p_j are two of them
+ * each, 22 bits; BF16 calls' queries are exact, their outputs rounded once, and
+ * their weights have 22 bits over the F16 cache where a sequence and key head has
+ * few rows (single tokens), else 11. (Heads past 256 values or of other than
+ * multiples of 8, and tensors off 16-byte alignment, take F32 products.) In 8 bits
+ * a value scale below 2^-126 may lose bits or count as 0. What a row does not see
+ * has no part in it, whatever it holds; positions on a page outside the cache are
+ * not seen, and *bad_page = 1. A row that sees nothing is zeros. Rows beside ones
+ * that see an infinity or a NaN may be done one by one, some hundred times as long.
  * head_dim is at most 512.
  * `longest` is the caller's guess of the longest sequence's positions (the page
  * table's room, where nothing better is known; 0: the work is not split): the work
- * is split by it, and any guess gives the same result within rounding. `workspace` (device, 16-byte aligned)
- * has at least the bytes that drift_paged_attention_workspace tells for the same
- * numbers (0: it may be NULL): for a decode step splits * tokens * heads *
- * (head_dim + 3) * 4, with no more splits than leave 16,384 blocks of a sequence,
- * key head and split (64 sequences, 32 heads over 8 of 128: at most 34 MB, however
- * wide the page tables are). The launches write it before they read it, so it may hold
- * anything before, and calls that may run at the same time need one each. The same call gives the same bits every time.
+ * is split by it, and any guess gives the same result within rounding. `workspace`
+ * (device, 16-byte aligned) has at least the bytes that
+ * drift_paged_attention_workspace tells for the same numbers (0: it may be NULL):
+ * for a decode step splits * tokens * heads * (head_dim + 3) * 4, with no more
+ * splits than leave 16,384 blocks of a sequence, key head and split (64 sequences,
+ * 32 heads over 8 of 128: at most 34 MB, however wide the page tables are). The
+ * launches write it before they read it, so it may hold anything before, and calls
+ * that may run at the same time need one each. The same call gives the same bits
+ * every time.
  * The reference's attention (kernels/attention.hip:7-34,227-229,446-456) is one
  * sequence's, without a window. */
 int drift_paged_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
