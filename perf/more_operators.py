@@ -144,7 +144,8 @@ def _starts(case):
 
 
 def _trees(case):
-    """What each drafted token sees of its sequence's, as rows of bits [tokens, words]: itself and its ancestors."""
+    """What each drafted token sees of its sequence's, as rows of bits [tokens, 64-bit words]: itself and its
+    ancestors."""
     each = _new_tokens(case)
     words = -(-int(each.max()) // 64)
     rows = np.zeros((int(each.sum()), words), np.uint64)
@@ -296,7 +297,7 @@ def _inputs(case, seed):
     s["queries"] = normal(case["tokens"], case["heads"], dim, dtype=TYPES[case["type"]], scale=2.0)
     s["scale"] = 1.0 / math.sqrt(dim)
     if op == "tree":
-        s["sees"] = torch.from_numpy(_trees(case).view(np.int64)).to(DEV)
+        s["sees"] = torch.from_numpy(_trees(case).view(np.int32)).to(DEV)
         s["out"] = torch.zeros_like(s["queries"])
     else:
         s["before"] = 0.01 * torch.exp(2.5 * normal(pages, kv, page))
@@ -388,7 +389,7 @@ def _plain_tree(s):
     start = s["starts"].long()[:, None, None]
     j = torch.arange(length, device=DEV)
     bits = s["sees"][rows]  # [sequences, most, words]
-    mine = (bits[..., None] >> torch.arange(64, device=DEV) & 1).flatten(2).bool()
+    mine = (bits[..., None] >> torch.arange(32, device=DEV) & 1).flatten(2).bool()
     mine &= torch.arange(mine.shape[2], device=DEV) < there.sum(1)[:, None, None]
     nth = (j - start).clamp(min=0, max=mine.shape[2] - 1).expand(count, rows.shape[1], length)
     seen = (j >= start) & (j < start + mine.shape[2]) & mine.gather(2, nth)
