@@ -24,6 +24,9 @@ _F64 = ctypes.c_double
 _PAGED_ROWS = [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P]
 _PAGED_ATTENTION = [_P, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32,
                     _I32, _I32, _P, _P, _I64, _P, _P]
+_TREE_ATTENTION = _PAGED_ATTENTION[:-5] + [_P, _I32] + _PAGED_ATTENTION[-5:]
+_ATTENTION_MASS = [_P, _P, _P, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P, _P,
+                   _P, _I64, _P, _P]
 
 # Argument types of every entry point, in the header's order.
 SIGNATURES = {
@@ -77,6 +80,15 @@ SIGNATURES = {
     "drift_paged_attention_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
     "drift_paged_attention_f32": (_I32, _PAGED_ATTENTION),
     "drift_paged_attention_bf16": (_I32, _PAGED_ATTENTION),
+    "drift_tree_attention_f32": (_I32, _TREE_ATTENTION),
+    "drift_tree_attention_bf16": (_I32, _TREE_ATTENTION),
+    "drift_attention_mass_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _P]),
+    "drift_attention_mass_f32": (_I32, _ATTENTION_MASS),
+    "drift_attention_mass_bf16": (_I32, _ATTENTION_MASS),
+    "drift_heaviest": (_I32, [_P, _P, _I32, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P]),
+    "drift_cache_keep_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _P]),
+    "drift_cache_keep": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _P, _I32, _I32, _I32,
+                                _I32, _I32, _P, _I64, _P, _P]),
     "drift_embedding_q8_0_f32": (_I32, [_P, _P, _P, _I64, _I64, _I32, _P, _P]),
     "drift_embedding_q8_0_bf16": (_I32, [_P, _P, _P, _I64, _I64, _I32, _P, _P]),
     "drift_embedding_f32": (_I32, [_P, _I32, _P, _P, _I64, _I64, _I32, _P, _P]),

@@ -47,6 +47,22 @@ __device__ __forceinline__ T uniform(T v) {
 // Positions a sequence can have: a tile past its last still counts in 32 bits.
 constexpr int64_t kMostPositions = INT32_MAX - 127;
 
+// A division by a page's units of 16 positions: with L = ceil(log2 page_units) and M =
+// ceil(2^(27 + L) / page_units), unit M / 2^(27 + L) is above the quotient by less than unit /
+// (2^27 page_units), so for a unit below 2^27 its whole part is the quotient's.
+struct UnitColumns {
+  uint32_t page_units, magic, shift;
+  // the column of a page table that unit `unit` of 16 positions is in
+  __device__ __forceinline__ uint32_t of(uint32_t unit) const { return (uint32_t)(((uint64_t)unit * magic) >> shift); }
+};
+
+inline UnitColumns unit_columns(int32_t page_size) {
+  UnitColumns c{(uint32_t)page_size / 16, 0, 27};
+  while (((uint64_t)c.page_units << 27) > ((uint64_t)1 << c.shift)) ++c.shift;
+  c.magic = (uint32_t)((((uint64_t)1 << c.shift) + c.page_units - 1) / c.page_units);
+  return c;
+}
+
 struct Span {
   int64_t first;         // its first token row
   int32_t rows;          // 0 where the sequence is not described rightly

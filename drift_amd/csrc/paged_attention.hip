@@ -37,15 +37,44 @@ struct AttentionArgs {
   float *statistics, *partials;
   int32_t few_slots, few_units;  // attend_few's rows of partials (0: by place), and units, of a sequence and key head
   int32_t few_rows;   // sequences of at most so many rows (tokens times group) are attend_few's, others attend_many's
-  // page_size / 16, and what divides a unit's number (below 2^27) by it exactly
-  uint32_t page_units, page_magic, page_shift;
+  UnitColumns columns;
+  // of a tree's rows (TREE): what each sees of its sequence's new tokens, `words` words of 32 bits a token
+  const uint32_t* sees;
+  int32_t words;
 };
 
-// The column of a page table that unit `unit` of 16 positions is in: with L = ceil(log2
-// page_units) and M = ceil(2^(27 + L) / page_units), unit M / 2^(27 + L) is above the quotient by
-// less than unit / (2^27 page_units), so its whole part is the quotient's.
-__device__ __forceinline__ uint32_t column_of(const AttentionArgs& a, uint32_t unit) {
-  return (uint32_t)(((uint64_t)unit * a.page_magic) >> a.page_shift);
+// Bits 0 .. n - 1.
+__device__ __forceinline__ uint64_t bits_below(int64_t n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// A tree's row's position: start - 1, and one for each of the sequence's new tokens that it sees.
+__device__ __forceinline__ int64_t tree_position(const AttentionArgs& a, const Span& span, int64_t nth) {
+  const uint32_t* sees = a.sees + (span.first + nth) * a.words;
+  int64_t position = span.start - 1;
+  for (int w = 0; (int64_t)w * 32 < span.rows && w < a.words; ++w)
+    position += __popc(sees[w] & (uint32_t)bits_below(span.rows - w * 32));
+  return position;
+}
+
+// What a tree's row sees of the 64 positions from `base` on: of those before `start` the
+// ones from `low` on and the first `sinks`, of the others those whose bits it has.
+__device__ __forceinline__ uint64_t tree_sees(const AttentionArgs& a, const Span& span, int64_t nth, int64_t base,
+                                              int64_t low, int64_t sinks) {
+  uint64_t seen = bits_below(span.start - base) & (~bits_below(low - base) | bits_below(sinks - base));
+  const int64_t at = base - span.start;  // the first of the positions among the new tokens
+  if (at > -64 && at < span.rows) {
+    const uint32_t* sees = a.sees + (span.first + nth) * a.words;
+    auto word = [&](int w) -> uint64_t { return w < a.words ? sees[w] : 0; };
+    uint64_t bits;
+    if (at < 0) {
+      bits = (word(0) | word(1) << 32) << -at;
+    } else {
+      const int w = (int)(at / 32), shift = (int)(at % 32);
+      bits = (word(w) | word(w + 1) << 32) >> shift;
+      if (shift != 0) bits |= word(w + 2) << (64 - shift);
+    }
+    seen |= bits & bits_below(span.rows - at);
+  }
+  return seen;
 }
 
 __device__ __forceinline__ float f16_value(uint32_t bits) {
@@ -97,18 +126,23 @@ struct RowState {
 // sums, every product of F32 values in F32 and one by one. It takes any head size and
 // whatever the cache holds. WIDE: keys and values on 16-byte alignment, heads of a
 // multiple of 8 values, read in eights; else one by one, at any alignment.
-template <typename T, bool I8, bool WIDE>
+template <typename T, bool I8, bool WIDE, bool TREE>
 __device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& a, const Span& span, int64_t nth, int h,
                                          int from, int step, RowScratch& r, RowState& state) {
   const int lane = threadIdx.x & (kWave - 1), kv = h / a.group;
-  const int64_t position = span.start + nth, row = ((span.first + nth) * a.heads + h) * a.dim;
+  // the last position that may be seen
+  const int64_t position = span.start + (TREE ? span.rows - 1 : nth), row = ((span.first + nth) * a.heads + h) * a.dim;
   wave_sync();
   for (int d = lane; d < a.dim; d += kWave) r.query[d] = load_one(queries + row + d);
   wave_sync();
   constexpr int kEach = kMaxHead / kWave;
   float sums[kEach] = {}, top = -kInfinity, total = 0.0f;
   bool any = false;
-  const int64_t low = a.window ? max(position - a.window + 1, (int64_t)0) : 0;
+  int64_t low = 0;
+  if (a.window) {
+    if constexpr (TREE) low = min(max(tree_position(a, span, nth) - a.window + 1, (int64_t)0), span.start);
+    else low = max(position - a.window + 1, (int64_t)0);
+  }
   const int64_t sink_end = a.window ? min((int64_t)a.sinks, low) : 0;
   for (int64_t tile = from; tile * kWave <= position; tile += step) {
     if (tile * kWave >= sink_end && (tile + 1) * kWave <= low) {  // what lies between is not seen
@@ -116,7 +150,9 @@ __device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& 
       if (tile * kWave > position) break;
     }
     const int64_t j = tile * kWave + lane;
-    bool seen = j <= position && (j >= low || j < sink_end);
+    bool seen;
+    if constexpr (TREE) seen = tree_sees(a, span, nth, tile * kWave, low, sink_end) >> lane & 1;
+    else seen = j <= position && (j >= low || j < sink_end);
     int64_t page = 0, off = 0;
     if (seen) {
       page = span.table[j / a.p.page_size];
@@ -206,11 +242,11 @@ __device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& 
 
 // One row by one wave, for the tile kernels' rows that came out as no numbers: slow,
 // and kept small, since its registers count in every kernel that calls it.
-template <typename T, bool I8>
+template <typename T, bool I8, bool TREE>
 __device__ __noinline__ void attend_row_of(const T* queries, T* out, const AttentionArgs& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
   RowState state;
-  row_part<T, I8, false>(queries, a, span, nth, h, 0, 1, r, state);
+  row_part<T, I8, false, TREE>(queries, a, span, nth, h, 0, 1, r, state);
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t row = ((span.first + nth) * a.heads + h) * a.dim;
   // nothing seen: zeros; nothing but scores of -infinity seen: 0 / 0, as the formula has it
@@ -223,12 +259,12 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const Atten
 
 // Copies of the arguments go by reference: the kernels' own then stay in scalar
 // registers (passed themselves, every use of theirs would read scratch memory).
-template <typename T, bool I8>
+template <typename T, bool I8, bool TREE>
 __device__ __forceinline__ void attend_row(const T* queries, T* out, const AttentionArgs& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
   const AttentionArgs args = a;
   const Span rows = span;
-  attend_row_of<T, I8>(queries, out, args, rows, nth, h, r);
+  attend_row_of<T, I8, TREE>(queries, out, args, rows, nth, h, r);
 }
 
 // Every row by itself, for what the tile kernels do not take: a block of four waves
@@ -238,7 +274,7 @@ __device__ __forceinline__ void attend_row(const T* queries, T* out, const Atten
 // (12.6 with a wave a row, value by value), over 8 of 100 1.13 ms (2.56).
 constexpr int kRowWaves = 4;
 
-template <typename T, bool I8, bool WIDE>
+template <typename T, bool I8, bool WIDE, bool TREE>
 __global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* queries, T* out, AttentionArgs a) {
   __shared__ RowScratch scratch[kRowWaves];
   __shared__ float tops[kRowWaves], totals[kRowWaves];
@@ -252,7 +288,7 @@ __global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* querie
   if (nth >= span.rows) return;
   const int h = blockIdx.x % (unsigned)a.heads;
   RowState state;
-  row_part<T, I8, WIDE>(queries, a, span, nth, h, wave, waves, scratch[wave], state);
+  row_part<T, I8, WIDE, TREE>(queries, a, span, nth, h, wave, waves, scratch[wave], state);
   wave_sync();
 #pragma unroll
   for (int i = 0; i < kMaxHead / kWave; ++i) scratch[wave].query[lane + i * kWave] = state.sums[i];
@@ -407,7 +443,7 @@ struct FewShared {
   float merged[kFewWaves][16][DP + 4], stats[kFewWaves][C * 16][3];
 };
 
-template <typename T, bool I8, int DP, int C>
+template <typename T, bool I8, bool TREE, int DP, int C>
 __device__ __forceinline__ void few_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
                                           FewShared<DP, C>& shared) {
   constexpr int kWaves = kFewWaves;
@@ -502,8 +538,8 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   // the page of unit u (-1: nothing of it is seen, or it names no page), and the unit's place in it
   auto page_of = [&](uint32_t u, uint32_t& off) -> int32_t {
     const uint32_t in = u > units ? units : u;
-    const uint32_t column = column_of(a, in);
-    off = (in - column * a.page_units) * 16;
+    const uint32_t column = a.columns.of(in);
+    off = (in - column * a.columns.page_units) * 16;
     const int32_t page = span.table[column];
     return page;
   };
@@ -791,16 +827,16 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
       RowScratch& scratch = *reinterpret_cast<RowScratch*>(&merged[wave][0][0]);
       for (; again; again &= again - 1) {
         const uint32_t row = row0 + c * 16 + __ffs(again) - 1;
-        attend_row<T, I8>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
+        attend_row<T, I8, TREE>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
       }
     }
   }
 }
 
-template <typename T, bool I8, int DP, int C>
+template <typename T, bool I8, bool TREE, int DP, int C>
 __global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, AttentionArgs a) {
   __shared__ FewShared<DP, C> shared;
-  few_block<T, I8, DP, C>(queries, out, a, blockIdx.x, shared);
+  few_block<T, I8, TREE, DP, C>(queries, out, a, blockIdx.x, shared);
 }
 
 // The many-rows kernel: 32 rows of queries a wave, four or eight waves a block
@@ -835,7 +871,7 @@ struct ManyTile {
   static constexpr int kBytes = I8 ? (kRange + 16 + 255) / 256 * 256 : kScales;
 };
 
-template <typename T, bool I8, int DP, int WAVES>
+template <typename T, bool I8, bool TREE, int DP, int WAVES>
 __device__ __forceinline__ void many_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
                                            unsigned blocks, char (&tiles)[2 * ManyTile<I8, DP>::kBytes]) {
   // BF16's weights have one term, 11 bits: a row's result is then within 2^-11 of its values' sizes before it is rounded
@@ -936,7 +972,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   // a scalar base and an offset that stays. Where pages hold whole tiles, eight
   // chunks of a value's row lie together; else two.
   const uint32_t last_unit = p1 / 16;
-  const bool wide = a.page_units % 4 == 0;
+  const bool wide = a.columns.page_units % 4 == 0;
   constexpr int kUnitThreads = 2 * DP;  // threads that stage a unit's keys, or its values where pages are narrow
   constexpr int kUnits = kThreads >= kUnitThreads ? kThreads / kUnitThreads : 1;  // units that all threads stage at once
   const int wave_unit = kUnits > 1 ? wave / (kUnitThreads / 64) : 0;
@@ -951,8 +987,8 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   uint32_t entry_off;
   auto load_entries = [&](int i) {
     const uint32_t at = min((uint32_t)list.tile(min(i, end - 1)) * 4 + (lane & 3), last_unit);
-    const uint32_t column = column_of(a, at);
-    entry_off = (at - column * a.page_units) * 16;
+    const uint32_t column = a.columns.of(at);
+    entry_off = (at - column * a.columns.page_units) * 16;
     entry = span.table[column];
   };
   struct Pages {
@@ -1380,29 +1416,29 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   RowScratch& scratch = reinterpret_cast<RowScratch*>(tiles)[wave];
   for (uint32_t rest_rows = (uint32_t)again | (uint32_t)(again >> 32); rest_rows; rest_rows &= rest_rows - 1) {
     const uint32_t row = row0 + wave_row + __ffs(rest_rows) - 1;
-    attend_row<T, I8>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
+    attend_row<T, I8, TREE>(queries, out, a, span, row / group, kv * a.group + (int)(row % group), scratch);
   }
 }
 
-template <typename T, bool I8, int DP, int WAVES>
+template <typename T, bool I8, bool TREE, int DP, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
   __shared__ __attribute__((aligned(16))) char tiles[2 * ManyTile<I8, DP>::kBytes];
-  many_block<T, I8, DP, WAVES>(queries, out, a, blockIdx.x, gridDim.x, tiles);
+  many_block<T, I8, TREE, DP, WAVES>(queries, out, a, blockIdx.x, gridDim.x, tiles);
 }
 
 // Both in one launch: the chunks' blocks, then the single tokens', whose reads fill the
 // time that the last chunks' products leave. 6 chunks (1,793 tokens) and 18 single tokens
 // over up to 6,000 positions, 28 heads over 4 of 128: 162 us, 226 in launches of their
 // own. The longest chunk's blocks bound it.
-template <typename T, bool I8, int DP>
+template <typename T, bool I8, bool TREE, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* queries, T* out, AttentionArgs few,
                                                                      AttentionArgs many, unsigned many_blocks) {
   constexpr size_t kMany = 2 * ManyTile<I8, DP>::kBytes, kFew = sizeof(FewShared<DP, 1>);
   __shared__ __attribute__((aligned(16))) char shared[kMany > kFew ? kMany : kFew];
   if (blockIdx.x < many_blocks)
-    many_block<T, I8, DP, 4>(queries, out, many, blockIdx.x, many_blocks, reinterpret_cast<char (&)[kMany]>(shared));
+    many_block<T, I8, TREE, DP, 4>(queries, out, many, blockIdx.x, many_blocks, reinterpret_cast<char (&)[kMany]>(shared));
   else
-    few_block<T, I8, DP, 1>(queries, out, few, blockIdx.x - many_blocks, reinterpret_cast<FewShared<DP, 1>&>(shared));
+    few_block<T, I8, TREE, DP, 1>(queries, out, few, blockIdx.x - many_blocks, reinterpret_cast<FewShared<DP, 1>&>(shared));
 }
 
 // Joins the splits of attend_few (FEW) or attend_many: a block takes up to
@@ -1411,7 +1447,7 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* qu
 template <bool FEW>
 constexpr int kJoinRows = FEW ? 16 : 32;
 
-template <typename T, bool I8, bool FEW, int DP>
+template <typename T, bool I8, bool TREE, bool FEW, int DP>
 __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
   // (many rows have few splits: two fours a lane let each wave have twice the rows on the way; 2 splits of 32,672 rows
   // of 128 values 9.4 us, 11.5 by one)
@@ -1503,7 +1539,7 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
     for (uint64_t again = __ballot(there && odd); again;) {
       const int which = (__ffsll((unsigned long long)again) - 1) / L;
       const uint32_t r = first + which, t = r / group;
-      attend_row<T, I8>(queries, out, a, span, t, kv * a.group + (int)(r - t * group), scratch[wave]);
+      attend_row<T, I8, TREE>(queries, out, a, span, t, kv * a.group + (int)(r - t * group), scratch[wave]);
       again &= L == 64 ? 0 : ~(((1ull << (L % 64)) - 1) << (which * L));
     }
   }
@@ -1623,15 +1659,15 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
 template <typename T, bool I8, int DP>
 constexpr int kManyTiles = DP > 128 ? 1 : DP <= 64 || (sizeof(T) == 2 && !I8) ? 4 : 2;
 
-template <typename T, bool I8, bool FEW, int DP>
+template <typename T, bool I8, bool TREE, bool FEW, int DP>
 int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, int64_t units, int rows, int tile,
          hipStream_t st) {
-  hipLaunchKernelGGL((attend_join<T, I8, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows<FEW>))), dim3(256),
+  hipLaunchKernelGGL((attend_join<T, I8, TREE, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows<FEW>))), dim3(256),
                      0, st, queries, out, a, rows, tile);
   return launched(entry);
 }
 
-template <typename T, bool I8, int DP>
+template <typename T, bool I8, bool TREE, int DP>
 int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArgs& a, const Plan& plan, hipStream_t st) {
   AttentionArgs few = a, many = a;
   const int few_tiles = plan.few16 ? 1 : kManyTiles<T, I8, DP>, few_rows = 16 * few_tiles;
@@ -1657,32 +1693,32 @@ int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArg
   const unsigned many_blocks = (unsigned)(many_units * many.splits * a.kv_heads);
   const dim3 block(256);
   if (plan.both) {
-    hipLaunchKernelGGL((attend_both<T, I8, DP>), dim3(many_blocks + few_blocks), block, 0, st, queries, out, few, many,
+    hipLaunchKernelGGL((attend_both<T, I8, TREE, DP>), dim3(many_blocks + few_blocks), block, 0, st, queries, out, few, many,
                        many_blocks);
   } else {
     if (few_blocks > 0) {
-      if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, DP, 1>), dim3(few_blocks), block, 0, st, queries, out, few);
-      else hipLaunchKernelGGL((attend_few<T, I8, DP, kManyTiles<T, I8, DP>>), dim3(few_blocks), block, 0, st, queries, out, few);
+      if (plan.few16) hipLaunchKernelGGL((attend_few<T, I8, TREE, DP, 1>), dim3(few_blocks), block, 0, st, queries, out, few);
+      else hipLaunchKernelGGL((attend_few<T, I8, TREE, DP, kManyTiles<T, I8, DP>>), dim3(few_blocks), block, 0, st, queries, out, few);
     }
     if (many_blocks > 0) {
       if constexpr (DP == 128) {
         if (plan.many_rows == 256)
-          hipLaunchKernelGGL((attend_many<T, I8, DP, 8>), dim3(many_blocks), dim3(512), 0, st, queries, out, many);
-        else hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
+          hipLaunchKernelGGL((attend_many<T, I8, TREE, DP, 8>), dim3(many_blocks), dim3(512), 0, st, queries, out, many);
+        else hipLaunchKernelGGL((attend_many<T, I8, TREE, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
       } else {
-        hipLaunchKernelGGL((attend_many<T, I8, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
+        hipLaunchKernelGGL((attend_many<T, I8, TREE, DP, 4>), dim3(many_blocks), block, 0, st, queries, out, many);
       }
     }
   }
   if (const int bad = launched(entry)) return bad;
   if (few_blocks > 0 && few.splits > 1)
-    if (const int bad = join<T, I8, true, DP>(entry, queries, out, few, few_units, few_rows, I8 ? 64 : 32, st)) return bad;
+    if (const int bad = join<T, I8, TREE, true, DP>(entry, queries, out, few, few_units, few_rows, I8 ? 64 : 32, st)) return bad;
   if (many_blocks > 0 && many.splits > 1)
-    return join<T, I8, false, DP>(entry, queries, out, many, many_units, plan.many_rows, 64, st);
+    return join<T, I8, TREE, false, DP>(entry, queries, out, many, many_units, plan.many_rows, 64, st);
   return 0;
 }
 
-template <typename T, bool I8>
+template <typename T, bool I8, bool TREE>
 int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, bool aligned, hipStream_t st) {
   const int64_t row_blocks = units_of(a.p, 1, 0, 1) * a.heads;
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
@@ -1691,20 +1727,20 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
   // (the tile kernels' offsets within a page, and rows of scales, have 32 bits)
   const bool small = (int64_t)a.p.page_size * a.kv_heads * a.dim * 2 < (int64_t)1 << 31 &&
                      (int64_t)a.p.cache_pages * a.kv_heads < (int64_t)1 << 31;
-  if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
+  if (TREE || !aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
     const dim3 grid((unsigned)row_blocks), block(kWave * (row_blocks * kRowWaves > kOneWaveBlocks ? 1 : kRowWaves));
     const bool wide = a.dim % 8 == 0 && aligned16(a.keys) && aligned16(a.values);
-    if (wide) hipLaunchKernelGGL((attend_rows<T, I8, true>), grid, block, 0, st, queries, out, a);
-    else hipLaunchKernelGGL((attend_rows<T, I8, false>), grid, block, 0, st, queries, out, a);
+    if (wide) hipLaunchKernelGGL((attend_rows<T, I8, true, TREE>), grid, block, 0, st, queries, out, a);
+    else hipLaunchKernelGGL((attend_rows<T, I8, false, TREE>), grid, block, 0, st, queries, out, a);
     return launched(entry);
   }
   a.few_rows = plan.few.splits == 0 ? 0 : plan.many.splits == 0 ? INT32_MAX : plan.few_rows;
-  if (a.dim <= 64) return launch_tiles<T, I8, 64>(entry, queries, out, a, plan, st);
-  if (a.dim <= 128) return launch_tiles<T, I8, 128>(entry, queries, out, a, plan, st);
-  return launch_tiles<T, I8, 256>(entry, queries, out, a, plan, st);
+  if (a.dim <= 64) return launch_tiles<T, I8, TREE, 64>(entry, queries, out, a, plan, st);
+  if (a.dim <= 128) return launch_tiles<T, I8, TREE, 128>(entry, queries, out, a, plan, st);
+  return launch_tiles<T, I8, TREE, 256>(entry, queries, out, a, plan, st);
 }
 
-template <typename T>
+template <typename T, bool TREE>
 int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a, int64_t longest, void* workspace,
                     int64_t workspace_bytes, void* stream) {
   clear_error();
@@ -1712,6 +1748,12 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   if (const int bad = check_attention(entry, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest)) return bad;
   if (a.p.tokens == 0 || a.p.sequences == 0) return 0;
   if (!queries || !out) return refuse("%s: null tensor", entry);
+  if (TREE) {
+    if (!a.sees) return refuse("%s: null tensor", entry);
+    if (a.words <= 0) return refuse("%s: %d words of what a row sees", entry, a.words);
+    if ((reinterpret_cast<uintptr_t>(a.sees) & 3) != 0)
+      return refuse("%s: what the rows see not aligned to its elements", entry);
+  }
   if ((const void*)queries == (const void*)out) return refuse("%s: out is queries", entry);
   if ((reinterpret_cast<uintptr_t>(queries) | reinterpret_cast<uintptr_t>(out)) % sizeof(T) != 0)
     return refuse("%s: queries or out not aligned to their elements", entry);
@@ -1720,10 +1762,7 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   if ((from > to ? from - to : to - from) / sizeof(T) < (uint64_t)a.p.tokens * a.heads * a.dim)
     return refuse("%s: out overlaps queries", entry);
   a.group = a.heads / a.kv_heads;
-  a.page_units = a.p.page_size / 16;
-  a.page_shift = 27;
-  while (((uint64_t)a.page_units << 27) > ((uint64_t)1 << a.page_shift)) ++a.page_shift;
-  a.page_magic = (uint32_t)((((uint64_t)1 << a.page_shift) + a.page_units - 1) / a.page_units);
+  a.columns = unit_columns(a.p.page_size);
   const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
                             a.p.offsets != nullptr, a.key_scales != nullptr, sizeof(T) == 4);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
@@ -1734,8 +1773,8 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   const bool aligned = a.dim % 8 == 0 && aligned16(queries) && aligned16(out) && aligned16(a.keys) && aligned16(a.values) &&
                        (!a.key_scales || (aligned16(a.key_scales) && aligned16(a.value_scales)));
   const hipStream_t st = (hipStream_t)stream;
-  return a.key_scales ? attend<T, true>(entry, queries, out, a, plan, aligned, st)
-                      : attend<T, false>(entry, queries, out, a, plan, aligned, st);
+  return a.key_scales ? attend<T, true, TREE>(entry, queries, out, a, plan, aligned, st)
+                      : attend<T, false, TREE>(entry, queries, out, a, plan, aligned, st);
 }
 
 }  // namespace
@@ -1759,10 +1798,10 @@ extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens
   return 0;
 }
 
-#define DRIFT_ATTENTION_ARGS                                                                                        \
+#define DRIFT_ATTENTION_ARGS(sees, words)                                                                                   \
   AttentionArgs {                                                                                                   \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, 0, 0, 0 \
+        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, {}, (const uint32_t*)sees, words \
   }
 
 extern "C" int drift_paged_attention_f32(const float* queries, const void* keys, const void* values,
@@ -1773,7 +1812,7 @@ extern "C" int drift_paged_attention_f32(const float* queries, const void* keys,
                                          int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                          int32_t sinks, int32_t longest, float* out, void* workspace,
                                          int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<float>("drift_paged_attention_f32", queries, out, DRIFT_ATTENTION_ARGS, longest, workspace,
+  return paged_attention<float, false>("drift_paged_attention_f32", queries, out, DRIFT_ATTENTION_ARGS(nullptr, 0), longest, workspace,
                                 workspace_bytes, stream);
 }
 
@@ -1785,6 +1824,31 @@ extern "C" int drift_paged_attention_bf16(const uint16_t* queries, const void* k
                                           int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                           int32_t sinks, int32_t longest, uint16_t* out, void* workspace,
                                           int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<uint16_t>("drift_paged_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS, longest,
+  return paged_attention<uint16_t, false>("drift_paged_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS(nullptr, 0), longest,
                                    workspace, workspace_bytes, stream);
+}
+
+extern "C" int drift_tree_attention_f32(const float* queries, const void* keys, const void* values,
+                                        const float* key_scales, const float* value_scales,
+                                        const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                                        const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,
+                                        int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                        int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
+                                        const int32_t* sees, int32_t words, float* out, void* workspace,
+                                        int64_t workspace_bytes, int32_t* bad_page, void* stream) {
+  return paged_attention<float, true>("drift_tree_attention_f32", queries, out, DRIFT_ATTENTION_ARGS(sees, words),
+                                      longest, workspace, workspace_bytes, stream);
+}
+
+extern "C" int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const void* values,
+                                         const float* key_scales, const float* value_scales,
+                                         const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                                         const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                                         int32_t start, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                         int32_t head_dim, int32_t page_size, float scale, int32_t window,
+                                         int32_t sinks, int32_t longest, const int32_t* sees, int32_t words,
+                                         uint16_t* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page,
+                                         void* stream) {
+  return paged_attention<uint16_t, true>("drift_tree_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS(sees, words),
+                                         longest, workspace, workspace_bytes, stream);
 }

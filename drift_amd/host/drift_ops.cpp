@@ -328,6 +328,48 @@ void checkAttention(const char* operation, const Tensor& queries, const PagedCac
             text("a window of ", window->positions, " positions with ", window->sinks, " sinks"));
 }
 
+int64_t checkSees(const char* operation, const Tensor& sees, int64_t tokens) {
+  require(sees.dtype == DType::I32 && sees.shape.rank() == 2 && sees.shape[0] == tokens && sees.shape[1] > 0,
+          text(operation, ": what the rows see is I32 [", tokens, ", words], not ", name(sees.dtype), " ",
+               sees.shape.str()));
+  return sees.shape[1];
+}
+
+void checkMass(const char* operation, const Tensor& mass, const PagedCache* cache) {
+  requireF32(operation, {&mass});
+  require(mass.shape.rank() == 3, text(operation, ": masses are [pages, kvHeads, pageSize], got ", mass.shape.str()));
+  if (cache)
+    require(mass.shape == Shape{cache->pages(), cache->kvHeads(), cache->pageSize},
+            text(operation, ": masses ", mass.shape.str(), " for a cache ", cache->keys.shape.str()));
+}
+
+int64_t checkTables(const char* operation, const Tensor& pageTables) {
+  require(pageTables.dtype == DType::I32 && pageTables.shape.rank() == 2,
+          text(operation, ": page tables are I32 [sequences, pages], not ", name(pageTables.dtype), " ",
+               pageTables.shape.str()));
+  return pageTables.shape[0];
+}
+
+void checkVector(const char* operation, const char* what, const Tensor& vector, int64_t count) {
+  require(vector.dtype == DType::I32 && vector.shape == Shape{count},
+          text(operation, ": ", what, " ", name(vector.dtype), " ", vector.shape.str(), " for ", count, " sequences"));
+}
+
+void checkKeep(const PagedCache& cache, const KeptRows& rows) {
+  const char* operation = "cacheKeep";
+  const int64_t count = checkTables(operation, rows.pageTables);
+  if (rows.counts) checkVector(operation, "counts", *rows.counts, count);
+  if (rows.starts) checkVector(operation, "starts", *rows.starts, count);
+  const Shape& kept = rows.kept.shape;
+  require(rows.kept.dtype == DType::I32 && (kept.rank() == 2 || kept.rank() == 3) && kept[0] == count &&
+              (kept.rank() == 2 || kept[1] == cache.kvHeads()),
+          text(operation, ": kept ", name(rows.kept.dtype), " ", kept.str(), " for ", count, " sequences of ",
+               cache.kvHeads(), " heads"));
+  if (rows.into)
+    require(checkTables(operation, *rows.into) == count,
+            text(operation, ": into ", rows.into->shape.str(), " for ", count, " sequences"));
+}
+
 // ops/LayoutOps.scala:73-80
 void checkSplitHalves(const Tensor& x, const Tensor& first, const Tensor& second) {
   checkElementwise("splitHalves", {&x});
@@ -945,8 +987,9 @@ int64_t HipOps::attentionWorkspace(const Tensor& queries, const PagedCache& cach
 
 void HipOps::attend(const char* operation, const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
                     float scale, const Tensor& out, const Tensor& workspace,
-                    const std::optional<AttentionWindow>& window, int32_t* badPage) {
+                    const std::optional<AttentionWindow>& window, int32_t* badPage, const Tensor* sees) {
   checkAttention(operation, queries, cache, out, window);
+  const int32_t words = sees ? (int32_t)checkSees(operation, *sees, queries.shape[0]) : 0;
   const auto from = reinterpret_cast<uintptr_t>(queries.data), to = reinterpret_cast<uintptr_t>(out.data);
   require((from > to ? from - to : to - from) >= (uintptr_t)queries.byteSize(),
           text(operation, from == to ? ": out is queries" : ": out overlaps queries"));
@@ -955,7 +998,23 @@ void HipOps::attend(const char* operation, const Tensor& queries, const PagedCac
   const auto kvHeads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();
   const int32_t positions = window ? (int32_t)window->positions : 0, sinks = window ? (int32_t)window->sinks : 0;
   const int64_t bytes = workspace.data ? workspace.byteSize() : 0;
-  if (isBf16(queries))
+  if (sees && isBf16(queries))
+    launched("drift_tree_attention_bf16",
+             drift_tree_attention_bf16(at<uint16_t>(queries), cache.keys.data, cache.values.data,
+                                       scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                       (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                       kvHeads, dimension, cache.pageSize, scale, positions, sinks, p.longest,
+                                       at<int32_t>(*sees), words, at<uint16_t>(out), workspace.data, bytes, badPage,
+                                       stream_));
+  else if (sees)
+    launched("drift_tree_attention_f32",
+             drift_tree_attention_f32(at<float>(queries), cache.keys.data, cache.values.data,
+                                      scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables, p.tablePages,
+                                      (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start, tokens, heads,
+                                      kvHeads, dimension, cache.pageSize, scale, positions, sinks, p.longest,
+                                      at<int32_t>(*sees), words, at<float>(out), workspace.data, bytes, badPage,
+                                      stream_));
+  else if (isBf16(queries))
     launched("drift_paged_attention_bf16",
              drift_paged_attention_bf16(at<uint16_t>(queries), cache.keys.data, cache.values.data,
                                         scalesOf(cache.keyScales), scalesOf(cache.valueScales), p.tables,
@@ -981,6 +1040,99 @@ void HipOps::attentionSequences(const Tensor& queries, const PagedCache& cache, 
                                 const Tensor& out, const Tensor& workspace,
                                 const std::optional<AttentionWindow>& window, int32_t* badPage) {
   attend("attentionSequences", queries, cache, sequences, scale, out, workspace, window, badPage);
+}
+
+void HipOps::attentionTree(const Tensor& queries, const PagedCache& cache, const Sequences& sequences,
+                           const Tensor& sees, float scale, const Tensor& out, const Tensor& workspace,
+                           const std::optional<AttentionWindow>& window, int32_t* badPage) {
+  attend("attentionTree", queries, cache, sequences, scale, out, workspace, window, badPage, &sees);
+}
+
+// ---- eviction from the paged cache
+
+int64_t HipOps::attentionMassWorkspace(const Tensor& queries, const PagedCache& cache, const Sequences& sequences) {
+  checkAttention("attentionMassWorkspace", queries, cache, queries, {});
+  const Paging p = pagingOf("attentionMassWorkspace", cache, sequences, queries.shape[0]);
+  int64_t bytes = 0;
+  const int code = drift_attention_mass_workspace(p.count, (int32_t)queries.shape[0], (int32_t)queries.shape[1],
+                                                  (int32_t)cache.kvHeads(), (int32_t)cache.headDimension(), p.longest,
+                                                  &bytes);
+  if (code != 0) throw HipException("drift_attention_mass_workspace", code, drift_last_error());
+  return bytes;
+}
+
+void HipOps::attentionMass(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, float scale,
+                           const Tensor& mass, const Tensor& workspace, const std::optional<Tensor>& before,
+                           int32_t* badPage) {
+  checkAttention("attentionMass", queries, cache, queries, {});
+  checkMass("attentionMass", mass, &cache);
+  if (before) checkMass("attentionMass", *before, &cache);
+  const Paging p = pagingOf("attentionMass", cache, sequences, queries.shape[0]);
+  const auto tokens = (int32_t)queries.shape[0], heads = (int32_t)queries.shape[1];
+  const auto kvHeads = (int32_t)cache.kvHeads(), dimension = (int32_t)cache.headDimension();
+  const float* held = before ? at<float>(*before) : nullptr;
+  const int64_t bytes = workspace.data ? workspace.byteSize() : 0;
+  if (isBf16(queries))
+    launched("drift_attention_mass_bf16",
+             drift_attention_mass_bf16(at<uint16_t>(queries), cache.keys.data, scalesOf(cache.keyScales), p.tables,
+                                       p.tablePages, (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start,
+                                       tokens, heads, kvHeads, dimension, cache.pageSize, scale, p.longest, held,
+                                       at<float>(mass), workspace.data, bytes, badPage, stream_));
+  else
+    launched("drift_attention_mass_f32",
+             drift_attention_mass_f32(at<float>(queries), cache.keys.data, scalesOf(cache.keyScales), p.tables,
+                                      p.tablePages, (int32_t)cache.pages(), p.starts, p.offsets, p.count, p.start,
+                                      tokens, heads, kvHeads, dimension, cache.pageSize, scale, p.longest, held,
+                                      at<float>(mass), workspace.data, bytes, badPage, stream_));
+}
+
+void HipOps::heaviest(const Tensor& mass, const Tensor& pageTables, const Tensor& lengths, int64_t sinks,
+                      int64_t recent, const Tensor& kept, const Tensor& counts, int32_t* badPage) {
+  const char* operation = "heaviest";
+  checkMass(operation, mass, nullptr);
+  const int64_t count = checkTables(operation, pageTables), pageSize = mass.shape[2];
+  require(pageSize > 0 && pageSize % 16 == 0, text("pages of ", pageSize, " tokens: not a multiple of 16"));
+  checks::checkVector(operation, "lengths", lengths, count);
+  checks::checkVector(operation, "counts", counts, count);
+  require(kept.dtype == DType::I32 && kept.shape.rank() == 3 && kept.shape[0] == count && kept.shape[1] == mass.shape[1],
+          text(operation, ": kept ", name(kept.dtype), " ", kept.shape.str(), " for ", count, " sequences of ",
+               mass.shape[1], " heads"));
+  const int64_t keep = kept.shape[2];
+  require(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
+          text(operation, ": the first ", sinks, " and the last ", recent, " positions of ", keep, " kept"));
+  launched("drift_heaviest",
+           drift_heaviest(at<float>(mass), at<int32_t>(pageTables), (int32_t)pageTables.shape[1],
+                          (int32_t)mass.shape[0], at<int32_t>(lengths), (int32_t)count, (int32_t)mass.shape[1],
+                          (int32_t)pageSize, (int32_t)sinks, (int32_t)recent, (int32_t)keep, at<int32_t>(kept),
+                          at<int32_t>(counts), badPage, stream_));
+}
+
+int64_t HipOps::cacheKeepWorkspace(const PagedCache& cache, const KeptRows& rows) {
+  checkKeep(cache, rows);
+  if (rows.into && rows.into->data != rows.pageTables.data) return 0;
+  int64_t bytes = 0;
+  const int code = drift_cache_keep_workspace((int32_t)rows.kept.shape[0], (int32_t)rows.kept.shape.last(),
+                                              (int32_t)cache.kvHeads(), (int32_t)cache.headDimension(),
+                                              cache.keyScales ? 1 : 0, &bytes);
+  if (code != 0) throw HipException("drift_cache_keep_workspace", code, drift_last_error());
+  return bytes;
+}
+
+void HipOps::cacheKeep(const PagedCache& cache, const KeptRows& rows, const Tensor& workspace,
+                       const std::optional<Tensor>& mass, int32_t* badPage) {
+  checkKeep(cache, rows);
+  if (mass) checkMass("cacheKeep", *mass, &cache);
+  const Shape& kept = rows.kept.shape;
+  launched("drift_cache_keep",
+           drift_cache_keep(cache.keys.data, cache.values.data, scalesOf(cache.keyScales), scalesOf(cache.valueScales),
+                            mass ? at<float>(*mass) : nullptr, at<int32_t>(rows.pageTables),
+                            (int32_t)rows.pageTables.shape[1], rows.into ? at<int32_t>(*rows.into) : nullptr,
+                            rows.into ? (int32_t)rows.into->shape[1] : 0, (int32_t)cache.pages(),
+                            at<int32_t>(rows.kept), kept.rank() == 3 ? (int32_t)kept[1] : 1,
+                            rows.counts ? at<int32_t>(*rows.counts) : nullptr,
+                            rows.starts ? at<int32_t>(*rows.starts) : nullptr, (int32_t)kept[0], (int32_t)kept.last(),
+                            (int32_t)cache.kvHeads(), (int32_t)cache.headDimension(), cache.pageSize, workspace.data,
+                            workspace.data ? workspace.byteSize() : 0, badPage, stream_));
 }
 
 // ---- tables

@@ -180,6 +180,15 @@ struct CacheRows {
   CacheRows(const Sequences& sequences) : sequences(sequences) {}
 };
 
+// Rows that cacheKeep moves: position starts[s] + i (without `starts` i) gets what
+// position kept[s, head, i] holds, for i < counts[s] (without `counts` all); all I32,
+// kept [sequences, kvHeads, most], or [sequences, most] for all heads alike. With
+// `into`, page tables [sequences, pages], rows go to those pages, else to the same.
+struct KeptRows {
+  Tensor pageTables, kept;
+  std::optional<Tensor> counts, starts, into;
+};
+
 // A table's storage type (tensor/DType.scala:14-66): values per block of
 // bytes, its GGUF type id (the kernels' `format`) and the alignment its
 // blocks' fields need.
@@ -269,6 +278,14 @@ void checkSequences(const char* operation, const Sequences& sequences, int64_t t
 int64_t checkCacheRows(const char* operation, const Tensor& k, const Tensor& v, const PagedCache& cache);
 void checkAttention(const char* operation, const Tensor& queries, const PagedCache& cache, const Tensor& out,
                     const std::optional<AttentionWindow>& window);
+// what a tree's rows see [tokens, words]: the words
+int64_t checkSees(const char* operation, const Tensor& sees, int64_t tokens);
+// masses [pages, kvHeads, pageSize], of `cache` where there is one
+void checkMass(const char* operation, const Tensor& mass, const PagedCache* cache);
+// page tables [sequences, pages]: the sequences
+int64_t checkTables(const char* operation, const Tensor& pageTables);
+void checkVector(const char* operation, const char* what, const Tensor& vector, int64_t count);
+void checkKeep(const PagedCache& cache, const KeptRows& rows);
 void checkSplitHalves(const Tensor& x, const Tensor& first, const Tensor& second);
 int checkConvert(const Tensor& x, const Tensor& out);  // the reference's conversion code
 }  // namespace checks
@@ -388,6 +405,33 @@ class HipOps {
                           const Tensor& out, const Tensor& workspace,
                           const std::optional<AttentionWindow>& window = {}, int32_t* badPage = nullptr);
 
+  // attention of trees of drafted tokens: as attentionSequences (and with its
+  // workspace), but of its sequence's new rows a row sees those that `sees` names
+  // (I32 [tokens, words], bit b of word w: row 32 w + b), and every position
+  // before them; `window` counts back from start - 1 + the rows that it sees
+  void attentionTree(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, const Tensor& sees,
+                     float scale, const Tensor& out, const Tensor& workspace,
+                     const std::optional<AttentionWindow>& window = {}, int32_t* badPage = nullptr);
+
+  // ---- eviction from the paged cache
+  // What the rows' attention weighs each position of their sequences, into mass F32
+  // [pages, kvHeads, pageSize], added to `before` (which may be mass) where the
+  // position precedes the rows. `workspace`: attentionMassWorkspace's bytes.
+  int64_t attentionMassWorkspace(const Tensor& queries, const PagedCache& cache, const Sequences& sequences);
+  void attentionMass(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, float scale,
+                     const Tensor& mass, const Tensor& workspace, const std::optional<Tensor>& before = {},
+                     int32_t* badPage = nullptr);
+  // The positions to keep, ascending, into kept I32 [sequences, kvHeads, keep]: of a
+  // sequence of lengths[s] > keep positions the first `sinks`, the last `recent` and
+  // the heaviest between, of a shorter one all; -1 past counts[s].
+  void heaviest(const Tensor& mass, const Tensor& pageTables, const Tensor& lengths, int64_t sinks, int64_t recent,
+                const Tensor& kept, const Tensor& counts, int32_t* badPage = nullptr);
+  // The kept rows moved together, all read before any is written; `mass` moves with
+  // them. `workspace`: cacheKeepWorkspace's bytes (none with rows.into).
+  int64_t cacheKeepWorkspace(const PagedCache& cache, const KeptRows& rows);
+  void cacheKeep(const PagedCache& cache, const KeptRows& rows, const Tensor& workspace,
+                 const std::optional<Tensor>& mass = {}, int32_t* badPage = nullptr);
+
   // ---- tables (ops/LinearOps.scala:16-33, ops/MemoryOps.scala:46)
   // An id outside the table (which the reference refuses) gets a zero row
   // and sets *badId (device int32) when given.
@@ -438,7 +482,7 @@ class HipOps {
                 const Tensor& v, int32_t* badPage);
   void attend(const char* operation, const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
               float scale, const Tensor& out, const Tensor& workspace, const std::optional<AttentionWindow>& window,
-              int32_t* badPage);
+              int32_t* badPage, const Tensor* sees = nullptr);
   void decodeRotated(const RotatedTable& table, const Tensor& out, const Tensor* ids, int32_t* badId);
 };
 

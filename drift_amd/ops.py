@@ -550,6 +550,43 @@ def checkAttention(operation: str, queries, cache, out) -> tuple:
     return tokens, heads
 
 
+def checkSees(operation: str, sees, tokens: int) -> int:
+    """What a tree's rows see [tokens, words]; returns the words."""
+    if not (sees.dtype == I32 and sees.dim() == 2 and sees.shape[0] == tokens and sees.shape[1] > 0):
+        raise ValueError(f"{operation}: what the rows see is I32 [{tokens}, words], not {_name(sees.dtype)} "
+                         f"{_shape(sees)}")
+    return sees.shape[1]
+
+
+def checkMass(operation: str, mass, cache=None) -> None:
+    """Masses F32 [pages, kvHeads, pageSize], of `cache` where there is one."""
+    requireF32(operation, mass)
+    if mass.dim() != 3:
+        raise ValueError(f"{operation}: masses are [pages, kvHeads, pageSize], got {_shape(mass)}")
+    if cache is not None and tuple(mass.shape) != (cache.pages, cache.kvHeads, cache.pageSize):
+        raise ValueError(f"{operation}: masses {_shape(mass)} for a cache {_shape(cache.keys)}")
+
+
+def checkTables(operation: str, pageTables, **vectors) -> int:
+    """Page tables I32 [sequences, pages], and I32 vectors [sequences] (None where there is none); returns the number
+    of sequences."""
+    if not (pageTables.dtype == I32 and pageTables.dim() == 2):
+        raise ValueError(f"{operation}: page tables are I32 [sequences, pages], not {_name(pageTables.dtype)} "
+                         f"{_shape(pageTables)}")
+    count = pageTables.shape[0]
+    for name, v in vectors.items():
+        if v is not None and not (v.dtype == I32 and v.dim() == 1 and v.shape[0] == count):
+            raise ValueError(f"{operation}: {name} {_name(v.dtype)} {_shape(v)} for {count} sequences")
+    return count
+
+
+def checkApart(operation: str, what: str, first, second) -> None:
+    """Two tensors that share no memory."""
+    ends = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (first, second)]
+    if ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]:
+        raise ValueError(f"{operation}: {what}")
+
+
 def checkSplitHalves(x, first, second) -> None:
     """ops/LayoutOps.scala:73-80 (F32, or BF16 here)."""
     checkElementwise("splitHalves", x)
@@ -621,7 +658,7 @@ class HipOps:
         self._quantizedValues: Optional[QuantizedValues] = None
         self._quantizedBuffer: Optional[torch.Tensor] = None
         self._scratch: Optional[torch.Tensor] = None
-        self._attentionBytes: dict = {}  # attention's workspace by its sizes
+        self._attentionBytes: dict = {}  # calls' workspaces by their sizes
 
     def _stream(self) -> int:
         if self.stream is not None:
@@ -1081,10 +1118,29 @@ class HipOps:
         self._attention("attentionSequences", queries, cache, paging, tensors, tokens, heads, paging[5], longest,
                         scale, out, window, badPage)
 
+    def attentionTree(self, queries, cache, sequences: Sequences, sees, scale: float, out,
+                      window: Optional[AttentionWindow] = None, badPage: Optional[torch.Tensor] = None) -> None:
+        """Attention of trees of drafted tokens, a tree a sequence: as
+        attentionSequences, but of its sequence's new rows a token sees those
+        that `sees` names (I32 [tokens, words], bit b of word w: the
+        sequence's row 32 w + b; its ancestors and itself), and every position
+        before them. The keys and values of row i lie at position starts[s] +
+        i, whatever its depth; with `window` the positions before the new
+        rows count back from starts[s] - 1 + the rows that the token sees
+        (what it hides of the new rows is the caller's to leave out).
+        `cacheKeep` then moves an accepted path's rows together."""
+        tokens, heads = checkAttention("attentionTree", queries, cache, out)
+        words = checkSees("attentionTree", sees, tokens)
+        paging, tensors = self._paging("attentionTree", cache, sequences, None, tokens)
+        room = sequences.pageTables.shape[1] * cache.pageSize
+        longest = min(sequences.longest, room) if sequences.longest else room
+        self._attention("attentionTree", queries, cache, paging, tensors, tokens, heads, paging[5], longest, scale,
+                        out, window, badPage, sees, words)
+
     def _attention(self, operation, queries, cache, paging, tensors, tokens, heads, count, longest, scale, out,
-                   window, badPage) -> None:
+                   window, badPage, sees=None, words=0) -> None:
         checkBadPage(operation, badPage)
-        self._onOneDevice(operation, (queries, out, badPage, *tensors))
+        self._onOneDevice(operation, (queries, out, badPage, sees, *tensors))
         apart = abs(queries.data_ptr() - out.data_ptr())
         if apart < queries.numel() * queries.element_size():
             raise ValueError(f"{operation}: out {'is' if apart == 0 else 'overlaps'} queries")
@@ -1093,25 +1149,140 @@ class HipOps:
         # scratch of this call's own, from torch's pool on the launch's stream: calls on several streams and
         # captured graphs never share it
         numbers = (count, tokens, heads, cache.kvHeads, cache.headDimension, positions, sinks, longest)
-        size = self._attentionBytes.get(numbers)
+        size = self._told("drift_paged_attention_workspace", *numbers)
+        workspace = self._workspace(size, queries.device)
+        keys, values, keyScales, valueScales, *_ = tensors
+        entry, tree = ("drift_paged_attention", ()) if sees is None else ("drift_tree_attention", (_ptr(sees), words))
+        self._launch(f"{entry}_{_suffix(queries.dtype)}", _ptr(queries), _ptr(keys), _ptr(values),
+                     _ptr(keyScales), _ptr(valueScales), *paging, tokens, heads, cache.kvHeads, cache.headDimension,
+                     cache.pageSize, scale, positions, sinks, longest, *tree, _ptr(out), _ptr(workspace), size,
+                     _ptr(badPage))
+
+    def _workspace(self, size: int, device) -> Optional[torch.Tensor]:
+        """Scratch of one call's own, from torch's pool on the launch's stream."""
+        if size == 0:
+            return None
+        if self.stream is None:
+            return torch.empty(size, dtype=torch.uint8, device=device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(size, dtype=torch.uint8, device=device)
+
+    # ---------------------------------------------------------------- eviction
+
+    def attentionMass(self, queries, cache, sequences: Sequences, scale: float, mass,
+                      before: Optional[torch.Tensor] = None, badPage: Optional[torch.Tensor] = None) -> None:
+        """What the rows' attention weighs each position of their sequences,
+        by which `heaviest` says which to keep: mass F32 [pages, kvHeads,
+        pageSize], at every position up to a sequence's last row, the sum over
+        the rows that see it and the heads of the key head of the row's weight
+        for it (queries, cache, sequences and scale as attentionSequences has
+        them), where the position precedes the rows added to `before` (laid
+        out the same, or `mass` itself; None: 0). Other positions are left as
+        they are. Two sequences that share a page leave either's sum there."""
+        operation = "attentionMass"
+        tokens, heads = checkAttention(operation, queries, cache, queries)
+        checkMass(operation, mass, cache)
+        if before is not None:
+            checkMass(operation, before, cache)
+        paging, tensors = self._paging(operation, cache, sequences, None, tokens)
+        checkBadPage(operation, badPage)
+        self._onOneDevice(operation, (queries, mass, before, badPage, *tensors))
+        if before is not None and before.data_ptr() != mass.data_ptr():
+            checkApart(operation, "mass overlaps before", mass, before)
+        room = sequences.pageTables.shape[1] * cache.pageSize
+        longest = min(sequences.longest or room, room, _MOST_POSITIONS)
+        numbers = (paging[5], tokens, heads, cache.kvHeads, cache.headDimension, longest)
+        size = self._told("drift_attention_mass_workspace", *numbers)
+        workspace = self._workspace(size, queries.device)
+        keys, _, keyScales, *_ = tensors
+        self._launch(f"drift_attention_mass_{_suffix(queries.dtype)}", _ptr(queries), _ptr(keys), _ptr(keyScales),
+                     *paging, tokens, heads, cache.kvHeads, cache.headDimension, cache.pageSize, scale, longest,
+                     _ptr(before), _ptr(mass), _ptr(workspace), size, _ptr(badPage))
+
+    def heaviest(self, mass, pageTables, lengths, sinks: int, recent: int, kept, counts,
+                 badPage: Optional[torch.Tensor] = None) -> None:
+        """The positions that each sequence and key head is to keep, into kept
+        I32 [sequences, kvHeads, keep]: of a sequence of lengths[s] > keep
+        positions (I32 [sequences]) the first `sinks`, the last `recent`, and
+        of those between the ones of the largest mass (equal ones the lower
+        positions; a NaN is above every number), of a shorter one all; in
+        ascending order, -1 past counts[s] = min(lengths[s], keep) (I32
+        [sequences]). mass is F32 [pages, kvHeads, pageSize], pageTables I32
+        [sequences, table pages]."""
+        operation = "heaviest"
+        checkMass(operation, mass)
+        pages, kvHeads, pageSize = mass.shape
+        if pageSize <= 0 or pageSize % 16 != 0:
+            raise ValueError(f"{operation}: pages of {pageSize} tokens: not a multiple of 16")
+        count = checkTables(operation, pageTables, lengths=lengths, counts=counts)
+        if not (kept.dtype == I32 and kept.dim() == 3 and tuple(kept.shape[:2]) == (count, kvHeads)):
+            raise ValueError(f"{operation}: kept {_name(kept.dtype)} {_shape(kept)} for {count} sequences of "
+                             f"{kvHeads} heads")
+        keep = kept.shape[2]
+        if sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"{operation}: the first {sinks} and the last {recent} positions of {keep} kept")
+        checkBadPage(operation, badPage)
+        self._onOneDevice(operation, (mass, pageTables, lengths, kept, counts, badPage))
+        checkApart(operation, "counts overlap lengths", lengths, counts)
+        self._launch("drift_heaviest", _ptr(mass), _ptr(pageTables), pageTables.shape[1], pages, _ptr(lengths), count,
+                     kvHeads, pageSize, sinks, recent, keep, _ptr(kept), _ptr(counts), _ptr(badPage))
+
+    def cacheKeep(self, cache, pageTables, kept, counts: Optional[torch.Tensor] = None,
+                  starts: Optional[torch.Tensor] = None, into: Optional[torch.Tensor] = None,
+                  mass: Optional[torch.Tensor] = None, badPage: Optional[torch.Tensor] = None) -> None:
+        """Moves rows of the cache (a KvCache or a QuantizedKvCache) together:
+        position starts[s] + i (None: i) of each sequence gets what position
+        kept[s, head, i] holds, for i < counts[s] (None: all); kept is I32
+        [sequences, kvHeads, most], or [sequences, most] for all heads alike,
+        in any order. Every row is read before any is written. With `into`,
+        page tables [sequences, pages], the rows go to those pages instead,
+        of which the lists may name none; the pages that rows go to belong to
+        one sequence each. `mass` (attentionMass's) moves with its positions.
+        Entries that are no position of a page of the cache move nothing,
+        `badPage` set.
+
+        After `heaviest` the cut sequences hold counts[s] positions: the next
+        calls' starts. After `attentionTree` kept are starts[s] + the accepted
+        path's rows, `starts` the sequences' starts."""
+        operation = "cacheKeep"
+        quantized = isinstance(cache, QuantizedKvCache)
+        if cache.keys.shape[1] != cache.pageSize:
+            raise ValueError(f"{operation}: pages of {cache.pageSize} tokens in a cache {_shape(cache.keys)}")
+        count = checkTables(operation, pageTables, counts=counts, starts=starts)
+        heads = kept.shape[1] if kept.dim() == 3 else 1
+        if not (kept.dtype == I32 and kept.dim() in (2, 3) and kept.shape[0] == count and
+                (kept.dim() == 2 or heads == cache.kvHeads)):
+            raise ValueError(f"{operation}: kept {_name(kept.dtype)} {_shape(kept)} for {count} sequences of "
+                             f"{cache.kvHeads} heads")
+        if into is not None and checkTables(operation, into) != count:
+            raise ValueError(f"{operation}: into {_shape(into)} for {count} sequences")
+        if mass is not None:
+            checkMass(operation, mass, cache)
+        checkBadPage(operation, badPage)
+        scales = (cache.keyScales, cache.valueScales) if quantized else (None, None)
+        self._onOneDevice(operation, (cache.keys, cache.values, *scales, mass, pageTables, into, kept, counts, starts,
+                                      badPage))
+        most, size = kept.shape[-1], 0
+        if into is None or into.data_ptr() == pageTables.data_ptr():
+            size = self._told("drift_cache_keep_workspace", count, most, cache.kvHeads, cache.headDimension,
+                              int(quantized))
+        workspace = self._workspace(size, kept.device)
+        self._launch("drift_cache_keep", _ptr(cache.keys), _ptr(cache.values), _ptr(scales[0]), _ptr(scales[1]),
+                     _ptr(mass), _ptr(pageTables), pageTables.shape[1], _ptr(into),
+                     0 if into is None else into.shape[1], cache.pages, _ptr(kept), heads, _ptr(counts), _ptr(starts),
+                     count, most, cache.kvHeads, cache.headDimension, cache.pageSize, _ptr(workspace), size,
+                     _ptr(badPage))
+
+    def _told(self, entry: str, *numbers) -> int:
+        """The bytes of scratch that `entry` tells for a call of these numbers."""
+        size = self._attentionBytes.get((entry, *numbers))
         if size is None:
             told = ctypes.c_int64()
-            _lib.call("drift_paged_attention_workspace", *numbers, ctypes.addressof(told))
-            size = self._attentionBytes[numbers] = told.value
+            _lib.call(entry, *numbers, ctypes.addressof(told))
             if len(self._attentionBytes) > 4096:
                 self._attentionBytes.clear()
-        if size == 0:
-            workspace = None
-        elif self.stream is None:
-            workspace = torch.empty(size, dtype=torch.uint8, device=queries.device)
-        else:
-            with torch.cuda.stream(self.stream):
-                workspace = torch.empty(size, dtype=torch.uint8, device=queries.device)
-        keys, values, keyScales, valueScales, *_ = tensors
-        self._launch(f"drift_paged_attention_{_suffix(queries.dtype)}", _ptr(queries), _ptr(keys), _ptr(values),
-                     _ptr(keyScales), _ptr(valueScales), *paging, tokens, heads, cache.kvHeads, cache.headDimension,
-                     cache.pageSize, scale, positions, sinks, longest, _ptr(out), _ptr(workspace), size,
-                     _ptr(badPage))
+            size = self._attentionBytes[(entry, *numbers)] = told.value
+        return size
 
     # ---------------------------------------------------------------- embedding, convert
 

@@ -95,6 +95,42 @@ final class DriftKernels(path: Path) {
   val pagedAttentionWorkspace = bind("drift_paged_attention_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P)
 
+  // ... longest, what the rows see and its words, ...
+  val treeAttention = twins("drift_tree_attention", P, P, P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, JAVA_INT, JAVA_INT, P, JAVA_INT, P, P,
+    JAVA_LONG, P, P)
+  val attentionMass = twins("drift_attention_mass", P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, P, P, P, JAVA_LONG, P, P)
+  val attentionMassWorkspace = bind("drift_attention_mass_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+    JAVA_INT, P)
+  val heaviest = bind("drift_heaviest", P, P, JAVA_INT, JAVA_INT, P, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+    JAVA_INT, P, P, P, P)
+  val cacheKeep = bind("drift_cache_keep", P, P, P, P, P, P, JAVA_INT, P, JAVA_INT, JAVA_INT, P, JAVA_INT, P, P,
+    JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, JAVA_LONG, P, P)
+  val cacheKeepWorkspace = bind("drift_cache_keep_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P)
+
+  /** The bytes of scratch that an `attentionMass` of these numbers takes. */
+  def massWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, longest: Int): Long = {
+    val arena = Arena.ofConfined()
+    try {
+      val bytes = arena.allocate(JAVA_LONG)
+      check("drift_attention_mass_workspace", (attentionMassWorkspace.invokeExact(sequences, tokens, heads, kvHeads,
+        headDimension, longest, bytes): Int))
+      bytes.get(JAVA_LONG, 0)
+    } finally arena.close()
+  }
+
+  /** The bytes of scratch that a `cacheKeep` in place of these numbers takes. */
+  def keepWorkspace(sequences: Int, most: Int, kvHeads: Int, headDimension: Int, quantized: Int): Long = {
+    val arena = Arena.ofConfined()
+    try {
+      val bytes = arena.allocate(JAVA_LONG)
+      check("drift_cache_keep_workspace", (cacheKeepWorkspace.invokeExact(sequences, most, kvHeads, headDimension,
+        quantized, bytes): Int))
+      bytes.get(JAVA_LONG, 0)
+    } finally arena.close()
+  }
+
   /** The bytes of scratch that a `pagedAttention` of these numbers takes. */
   def attentionWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, window: Int,
                          sinks: Int, longest: Int): Long = {

@@ -424,6 +424,93 @@ int drift_paged_attention_bf16(const uint16_t* queries, const void* keys, const 
                                uint16_t* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page,
                                void* stream);
 
+/* Attention of trees of drafted tokens: drift_paged_attention_* with the rows of a
+ * sequence seeing, of its new tokens, those that `sees` names (device int32
+ * [tokens, words], bit b of word w of a row: its sequence's new token 32 w + b, at
+ * position start + 32 w + b of the cache; bits of tokens that the sequence does not
+ * have count for nothing, and tokens past the words are not seen). Every position
+ * before the new tokens is seen; with a window those j > P - window or j < sinks,
+ * P = start - 1 + the new tokens that the row sees, its depth in the tree (what the
+ * window hides of the new tokens is the caller's to leave out). A row that sees nothing
+ * is zeros. The workspace is drift_paged_attention_workspace's. For a
+ * verified chain (each token seeing those up to itself) it is drift_paged_attention_*.
+ * Replaces nothing of the reference, which drafts one chain. */
+int drift_tree_attention_f32(const float* queries, const void* keys, const void* values, const float* key_scales,
+                             const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                             int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                             int32_t start, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                             int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
+                             const int32_t* sees, int32_t words, float* out, void* workspace, int64_t workspace_bytes,
+                             int32_t* bad_page, void* stream);
+int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const void* values, const float* key_scales,
+                              const float* value_scales, const int32_t* page_tables, int32_t table_pages,
+                              int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,
+                              int32_t start, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                              int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
+                              const int32_t* sees, int32_t words, uint16_t* out, void* workspace,
+                              int64_t workspace_bytes, int32_t* bad_page, void* stream);
+
+/* ---------------------------------------------------------------- eviction from the paged cache
+ * drift_attention_mass_*: what the rows' attention weighs each position of their
+ * sequences: mass [cache_pages, kv_heads, page_size] (F32), at every position up to
+ * a sequence's last row's, the sum over its rows that see it and the heads of the key
+ * head of p_j = exp(scale q.k_j - m) / sum exp(scale q.k_j - m), added to `before`
+ * (laid out the same; may be mass itself, not otherwise share memory with it; NULL: 0)
+ * where the position precedes the sequence's rows. Rows, paging, scores and workspace
+ * rules are drift_paged_attention_*'s, without a window; other positions of mass are
+ * left as they are, and so are ones on a page outside the cache, *bad_page set. The
+ * same call gives the same bits every time. Two sequences that share a page leave
+ * either's sum there. keys and values of drift_paged_write_*: the values are not read.
+ *
+ * drift_heaviest: the `keep` positions that each sequence and key head is to keep:
+ * of a sequence of lengths[s] > keep positions the first `sinks`, the last `recent`,
+ * and of those between the keep - sinks - recent of the largest mass (equal ones the
+ * lower positions; 0 and -0 are equal, a NaN is above every number, a position on a
+ * page outside the cache below, *bad_page set); of a shorter one all. kept [sequences, kv_heads,
+ * keep] has them in ascending order, -1 past counts[s] = min(lengths[s], keep); a
+ * length below 0 or past the page table counts as 0, *bad_page set.
+ *
+ * drift_cache_keep: moves rows of the cache: for each sequence, key head and i <
+ * counts[s] (NULL: `most`), position starts[s] + i (NULL: i) gets the key and value
+ * (codes and scales in 8 bits), and in `mass` (nullable) the mass, that position
+ * kept[s, head, i] holds; kept is [sequences, kept_heads, most], kept_heads 1 (the
+ * same list for every head) or kv_heads, in any order. Every row is read before
+ * any is written: in place (`into` NULL) lists may move rows over each other. With
+ * `into`, page tables [sequences, into_pages], rows go to positions of those pages,
+ * which may hold none that the lists name (else what moves there is either); the
+ * pages that rows go to belong to one sequence each. Entries that are no position of
+ * their page table, or lie on a page outside the cache, and rows that would go to
+ * one, move nothing, and a count outside 0 .. most or a start below 0 leaves its
+ * sequence as it is; *bad_page is set. In place it takes the workspace (device, 16-byte
+ * aligned) that drift_cache_keep_workspace tells, written before it is read; with
+ * `into` none.
+ * Replaces nothing of the reference, whose cache only grows
+ * (src/drift/runner/ops/KvCache.scala:5-22). */
+int drift_attention_mass_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                   int32_t head_dim, int32_t longest, int64_t* bytes);
+int drift_attention_mass_f32(const float* queries, const void* keys, const float* key_scales,
+                             const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                             const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,
+                             int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                             float scale, int32_t longest, const float* before, float* mass, void* workspace,
+                             int64_t workspace_bytes, int32_t* bad_page, void* stream);
+int drift_attention_mass_bf16(const uint16_t* queries, const void* keys, const float* key_scales,
+                              const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                              const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,
+                              int32_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page_size,
+                              float scale, int32_t longest, const float* before, float* mass, void* workspace,
+                              int64_t workspace_bytes, int32_t* bad_page, void* stream);
+int drift_heaviest(const float* mass, const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
+                   const int32_t* lengths, int32_t sequences, int32_t kv_heads, int32_t page_size, int32_t sinks,
+                   int32_t recent, int32_t keep, int32_t* kept, int32_t* counts, int32_t* bad_page, void* stream);
+int drift_cache_keep_workspace(int32_t sequences, int32_t most, int32_t kv_heads, int32_t head_dim, int32_t quantized,
+                               int64_t* bytes);
+int drift_cache_keep(void* keys, void* values, float* key_scales, float* value_scales, float* mass,
+                     const int32_t* page_tables, int32_t table_pages, const int32_t* into, int32_t into_pages,
+                     int32_t cache_pages, const int32_t* kept, int32_t kept_heads, const int32_t* counts,
+                     const int32_t* starts, int32_t sequences, int32_t most, int32_t kv_heads, int32_t head_dim,
+                     int32_t page_size, void* workspace, int64_t workspace_bytes, int32_t* bad_page, void* stream);
+
 /* ---------------------------------------------------------------- embedding
  * Rows `ids` of a Q8_0 table ([vocab, cols], cols a multiple of 32: per 32
  * values a 34-byte block, fp16 scale d then 32 int8 codes), decoded as

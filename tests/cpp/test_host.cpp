@@ -789,6 +789,125 @@ GPU_TEST(paged_attention_over_both_caches) {
   }
 }
 
+CHECK_TEST(trees_masses_and_moves_are_checked) {
+  HipOps hip;
+  const KvCache cache = KvCache::of(fake(DType::F16, {2, 16, 2, 64}), fake(DType::F16, {2, 2, 64, 16}), 16);
+  const Tensor q = fake(DType::F32, {3, 4, 64}), out = fake(DType::F32, {3, 4, 64}, 8192), none{DType::U8, {0}, nullptr};
+  const Sequences s{fake(DType::I32, {2, 2}), fake(DType::I32, {2}), fake(DType::I32, {3}), 0};
+  refused([&] { hip.attentionTree(q, cache, s, fake(DType::I32, {2, 1}), 1.0f, out, none); },
+          "attentionTree: what the rows see is I32 [3, words], not I32 [2×1]");
+  refused([&] { hip.attentionTree(q, cache, s, fake(DType::I32, {3, 1}), 1.0f, q, none); }, "attentionTree: out is queries");
+  const Tensor mass = fake(DType::F32, {2, 2, 16});
+  refused([&] { hip.attentionMass(q, cache, s, 1.0f, fake(DType::F32, {2, 16, 2}), none); },
+          "attentionMass: masses [2×16×2] for a cache [2×16×2×64]");
+  refused([&] { hip.attentionMass(q, cache, s, 1.0f, mass, none, fake(DType::F32, {2, 32})); },
+          "attentionMass: masses are [pages, kvHeads, pageSize], got [2×32]");
+  expect(hip.attentionMassWorkspace(q, cache, s) > 0, "scratch of masses");
+  refused<HipException>([&] { hip.attentionMass(q, cache, s, 1.0f, mass, none); }, "workspace");
+  const Tensor lengths = fake(DType::I32, {2}), counts = fake(DType::I32, {2}, 8192), kept = fake(DType::I32, {2, 2, 8});
+  refused([&] { hip.heaviest(mass, s.pageTables, lengths, 5, 4, kept, counts); },
+          "heaviest: the first 5 and the last 4 positions of 8 kept");
+  refused([&] { hip.heaviest(mass, s.pageTables, lengths, 1, 1, fake(DType::I32, {2, 3, 8}), counts); },
+          "heaviest: kept I32 [2×3×8] for 2 sequences of 2 heads");
+  refused([&] { hip.heaviest(mass, s.pageTables, fake(DType::I32, {3}), 1, 1, kept, counts); },
+          "heaviest: lengths I32 [3] for 2 sequences");
+  refused<HipException>([&] { hip.heaviest(mass, s.pageTables, lengths, 1, 1, kept, lengths); }, "counts overlap lengths");
+  KeptRows rows{s.pageTables, kept, {}, {}, {}};
+  expect(hip.cacheKeepWorkspace(cache, rows) > 0, "scratch of rows moved in place");
+  refused<HipException>([&] { hip.cacheKeep(cache, rows, none); }, "workspace");
+  rows.into = fake(DType::I32, {3, 2}, 8192);
+  refused([&] { hip.cacheKeep(cache, rows, none); }, "cacheKeep: into [3×2] for 2 sequences");
+  rows.into = fake(DType::I32, {2, 5}, 8192);
+  expect(hip.cacheKeepWorkspace(cache, rows) == 0, "no scratch into other pages");
+  rows.kept = fake(DType::I32, {2, 3, 8});
+  refused([&] { hip.cacheKeep(cache, rows, none); }, "cacheKeep: kept I32 [2×3×8] for 2 sequences of 2 heads");
+}
+
+GPU_TEST(a_cache_cut_to_its_heaviest) {
+  // one sequence of 90 positions over the F16 cache: what one row's attention
+  // weighs them, the 24 heaviest with the first and the last, the cache cut to
+  // them, and a tree of two nodes over what is left. The values are whole
+  // numbers of 1/8 up to 2, exact in F16; a weight's bar is 1e-4 as above.
+  HipOps hip;
+  Device dev;
+  const int kh = 2, heads = 4, dim = 64, page = 16, pages = 8, n = 90, keep = 26;
+  const std::vector<int32_t> table = {5, 2, 7, 0, 3, 1, 6, 4};
+  std::mt19937 rng(9);
+  auto eighths = [&](size_t count) {
+    std::vector<float> x(count);
+    for (float& v : x) v = (float)((int)(rng() % 33) - 16) / 8.0f;
+    return x;
+  };
+  const std::vector<float> k = eighths((size_t)n * kh * dim), v = eighths((size_t)n * kh * dim), q = eighths(heads * dim);
+  const std::vector<uint16_t> blank((size_t)pages * page * kh * dim, 0);
+  const KvCache cache = KvCache::of(dev.upload(DType::F16, {pages, page, kh, dim}, blank),
+                                    dev.upload(DType::F16, {pages, kh, dim, page}, blank), page);
+  const Tensor tables = dev.upload(DType::I32, {1, pages}, table);
+  const auto sequences = [&](int32_t start, int32_t rows) {
+    return Sequences{tables, dev.upload(DType::I32, {1}, std::vector<int32_t>{start}),
+                     dev.upload(DType::I32, {2}, std::vector<int32_t>{0, rows}), 0};
+  };
+  hip.cacheWriteSequences(dev.upload(DType::F32, {n, kh, dim}, k), dev.upload(DType::F32, {n, kh, dim}, v), cache,
+                          sequences(0, n));
+  const Tensor mass = dev.upload(DType::F32, {pages, kh, page}, std::vector<float>((size_t)pages * kh * page, 0.0f));
+  const Tensor qd = dev.upload(DType::F32, {1, heads, dim}, q);
+  const Sequences last = sequences(n - 1, 1);
+  hip.attentionMass(qd, cache, last, 0.125f, mass, dev.empty(DType::U8, {hip.attentionMassWorkspace(qd, cache, last)}), mass);
+  const std::vector<float> gathered = dev.download<float>(mass);
+  std::vector<std::vector<double>> want(kh, std::vector<double>(n, 0.0));
+  const auto weights = [&](int h, const std::vector<int>& at) {
+    std::vector<double> p;
+    double sum = 0, top = -1e300;
+    for (int j : at) {
+      double dot = 0;
+      for (int d = 0; d < dim; ++d) dot += (double)q[h * dim + d] * k[((size_t)j * kh + h / (heads / kh)) * dim + d];
+      p.push_back(0.125 * dot);
+      top = std::max(top, p.back());
+    }
+    for (double& x : p) sum += x = std::exp(x - top);
+    for (double& x : p) x /= sum;
+    return p;
+  };
+  std::vector<int> every(n);
+  for (int j = 0; j < n; ++j) every[j] = j;
+  for (int h = 0; h < heads; ++h) {
+    const std::vector<double> p = weights(h, every);
+    for (int j = 0; j < n; ++j) want[h / (heads / kh)][j] += p[j];
+  }
+  for (int h = 0; h < kh; ++h)
+    for (int j = 0; j < n; ++j)
+      expect(std::fabs(gathered[(size_t)(table[j / page] * kh + h) * page + j % page] - want[h][j]) < 1e-4, "a mass");
+  const Tensor kept = dev.empty(DType::I32, {1, kh, keep}), counts = dev.empty(DType::I32, {1});
+  hip.heaviest(mass, tables, dev.upload(DType::I32, {1}, std::vector<int32_t>{n}), 1, 1, kept, counts);
+  const std::vector<int32_t> chosen = dev.download<int32_t>(kept);
+  expect(dev.download<int32_t>(counts)[0] == keep, "the count");
+  KeptRows rows{tables, kept, counts, {}, {}};
+  hip.cacheKeep(cache, rows, dev.empty(DType::U8, {hip.cacheKeepWorkspace(cache, rows)}), mass);
+  // the last two kept positions as a tree's nodes: the second row sees itself and not the first
+  const Sequences tree = sequences(keep - 2, 2);
+  const Tensor out = dev.empty(DType::F32, {2, heads, dim});
+  std::vector<float> twice(q);
+  twice.insert(twice.end(), q.begin(), q.end());
+  const Tensor q2 = dev.upload(DType::F32, {2, heads, dim}, twice);
+  hip.attentionTree(q2, cache, tree, dev.upload(DType::I32, {2, 1}, std::vector<int32_t>{1, 2}), 0.125f, out,
+                    dev.empty(DType::U8, {hip.attentionWorkspace(q2, cache, tree)}));
+  const std::vector<float> got = dev.download<float>(out);
+  for (int h = 0; h < heads; ++h) {
+    const int32_t* mine = chosen.data() + h / (heads / kh) * keep;
+    expect(mine[0] == 0 && mine[keep - 1] == n - 1, "the first and the last");
+    for (int row = 0; row < 2; ++row) {
+      std::vector<int> at(mine, mine + keep - 2);
+      at.push_back(mine[keep - 2 + row]);
+      const std::vector<double> p = weights(h, at);
+      for (int d = 0; d < dim; ++d) {
+        double x = 0;
+        for (size_t j = 0; j < at.size(); ++j) x += p[j] * v[((size_t)at[j] * kh + h / (heads / kh)) * dim + d];
+        expect(std::fabs(x - got[((size_t)row * heads + h) * dim + d]) < 1e-4, "a tree's row over what is left");
+      }
+    }
+  }
+}
+
 GPU_TEST(stored_and_rotated_tables) {
   HipOps hip;
   Device dev;
