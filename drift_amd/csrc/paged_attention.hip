@@ -3,7 +3,9 @@
 //
 // Token t of a sequence sits at position P = start + t and sees the positions
 // j <= P of its own sequence (its own key, written before, among them); with a
-// window only those with j > P - window, or j < sinks. Query head h reads key
+// window only those with j > P - window, or j < sinks. TREE: the tokens are a tree's,
+// and of their own positions each sees those whose bits it has; its own P, for
+// the window over the positions before them, is start - 1 + their number. Query head h reads key
 // head h / (heads / kv_heads):
 //   s_j = scale q.k_j,  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
 // over the visible j, in one pass with the running maximum m and sum, in F32. A
@@ -77,6 +79,21 @@ __device__ __forceinline__ uint64_t tree_sees(const AttentionArgs& a, const Span
   return seen;
 }
 
+// The first position of a tree's row among those before `start`, but for the sinks.
+__device__ __forceinline__ int64_t tree_low(const AttentionArgs& a, const Span& span, int64_t nth) {
+  return a.window ? min(max(tree_position(a, span, nth) - a.window + 1, (int64_t)0), span.start) : 0;
+}
+
+// The least position that the rows from token `nth` on may have, and the last that those up to it may see.
+template <bool TREE>
+__device__ __forceinline__ int64_t first_position(const Span& span, uint32_t nth) {
+  return TREE ? max(span.start, (int64_t)1) - 1 : span.start + nth;
+}
+template <bool TREE>
+__device__ __forceinline__ int64_t last_position(const Span& span, uint32_t nth) {
+  return span.start + (TREE ? span.rows - 1 : nth);
+}
+
 __device__ __forceinline__ float f16_value(uint32_t bits) {
   return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
@@ -139,10 +156,8 @@ __device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& 
   float sums[kEach] = {}, top = -kInfinity, total = 0.0f;
   bool any = false;
   int64_t low = 0;
-  if (a.window) {
-    if constexpr (TREE) low = min(max(tree_position(a, span, nth) - a.window + 1, (int64_t)0), span.start);
-    else low = max(position - a.window + 1, (int64_t)0);
-  }
+  if constexpr (TREE) low = tree_low(a, span, nth);
+  else if (a.window) low = max(position - a.window + 1, (int64_t)0);
   const int64_t sink_end = a.window ? min((int64_t)a.sinks, low) : 0;
   for (int64_t tile = from; tile * kWave <= position; tile += step) {
     if (tile * kWave >= sink_end && (tile + 1) * kWave <= low) {  // what lies between is not seen
@@ -473,7 +488,8 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   const int rows = (int)min((int64_t)span.rows * a.group - nth * (C * 16), (int64_t)(C * 16));
   if (rows <= 0 || (int64_t)span.rows * a.group > a.few_rows) return;
   const uint32_t row0 = (uint32_t)nth * (C * 16), group = (uint32_t)a.group;
-  const uint32_t p0 = (uint32_t)span.start + row0 / group, p1 = (uint32_t)span.start + (row0 + rows - 1) / group;
+  const uint32_t p0 = (uint32_t)first_position<TREE>(span, row0 / group);
+  const uint32_t p1 = (uint32_t)last_position<TREE>(span, (row0 + rows - 1) / group);
   const TileList list = tiles_of(a, p0, p1, TOK);
   const int each = split_tiles(a, list.count);
   const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
@@ -483,12 +499,13 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
   // the rows' queries as B operands: column col, values 8 g .. of each 32 (8 bits: of each 64, 16 g ..)
   f16x8 query[C][KS][TERMS];
   float row_scale[C];
-  uint32_t position[C];
+  uint32_t position[C], low[TREE ? C : 1];  // (TREE: a row's token, and what tree_low has)
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int r = c * 16 + col;
     const uint32_t row = row0 + min(r, rows - 1), token = row / group;
-    position[c] = (uint32_t)span.start + token;
+    position[c] = TREE ? token : (uint32_t)span.start + token;
+    if constexpr (TREE) low[c] = (uint32_t)tree_low(a, span, token);
     const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
     float v[KS][8];
     uint32_t most = 0;
@@ -651,7 +668,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
 #pragma unroll
       for (int e = 0; e < 16; ++e) value_log[e] = __builtin_amdgcn_logf(value_log[e]);
     // whether every row sees the whole tile
-    const bool whole = base + TOK - 1 <= p0 &&
+    const bool whole = (TREE ? base + TOK <= (uint32_t)span.start : base + TOK - 1 <= p0) &&
                        (a.window == 0 || base + (uint32_t)a.window > p1 || base + TOK - 1 < (uint32_t)a.sinks) &&
                        __all(okay);
     float weight[C][NT][4];  // TOK / 4 consecutive positions
@@ -666,7 +683,13 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
           if constexpr (I8) x *= key_scale[4 * t + e];
           score[c][t][e] = x;
         }
-      if (!whole)
+      if (TREE && !whole) {
+        const uint32_t sees = okay ? (uint32_t)tree_sees(a, span, position[c], mine, low[TREE ? c : 0], a.sinks) : 0;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) score[c][t][e] = sees >> (4 * t + e) & 1 ? score[c][t][e] : -kInfinity;
+      } else if (!whole)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -908,7 +931,8 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   const int rows = (int)min((int64_t)span.rows * a.group - nth * kRows, (int64_t)kRows);
   if (rows <= 0 || (int64_t)span.rows * a.group <= a.few_rows) return;
   const uint32_t row0 = (uint32_t)nth * kRows, group = (uint32_t)a.group, start = (uint32_t)span.start;
-  const uint32_t p0 = start + row0 / group, p1 = start + (row0 + rows - 1) / group;
+  const uint32_t p0 = (uint32_t)first_position<TREE>(span, row0 / group);
+  const uint32_t p1 = (uint32_t)last_position<TREE>(span, (row0 + rows - 1) / group);
   const TileList list = tiles_of(a, p0, p1, TOK);
   const int each = split_tiles(a, list.count);
   const int begin = uniform(split * each), end = uniform(min(begin + each, list.count));
@@ -918,11 +942,12 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   // ---- this wave's rows
   const int wave_row = wave * 32;
   const bool idle = wave_row >= rows;
-  const uint32_t w0 = start + (row0 + min(wave_row, rows - 1)) / group;
-  const uint32_t w1 = start + (row0 + min(wave_row + 32, rows) - 1) / group;
+  const uint32_t w0 = (uint32_t)first_position<TREE>(span, (row0 + min(wave_row, rows - 1)) / group);
+  const uint32_t w1 = (uint32_t)last_position<TREE>(span, (row0 + min(wave_row + 32, rows) - 1) / group);
   f16x8 query[KS][TERMS];
   const uint32_t row = row0 + min(wave_row + col, rows - 1), token = row / group;
   const uint32_t position = start + token;
+  const uint32_t row_low = TREE ? (uint32_t)tree_low(a, span, token) : 0;
   const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
   uint32_t most = 0;
   float v[KS][8];
@@ -1187,7 +1212,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
     // whether any, and whether every row of the wave sees the tile
     if (idle || base > w1) continue;
     if (a.window && base + TOK - 1 + (uint32_t)a.window <= w0 && base >= (uint32_t)a.sinks) continue;
-    const bool whole = okay_then == 15u && base + TOK - 1 <= w0 &&
+    const bool whole = okay_then == 15u && (TREE ? base + TOK <= start : base + TOK - 1 <= w0) &&
                        (a.window == 0 || base + (uint32_t)a.window > w1 || base + TOK - 1 < (uint32_t)a.sinks);
     bool apart = false, change = false;
     float factor = 1.0f;  // what the results so far are multiplied by, where there is a change
@@ -1248,14 +1273,21 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
         }
     }
     if (!whole) {
-      int mine = (int)base + h * 8;
-      asm volatile("" : "+v"(mine));  // (or what depends on it alone is kept for every tile)
-      const int last = (int)position, low = a.window ? last - a.window + 1 : INT32_MIN;
+      if constexpr (TREE) {
+        const uint64_t sees = tree_sees(a, span, token, base, row_low, a.sinks) >> (h * 8);
 #pragma unroll
-      for (int n = 0; n < 32; ++n) {
-        const int j = mine + n / 8 * 16 + n % 8;
-        const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
-        score[n / 16][n % 16] = seen ? score[n / 16][n % 16] : -kInfinity;
+        for (int n = 0; n < 32; ++n)
+          score[n / 16][n % 16] = sees >> (n / 8 * 16 + n % 8) & 1 ? score[n / 16][n % 16] : -kInfinity;
+      } else {
+        int mine = (int)base + h * 8;
+        asm volatile("" : "+v"(mine));  // (or what depends on it alone is kept for every tile)
+        const int last = (int)position, low = a.window ? last - a.window + 1 : INT32_MIN;
+#pragma unroll
+        for (int n = 0; n < 32; ++n) {
+          const int j = mine + n / 8 * 16 + n % 8;
+          const bool seen = (j <= last) & ((j >= low) | (j < a.sinks));
+          score[n / 16][n % 16] = seen ? score[n / 16][n % 16] : -kInfinity;
+        }
       }
       if (okay_then != 15u)
 #pragma unroll
@@ -1468,7 +1500,7 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
   const uint32_t row0 = (uint32_t)nth * rows;
   if (row0 + part * kRows >= all || (all <= (uint32_t)a.few_rows) != FEW) return;
   const uint32_t last = min(row0 + rows, all) - 1, end = min(row0 + (part + 1) * kRows, last + 1);
-  const TileList list = tiles_of(a, span.start + row0 / group, span.start + last / group, tile);
+  const TileList list = tiles_of(a, first_position<TREE>(span, row0 / group), last_position<TREE>(span, last / group), tile);
   const int each = split_tiles(a, list.count), splits = (list.count + each - 1) / each;
   if (splits == 1) return;
   for (uint32_t first = row0 + part * kRows + wave * (64 / L); first < end; first += 4 * (64 / L)) {
@@ -1727,7 +1759,7 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
   // (the tile kernels' offsets within a page, and rows of scales, have 32 bits)
   const bool small = (int64_t)a.p.page_size * a.kv_heads * a.dim * 2 < (int64_t)1 << 31 &&
                      (int64_t)a.p.cache_pages * a.kv_heads < (int64_t)1 << 31;
-  if (TREE || !aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
+  if (!aligned || !small || a.dim > 256 || a.p.cache_pages == 0 || blocks > kOneWaveBlocks / 4) {
     const dim3 grid((unsigned)row_blocks), block(kWave * (row_blocks * kRowWaves > kOneWaveBlocks ? 1 : kRowWaves));
     const bool wide = a.dim % 8 == 0 && aligned16(a.keys) && aligned16(a.values);
     if (wide) hipLaunchKernelGGL((attend_rows<T, I8, true, TREE>), grid, block, 0, st, queries, out, a);
