@@ -82,7 +82,7 @@ SIGNATURES = {
     "drift_paged_attention_bf16": (_I32, _PAGED_ATTENTION),
     "drift_tree_attention_f32": (_I32, _TREE_ATTENTION),
     "drift_tree_attention_bf16": (_I32, _TREE_ATTENTION),
-    "drift_attention_mass_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _P]),
+    "drift_attention_mass_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
     "drift_attention_mass_f32": (_I32, _ATTENTION_MASS),
     "drift_attention_mass_bf16": (_I32, _ATTENTION_MASS),
     "drift_heaviest": (_I32, [_P, _P, _I32, _I32, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P]),

@@ -1053,10 +1053,11 @@ void HipOps::attentionTree(const Tensor& queries, const PagedCache& cache, const
 int64_t HipOps::attentionMassWorkspace(const Tensor& queries, const PagedCache& cache, const Sequences& sequences) {
   checkAttention("attentionMassWorkspace", queries, cache, queries, {});
   const Paging p = pagingOf("attentionMassWorkspace", cache, sequences, queries.shape[0]);
+  const int64_t room = std::min<int64_t>((int64_t)p.tablePages * cache.pageSize, MostPositions);
   int64_t bytes = 0;
   const int code = drift_attention_mass_workspace(p.count, (int32_t)queries.shape[0], (int32_t)queries.shape[1],
-                                                  (int32_t)cache.kvHeads(), (int32_t)cache.headDimension(), p.longest,
-                                                  &bytes);
+                                                  (int32_t)cache.kvHeads(), (int32_t)cache.headDimension(), (int32_t)room,
+                                                  p.longest, &bytes);
   if (code != 0) throw HipException("drift_attention_mass_workspace", code, drift_last_error());
   return bytes;
 }

@@ -1189,9 +1189,9 @@ class HipOps:
         self._onOneDevice(operation, (queries, mass, before, badPage, *tensors))
         if before is not None and before.data_ptr() != mass.data_ptr():
             checkApart(operation, "mass overlaps before", mass, before)
-        room = sequences.pageTables.shape[1] * cache.pageSize
-        longest = min(sequences.longest or room, room, _MOST_POSITIONS)
-        numbers = (paging[5], tokens, heads, cache.kvHeads, cache.headDimension, longest)
+        room = min(sequences.pageTables.shape[1] * cache.pageSize, _MOST_POSITIONS)
+        longest = min(sequences.longest or room, room)
+        numbers = (paging[5], tokens, heads, cache.kvHeads, cache.headDimension, room, longest)
         size = self._told("drift_attention_mass_workspace", *numbers)
         workspace = self._workspace(size, queries.device)
         keys, _, keyScales, *_ = tensors

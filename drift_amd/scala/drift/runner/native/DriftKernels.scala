@@ -102,7 +102,7 @@ final class DriftKernels(path: Path) {
   val attentionMass = twins("drift_attention_mass", P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT, JAVA_INT,
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, P, P, P, JAVA_LONG, P, P)
   val attentionMassWorkspace = bind("drift_attention_mass_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
-    JAVA_INT, P)
+    JAVA_INT, JAVA_INT, P)
   val heaviest = bind("drift_heaviest", P, P, JAVA_INT, JAVA_INT, P, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
     JAVA_INT, P, P, P, P)
   val cacheKeep = bind("drift_cache_keep", P, P, P, P, P, P, JAVA_INT, P, JAVA_INT, JAVA_INT, P, JAVA_INT, P, P,
@@ -110,12 +110,13 @@ final class DriftKernels(path: Path) {
   val cacheKeepWorkspace = bind("drift_cache_keep_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P)
 
   /** The bytes of scratch that an `attentionMass` of these numbers takes. */
-  def massWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, longest: Int): Long = {
+  def massWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, room: Int,
+                    longest: Int): Long = {
     val arena = Arena.ofConfined()
     try {
       val bytes = arena.allocate(JAVA_LONG)
       check("drift_attention_mass_workspace", (attentionMassWorkspace.invokeExact(sequences, tokens, heads, kvHeads,
-        headDimension, longest, bytes): Int))
+        headDimension, room, longest, bytes): Int))
       bytes.get(JAVA_LONG, 0)
     } finally arena.close()
   }

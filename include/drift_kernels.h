@@ -456,8 +456,12 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * a sequence's last row's, the sum over its rows that see it and the heads of the key
  * head of p_j = exp(scale q.k_j - m) / sum exp(scale q.k_j - m), added to `before`
  * (laid out the same; may be mass itself, not otherwise share memory with it; NULL: 0)
- * where the position precedes the sequence's rows. Rows, paging, scores and workspace
- * rules are drift_paged_attention_*'s, without a window; other positions of mass are
+ * where the position precedes the sequence's rows. Rows, paging and scores are
+ * drift_paged_attention_*'s, without a window, and so are the rules of the workspace,
+ * whose bytes drift_attention_mass_workspace tells (`room`: table_pages * page_size,
+ * at most 2147483520): of few rows a sequence it holds their scores, 4 bytes a row and
+ * position of room up to 512 MiB in all (64 sequences' step, 32 heads, 8,016 positions: 66 MB), of
+ * many a copy of the queries. Other positions of mass are
  * left as they are, and so are ones on a page outside the cache, *bad_page set. The
  * same call gives the same bits every time. Two sequences that share a page leave
  * either's sum there. keys and values of drift_paged_write_*: the values are not read.
@@ -487,7 +491,7 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * Replaces nothing of the reference, whose cache only grows
  * (src/drift/runner/ops/KvCache.scala:5-22). */
 int drift_attention_mass_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
-                                   int32_t head_dim, int32_t longest, int64_t* bytes);
+                                   int32_t head_dim, int32_t room, int32_t longest, int64_t* bytes);
 int drift_attention_mass_f32(const float* queries, const void* keys, const float* key_scales,
                              const int32_t* page_tables, int32_t table_pages, int32_t cache_pages,
                              const int32_t* starts, const int32_t* offsets, int32_t sequences, int32_t start,

@@ -203,11 +203,12 @@ def told(entry, *numbers):
 
 
 def test_the_workspaces_are_told():
-    assert refusal("drift_attention_mass_workspace", 1, 1, 8, 2, 128, 10, None).endswith("null bytes")
-    assert "7 heads over 2" in told("drift_attention_mass_workspace", 1, 1, 7, 2, 128, 10)[0]
-    assert "longest" in told("drift_attention_mass_workspace", 1, 1, 8, 2, 128, -1)[0]
-    for numbers in ((1, 1, 8, 2, 128, 10), (64, 64, 32, 8, 128, 2 ** 31 - 1), (1, 0, 8, 2, 64, 0), (0, 5, 8, 2, 64, 5),
-                    (3, 2 ** 20, 64, 8, 256, 2 ** 20)):
+    assert refusal("drift_attention_mass_workspace", 1, 1, 8, 2, 128, 16, 10, None).endswith("null bytes")
+    assert "7 heads over 2" in told("drift_attention_mass_workspace", 1, 1, 7, 2, 128, 16, 10)[0]
+    assert "longest" in told("drift_attention_mass_workspace", 1, 1, 8, 2, 128, 16, -1)[0]
+    assert "room for -1" in told("drift_attention_mass_workspace", 1, 1, 8, 2, 128, -1, 5)[0]
+    for numbers in ((1, 1, 8, 2, 128, 16, 10), (64, 64, 32, 8, 128, 2 ** 31 - 1, 2 ** 31 - 1), (1, 0, 8, 2, 64, 0, 0),
+                    (0, 5, 8, 2, 64, 16, 5), (3, 2 ** 20, 64, 8, 256, 2 ** 21, 2 ** 20), (1, 1, 1, 1, 1, 0, 0)):
         code, size = told("drift_attention_mass_workspace", *numbers)
         assert code == "code 0" and 0 <= size < 1 << 40
     assert refusal("drift_cache_keep_workspace", 1, 1, 8, 128, 0, None).endswith("null bytes")
