@@ -14,6 +14,7 @@
 #include "products.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace drift {
 namespace {
@@ -23,9 +24,8 @@ constexpr float kLog2E = 1.44269504088896340736f;
 
 // What the position sums need of a row: its scores' factor, in powers of two (NaN: the
 // row is no numbers), its largest score and one over its sum.
-struct Row {
-  float scale, top, inverse, spare;
-};
+typedef f32x4 Row;
+enum { kScale, kTop, kInverse };
 
 struct MassArgs {
   Paging p;
@@ -45,6 +45,7 @@ struct MassArgs {
   // positions in `splits` of at least `chunk` tiles for the statistics; rows in `parts` for the sums, of positions below
   // `summed`, a block every `strides`-th tile of positions
   int32_t splits, chunk, parts, summed, strides;
+  int32_t wide;  // masses on 16-byte alignment
 };
 
 // Rows of a sequence and key head lie together in the workspace: row r is token r / group, head r % group.
@@ -74,9 +75,21 @@ __device__ __forceinline__ bool place_of(const MassArgs& a, const Span& span, in
   return true;
 }
 
-// A position's sum into its mass.
-__device__ __forceinline__ void store_mass(const MassArgs& a, const Span& span, int64_t j, const Place& place, float sum) {
-  a.mass[place.word] = a.before && j < span.start ? a.before[place.word] + sum : sum;
+// Sums of the four positions from j on (a multiple of four: on one page) into their masses.
+__device__ __forceinline__ void store_masses(const MassArgs& a, const Span& span, int64_t j, int kv, const float (&sum)[4]) {
+  const int64_t length = span.start + span.rows;
+  Place place;
+  if (j >= length || !place_of(a, span, j, kv, place)) return;
+  if (a.wide && j + 4 <= length && (!a.before || j + 4 <= span.start || j >= span.start)) {
+    f32x4 x = {sum[0], sum[1], sum[2], sum[3]};
+    if (a.before && j < span.start) x += *(const f32x4*)(a.before + place.word);
+    *(f32x4*)(a.mass + place.word) = x;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < length)
+      a.mass[place.word + e] = a.before && j + e < span.start ? a.before[place.word + e] + sum[e] : sum[e];
 }
 
 // The score of a row and a position, by F32 products one after another.
@@ -201,20 +214,35 @@ __device__ __forceinline__ float take_query(const T* q, const MassArgs& a, At d_
 // Scores that came out as NaN, taken again by themselves: a term of F16 may have met an
 // infinity that the whole number would have made one of.
 template <typename T, bool I8>
-__device__ __noinline__ float score_again(const T* queries, const MassArgs& a, const Span& span, int kv, uint32_t row,
-                                          int64_t j) {
+__device__ __noinline__ float score_again_of(const T* query, const MassArgs& a, const Span& span, int kv, int64_t j) {
   Place place;
   if (!place_of(a, span, j, kv, place)) return -kInfinity;
-  return score_of<T, I8>(a, query_of(queries, a, span, kv, row), place) * kLog2E;
+  return score_of<T, I8>(a, query, place) * kLog2E;
+}
+
+// Of a lane's scores x[n], of positions at(n), those that are NaN. Copies of the arguments go by
+// reference: the kernels' own then stay in scalar registers (passed themselves, every
+// use of theirs would read scratch memory).
+template <typename T, bool I8, int N, typename At>
+__device__ __forceinline__ void scores_again(const T* query, const MassArgs& a, const Span& span, int kv, At at,
+                                             float factor, float (&x)[N]) {
+  const MassArgs args = a;
+  const Span rows = span;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (x[n] != x[n]) x[n] = score_again_of<T, I8>(query, args, rows, kv, at(n)) * factor;
 }
 
 // How far, in powers of two, a score may pass what weights are taken against: sums of weights up to 2^kSlack each stay
 // numbers, and those 2^-126 of the least.
 constexpr float kSlack = 32.0f;
 
-// (nothing but scores of -infinity seen: 0 / 0, as the formula has it)
+// A row's constants, the weights taken against a number that no score passes: the sum of weights against `top` is no less
+// than the largest of them. (Nothing but scores of -infinity seen: 0 / 0, as the formula has it.)
 __device__ __forceinline__ Row row_of(float scale, float top, float total) {
-  return Row{scale, top, top == -kInfinity || scale != scale ? __builtin_nanf("") : 1.0f / total, 0.0f};
+  const float most = top + ceilf(log2f(total));
+  const float inverse = exp2f(most - top) / total;
+  return Row{scale, most, top == -kInfinity || scale != scale ? __builtin_nanf("") : inverse, 0.0f};
 }
 
 // Largest scores and sums, in powers of two, of two parts as one's.
@@ -237,12 +265,14 @@ __device__ __forceinline__ SplitTiles split_tiles(const MassArgs& a, uint32_t la
 }
 
 // Scores of units of 16 rows, kept, and their statistics: positions in tiles of 32 (F16)
-// or 64 (8 bits) that a block's waves take in turn, keys straight from memory into the
-// operands of 16 x 16 x 32 products, S^T = K Q^T: the result's column (lane % 16) is a
-// row, its rows are positions, dealt out so that a lane has TOK / 4 consecutive ones.
+// or 64 (8 bits), keys straight from memory into the operands of 16 x 16 x 32
+// products, S^T = K Q^T: the result's column (lane % 16) is a row, its rows are
+// positions, dealt out so that a lane has TOK / 4 consecutive ones. A block's four waves
+// take its split's tiles in turn.
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* queries, MassArgs a) {
-  constexpr int kWaves = 4, TOK = I8 ? 64 : 32, NT = TOK / 16, TERMS = sizeof(T) == 4 ? 2 : 1, KS = DP / 32;
+  constexpr int kWaves = 4;
+  constexpr int TOK = I8 ? 64 : 32, NT = TOK / 16, TERMS = sizeof(T) == 4 ? 2 : 1, KS = DP / 32;
   __shared__ float stats[kWaves][16][2];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const int kv = blockIdx.x % (unsigned)a.kv_heads;
@@ -287,9 +317,11 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
     return w;
   };
   constexpr int kKeyLoads = I8 ? KS / 2 : KS;  // 16-byte loads a position
-  uint4 keys[NT][kKeyLoads];
-  float key_scale[I8 ? 16 : 1];
-  auto load_keys = [&](const Places& w) {
+  struct Keys {
+    u32x4 raw[NT][kKeyLoads];
+    float scale[I8 ? 16 : 1];
+  };
+  auto load_keys = [&](const Places& w, Keys& to) {
     const int32_t page = (uint32_t)w.key_page < (uint32_t)a.p.cache_pages ? w.key_page : 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -301,14 +333,14 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
           const int8_t* key = (const int8_t*)a.keys + at;
           const int d = k * 64 + g * 16;
           if (a.dim == DP) {
-            keys[t][k] = __builtin_bit_cast(uint4, *(const u32x4_8*)(key + d));
+            to.raw[t][k] = *(const u32x4_8*)(key + d);
           } else {
             const u32x2 x = *(const u32x2*)(key + (d < a.dim ? d : 0)), y = *(const u32x2*)(key + (d + 8 < a.dim ? d + 8 : 0));
-            keys[t][k] = make_uint4(x.x, x.y, y.x, y.y);
+            to.raw[t][k] = u32x4{x.x, x.y, y.x, y.y};
           }
         } else {
           const int d = k * 32 + g * 8;
-          keys[t][k] = *(const uint4*)((const uint16_t*)a.keys + at + (d < a.dim ? d : 0));
+          to.raw[t][k] = *(const u32x4*)((const uint16_t*)a.keys + at + (d < a.dim ? d : 0));
         }
       }
     }
@@ -318,25 +350,16 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const float4 x = *(const float4*)(from + e);
-        key_scale[e] = x.x, key_scale[e + 1] = x.y, key_scale[e + 2] = x.z, key_scale[e + 3] = x.w;
+        to.scale[e] = x.x, to.scale[e + 1] = x.y, to.scale[e + 2] = x.z, to.scale[e + 3] = x.w;
       }
     }
   };
 
   float top = -kInfinity, total = 0.0f;
-  int i = begin + wave;
-  Places now = places_of(i), next = places_of(i + kWaves);
-  if (i < end) load_keys(now);
-  for (; i < end; i += kWaves) {
+  auto take_tile = [&](int i, bool okay, const Keys& keys) {
     const uint32_t mine = (uint32_t)i * TOK + g * (TOK / 4);  // the lane's first position
-    const bool okay = (uint32_t)now.own_page < (uint32_t)a.p.cache_pages;
     if (!okay && mine <= p1) flag_bad(a.p);
     f32x4 score[NT];
-    // (the next tile's scales overwrite these)
-    float scale[I8 ? 16 : 1];
-    if constexpr (I8)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) scale[e] = key_scale[e];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       score[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -344,20 +367,16 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
       for (int k = 0; k < KS; ++k) {
         f16x8 key;
         if constexpr (I8) {
-          const uint4 w = keys[t][k / 2];
+          const u32x4 w = keys.raw[t][k / 2];
           key = k % 2 ? codes_f16(w.z, w.w) : codes_f16(w.x, w.y);
         } else {
-          key = __builtin_bit_cast(f16x8, keys[t][k]);
+          key = __builtin_bit_cast(f16x8, keys.raw[t][k]);
         }
 #pragma unroll
         for (int m = 0; m < TERMS; ++m)
           score[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, query[k][m], score[t], 0, 0, 0);
       }
     }
-    if (i + kWaves < end) load_keys(next);
-    now = next;
-    next = places_of(i + 2 * kWaves);
-
     const bool whole = (uint32_t)(i + 1) * TOK - 1 <= p0 && __all(okay);
     bool odd = false;
 #pragma unroll
@@ -365,17 +384,19 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float x = score[t][e] * row_scale;
-        if constexpr (I8) x *= scale[4 * t + e];
+        if constexpr (I8) x *= keys.scale[4 * t + e];
         if (!whole) x = (okay & (mine + 4 * t + e <= position)) ? x : -kInfinity;
         odd |= x != x;
         score[t][e] = x;
       }
-    if (__any(odd) && row_scale == row_scale)
+    if (__any(odd && row_scale == row_scale)) {
+      float x[4 * NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int n = 0; n < 4 * NT; ++n) x[n] = score[n / 4][n % 4];
+      scores_again<T, I8>(query_of(queries, a, span, kv, row), a, span, kv, [&](int n) { return (int64_t)mine + n; }, 1.0f, x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (score[t][e] != score[t][e]) score[t][e] = score_again<T, I8>(queries, a, span, kv, row, mine + 4 * t + e);
+      for (int n = 0; n < 4 * NT; ++n) score[n / 4][n % 4] = x[n];
+    }
     float high = top;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -392,6 +413,28 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
     if (col < rows && mine < a.room)
 #pragma unroll
       for (int t = 0; t < NT; ++t) *(f32x4*)(scores + mine + 4 * t) = score[t];
+  };
+  // Keys of two tiles on their way. A tile's places are asked for before the keys of the tile before it are: loads
+  // come back in their order, and to wait for the places is then no wait for those keys.
+  Keys keys0, keys1;
+  int i = begin + wave;
+  const Places first0 = places_of(i), first1 = places_of(i + kWaves);
+  Places next = places_of(i + 2 * kWaves);
+  auto in_cache = [&](const Places& w) { return (uint32_t)w.own_page < (uint32_t)a.p.cache_pages; };
+  bool okay0 = in_cache(first0), okay1 = in_cache(first1);
+  if (i < end) load_keys(first0, keys0);
+  if (i + kWaves < end) load_keys(first1, keys1);
+  auto step = [&](Keys& keys, bool& okay) {
+    const Places coming = next;
+    next = places_of(i + 3 * kWaves);
+    take_tile(i, okay, keys);
+    okay = in_cache(coming);
+    if (i + 2 * kWaves < end) load_keys(coming, keys);
+    i += kWaves;
+  };
+  while (i < end) {
+    step(keys0, okay0);
+    if (i < end) step(keys1, okay1);
   }
   // the four lanes' of a row, then the waves'
 #pragma unroll
@@ -399,11 +442,11 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
     join_statistics(top, total, __shfl_xor(top, mask, kWave), __shfl_xor(total, mask, kWave));
   if (g == 0) stats[wave][col][0] = top, stats[wave][col][1] = total;
   __syncthreads();
-  if ((int)threadIdx.x < rows) {
-    top = stats[0][threadIdx.x][0], total = stats[0][threadIdx.x][1];
+  if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) join_statistics(top, total, stats[w][threadIdx.x][0], stats[w][threadIdx.x][1]);
-    float* to = a.statistics + (split * a.rows + row_place(a, span, kv) + row0 + threadIdx.x) * 2;
+  for (int w = 1; w < kWaves; ++w) join_statistics(top, total, stats[w][col][0], stats[w][col][1]);
+  if (g == 0 && col < rows) {
+    float* to = a.statistics + (split * a.rows + row_place(a, span, kv) + row) * 2;
     to[0] = top, to[1] = total;
   }
 }
@@ -423,7 +466,7 @@ __global__ void __launch_bounds__(256) few_sums(MassArgs a) {
   bool staged = false;
   for (int64_t base = (int64_t)(rest % (unsigned)a.strides) * 1024; base < length; base += (int64_t)a.strides * 1024) {
     const int64_t j = base + threadIdx.x * 4;
-    double sum[4] = {};
+    float sum[4] = {};
     for (uint32_t row0 = 0; row0 < rows; row0 += kBatch) {
       if (rows > kBatch || !staged) {
         __syncthreads();
@@ -433,6 +476,7 @@ __global__ void __launch_bounds__(256) few_sums(MassArgs a) {
           const int splits = split_tiles(a, (uint32_t)span.start + end / group, I8 ? 64 : 32).count;
           const float* st = a.statistics + (first + row) * 2;
           float top = st[0], total = st[1];
+#pragma unroll 4
           for (int i = 1; i < splits; ++i) join_statistics(top, total, st[i * a.rows * 2], st[i * a.rows * 2 + 1]);
           // (nothing but scores of -infinity seen: 0 / 0, as the formula has it)
           constants[threadIdx.x] = make_float2(top, top == -kInfinity ? __builtin_nanf("") : 1.0f / total);
@@ -441,25 +485,29 @@ __global__ void __launch_bounds__(256) few_sums(MassArgs a) {
         staged = true;
       }
       if (j >= length) continue;
-      const uint32_t count = min(rows - row0, (uint32_t)kBatch);
-      // the rows before a position's own token do not see it, and have no scores there
-      const int64_t hidden = (j + 3 - span.start) * group - row0;
-      for (uint32_t r = 0; r < count; ++r) {
-        if ((int64_t)r >= (j - span.start) * group - row0) {
-          const f32x4 x = *(const f32x4*)(a.scores + (first + row0 + r) * a.room + j);
-          const float2 c = constants[r];
+      const int count = (int)min(rows - row0, (uint32_t)kBatch);
+      // rows from `some` on see the first position, from `all` on all four: before their own token rows have no scores
+      auto sees = [&](int64_t at) { return (int)min(max((at - span.start) * group - row0, (int64_t)0), (int64_t)count); };
+      const int some = sees(j), all = sees(j + 3);
+      const float* from = a.scores + (first + row0) * a.room + j;
+      for (int r = some; r < all; ++r) {
+        const f32x4 x = *(const f32x4*)(from + r * a.room);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = exp2_fast(x[e] - c.x) * c.y;
-            if ((int64_t)r >= hidden || (int64_t)r >= (j + e - span.start) * group - row0) sum[e] += p;
-          }
-        }
+        for (int e = 0; e < 4; ++e)
+          if (r >= sees(j + e)) sum[e] = fmaf(exp2_fast(x[e] - constants[r].x), constants[r].y, sum[e]);
       }
+      float part[4] = {};
+#pragma unroll 4
+      for (int r = all; r < count; ++r) {
+        const f32x4 x = *(const f32x4*)(from + r * a.room);
+        const float2 c = constants[r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e] = fmaf(exp2_fast(x[e] - c.x), c.y, part[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += part[e];
     }
-    for (int e = 0; e < 4; ++e) {
-      Place place;
-      if (j + e < length && place_of(a, span, j + e, kv, place)) store_mass(a, span, j + e, place, (float)sum[e]);
-    }
+    store_masses(a, span, j, kv, sum);
   }
 }
 
@@ -516,88 +564,118 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_statistics(const T
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) *(f16x8*)(a.halves + (place * TERMS + t) * DP + k * 16 + h * 8) = query[k][t];
 
-  // ---- staging: a thread's chunks of a tile
+  // ---- staging: a thread's chunks of a tile. Chunk n of a thread is of a unit that its whole wave shares, so that
+  // a load is a scalar base and an offset that stays. A tile's four units are one a lane of four.
   const uint32_t last_unit = p1 / 16;
-  struct Units {
-    int32_t page[kLoads], scale_page;
-    uint32_t off[kLoads], scale_off;
+  constexpr int kBytes = I8 ? 1 : 2;
+  const uint32_t position_bytes = (uint32_t)a.kv_heads * a.dim * kBytes, key_head = (uint32_t)kv * a.dim * kBytes;
+  struct Entries {
+    int32_t page;
+    uint32_t off;
   };
-  auto unit_at = [&](uint32_t unit, uint32_t& off) {
-    const uint32_t in = min(unit, last_unit), column = a.columns.of(in);
-    off = (in - column * a.columns.page_units) * 16;
-    return span.table[column];
+  auto entries_of = [&](int i) {
+    const uint32_t at = min((uint32_t)min(i, end - 1) * 4 + (lane & 3), last_unit), column = a.columns.of(at);
+    return Entries{span.table[column], (at - column * a.columns.page_units) * 16};
   };
-  auto load_units = [&](int i, Units& u) {
-    const uint32_t first = (uint32_t)min(i, end - 1) * 4;
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) u.page[n] = unit_at(first + (thread + n * kThreads) / (DP / 8) / 16, u.off[n]);
-    if (I8) u.scale_page = unit_at(first + lane / 16, u.scale_off);
+  auto at_lane = [](uint64_t x, int u) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)x, u);
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), u) << 32) | lo;
   };
-  auto in_cache = [&](int32_t page) { return (uint32_t)page < (uint32_t)a.p.cache_pages; };
-  uint4 raw[kLoads];
-  float scale_raw = 0.0f;
-  auto load_tile = [&](const Units& u) {
+  constexpr int kTokens = 64 / (DP / 8), kStep = kThreads / (DP / 8);  // positions a wave stages at once, and all four
+  const int own_token = lane / (DP / 8) + wave * kTokens, own_chunk = lane % (DP / 8);
+  const uint32_t own_at = (uint32_t)(own_token % 16) * position_bytes + key_head +
+                          (own_chunk * 8 < a.dim ? own_chunk * 8 * kBytes : 0);
+  struct Raw {
+    u32x4 chunk[kLoads];
+    float scale;
+    uint32_t okay;  // which of the tile's units lie in the cache
+  };
+  auto load_tile = [&](const Entries& units, Raw& raw) {
+    const bool okay = (uint32_t)units.page < (uint32_t)a.p.cache_pages;
+    if (!okay) flag_bad(a.p);
+    const uint64_t page = okay ? units.page : 0;
+    const uint64_t from = (page * a.p.page_size + units.off) * position_bytes;
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
-      const int chunk = (thread + n * kThreads) % (DP / 8) * 8, token = (thread + n * kThreads) / (DP / 8) % 16;
-      const int64_t page = in_cache(u.page[n]) ? u.page[n] : 0;
-      const int64_t at = ((page * a.p.page_size + u.off[n] + token) * a.kv_heads + kv) * a.dim + (chunk < a.dim ? chunk : 0);
+      const char* at = (const char*)a.keys + at_lane(from, (n * kStep + wave * kTokens) / 16) +
+                       (n * kStep % 16 * position_bytes) + own_at;
       if constexpr (I8) {
-        const u32x2 x = *(const u32x2*)((const int8_t*)a.keys + at);
-        raw[n].x = x.x, raw[n].y = x.y;
+        const u32x2 x = *(const u32x2*)at;
+        raw.chunk[n].x = x.x, raw.chunk[n].y = x.y;
       } else {
-        raw[n] = *(const uint4*)((const uint16_t*)a.keys + at);
+        raw.chunk[n] = *(const u32x4*)at;
       }
     }
     if (I8 && wave == 0) {
-      const int64_t page = in_cache(u.scale_page) ? u.scale_page : 0;
-      scale_raw = a.key_scales[(page * a.kv_heads + kv) * a.p.page_size + u.scale_off + lane % 16];
+      const uint32_t off = (uint32_t)__shfl((int)units.off, lane / 16, kWave);
+      const int64_t its = __shfl((int)page, lane / 16, kWave);
+      raw.scale = a.key_scales[(its * a.kv_heads + kv) * a.p.page_size + off + lane % 16];
     }
+    raw.okay = (uint32_t)__ballot(okay) & 15u;
   };
-  auto store_tile = [&](char* tile) {
+  const int own_place = chunk_place<DP>(own_token, own_chunk);
+  auto store_tile = [&](char* tile, const Raw& raw) {
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
-      const int q = thread + n * kThreads;
-      *(uint4*)(tile + chunk_place<DP>(q / (DP / 8), q % (DP / 8))) =
-          I8 ? __builtin_bit_cast(uint4, codes_f16(raw[n].x, raw[n].y)) : raw[n];
+      // (16 positions on, and for narrow heads 32, the exclusive or is the same; for wide ones 8 on it has bit 3 turned)
+      const int to = kStep % 16 ? chunk_place<DP>(own_token + n * kStep, own_chunk) : own_place + n * kStep * DP * 2;
+      *(u32x4*)(tile + to) = I8 ? __builtin_bit_cast(u32x4, codes_f16(raw.chunk[n].x, raw.chunk[n].y)) : raw.chunk[n];
     }
-    if (I8 && wave == 0) ((float*)(tile + kScales))[lane] = scale_raw;
+    if (I8 && wave == 0) ((float*)(tile + kScales))[lane] = raw.scale;
   };
-  // a tile's units that lie in the cache, one a lane of four
-  auto okay_of = [&](int i) {
-    uint32_t off;
-    const bool okay = in_cache(unit_at((uint32_t)i * 4 + (lane & 3), off));
-    if (!okay) flag_bad(a.p);
-    return (uint32_t)__ballot(okay) & 15u;
-  };
+  const int key_from = chunk_place<DP>(col, h);
 
   float top = -kInfinity, total = 0.0f;
-  Units units;
-  load_units(begin, units);
-  load_tile(units);
-  load_units(begin + 1, units);
-  store_tile(tiles);
-  for (int i = begin; i < end; ++i) {
+  // A tile is asked for two tiles ahead, and its entries before the tile before it is: loads come back in their order,
+  // and to wait for the entries is then no wait for that tile.
+  Raw raw0, raw1;
+  load_tile(entries_of(begin), raw0);
+  const Entries second = entries_of(begin + 1);
+  Entries next = entries_of(begin + 2);
+  uint32_t okay = raw0.okay;
+  if (begin + 1 < end) load_tile(second, raw1);
+  store_tile(tiles, raw0);
+  auto take_tile = [&](int i, Raw& ahead, const Raw& coming) {
     const int now = ((i - begin) & 1) * kTileBytes;
-    if (i + 1 < end) load_tile(units);
-    load_units(i + 2, units);
+    const Entries units = next;
+    next = entries_of(i + 3);
+    if (i + 2 < end) load_tile(units, ahead);
     __syncthreads();
     const uint32_t base = (uint32_t)i * TOK;
-    const uint32_t okay = okay_of(i);
     if (!idle && base <= w1) {
       const bool whole = okay == 15u && base + TOK - 1 <= w0;
       f32x16 score[2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
         for (int e = 0; e < 16; ++e) score[half][e] = 0.0f;
+      {
+        // operands four at a time, the next four on their way while these are multiplied
+        f16x8 keys[2][4];
+        auto load_keys = [&](int n, f16x8 (&to)[4]) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const f16x8 key = *(const f16x8*)(tiles + now + chunk_place<DP>(half * 32 + col, 2 * k + h));
+          for (int e = 0; e < 4; ++e) {
+            // (the exclusive or with k, in the low bits of places that are multiples of 128, gives them from one)
+            const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
+            to[e] = *(const f16x8*)(tiles + ((now + key_from) ^ (k % 8 * 32)) + half * 32 * DP * 2 + k / 8 * 256);
+          }
+        };
+        load_keys(0, keys[0]);
+        __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int m = 0; m < TERMS; ++m)
-            score[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, query[k][m], score[half], 0, 0, 0);
+        for (int n = 0; n < KS / 2; ++n) {
+          if (n + 1 < KS / 2) load_keys(n + 1, keys[(n + 1) % 2]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int half = (4 * n + e) / KS, k = (4 * n + e) % KS;
+#pragma unroll
+            for (int m = 0; m < TERMS; ++m)
+              score[half] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[n % 2][e], query[k][m], score[half], 0, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
       // score[half][e] is row col, position base + 32 half + 8 (e / 4) + 4 h + e % 4
       if constexpr (I8)
@@ -616,7 +694,10 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_statistics(const T
           score[n / 16][e] = seen ? score[n / 16][e] : -kInfinity;
         }
       };
-      if (!whole) mask();
+      if (!whole) {
+        asm volatile("");  // (a branch, not a choice for every score)
+        mask();
+      }
       // What weights are taken against is raised only when a score passes it by more than kSlack: while that bound is
       // not below 0, the numbers' bits compare as whole numbers do (a NaN may pass it, or reaches the sum by itself).
       auto raise = [&]() {
@@ -641,18 +722,26 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_statistics(const T
       if (__any(!(bound >= 0.0f) || most > __float_as_int(bound))) raise();
       float sum = weigh();
       if (__any(sum != sum && row_scale == row_scale)) {
+        float x[32];
 #pragma unroll
-        for (int n = 0; n < 32; ++n) {
-          const int e = n % 16, in = n / 16 * 32 + e / 4 * 8 + e % 4 + 4 * h;
-          if (score[n / 16][e] != score[n / 16][e])
-            score[n / 16][e] = score_again<T, I8>(queries, a, span, kv, row, base + in) * row_inverse;
-        }
+        for (int n = 0; n < 32; ++n) x[n] = score[n / 16][n % 16];
+        scores_again<T, I8>(query_of(queries, a, span, kv, row), a, span, kv,
+                            [&](int n) { return (int64_t)base + n / 16 * 32 + n % 16 / 4 * 8 + n % 4 + 4 * h; }, row_inverse, x);
+#pragma unroll
+        for (int n = 0; n < 32; ++n) score[n / 16][n % 16] = x[n];
         raise();
         sum = weigh();
       }
       total += sum;
     }
-    if (i + 1 < end) store_tile(tiles + (kTileBytes - now));
+    if (i + 1 < end) {
+      store_tile(tiles + (kTileBytes - now), coming);
+      okay = coming.okay;
+    }
+  };
+  for (int i = begin; i < end; i += 2) {
+    take_tile(i, raw0, raw1);
+    if (i + 1 < end) take_tile(i + 1, raw1, raw0);
   }
   join_statistics(top, total, __shfl_xor(top, 32, kWave), __shfl_xor(total, 32, kWave));
   if (h != 0 || !mine) return;
@@ -673,11 +762,12 @@ __global__ void __launch_bounds__(128) many_rows(MassArgs a) {
   const int splits = split_tiles(a, (uint32_t)span.start + last / (uint32_t)a.group, 64).count;
   const int64_t place = row_place(a, span, kv) + row;
   float top = a.statistics[place * 2], total = a.statistics[place * 2 + 1];
+#pragma unroll 8
   for (int i = 1; i < splits; ++i) {
     const float* st = a.statistics + (i * a.rows + place) * 2;
     join_statistics(top, total, st[0], st[1]);
   }
-  a.constants[place] = row_of(a.constants[place].scale, top, total);
+  a.constants[place] = row_of(a.constants[place][kScale], top, total);
 }
 
 // Many rows' positions: 32 SETS a wave, whose keys stay in its registers, 128 SETS a block, while the
@@ -686,7 +776,17 @@ __global__ void __launch_bounds__(128) many_rows(MassArgs a) {
 // until the last. A block has every `parts`-th part of the rows that see its tile of positions.
 //
 // A score that is NaN where its row is numbers is one of -infinity (a key's infinity met a zero term): had it
-// been NaN or infinity the row would not be. So a NaN weight counts as 0, times a row's inverse that may be NaN.
+// been NaN or infinity the row would not be. So a NaN weight counts as 0, times an inverse that is NaN where the row is.
+
+// The sum over a half of a wave, in every lane of it.
+__device__ __forceinline__ float half_sum(float v) {
+  v += __int_as_float(dpp_move32<0xb1>(__float_as_int(v)));   // quad_perm [1, 0, 3, 2]
+  v += __int_as_float(dpp_move32<0x4e>(__float_as_int(v)));   // quad_perm [2, 3, 0, 1]
+  v += __int_as_float(dpp_move32<0x141>(__float_as_int(v)));  // row_half_mirror
+  v += __int_as_float(dpp_move32<0x140>(__float_as_int(v)));  // row_mirror
+  return v + __shfl_xor(v, 16, kWave);
+}
+
 template <typename T, bool I8, int DP>
 constexpr int kSumRows = (sizeof(T) == 4 ? 2 : 1) * DP > 256 ? 32 : 64;
 template <int DP>
@@ -717,6 +817,27 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
     const int from = j0 > start ? (int)((j0 - start) * group / RT) : 0;
     const int each = parted ? (all_tiles - from + a.parts - 1) / a.parts : all_tiles;
     const int begin = min(from + part * each, all_tiles), end = min(begin + each, all_tiles);
+
+    // ---- the rows
+    u32x4 raw[kLoads];
+    Row constants[RT / 32], coming[RT / 32];
+    auto load_tile = [&](int i) {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) {
+        const int q = thread + n * 256, row = q / (TERMS * DP / 8), chunk = q % (TERMS * DP / 8);
+        raw[n] = *(const u32x4*)(a.halves + (first + min((uint32_t)(i * RT + row), rows - 1)) * (TERMS * DP) + chunk * 8);
+      }
+#pragma unroll
+      for (int r = 0; r < RT / 32; ++r) coming[r] = a.constants[first + min((uint32_t)(i * RT + r * 32 + col), rows - 1)];
+    };
+    auto store_tile = [&](char* to) {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) {
+        const int q = thread + n * 256, row = q / (TERMS * DP / 8), chunk = q % (TERMS * DP / 8);
+        *(u32x4*)(to + chunk / (DP / 8) * kTermBytes + chunk_place<DP>(row, chunk % (DP / 8))) = raw[n];
+      }
+    };
+    if (begin < end) load_tile(begin);
 
     // ---- the wave's positions
     const uint32_t base = j0 + wave * 32 * SETS;
@@ -752,36 +873,19 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
         }
     }
 
-    // ---- the rows
-    uint4 raw[kLoads];
-    Row constants[RT / 32], coming[RT / 32];
-    auto load_tile = [&](int i) {
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n) {
-        const int q = thread + n * 256, row = q / (TERMS * DP / 8), chunk = q % (TERMS * DP / 8);
-        raw[n] = *(const uint4*)(a.halves + (first + min((uint32_t)(i * RT + row), rows - 1)) * (TERMS * DP) + chunk * 8);
-      }
-#pragma unroll
-      for (int r = 0; r < RT / 32; ++r) coming[r] = a.constants[first + min((uint32_t)(i * RT + r * 32 + col), rows - 1)];
-    };
-    auto store_tile = [&](char* to) {
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n) {
-        const int q = thread + n * 256, row = q / (TERMS * DP / 8), chunk = q % (TERMS * DP / 8);
-        *(uint4*)(to + chunk / (DP / 8) * kTermBytes + chunk_place<DP>(row, chunk % (DP / 8))) = raw[n];
-      }
-    };
+    const int query_from = chunk_place<DP>(col, h);
     float sum[SETS][16];
 #pragma unroll
     for (int set = 0; set < SETS; ++set)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum[set][e] = 0.0f;
     if (begin < end) {
-      load_tile(begin);
       __syncthreads();  // (the tiles of the positions before are used up)
       store_tile(tiles);
     }
-    for (int i = begin; i < end; ++i) {
+    // WHOLE: every row of the tile sees every position of the block
+    auto take_tile = [&](int i, auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
       const int now = ((i - begin) & 1) * kTileBytes;
 #pragma unroll
       for (int r = 0; r < RT / 32; ++r) constants[r] = coming[r];
@@ -791,75 +895,96 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
       for (int r = 0; r < RT / 32; ++r) {
         const uint32_t row0 = (uint32_t)i * RT + r * 32;
         // (the wave's first position is past the last row's own: nothing is seen)
-        if (row0 >= rows || base > start + min(row0 + 31, rows - 1) / group) continue;
-        const bool whole = row0 + 32 <= rows && base + 32 * SETS - 1 <= start + row0 / group;
+        if (!WHOLE && (row0 >= rows || base > start + min(row0 + 31, rows - 1) / group)) continue;
         f32x16 score[SETS];
 #pragma unroll
         for (int set = 0; set < SETS; ++set)
 #pragma unroll
           for (int e = 0; e < 16; ++e) score[set][e] = 0.0f;
+        {
+          // operands four at a time, as above
+          constexpr int kAll = KS * TERMS;
+          f16x8 query[2][4];
+          auto load_query = [&](int n, f16x8 (&to)[4]) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+            for (int e = 0; e < 4; ++e) {
+              const int k = (4 * n + e) / TERMS, term = (4 * n + e) % TERMS;
+              to[e] = *(const f16x8*)(tiles + ((now + query_from) ^ (k % 8 * 32)) + term * kTermBytes + r * 32 * DP * 2 +
+                                      k / 8 * 256);
+            }
+          };
+          load_query(0, query[0]);
+          __builtin_amdgcn_s_setprio(1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t) {
-            const f16x8 query = *(const f16x8*)(tiles + now + t * kTermBytes + chunk_place<DP>(r * 32 + col, 2 * k + h));
+          for (int n = 0; n < kAll / 4; ++n) {
+            if (n + 1 < kAll / 4) load_query(n + 1, query[(n + 1) % 2]);
 #pragma unroll
-            for (int set = 0; set < SETS; ++set)
-              score[set] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key[set][k], query, score[set], 0, 0, 0);
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int set = 0; set < SETS; ++set)
+                score[set] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key[set][(4 * n + e) / TERMS], query[n % 2][e], score[set], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
           }
+          __builtin_amdgcn_s_setprio(0);
+        }
         const Row c = constants[r];
         // positions base + 32 set + 8 (e / 4) + 4 h + e % 4, of which the row sees those up to its own
-        const int seen = row0 + col < rows ? (int)(start + (row0 + col) / group - base) - 4 * h : -1;
+        int seen = INT32_MAX;
+        if (!WHOLE) seen = row0 + col < rows ? (int)(start + (row0 + col) / group - base) - 4 * h : -1;
 #pragma unroll
         for (int set = 0; set < SETS; ++set)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x = score[set][e];
             if constexpr (I8) x *= key_scale[set][e];
-            const float p = fmaxf(exp2_fast(fmaf(x, c.scale, -c.top)), 0.0f);
-            if (whole) sum[set][e] = fmaf(p, c.inverse, sum[set][e]);
-            else sum[set][e] = set * 32 + e / 4 * 8 + e % 4 <= seen ? fmaf(p, c.inverse, sum[set][e]) : sum[set][e];
+            // (at most 1 but for NaN, of which the bounds make 0)
+            const float p = __builtin_amdgcn_fmed3f(exp2_fast(fmaf(x, c[kScale], -c[kTop])), 0.0f, 1.0f);
+            const float next = fmaf(p, c[kInverse], sum[set][e]);
+            sum[set][e] = set * 32 + e / 4 * 8 + e % 4 <= seen ? next : sum[set][e];
           }
       }
       if (i + 1 < end) store_tile(tiles + (kTileBytes - now));
-    }
+    };
+    // rows from token `all` on see all the block's positions; the last tile may have fewer rows
+    const uint32_t all = j0 + kPositions > start + 1 ? j0 + kPositions - 1 - start : 0;
+    const int first_whole = (int)min(((uint64_t)all * group + RT - 1) / RT, (uint64_t)all_tiles);
+    int i = begin;
+    for (; i < min(first_whole, end); ++i) take_tile(i, std::false_type());
+    for (; i < min((int)(rows / RT), end); ++i) take_tile(i, std::true_type());
+    for (; i < end; ++i) take_tile(i, std::false_type());
 
     // ---- the lanes' rows added up: lanes 0 to 3 of each half have four positions of every set each
 #pragma unroll
     for (int set = 0; set < SETS; ++set) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-#pragma unroll
-        for (int mask = 1; mask < 32; mask <<= 1) sum[set][e] += __shfl_xor(sum[set][e], mask, kWave);
+      for (int e = 0; e < 16; ++e) sum[set][e] = half_sum(sum[set][e]);
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (col == q)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t j = base + set * 32 + 8 * q + 4 * h + e;
-            if (j >= length) continue;
-            if (parted) {
-              a.partials[(((int64_t)part * a.p.sequences + s) * a.kv_heads + kv) * a.summed + j] = sum[set][4 * q + e];
-            } else {
-              Place place;
-              if (place_of(a, span, j, kv, place)) store_mass(a, span, j, place, sum[set][4 * q + e]);
-            }
-          }
+        if (col == q) {
+          const uint32_t j = base + set * 32 + 8 * q + 4 * h;
+          const float four[4] = {sum[set][4 * q], sum[set][4 * q + 1], sum[set][4 * q + 2], sum[set][4 * q + 3]};
+          if (!parted) store_masses(a, span, j, kv, four);
+          else if (j < length)
+            *(f32x4*)(a.partials + (((int64_t)part * a.p.sequences + s) * a.kv_heads + kv) * a.summed + j) =
+                f32x4{four[0], four[1], four[2], four[3]};
+        }
     }
   }
 }
 
-// Positions' sums over the parts of many rows.
-__global__ void __launch_bounds__(256) many_parts(MassArgs a) {
+// Positions' sums over the parts of many rows, four a thread.
+__global__ void __launch_bounds__(64) many_parts(MassArgs a) {
   const int kv = blockIdx.y % (unsigned)a.kv_heads, s = blockIdx.y / (unsigned)a.kv_heads;
   const Span span = span_of<false>(a.p, s);
-  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t j = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
   if (span.rows == 0 || j >= min(span.start + span.rows, (int64_t)a.summed)) return;
-  float sum = 0.0f;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
   for (int part = 0; part < a.parts; ++part)
-    sum += a.partials[(((int64_t)part * a.p.sequences + s) * a.kv_heads + kv) * a.summed + j];
-  Place place;
-  if (place_of(a, span, j, kv, place)) store_mass(a, span, j, place, sum);
+    sum += *(const f32x4*)(a.partials + (((int64_t)part * a.p.sequences + s) * a.kv_heads + kv) * a.summed + j);
+  const float four[4] = {sum[0], sum[1], sum[2], sum[3]};
+  store_masses(a, span, j, kv, four);
 }
 
 // ------------------------------------------------------------------ host side
@@ -914,7 +1039,7 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     const int64_t positions = dim <= 128 ? 256 : 128, tiles = ceil_div(seen, positions);
     p.strides = (int)std::min(tiles, std::max<int64_t>(kSplitBlocks / units, 1));
     const int64_t row_tiles = ceil_div((by_offsets || sequences == 1 ? tokens : 1) * group, 64);
-    p.parts = (int)std::max<int64_t>(std::min({1024 / (units * tiles), ceil_div(row_tiles, 4), (int64_t)16}), 1);
+    p.parts = (int)std::max<int64_t>(std::min({(int64_t)2048 / (units * tiles), ceil_div(row_tiles, 4), (int64_t)16}), 1);
     p.summed = p.parts > 1 ? tiles * positions : 0;
   }
   at(p.split.splits * rows * 8);
@@ -949,7 +1074,7 @@ int launch_products(const char* entry, const T* queries, const MassArgs& a, cons
   hipLaunchKernelGGL((many_sums<T, I8, DP>), dim3((unsigned)(units * a.strides * a.parts)), block, 0, st, a);
   if (const int bad = launched(entry)) return bad;
   if (a.parts > 1) {
-    hipLaunchKernelGGL(many_parts, dim3((unsigned)ceil_div(a.summed, 256), (unsigned)units), block, 0, st, a);
+    hipLaunchKernelGGL(many_parts, dim3((unsigned)ceil_div(a.summed, 256), (unsigned)units), dim3(64), 0, st, a);
     return launched(entry);
   }
   return 0;
@@ -1013,6 +1138,7 @@ int attention_mass(const char* entry, const T* queries, MassArgs a, int64_t long
   a.rows = (int64_t)a.p.tokens * a.heads;
   a.group = a.heads / a.kv_heads;
   a.columns = unit_columns(a.p.page_size);
+  a.wide = aligned16(a.mass) && aligned16(a.before);
   const bool aligned = a.dim % 8 == 0 && aligned16(queries) && aligned16(a.keys) && aligned16(a.key_scales);
   return a.key_scales ? launch_mass<T, true>(entry, queries, a, plan, aligned, longest, (hipStream_t)stream)
                       : launch_mass<T, false>(entry, queries, a, plan, aligned, longest, (hipStream_t)stream);
@@ -1039,7 +1165,7 @@ extern "C" int drift_attention_mass_workspace(int32_t sequences, int32_t tokens,
   MassArgs {                                                                                                        \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
         kv_heads, head_dim, 0, scale, keys, key_scales, before, mass, {}, 0, 0, nullptr, nullptr, nullptr, nullptr, \
-        nullptr, 1, 1, 1, 0, 1                                                                                      \
+        nullptr, 1, 1, 1, 0, 1, 0                                                                                   \
   }
 
 extern "C" int drift_attention_mass_f32(const float* queries, const void* keys, const float* key_scales,
