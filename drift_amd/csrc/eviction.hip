@@ -38,10 +38,12 @@ constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave, kBins = 20
 // lowest first. Three passes over the orders' digits of 11, 11 and 10 bits find it,
 // each by a histogram in LDS of the candidates that share the digits so far; two more
 // write the positions in their order, by counts of the waves before and ballots.
+// EACH: the candidates a lane keeps in registers; 0: more, read again in each pass.
+template <int EACH>
 __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
   __shared__ uint32_t bins[kBins];
   __shared__ uint32_t sums[2][kPickWaves];
-  __shared__ uint32_t found[2];
+  __shared__ uint32_t found[3];
   const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
   const int s = blockIdx.x / (unsigned)a.kv_heads, kv = blockIdx.x % (unsigned)a.kv_heads;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.keep;
@@ -61,14 +63,42 @@ __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
   if (wanted == 0) return;
   const uint32_t candidates = (uint32_t)(length - a.sinks - a.recent);  // more than are wanted
   const int32_t* table = a.tables + (int64_t)s * a.table_pages;
-  auto order_at = [&](uint32_t candidate) -> uint32_t {
-    const uint32_t j = candidate + a.sinks, unit = j / 16, column = a.columns.of(unit);
-    const int32_t page = table[column];
+  auto column_of = [&](uint32_t candidate) { return a.columns.of((candidate + a.sinks) / 16); };
+  auto order_at = [&](uint32_t candidate, int32_t page) -> uint32_t {
     if (page < 0 || page >= a.cache_pages) {
       if (a.bad_page) *a.bad_page = 1;
       return 0;
     }
-    return order_of(a.mass[((int64_t)page * a.kv_heads + kv) * a.page_size + (j - column * a.columns.page_units * 16)]);
+    const uint32_t j = candidate + a.sinks, off = j - column_of(candidate) * a.columns.page_units * 16;
+    return order_of(a.mass[((int64_t)page * a.kv_heads + kv) * a.page_size + off]);
+  };
+  // a wave's candidates lie together, a lane has every 64th of them: their places then follow from the waves' before
+  const uint32_t each = (candidates + kPickThreads - 1) / kPickThreads;  // of a lane
+  const uint32_t begin = min(wave * each * kWave, candidates), end = min(begin + each * kWave, candidates);
+  uint32_t kept_order[EACH > 0 ? EACH : 1];
+  if constexpr (EACH > 0) {
+    int32_t page[EACH];
+#pragma unroll
+    for (int n = 0; n < EACH; ++n)
+      page[n] = begin + n * kWave + lane < end ? table[column_of(begin + n * kWave + lane)] : 0;
+#pragma unroll
+    for (int n = 0; n < EACH; ++n)
+      kept_order[n] = begin + n * kWave + lane < end ? order_at(begin + n * kWave + lane, page[n]) : 0;
+  }
+  // `take` with each of the lane's orders, and whether there is one; whole waves
+  auto for_each = [&](auto take) {
+    if constexpr (EACH > 0) {
+#pragma unroll
+      for (int n = 0; n < EACH; ++n) {
+        const uint32_t i = begin + n * kWave;
+        if (i < end) take(i + lane, i + lane < end, kept_order[n]);
+      }
+    } else {
+      for (uint32_t i = begin; i < end; i += kWave) {
+        const bool in = i + lane < end;
+        take(i + lane, in, in ? order_at(i + lane, table[column_of(i + lane)]) : 0u);
+      }
+    }
   };
 
   uint32_t digits = 0, known = 0, left = wanted;  // the threshold's digits so far, and how many are wanted of those that share them
@@ -76,10 +106,19 @@ __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
     for (int i = thread; i < kBins; i += kPickThreads) bins[i] = 0;
     __syncthreads();
-    for (uint32_t i = thread; i < candidates; i += kPickThreads) {
-      const uint32_t order = order_at(i);
-      if ((order & known) == digits) atomicAdd(&bins[order >> shift & (width - 1)], 1u);
-    }
+    for_each([&](uint32_t, bool in, uint32_t order) {
+      const bool counts = in && (order & known) == digits;
+      const uint32_t bin = order >> shift & (width - 1);
+      // (equal masses, as before the first call, are one addition a wave)
+      const uint64_t all = __ballot(counts);
+      if (all == 0) return;
+      const uint32_t one = uniform(__shfl(bin, __ffsll((unsigned long long)all) - 1, kWave));
+      if (__all(!counts || bin == one)) {
+        if (lane == 0) atomicAdd(&bins[one], (uint32_t)__popcll(all));
+      } else if (counts) {
+        atomicAdd(&bins[bin], 1u);
+      }
+    });
     __syncthreads();
     // a thread's two bins, the highest first; those above them
     const int bin = kBins - 2 - 2 * thread;
@@ -94,41 +133,38 @@ __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
     __syncthreads();
     uint32_t above = upto - high - low;
     for (int w = 0; w < wave; ++w) above += sums[0][w];
-    if (above < left && left <= above + high) found[0] = bin + 1, found[1] = above;
-    else if (above + high < left && left <= above + high + low) found[0] = bin, found[1] = above + high;
+    if (above < left && left <= above + high) found[0] = bin + 1, found[1] = above, found[2] = high;
+    else if (above + high < left && left <= above + high + low) found[0] = bin, found[1] = above + high, found[2] = low;
     __syncthreads();
     digits |= found[0] << shift;
     known |= (uint32_t)(width - 1) << shift;
     left -= found[1];
+    const bool all_taken = found[2] == left;
     __syncthreads();
+    if (all_taken) break;  // (every candidate that shares the digits: those with more digits are all taken)
   }
 
-  // a wave's candidates lie together, so that their places follow from the waves' before
-  const uint32_t each = (candidates + kPickThreads - 1) / kPickThreads * kWave;
-  const uint32_t begin = min(wave * each, candidates), end = min(begin + each, candidates);
+  // above the threshold, or (left of them, the lowest first) sharing its digits
   uint32_t more = 0, equal = 0;
-  for (uint32_t i = begin; i < end; i += kWave) {
-    const uint32_t order = i + lane < end ? order_at(i + lane) : 0;
-    const bool in = i + lane < end;
-    more += __popcll(__ballot(in && order > digits));
-    equal += __popcll(__ballot(in && order == digits));
-  }
+  for_each([&](uint32_t, bool in, uint32_t order) {
+    more += __popcll(__ballot(in && (order & known) > digits));
+    equal += __popcll(__ballot(in && (order & known) == digits));
+  });
   if (lane == 0) sums[0][wave] = more, sums[1][wave] = equal;
   __syncthreads();
   uint32_t more_before = 0, equal_before = 0;
   for (int w = 0; w < wave; ++w) more_before += sums[0][w], equal_before += sums[1][w];
   uint32_t place = a.sinks + more_before + min(equal_before, left);
   const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t i = begin; i < end; i += kWave) {
-    const bool in = i + lane < end;
-    const uint32_t order = in ? order_at(i + lane) : 0;
-    const uint64_t ties = __ballot(in && order == digits);
-    const bool taken = in && (order > digits || (order == digits && equal_before + __popcll(ties & below) < left));
+  for_each([&](uint32_t i, bool in, uint32_t order) {
+    const bool tie = in && (order & known) == digits;
+    const uint64_t ties = __ballot(tie);
+    const bool taken = (in && (order & known) > digits) || (tie && equal_before + __popcll(ties & below) < left);
     const uint64_t all = __ballot(taken);
-    if (taken) kept[place + __popcll(all & below)] = (int32_t)(i + lane + a.sinks);
+    if (taken) kept[place + __popcll(all & below)] = (int32_t)(i + a.sinks);
     place += __popcll(all);
     equal_before += __popcll(ties);
-  }
+  });
 }
 
 // ------------------------------------------------------------------ the kept rows' move
@@ -208,6 +244,223 @@ __global__ void __launch_bounds__(256) move_rows(KeepArgs a, int64_t rows, int64
   }
 }
 
+// Rows in chunks of 128 by a block: a block has a sequence's and key head's keys with
+// their words (scales and masses), or 64 dimensions of its values, which share
+// nothing; the cache's bits pass through registers.
+//
+// Keys go row by row in pieces of PIECE bytes. Of values, which lie transposed, a lane has a dimension and a wave
+// 32 rows: each is a load of one number a lane, and 16 rows that go to a whole unit of
+// 16 positions are one store (two for F16) of a lane.
+//
+// In place, what a chunk reads has to be read before another's rows are written over
+// it. A block that has a whole list keeps to it chunk by chunk where every row comes from its own place or from
+// behind it, or from before all places that rows go to (an ascending list does): later rows' sources are then
+// not among the places of earlier ones. Else it puts all rows by first. Where lists are long and few, their chunks
+// are blocks of two launches instead, one that puts rows by and one that brings them back.
+enum KeepMode { kWalk, kDirect, kPutBy, kBringBack };
+constexpr int kKeepRows = 128;
+
+template <typename E, int PIECE, int PIECES>
+struct KeepChunk {
+  static constexpr int kWords = PIECE / 4;
+  typedef uint32_t Piece __attribute__((ext_vector_type(kWords)));
+  Piece keys[PIECES];
+  float words[3];
+  u32x4 values[2][sizeof(E)];
+};
+
+template <typename E, int PIECE, int PIECES, int MODE>
+__global__ void __launch_bounds__(256) keep_rows(KeepArgs a, int chunks) {
+  using Chunk = KeepChunk<E, PIECE, PIECES>;
+  using Piece = typename Chunk::Piece;
+  constexpr int kBytes = sizeof(E);
+  __shared__ int64_t from[kKeepRows], to[kKeepRows], word_from[kKeepRows], word_to[kKeepRows];
+  __shared__ uint64_t moves[2];  // which of the chunk's rows move
+  const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
+  const int parts = 1 + (a.dim + 63) / 64;
+  unsigned block = blockIdx.x;
+  const int own_chunk = MODE == kWalk ? 0 : block % (unsigned)chunks;
+  if (MODE != kWalk) block /= (unsigned)chunks;
+  const int kv = block % (unsigned)a.kv_heads, part = block / (unsigned)a.kv_heads % (unsigned)parts;
+  const int s = block / (unsigned)a.kv_heads / (unsigned)parts;
+  const int32_t count = a.counts ? a.counts[s] : a.most, start = a.starts ? a.starts[s] : 0;
+  if (count < 0 || count > a.most || start < 0) {
+    if (a.bad_page) *a.bad_page = 1;
+    return;
+  }
+  const int32_t* kept = a.kept + ((int64_t)s * a.kept_heads + (a.kept_heads == 1 ? 0 : kv)) * a.most;
+  const int32_t *table = a.tables + (int64_t)s * a.table_pages, *into = a.into + (int64_t)s * a.into_pages;
+  const int row_pieces = a.dim * kBytes / PIECE, d = (part - 1) * 64 + lane;  // (of values: the lane's dimension)
+  E* const values = (E*)a.values;
+  float* const words[3] = {a.key_scales, a.value_scales, a.mass};
+
+  // where the chunk's rows lie and where they go
+  auto place_rows = [&](int chunk) {
+    if (thread < kKeepRows) {
+      const int i = chunk * kKeepRows + thread;
+      bool good = i < count;
+      int64_t page = 0, off = 0, its_page = 0, its_off = 0;
+      if (good) {
+        good = place_of(a, table, a.table_pages, kept[i], page, off) &&
+               place_of(a, into, a.into_pages, (int64_t)start + i, its_page, its_off);
+        if (!good && a.bad_page) *a.bad_page = 1;
+      }
+      if (!good) page = off = its_page = its_off = 0;
+      if (part == 0) {
+        from[thread] = ((page * a.page_size + off) * a.kv_heads + kv) * a.dim;
+        to[thread] = ((its_page * a.page_size + its_off) * a.kv_heads + kv) * a.dim;
+        word_from[thread] = (page * a.kv_heads + kv) * a.page_size + off;
+        word_to[thread] = (its_page * a.kv_heads + kv) * a.page_size + its_off;
+      } else {
+        from[thread] = (page * a.kv_heads + kv) * a.dim * a.page_size + off;
+        to[thread] = (its_page * a.kv_heads + kv) * a.dim * a.page_size + its_off;
+      }
+      const uint64_t good_rows = __ballot(good);
+      if (lane == 0) moves[wave] = good_rows;
+    }
+    __syncthreads();
+  };
+  auto moves_row = [&](int row) { return (bool)(moves[row / 64] >> (row % 64) & 1); };
+  auto read_rows = [&](Chunk& c) {
+    if (part == 0) {
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) {
+        const int q = thread + n * 256, row = q / row_pieces;
+        if (row < kKeepRows && moves_row(row))
+          c.keys[n] = *(const Piece*)((const char*)a.keys + from[row] * kBytes + (q - row * row_pieces) * PIECE);
+      }
+      if (thread < kKeepRows && moves_row(thread))
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+          if (words[w]) c.words[w] = words[w][word_from[thread]];
+    } else if (d < a.dim) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t x[16];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) x[n] = (uint32_t)values[uniform(from[wave * 32 + u * 16 + n]) + (int64_t)d * a.page_size];
+#pragma unroll
+        for (int n = 0; n < 4 * kBytes; ++n) {
+          uint32_t word = 0;
+#pragma unroll
+          for (int e = 0; e < 4 / kBytes; ++e) word |= x[n * (4 / kBytes) + e] << (8 * kBytes * e);
+          c.values[u][n / 4][n % 4] = word;
+        }
+      }
+    }
+  };
+  auto write_rows = [&](const Chunk& c, bool units) {
+    if (part == 0) {
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) {
+        const int q = thread + n * 256, row = q / row_pieces;
+        if (row < kKeepRows && moves_row(row))
+          *(Piece*)((char*)a.keys + to[row] * kBytes + (q - row * row_pieces) * PIECE) = c.keys[n];
+      }
+      if (thread < kKeepRows && moves_row(thread))
+#pragma unroll
+        for (int w = 0; w < 3; ++w)
+          if (words[w]) words[w][word_to[thread]] = c.words[w];
+    } else if (d < a.dim) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row0 = wave * 32 + u * 16;
+        const uint32_t moving = (uint32_t)(moves[row0 / 64] >> (row0 % 64)) & 0xffffu;
+        if (units && moving == 0xffffu) {
+          u32x4* const unit = (u32x4*)(values + uniform(to[row0]) + (int64_t)d * a.page_size);
+#pragma unroll
+          for (int n = 0; n < kBytes; ++n) unit[n] = c.values[u][n];
+        } else {
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            if (moving >> n & 1)
+              values[uniform(to[row0 + n]) + (int64_t)d * a.page_size] =
+                  (E)(c.values[u][n * kBytes / 16][n * kBytes % 16 / 4] >> (n * kBytes % 4 * 8));
+        }
+      }
+    }
+  };
+  // a thread's own pieces of a chunk, put by and brought back
+  constexpr int kSlots = PIECES * PIECE / 16 > 2 * kBytes ? PIECES * PIECE / 16 : 2 * kBytes;
+  auto slot_of = [&](int chunk) {
+    return (u32x4*)a.scratch + (((int64_t)block * chunks + chunk) * (kSlots + 1) * 256 + thread);
+  };
+  auto put_by = [&](const Chunk& c, u32x4* slot) {
+    if (part == 0) {
+#pragma unroll
+      for (int n = 0; n < PIECES; n += 16 / PIECE) {
+        u32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = c.keys[n + e / Chunk::kWords][e % Chunk::kWords];
+        slot[n * PIECE / 16 * 256] = x;
+      }
+      slot[kSlots * 256] = u32x4{__float_as_uint(c.words[0]), __float_as_uint(c.words[1]), __float_as_uint(c.words[2]), 0};
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2 * kBytes; ++n) slot[n * 256] = c.values[n / kBytes][n % kBytes];
+    }
+  };
+  auto bring_back = [&](Chunk& c, const u32x4* slot) {
+    if (part == 0) {
+#pragma unroll
+      for (int n = 0; n < PIECES; n += 16 / PIECE) {
+        const u32x4 x = slot[n * PIECE / 16 * 256];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c.keys[n + e / Chunk::kWords][e % Chunk::kWords] = x[e];
+      }
+      const u32x4 x = slot[kSlots * 256];
+#pragma unroll
+      for (int w = 0; w < 3; ++w) c.words[w] = __uint_as_float(x[w]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2 * kBytes; ++n) c.values[n / kBytes][n % kBytes] = slot[n * 256];
+    }
+  };
+
+  const bool units = start % 16 == 0;
+  Chunk c{};
+  if constexpr (MODE != kWalk) {
+    if (own_chunk * kKeepRows >= count) return;
+    place_rows(own_chunk);
+    if (MODE == kBringBack) bring_back(c, slot_of(own_chunk));
+    else read_rows(c);
+    if (MODE == kPutBy) put_by(c, slot_of(own_chunk));
+    else write_rows(c, units);
+    return;
+  }
+  const int all = (count + kKeepRows - 1) / kKeepRows;
+  bool by_place = true;
+  if (all > 1) {
+    bool here = true;
+    for (int i = thread; i < count; i += 256) here &= kept[i] >= (int64_t)start + i || kept[i] < start;
+    by_place = __syncthreads_and(here);
+  }
+  if (by_place) {
+    for (int chunk = 0; chunk < all; ++chunk) {
+      place_rows(chunk);
+      read_rows(c);
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows have come
+      __syncthreads();
+      write_rows(c, units);
+      __syncthreads();  // (the places are used up)
+    }
+    return;
+  }
+  for (int chunk = 0; chunk < all; ++chunk) {
+    place_rows(chunk);
+    read_rows(c);
+    put_by(c, slot_of(chunk));
+    __syncthreads();
+  }
+  for (int chunk = 0; chunk < all; ++chunk) {
+    place_rows(chunk);
+    bring_back(c, slot_of(chunk));
+    write_rows(c, units);
+    __syncthreads();
+  }
+}
+
+// Bytes of scratch of a row that is put by on its own (move_rows).
 int64_t scratch_row(int32_t dim, bool quantized) { return ceil_div((int64_t)dim * 2 * (quantized ? 1 : 2), 4) * 4 + 12; }
 
 int check_keep(const char* entry, int32_t sequences, int32_t most, int32_t kv_heads, int32_t dim) {
@@ -218,12 +471,62 @@ int check_keep(const char* entry, int32_t sequences, int32_t most, int32_t kv_he
   return 0;
 }
 
+// Pieces of keys that a thread has of a chunk; 0: none that the kernel is made for.
+int pieces_of(int32_t dim, bool quantized, int& piece) {
+  const int64_t bytes = (int64_t)dim * (quantized ? 1 : 2);
+  piece = bytes % 16 == 0 ? 16 : 8;
+  if (bytes % piece != 0) return 0;
+  const int64_t pieces = ceil_div(kKeepRows * bytes / piece, 256);
+  return pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 0;
+}
+
 int64_t keep_bytes(int32_t sequences, int32_t most, int32_t kv_heads, int32_t dim, bool quantized) {
-  return (int64_t)sequences * most * kv_heads * scratch_row(dim, quantized);
+  const int64_t by_rows = (int64_t)sequences * most * kv_heads * scratch_row(dim, quantized);
+  int piece;
+  const int pieces = pieces_of(dim, quantized, piece), slots = std::max(pieces * piece / 16, quantized ? 2 : 4);
+  const int64_t by_chunks = (int64_t)sequences * kv_heads * (1 + ceil_div(dim, 64)) * ceil_div(most, kKeepRows) *
+                            (slots + 1) * 256 * 16;
+  return ceil_div(pieces == 0 ? by_rows : std::max(by_rows, by_chunks), 16) * 16;
+}
+
+template <typename E, int PIECE, int PIECES>
+int keep_chunks(const char* entry, const KeepArgs& a, bool apart, hipStream_t st) {
+  const int chunks = (int)ceil_div(a.most, kKeepRows);
+  const int64_t lists = (int64_t)a.sequences * a.kv_heads * (1 + ceil_div(a.dim, 64));
+  const dim3 block(256), each((unsigned)(lists * chunks)), walk((unsigned)lists);
+  if (apart || chunks == 1) {
+    if (chunks == 1) hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kWalk>), walk, block, 0, st, a, chunks);
+    else hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kDirect>), each, block, 0, st, a, chunks);
+    return launched(entry);
+  }
+  if (lists >= 512) {
+    hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kWalk>), walk, block, 0, st, a, chunks);
+    return launched(entry);
+  }
+  hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kPutBy>), each, block, 0, st, a, chunks);
+  if (const int bad = launched(entry)) return bad;
+  hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kBringBack>), each, block, 0, st, a, chunks);
+  return launched(entry);
 }
 
 template <typename E>
 int keep(const char* entry, const KeepArgs& a, bool apart, hipStream_t st) {
+  int piece;
+  const int pieces = pieces_of(a.dim, sizeof(E) == 1, piece);
+  const int64_t blocks = (int64_t)a.sequences * a.kv_heads * (1 + ceil_div(a.dim, 64)) * ceil_div(a.most, kKeepRows);
+  if (pieces > 0 && a.cache_pages > 0 && blocks <= kOneWaveBlocks / 4 && aligned16(a.keys) && aligned16(a.values)) {
+#define DRIFT_KEEP(PIECE, PIECES) \
+  if (piece == PIECE && pieces == PIECES) return keep_chunks<E, PIECE, PIECES>(entry, a, apart, st);
+    DRIFT_KEEP(16, 4)
+    DRIFT_KEEP(16, 8)
+    DRIFT_KEEP(16, 16)
+    if constexpr (sizeof(E) == 1) {
+      DRIFT_KEEP(8, 4)
+      DRIFT_KEEP(8, 8)
+      DRIFT_KEEP(8, 16)
+    }
+#undef DRIFT_KEEP
+  }
   const int64_t rows = (int64_t)a.sequences * a.kv_heads * a.most, row_bytes = scratch_row(a.dim, sizeof(E) == 1);
   const dim3 grid((unsigned)ceil_div(rows, 4)), block(256);
   if (apart) {
@@ -271,7 +574,14 @@ extern "C" int drift_heaviest(const float* mass, const int32_t* page_tables, int
     return refuse("%s: counts overlap lengths", entry);  // (each head's block reads its sequence's length)
   const HeaviestArgs a{mass, page_tables, lengths, sequences, table_pages, cache_pages, page_size, kv_heads,
                        sinks, recent, keep, kept, counts, bad_page, unit_columns(page_size)};
-  hipLaunchKernelGGL(pick_heaviest, dim3((unsigned)(sequences * kv_heads)), dim3(kPickThreads), 0, (hipStream_t)stream, a);
+  // (no sequence has more candidates than its page table has room for)
+  const int64_t each = ceil_div(std::max<int64_t>((int64_t)table_pages * page_size - sinks - recent, 0), kPickThreads);
+  const dim3 grid((unsigned)(sequences * kv_heads)), block(kPickThreads);
+  const hipStream_t st = (hipStream_t)stream;
+  if (each <= 2) hipLaunchKernelGGL(pick_heaviest<2>, grid, block, 0, st, a);
+  else if (each <= 8) hipLaunchKernelGGL(pick_heaviest<8>, grid, block, 0, st, a);
+  else if (each <= 32) hipLaunchKernelGGL(pick_heaviest<32>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(pick_heaviest<0>, grid, block, 0, st, a);
   return launched(entry);
 }
 
