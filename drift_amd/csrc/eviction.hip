@@ -40,7 +40,7 @@ constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave, kBins = 20
 // write the positions in their order, by counts of the waves before and ballots.
 // EACH: the candidates a lane keeps in registers; 0: more, read again in each pass.
 template <int EACH>
-__global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
+__global__ void __launch_bounds__(kPickThreads, EACH > 0 && EACH <= 16 ? 8 : 4) pick_heaviest(HeaviestArgs a) {
   __shared__ uint32_t bins[kBins];
   __shared__ uint32_t sums[2][kPickWaves];
   __shared__ uint32_t found[3];
@@ -94,9 +94,17 @@ __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
         if (i < end) take(i + lane, i + lane < end, kept_order[n]);
       }
     } else {
-      for (uint32_t i = begin; i < end; i += kWave) {
-        const bool in = i + lane < end;
-        take(i + lane, in, in ? order_at(i + lane, table[column_of(i + lane)]) : 0u);
+      constexpr int kAhead = 16;  // on their way together
+      for (uint32_t i = begin; i < end; i += kAhead * kWave) {
+        int32_t page[kAhead];
+        uint32_t order[kAhead];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) page[n] = table[column_of(min(i + n * kWave + lane, end - 1))];
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) order[n] = order_at(min(i + n * kWave + lane, end - 1), page[n]);
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n)
+          if (i + n * kWave < end) take(i + n * kWave + lane, i + n * kWave + lane < end, order[n]);
       }
     }
   };
@@ -110,11 +118,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_heaviest(HeaviestArgs a) {
       const bool counts = in && (order & known) == digits;
       const uint32_t bin = order >> shift & (width - 1);
       // (equal masses, as before the first call, are one addition a wave)
-      const uint64_t all = __ballot(counts);
-      if (all == 0) return;
-      const uint32_t one = uniform(__shfl(bin, __ffsll((unsigned long long)all) - 1, kWave));
-      if (__all(!counts || bin == one)) {
-        if (lane == 0) atomicAdd(&bins[one], (uint32_t)__popcll(all));
+      if (__all(counts && bin == uniform(bin))) {
+        if (lane == 0) atomicAdd(&bins[bin], (uint32_t)kWave);
       } else if (counts) {
         atomicAdd(&bins[bin], 1u);
       }
@@ -248,9 +253,10 @@ __global__ void __launch_bounds__(256) move_rows(KeepArgs a, int64_t rows, int64
 // their words (scales and masses), or 64 dimensions of its values, which share
 // nothing; the cache's bits pass through registers.
 //
-// Keys go row by row in pieces of PIECE bytes. Of values, which lie transposed, a lane has a dimension and a wave
-// 32 rows: each is a load of one number a lane, and 16 rows that go to a whole unit of
-// 16 positions are one store (two for F16) of a lane.
+// Keys go row by row in pieces of PIECE bytes. Of values, which lie transposed, a lane has a
+// dimension and a wave 32 rows: 16 bytes of neighbouring positions a load, once for the
+// rows that lie in them, and 16 rows that go to a whole unit of 16 positions leave in one
+// store of a lane (two for F16). So values of rows far apart cost their whole lines.
 //
 // In place, what a chunk reads has to be read before another's rows are written over
 // it. A block that has a whole list keeps to it chunk by chunk where every row comes from its own place or from
@@ -260,204 +266,244 @@ __global__ void __launch_bounds__(256) move_rows(KeepArgs a, int64_t rows, int64
 enum KeepMode { kWalk, kDirect, kPutBy, kBringBack };
 constexpr int kKeepRows = 128;
 
-template <typename E, int PIECE, int PIECES>
-struct KeepChunk {
-  static constexpr int kWords = PIECE / 4;
-  typedef uint32_t Piece __attribute__((ext_vector_type(kWords)));
-  Piece keys[PIECES];
-  float words[3];
-  u32x4 values[2][sizeof(E)];
+// A chunk's places. A walk has three of them: the next chunk's are made while this one's rows are on
+// their way, and a wave that is a chunk behind still finds its own.
+struct KeepPlaces {
+  int64_t from[kKeepRows], to[kKeepRows], word_from[kKeepRows], word_to[kKeepRows];
+  uint64_t moves[2];  // which of its rows move
 };
+
+// A list as a block has it.
+struct KeepList {
+  int s, kv, part;
+  int32_t count, start;
+  const int32_t *kept, *table, *into;
+};
+
+__device__ __forceinline__ void place_rows(const KeepArgs& a, const KeepList& l, int chunk, KeepPlaces& p) {
+  const int thread = threadIdx.x;
+  if (thread >= kKeepRows) return;
+  const int i = chunk * kKeepRows + thread;
+  int64_t page = 0, off = 0, its_page = 0, its_off = 0;
+  bool good = i < l.count;
+  if (good) {
+    good = place_of(a, l.table, a.table_pages, l.kept[i], page, off) &&
+           place_of(a, l.into, a.into_pages, (int64_t)l.start + i, its_page, its_off);
+    if (!good && a.bad_page) *a.bad_page = 1;
+  }
+  if (!good) page = off = its_page = its_off = 0;
+  if (l.part == 0) {
+    p.from[thread] = ((page * a.page_size + off) * a.kv_heads + l.kv) * a.dim;
+    p.to[thread] = ((its_page * a.page_size + its_off) * a.kv_heads + l.kv) * a.dim;
+    p.word_from[thread] = (page * a.kv_heads + l.kv) * a.page_size + off;
+    p.word_to[thread] = (its_page * a.kv_heads + l.kv) * a.page_size + its_off;
+  } else {
+    p.from[thread] = (page * a.kv_heads + l.kv) * a.dim * a.page_size + off;
+    p.to[thread] = (its_page * a.kv_heads + l.kv) * a.dim * a.page_size + its_off;
+  }
+  const uint64_t rows = __ballot(good);
+  if (thread % kWave == 0) p.moves[thread / kWave] = rows;
+}
+
+// What a thread has of a chunk of keys: its piece of every `step`-th row from `row0` on, and a row's words.
+template <typename E, int PIECE, int PIECES>
+struct KeyRows {
+  static constexpr int kSlots = PIECES * PIECE / 16 + 1;
+  typedef uint32_t Piece __attribute__((ext_vector_type(PIECE / 4)));
+  Piece piece[PIECES];
+  u32x4 words;
+  int step, row0, at;
+
+  __device__ __forceinline__ KeyRows(const KeepArgs& a, const KeepList&) {
+    const int pieces = a.dim * (int)sizeof(E) / PIECE;
+    step = 256 / pieces, row0 = threadIdx.x / pieces, at = (threadIdx.x - row0 * pieces) * PIECE;
+    if (row0 >= step) row0 = kKeepRows;  // (a row's last threads, where rows do not divide the block: none)
+  }
+  __device__ __forceinline__ bool has(const KeepPlaces& p, int n) const {
+    const int row = row0 + n * step;
+    return row < kKeepRows && (p.moves[row / 64] >> (row % 64) & 1);
+  }
+  __device__ __forceinline__ void read(const KeepArgs& a, const KeepList&, const KeepPlaces& p) {
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+      if (has(p, n)) piece[n] = *(const Piece*)((const char*)a.keys + p.from[row0 + n * step] * sizeof(E) + at);
+    const int row = threadIdx.x;
+    if (row < kKeepRows && (p.moves[row / 64] >> (row % 64) & 1)) {
+      if (a.key_scales) words[0] = __float_as_uint(a.key_scales[p.word_from[row]]);
+      if (a.value_scales) words[1] = __float_as_uint(a.value_scales[p.word_from[row]]);
+      if (a.mass) words[2] = __float_as_uint(a.mass[p.word_from[row]]);
+    }
+  }
+  __device__ __forceinline__ void write(const KeepArgs& a, const KeepList&, const KeepPlaces& p) const {
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+      if (has(p, n)) *(Piece*)((char*)a.keys + p.to[row0 + n * step] * sizeof(E) + at) = piece[n];
+    const int row = threadIdx.x;
+    if (row < kKeepRows && (p.moves[row / 64] >> (row % 64) & 1)) {
+      if (a.key_scales) a.key_scales[p.word_to[row]] = __uint_as_float(words[0]);
+      if (a.value_scales) a.value_scales[p.word_to[row]] = __uint_as_float(words[1]);
+      if (a.mass) a.mass[p.word_to[row]] = __uint_as_float(words[2]);
+    }
+  }
+  __device__ __forceinline__ void put_by(u32x4* slot) const {
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+      if constexpr (PIECE == 16) slot[n * 256] = piece[n];
+      else if (n % 2 == 0) slot[n / 2 * 256] = u32x4{piece[n][0], piece[n][1], piece[n + 1][0], piece[n + 1][1]};
+    }
+    slot[(kSlots - 1) * 256] = words;
+  }
+  __device__ __forceinline__ void bring_back(const u32x4* slot) {
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+      if constexpr (PIECE == 16) {
+        piece[n] = slot[n * 256];
+      } else if (n % 2 == 0) {
+        const u32x4 x = slot[n / 2 * 256];
+        piece[n] = Piece{x[0], x[1]}, piece[n + 1] = Piece{x[2], x[3]};
+      }
+    }
+    words = slot[(kSlots - 1) * 256];
+  }
+};
+
+// Of values: a dimension of the wave's 32 rows, as two units.
+template <typename E>
+struct ValueRows {
+  static constexpr int kBytes = sizeof(E), kSlots = 2 * kBytes;
+  static constexpr int kRun = 16 / kBytes;  // positions a load
+  u32x4 unit[2][kBytes];
+  int d, row0;
+
+  __device__ __forceinline__ ValueRows(const KeepArgs&, const KeepList& l) {
+    d = (l.part - 1) * 64 + (threadIdx.x & (kWave - 1)), row0 = uniform((int)threadIdx.x / kWave) * 32;
+  }
+  __device__ __forceinline__ void read(const KeepArgs& a, const KeepList&, const KeepPlaces& p) {
+    if (d >= a.dim) return;
+    const E* const values = (const E*)a.values + (int64_t)d * a.page_size;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // (places and dimensions are multiples of 16 positions but for `off`, so that a run lies at a multiple of its size)
+      int64_t from[16];
+      u32x4 run[16], now = {0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        from[n] = uniform(p.from[row0 + u * 16 + n]);
+        if (n == 0 || from[n] / kRun != from[n - 1] / kRun) run[n] = *(const u32x4*)(values + from[n] / kRun * kRun);
+      }
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        if (n == 0 || from[n] / kRun != from[n - 1] / kRun) now = run[n];
+        const int in = (int)(from[n] % kRun) * kBytes;  // bytes
+        const uint32_t low = in & 4 ? now[1] : now[0], high = in & 4 ? now[3] : now[2];
+        const uint32_t x = (in & 8 ? high : low) >> (in % 4 * 8) & (kBytes == 1 ? 0xffu : 0xffffu);
+        const int to = n * kBytes;
+        if (to % 4 == 0) unit[u][to / 16][to % 16 / 4] = x;
+        else unit[u][to / 16][to % 16 / 4] |= x << (to % 4 * 8);
+      }
+    }
+  }
+  __device__ __forceinline__ void write(const KeepArgs& a, const KeepList& l, const KeepPlaces& p) const {
+    if (d >= a.dim) return;
+    E* const values = (E*)a.values + (int64_t)d * a.page_size;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int first = row0 + u * 16;
+      const uint32_t moving = uniform((uint32_t)(p.moves[first / 64] >> (first % 64)) & 0xffffu);
+      if (moving == 0) continue;
+      if (l.start % 16 == 0 && moving == 0xffffu) {
+        u32x4* const to = (u32x4*)(values + uniform(p.to[first]));
+#pragma unroll
+        for (int n = 0; n < kBytes; ++n) to[n] = unit[u][n];
+      } else {
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          if (moving >> n & 1)
+            values[uniform(p.to[first + n])] = (E)(unit[u][n * kBytes / 16][n * kBytes % 16 / 4] >> (n * kBytes % 4 * 8));
+      }
+    }
+  }
+  __device__ __forceinline__ void put_by(u32x4* slot) const {
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) slot[n * 256] = unit[n / kBytes][n % kBytes];
+  }
+  __device__ __forceinline__ void bring_back(const u32x4* slot) {
+#pragma unroll
+    for (int n = 0; n < kSlots; ++n) unit[n / kBytes][n % kBytes] = slot[n * 256];
+  }
+};
+
+// `slots`: 16-byte places that a thread has in the workspace for a chunk.
+template <typename Rows, int MODE>
+__device__ __forceinline__ void keep_part(const KeepArgs& a, const KeepList& l, unsigned list, int chunk, int chunks,
+                                          int slots, KeepPlaces* sets) {
+  Rows rows(a, l);
+  auto slot_of = [&](int chunk) { return (u32x4*)a.scratch + (((int64_t)list * chunks + chunk) * slots * 256 + threadIdx.x); };
+  if constexpr (MODE != kWalk) {
+    if (chunk * kKeepRows >= l.count) return;
+    place_rows(a, l, chunk, sets[0]);
+    __syncthreads();
+    if (MODE == kBringBack) rows.bring_back(slot_of(chunk));
+    else rows.read(a, l, sets[0]);
+    if (MODE == kPutBy) rows.put_by(slot_of(chunk));
+    else rows.write(a, l, sets[0]);
+  } else {
+    const int all = (l.count + kKeepRows - 1) / kKeepRows;
+    if (all == 0) return;
+    place_rows(a, l, 0, sets[0]);
+    bool by_place = true;
+    if (all > 1)
+      for (int i = threadIdx.x; i < l.count; i += 256) by_place &= l.kept[i] >= (int64_t)l.start + i || l.kept[i] < l.start;
+    if (__syncthreads_and(by_place)) {
+      for (int i = 0; i < all; ++i) {
+        const KeepPlaces& p = sets[i % 3];
+        rows.read(a, l, p);
+        if (i + 1 < all) place_rows(a, l, i + 1, sets[(i + 1) % 3]);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows have come
+        __syncthreads();
+        rows.write(a, l, p);
+      }
+      return;
+    }
+    for (int back = 0; back < 2; ++back)
+      for (int i = 0; i < all; ++i) {
+        __syncthreads();
+        place_rows(a, l, i, sets[0]);
+        __syncthreads();
+        if (back) {
+          rows.bring_back(slot_of(i));
+          rows.write(a, l, sets[0]);
+        } else {
+          rows.read(a, l, sets[0]);
+          rows.put_by(slot_of(i));
+        }
+      }
+  }
+}
+
+template <typename E, int PIECE, int PIECES>
+constexpr int kKeepSlots = KeyRows<E, PIECE, PIECES>::kSlots > ValueRows<E>::kSlots ? KeyRows<E, PIECE, PIECES>::kSlots
+                                                                                    : ValueRows<E>::kSlots;
 
 template <typename E, int PIECE, int PIECES, int MODE>
 __global__ void __launch_bounds__(256) keep_rows(KeepArgs a, int chunks) {
-  using Chunk = KeepChunk<E, PIECE, PIECES>;
-  using Piece = typename Chunk::Piece;
-  constexpr int kBytes = sizeof(E);
-  __shared__ int64_t from[kKeepRows], to[kKeepRows], word_from[kKeepRows], word_to[kKeepRows];
-  __shared__ uint64_t moves[2];  // which of the chunk's rows move
-  const int thread = threadIdx.x, lane = thread & (kWave - 1), wave = uniform(thread / kWave);
+  __shared__ KeepPlaces sets[MODE == kWalk ? 3 : 1];
   const int parts = 1 + (a.dim + 63) / 64;
-  unsigned block = blockIdx.x;
-  const int own_chunk = MODE == kWalk ? 0 : block % (unsigned)chunks;
-  if (MODE != kWalk) block /= (unsigned)chunks;
-  const int kv = block % (unsigned)a.kv_heads, part = block / (unsigned)a.kv_heads % (unsigned)parts;
-  const int s = block / (unsigned)a.kv_heads / (unsigned)parts;
-  const int32_t count = a.counts ? a.counts[s] : a.most, start = a.starts ? a.starts[s] : 0;
-  if (count < 0 || count > a.most || start < 0) {
+  const unsigned list = MODE == kWalk ? blockIdx.x : blockIdx.x / (unsigned)chunks;
+  const int chunk = MODE == kWalk ? 0 : blockIdx.x % (unsigned)chunks;
+  KeepList l;
+  l.kv = list % (unsigned)a.kv_heads, l.part = list / (unsigned)a.kv_heads % (unsigned)parts;
+  l.s = list / (unsigned)a.kv_heads / (unsigned)parts;
+  l.count = a.counts ? uniform(a.counts[l.s]) : a.most, l.start = a.starts ? uniform(a.starts[l.s]) : 0;
+  if (l.count < 0 || l.count > a.most || l.start < 0) {
     if (a.bad_page) *a.bad_page = 1;
     return;
   }
-  const int32_t* kept = a.kept + ((int64_t)s * a.kept_heads + (a.kept_heads == 1 ? 0 : kv)) * a.most;
-  const int32_t *table = a.tables + (int64_t)s * a.table_pages, *into = a.into + (int64_t)s * a.into_pages;
-  const int row_pieces = a.dim * kBytes / PIECE, d = (part - 1) * 64 + lane;  // (of values: the lane's dimension)
-  E* const values = (E*)a.values;
-  float* const words[3] = {a.key_scales, a.value_scales, a.mass};
-
-  // where the chunk's rows lie and where they go
-  auto place_rows = [&](int chunk) {
-    if (thread < kKeepRows) {
-      const int i = chunk * kKeepRows + thread;
-      bool good = i < count;
-      int64_t page = 0, off = 0, its_page = 0, its_off = 0;
-      if (good) {
-        good = place_of(a, table, a.table_pages, kept[i], page, off) &&
-               place_of(a, into, a.into_pages, (int64_t)start + i, its_page, its_off);
-        if (!good && a.bad_page) *a.bad_page = 1;
-      }
-      if (!good) page = off = its_page = its_off = 0;
-      if (part == 0) {
-        from[thread] = ((page * a.page_size + off) * a.kv_heads + kv) * a.dim;
-        to[thread] = ((its_page * a.page_size + its_off) * a.kv_heads + kv) * a.dim;
-        word_from[thread] = (page * a.kv_heads + kv) * a.page_size + off;
-        word_to[thread] = (its_page * a.kv_heads + kv) * a.page_size + its_off;
-      } else {
-        from[thread] = (page * a.kv_heads + kv) * a.dim * a.page_size + off;
-        to[thread] = (its_page * a.kv_heads + kv) * a.dim * a.page_size + its_off;
-      }
-      const uint64_t good_rows = __ballot(good);
-      if (lane == 0) moves[wave] = good_rows;
-    }
-    __syncthreads();
-  };
-  auto moves_row = [&](int row) { return (bool)(moves[row / 64] >> (row % 64) & 1); };
-  auto read_rows = [&](Chunk& c) {
-    if (part == 0) {
-#pragma unroll
-      for (int n = 0; n < PIECES; ++n) {
-        const int q = thread + n * 256, row = q / row_pieces;
-        if (row < kKeepRows && moves_row(row))
-          c.keys[n] = *(const Piece*)((const char*)a.keys + from[row] * kBytes + (q - row * row_pieces) * PIECE);
-      }
-      if (thread < kKeepRows && moves_row(thread))
-#pragma unroll
-        for (int w = 0; w < 3; ++w)
-          if (words[w]) c.words[w] = words[w][word_from[thread]];
-    } else if (d < a.dim) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t x[16];
-#pragma unroll
-        for (int n = 0; n < 16; ++n) x[n] = (uint32_t)values[uniform(from[wave * 32 + u * 16 + n]) + (int64_t)d * a.page_size];
-#pragma unroll
-        for (int n = 0; n < 4 * kBytes; ++n) {
-          uint32_t word = 0;
-#pragma unroll
-          for (int e = 0; e < 4 / kBytes; ++e) word |= x[n * (4 / kBytes) + e] << (8 * kBytes * e);
-          c.values[u][n / 4][n % 4] = word;
-        }
-      }
-    }
-  };
-  auto write_rows = [&](const Chunk& c, bool units) {
-    if (part == 0) {
-#pragma unroll
-      for (int n = 0; n < PIECES; ++n) {
-        const int q = thread + n * 256, row = q / row_pieces;
-        if (row < kKeepRows && moves_row(row))
-          *(Piece*)((char*)a.keys + to[row] * kBytes + (q - row * row_pieces) * PIECE) = c.keys[n];
-      }
-      if (thread < kKeepRows && moves_row(thread))
-#pragma unroll
-        for (int w = 0; w < 3; ++w)
-          if (words[w]) words[w][word_to[thread]] = c.words[w];
-    } else if (d < a.dim) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row0 = wave * 32 + u * 16;
-        const uint32_t moving = (uint32_t)(moves[row0 / 64] >> (row0 % 64)) & 0xffffu;
-        if (units && moving == 0xffffu) {
-          u32x4* const unit = (u32x4*)(values + uniform(to[row0]) + (int64_t)d * a.page_size);
-#pragma unroll
-          for (int n = 0; n < kBytes; ++n) unit[n] = c.values[u][n];
-        } else {
-#pragma unroll
-          for (int n = 0; n < 16; ++n)
-            if (moving >> n & 1)
-              values[uniform(to[row0 + n]) + (int64_t)d * a.page_size] =
-                  (E)(c.values[u][n * kBytes / 16][n * kBytes % 16 / 4] >> (n * kBytes % 4 * 8));
-        }
-      }
-    }
-  };
-  // a thread's own pieces of a chunk, put by and brought back
-  constexpr int kSlots = PIECES * PIECE / 16 > 2 * kBytes ? PIECES * PIECE / 16 : 2 * kBytes;
-  auto slot_of = [&](int chunk) {
-    return (u32x4*)a.scratch + (((int64_t)block * chunks + chunk) * (kSlots + 1) * 256 + thread);
-  };
-  auto put_by = [&](const Chunk& c, u32x4* slot) {
-    if (part == 0) {
-#pragma unroll
-      for (int n = 0; n < PIECES; n += 16 / PIECE) {
-        u32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = c.keys[n + e / Chunk::kWords][e % Chunk::kWords];
-        slot[n * PIECE / 16 * 256] = x;
-      }
-      slot[kSlots * 256] = u32x4{__float_as_uint(c.words[0]), __float_as_uint(c.words[1]), __float_as_uint(c.words[2]), 0};
-    } else {
-#pragma unroll
-      for (int n = 0; n < 2 * kBytes; ++n) slot[n * 256] = c.values[n / kBytes][n % kBytes];
-    }
-  };
-  auto bring_back = [&](Chunk& c, const u32x4* slot) {
-    if (part == 0) {
-#pragma unroll
-      for (int n = 0; n < PIECES; n += 16 / PIECE) {
-        const u32x4 x = slot[n * PIECE / 16 * 256];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c.keys[n + e / Chunk::kWords][e % Chunk::kWords] = x[e];
-      }
-      const u32x4 x = slot[kSlots * 256];
-#pragma unroll
-      for (int w = 0; w < 3; ++w) c.words[w] = __uint_as_float(x[w]);
-    } else {
-#pragma unroll
-      for (int n = 0; n < 2 * kBytes; ++n) c.values[n / kBytes][n % kBytes] = slot[n * 256];
-    }
-  };
-
-  const bool units = start % 16 == 0;
-  Chunk c{};
-  if constexpr (MODE != kWalk) {
-    if (own_chunk * kKeepRows >= count) return;
-    place_rows(own_chunk);
-    if (MODE == kBringBack) bring_back(c, slot_of(own_chunk));
-    else read_rows(c);
-    if (MODE == kPutBy) put_by(c, slot_of(own_chunk));
-    else write_rows(c, units);
-    return;
-  }
-  const int all = (count + kKeepRows - 1) / kKeepRows;
-  bool by_place = true;
-  if (all > 1) {
-    bool here = true;
-    for (int i = thread; i < count; i += 256) here &= kept[i] >= (int64_t)start + i || kept[i] < start;
-    by_place = __syncthreads_and(here);
-  }
-  if (by_place) {
-    for (int chunk = 0; chunk < all; ++chunk) {
-      place_rows(chunk);
-      read_rows(c);
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows have come
-      __syncthreads();
-      write_rows(c, units);
-      __syncthreads();  // (the places are used up)
-    }
-    return;
-  }
-  for (int chunk = 0; chunk < all; ++chunk) {
-    place_rows(chunk);
-    read_rows(c);
-    put_by(c, slot_of(chunk));
-    __syncthreads();
-  }
-  for (int chunk = 0; chunk < all; ++chunk) {
-    place_rows(chunk);
-    bring_back(c, slot_of(chunk));
-    write_rows(c, units);
-    __syncthreads();
-  }
+  l.kept = a.kept + ((int64_t)l.s * a.kept_heads + (a.kept_heads == 1 ? 0 : l.kv)) * a.most;
+  l.table = a.tables + (int64_t)l.s * a.table_pages, l.into = a.into + (int64_t)l.s * a.into_pages;
+  constexpr int kSlots = kKeepSlots<E, PIECE, PIECES>;
+  if (l.part == 0) keep_part<KeyRows<E, PIECE, PIECES>, MODE>(a, l, list, chunk, chunks, kSlots, sets);
+  else keep_part<ValueRows<E>, MODE>(a, l, list, chunk, chunks, kSlots, sets);
 }
 
 // Bytes of scratch of a row that is put by on its own (move_rows).
@@ -475,17 +521,17 @@ int check_keep(const char* entry, int32_t sequences, int32_t most, int32_t kv_he
 int pieces_of(int32_t dim, bool quantized, int& piece) {
   const int64_t bytes = (int64_t)dim * (quantized ? 1 : 2);
   piece = bytes % 16 == 0 ? 16 : 8;
-  if (bytes % piece != 0) return 0;
-  const int64_t pieces = ceil_div(kKeepRows * bytes / piece, 256);
+  if (bytes % piece != 0 || (piece == 8 && !quantized) || bytes / piece > 256) return 0;
+  const int64_t pieces = ceil_div(kKeepRows, 256 / (bytes / piece));
   return pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 0;
 }
 
 int64_t keep_bytes(int32_t sequences, int32_t most, int32_t kv_heads, int32_t dim, bool quantized) {
   const int64_t by_rows = (int64_t)sequences * most * kv_heads * scratch_row(dim, quantized);
   int piece;
-  const int pieces = pieces_of(dim, quantized, piece), slots = std::max(pieces * piece / 16, quantized ? 2 : 4);
+  const int pieces = pieces_of(dim, quantized, piece), slots = std::max(pieces * piece / 16 + 1, quantized ? 2 : 4);
   const int64_t by_chunks = (int64_t)sequences * kv_heads * (1 + ceil_div(dim, 64)) * ceil_div(most, kKeepRows) *
-                            (slots + 1) * 256 * 16;
+                            slots * 256 * 16;
   return ceil_div(pieces == 0 ? by_rows : std::max(by_rows, by_chunks), 16) * 16;
 }
 
@@ -499,7 +545,9 @@ int keep_chunks(const char* entry, const KeepArgs& a, bool apart, hipStream_t st
     else hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kDirect>), each, block, 0, st, a, chunks);
     return launched(entry);
   }
-  if (lists >= 512) {
+  // (16 sequences of 8 heads of 128, 384 lists of 4,096 rows, 255 us one way and 277 the other, of 500 31 and 36; 8
+  // sequences, 192 lists, 200 and 140; one, 24 lists, 178 and 27)
+  if (lists >= 256) {
     hipLaunchKernelGGL((keep_rows<E, PIECE, PIECES, kWalk>), walk, block, 0, st, a, chunks);
     return launched(entry);
   }
@@ -580,6 +628,7 @@ extern "C" int drift_heaviest(const float* mass, const int32_t* page_tables, int
   const hipStream_t st = (hipStream_t)stream;
   if (each <= 2) hipLaunchKernelGGL(pick_heaviest<2>, grid, block, 0, st, a);
   else if (each <= 8) hipLaunchKernelGGL(pick_heaviest<8>, grid, block, 0, st, a);
+  else if (each <= 16) hipLaunchKernelGGL(pick_heaviest<16>, grid, block, 0, st, a);
   else if (each <= 32) hipLaunchKernelGGL(pick_heaviest<32>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(pick_heaviest<0>, grid, block, 0, st, a);
   return launched(entry);
