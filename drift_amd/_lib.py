@@ -80,6 +80,7 @@ SIGNATURES = {
     "drift_paged_attention_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
     "drift_paged_attention_f32": (_I32, _PAGED_ATTENTION),
     "drift_paged_attention_bf16": (_I32, _PAGED_ATTENTION),
+    "drift_tree_attention_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
     "drift_tree_attention_f32": (_I32, _TREE_ATTENTION),
     "drift_tree_attention_bf16": (_I32, _TREE_ATTENTION),
     "drift_attention_mass_workspace": (_I32, [_I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),

@@ -1539,7 +1539,7 @@ struct Plan {
 constexpr int kFewRows = 64;
 
 Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t window,
-             int64_t sinks, int64_t longest, bool by_offsets, bool quantized, bool f32) {
+             int64_t sinks, int64_t longest, bool by_offsets, bool quantized, bool f32, bool tree) {
   Plan p{0, true, 128, {0, 1}, {0, 1}, false, 0, 0, 0, 0, 0, 0, 0, 0};
   if (sequences <= 0 || tokens <= 0) return p;
   const int64_t group = heads / kv_heads, each = by_offsets ? tokens : ceil_div(tokens, sequences);
@@ -1550,7 +1550,12 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   // chunk's few rows are better off among attend_many's: a mixed batch of 24 sequences, 18 of one token, 162 us, 251
   // with units of 64 rows for all up to 64 (in launches of their own; 226 with 16).
   p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
-  p.few16 = p.few_rows == 16 ? true : by_offsets ? tokens * group <= sequences * 16 : each * group <= 16;
+  // Trees have 16 to some hundred rows each, of positions that memory has to bring for all of them: in units of 16 by
+  // waves two a SIMD, and past 16 rows among attend_many's, whose tiles serve 128 (us, as above / so: 8 nodes of one
+  // sequence, 32 rows, 29 / 15, 8 sequences of 12 nodes at 3,000 positions 122 / 36, 64 of 8 at 4,000 318 / 181, over 8
+  // bits 266 / 203, 16 of 20 rows over 24 heads of their own 222 / 156).
+  if (tree && each * group > kFewRows) p.few_rows = 16;
+  p.few16 = p.few_rows == 16 || tree ? true : by_offsets ? tokens * group <= sequences * 16 : each * group <= 16;
   // Up to 768 positions a second launch takes longer than it saves (one token at 517 12.5 us, 14.2 in splits, at 767 13.5
   // and 13.8, at 1,023 15.9 and 14.3; heads of 256 over 8 bits at 500 16.4 and 17.7, at 760 20.1 and 17.7). Splits of
   // 1,024 positions at most even out sequences of unlike lengths (64 of 400 to 8,000 251 us, in splits of 512 259, of 2,048
@@ -1577,7 +1582,9 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     }
     p.many_rows = large && dim > 64 && dim <= 128 ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
-    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, 8, 1 << 25);
+    // (a tile of wide heads takes long enough for splits of 4: 5 trees in a window of 1,024, F32 heads of 256, 59 us in
+    // splits of 8, 49 of 4)
+    p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, tree && dim > 128 ? 4 : 8, 1 << 25);
   }
   p.few_most = std::min(each * group, (int64_t)p.few_rows);
   // single tokens' blocks after the chunks' in one launch: the mixed batch 162 us, 226 in two, 203 the other way round
@@ -1708,7 +1715,7 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
   a.group = a.heads / a.kv_heads;
   a.columns = unit_columns(a.p.page_size);
   const Plan plan = plan_of(a.p.sequences, a.p.tokens, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest,
-                            a.p.offsets != nullptr, a.key_scales != nullptr, sizeof(T) == 4);
+                            a.p.offsets != nullptr, a.key_scales != nullptr, sizeof(T) == 4, TREE);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes || !aligned16(workspace)))
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,
                   (long long)plan.bytes);
@@ -1726,20 +1733,33 @@ int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a
 
 using namespace drift;
 
-extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
-                                               int32_t head_dim, int32_t window, int32_t sinks, int32_t longest,
-                                               int64_t* bytes) {
+namespace {
+int attention_workspace(const char* entry, int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                        int32_t head_dim, int32_t window, int32_t sinks, int32_t longest, bool tree, int64_t* bytes) {
   clear_error();
-  if (!bytes) return refuse("drift_paged_attention_workspace: null bytes");
+  if (!bytes) return refuse("%s: null bytes", entry);
   *bytes = 0;
-  if (const int bad = check_attention("drift_paged_attention_workspace", heads, kv_heads, head_dim, window, sinks,
-                                      longest))
-    return bad;
+  if (const int bad = check_attention(entry, heads, kv_heads, head_dim, window, sinks, longest)) return bad;
   // with offsets or without, over either cache, in either type
   for (int kind = 0; kind < 8; ++kind)
     *bytes = std::max(*bytes, plan_of(sequences, tokens, heads, kv_heads, head_dim, window, sinks, longest, kind & 1,
-                                      kind & 2, kind & 4).bytes);
+                                      kind & 2, kind & 4, tree).bytes);
   return 0;
+}
+}  // namespace
+
+extern "C" int drift_paged_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                               int32_t head_dim, int32_t window, int32_t sinks, int32_t longest,
+                                               int64_t* bytes) {
+  return attention_workspace("drift_paged_attention_workspace", sequences, tokens, heads, kv_heads, head_dim, window,
+                             sinks, longest, false, bytes);
+}
+
+extern "C" int drift_tree_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                              int32_t head_dim, int32_t window, int32_t sinks, int32_t longest,
+                                              int64_t* bytes) {
+  return attention_workspace("drift_tree_attention_workspace", sequences, tokens, heads, kv_heads, head_dim, window,
+                             sinks, longest, true, bytes);
 }
 
 #define DRIFT_ATTENTION_ARGS(sees, words)                                                                                   \

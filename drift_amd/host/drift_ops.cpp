@@ -972,17 +972,31 @@ void HipOps::cacheReadSequences(const PagedCache& cache, const Sequences& sequen
   readRows("cacheReadSequences", cache, sequences, k, v, badPage);
 }
 
+namespace {
+template <typename Tell, typename P>
+int64_t toldWorkspace(const char* entry, Tell tell, const P& p, const Tensor& queries, const PagedCache& cache,
+                      const std::optional<AttentionWindow>& window) {
+  int64_t bytes = 0;
+  const int code = tell(p.count, (int32_t)queries.shape[0], (int32_t)queries.shape[1], (int32_t)cache.kvHeads(),
+                        (int32_t)cache.headDimension(), window ? (int32_t)window->positions : 0,
+                        window ? (int32_t)window->sinks : 0, p.longest, &bytes);
+  if (code != 0) throw HipException(entry, code, drift_last_error());
+  return bytes;
+}
+}  // namespace
+
 int64_t HipOps::attentionWorkspace(const Tensor& queries, const PagedCache& cache, const CacheRows& rows,
                                    const std::optional<AttentionWindow>& window) {
   checkAttention("attentionWorkspace", queries, cache, queries, window);
-  const Paging p = pagingOf("attentionWorkspace", cache, rows, queries.shape[0]);
-  int64_t bytes = 0;
-  const int code = drift_paged_attention_workspace(
-      p.count, (int32_t)queries.shape[0], (int32_t)queries.shape[1], (int32_t)cache.kvHeads(),
-      (int32_t)cache.headDimension(), window ? (int32_t)window->positions : 0, window ? (int32_t)window->sinks : 0,
-      p.longest, &bytes);
-  if (code != 0) throw HipException("drift_paged_attention_workspace", code, drift_last_error());
-  return bytes;
+  return toldWorkspace("drift_paged_attention_workspace", drift_paged_attention_workspace,
+                       pagingOf("attentionWorkspace", cache, rows, queries.shape[0]), queries, cache, window);
+}
+
+int64_t HipOps::attentionTreeWorkspace(const Tensor& queries, const PagedCache& cache, const Sequences& sequences,
+                                       const std::optional<AttentionWindow>& window) {
+  checkAttention("attentionTreeWorkspace", queries, cache, queries, window);
+  return toldWorkspace("drift_tree_attention_workspace", drift_tree_attention_workspace,
+                       pagingOf("attentionTreeWorkspace", cache, sequences, queries.shape[0]), queries, cache, window);
 }
 
 void HipOps::attend(const char* operation, const Tensor& queries, const PagedCache& cache, const CacheRows& rows,

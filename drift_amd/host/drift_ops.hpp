@@ -405,10 +405,12 @@ class HipOps {
                           const Tensor& out, const Tensor& workspace,
                           const std::optional<AttentionWindow>& window = {}, int32_t* badPage = nullptr);
 
-  // attention of trees of drafted tokens: as attentionSequences (and with its
-  // workspace), but of its sequence's new rows a row sees those that `sees` names
+  // attention of trees of drafted tokens: as attentionSequences (with a workspace of
+  // attentionTreeWorkspace's bytes), but of its sequence's new rows a row sees those that `sees` names
   // (I32 [tokens, words], bit b of word w: row 32 w + b), and every position
   // before them; `window` counts back from start - 1 + the rows that it sees
+  int64_t attentionTreeWorkspace(const Tensor& queries, const PagedCache& cache, const Sequences& sequences,
+                                 const std::optional<AttentionWindow>& window = {});
   void attentionTree(const Tensor& queries, const PagedCache& cache, const Sequences& sequences, const Tensor& sees,
                      float scale, const Tensor& out, const Tensor& workspace,
                      const std::optional<AttentionWindow>& window = {}, int32_t* badPage = nullptr);

@@ -1149,10 +1149,10 @@ class HipOps:
         # scratch of this call's own, from torch's pool on the launch's stream: calls on several streams and
         # captured graphs never share it
         numbers = (count, tokens, heads, cache.kvHeads, cache.headDimension, positions, sinks, longest)
-        size = self._told("drift_paged_attention_workspace", *numbers)
+        entry, tree = ("drift_paged_attention", ()) if sees is None else ("drift_tree_attention", (_ptr(sees), words))
+        size = self._told(f"{entry}_workspace", *numbers)
         workspace = self._workspace(size, queries.device)
         keys, values, keyScales, valueScales, *_ = tensors
-        entry, tree = ("drift_paged_attention", ()) if sees is None else ("drift_tree_attention", (_ptr(sees), words))
         self._launch(f"{entry}_{_suffix(queries.dtype)}", _ptr(queries), _ptr(keys), _ptr(values),
                      _ptr(keyScales), _ptr(valueScales), *paging, tokens, heads, cache.kvHeads, cache.headDimension,
                      cache.pageSize, scale, positions, sinks, longest, *tree, _ptr(out), _ptr(workspace), size,

@@ -99,6 +99,8 @@ final class DriftKernels(path: Path) {
   val treeAttention = twins("drift_tree_attention", P, P, P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT,
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, JAVA_INT, JAVA_INT, P, JAVA_INT, P, P,
     JAVA_LONG, P, P)
+  val treeAttentionWorkspace = bind("drift_tree_attention_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
+    JAVA_INT, JAVA_INT, JAVA_INT, P)
   val attentionMass = twins("drift_attention_mass", P, P, P, P, JAVA_INT, JAVA_INT, P, P, JAVA_INT, JAVA_INT, JAVA_INT,
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_FLOAT, JAVA_INT, P, P, P, JAVA_LONG, P, P)
   val attentionMassWorkspace = bind("drift_attention_mass_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT,
@@ -108,6 +110,18 @@ final class DriftKernels(path: Path) {
   val cacheKeep = bind("drift_cache_keep", P, P, P, P, P, P, JAVA_INT, P, JAVA_INT, JAVA_INT, P, JAVA_INT, P, P,
     JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P, JAVA_LONG, P, P)
   val cacheKeepWorkspace = bind("drift_cache_keep_workspace", JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, JAVA_INT, P)
+
+  /** The bytes of scratch that a `treeAttention` of these numbers takes. */
+  def treeWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, window: Int, sinks: Int,
+                    longest: Int): Long = {
+    val arena = Arena.ofConfined()
+    try {
+      val bytes = arena.allocate(JAVA_LONG)
+      check("drift_tree_attention_workspace", (treeAttentionWorkspace.invokeExact(sequences, tokens, heads, kvHeads,
+        headDimension, window, sinks, longest, bytes): Int))
+      bytes.get(JAVA_LONG, 0)
+    } finally arena.close()
+  }
 
   /** The bytes of scratch that an `attentionMass` of these numbers takes. */
   def massWorkspace(sequences: Int, tokens: Int, heads: Int, kvHeads: Int, headDimension: Int, room: Int,

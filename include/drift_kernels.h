@@ -432,9 +432,11 @@ int drift_paged_attention_bf16(const uint16_t* queries, const void* keys, const 
  * before the new tokens is seen; with a window those j > P - window or j < sinks,
  * P = start - 1 + the new tokens that the row sees, its depth in the tree (what the
  * window hides of the new tokens is the caller's to leave out). A row that sees nothing
- * is zeros. The workspace is drift_paged_attention_workspace's. For a
+ * is zeros. The workspace has drift_tree_attention_workspace's bytes. For a
  * verified chain (each token seeing those up to itself) it is drift_paged_attention_*.
  * Replaces nothing of the reference, which drafts one chain. */
+int drift_tree_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                   int32_t head_dim, int32_t window, int32_t sinks, int32_t longest, int64_t* bytes);
 int drift_tree_attention_f32(const float* queries, const void* keys, const void* values, const float* key_scales,
                              const float* value_scales, const int32_t* page_tables, int32_t table_pages,
                              int32_t cache_pages, const int32_t* starts, const int32_t* offsets, int32_t sequences,

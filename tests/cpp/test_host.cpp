@@ -890,7 +890,7 @@ GPU_TEST(a_cache_cut_to_its_heaviest) {
   twice.insert(twice.end(), q.begin(), q.end());
   const Tensor q2 = dev.upload(DType::F32, {2, heads, dim}, twice);
   hip.attentionTree(q2, cache, tree, dev.upload(DType::I32, {2, 1}, std::vector<int32_t>{1, 2}), 0.125f, out,
-                    dev.empty(DType::U8, {hip.attentionWorkspace(q2, cache, tree)}));
+                    dev.empty(DType::U8, {hip.attentionTreeWorkspace(q2, cache, tree)}));
   const std::vector<float> got = dev.download<float>(out);
   for (int h = 0; h < heads; ++h) {
     const int32_t* mine = chosen.data() + h / (heads / kh) * keep;

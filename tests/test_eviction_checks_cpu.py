@@ -203,6 +203,11 @@ def told(entry, *numbers):
 
 
 def test_the_workspaces_are_told():
+    assert refusal("drift_tree_attention_workspace", 1, 1, 8, 2, 128, 0, 0, 10, None).endswith("null bytes")
+    assert "7 heads over 2" in told("drift_tree_attention_workspace", 1, 1, 7, 2, 128, 0, 0, 10)[0]
+    for numbers in ((1, 8, 32, 8, 128, 0, 0, 525), (64, 2000, 32, 8, 256, 4096, 4, 2 ** 31 - 1), (0, 5, 8, 2, 64, 0, 0, 5)):
+        code, size = told("drift_tree_attention_workspace", *numbers)
+        assert code == "code 0" and 0 <= size < 1 << 40
     assert refusal("drift_attention_mass_workspace", 1, 1, 8, 2, 128, 16, 10, None).endswith("null bytes")
     assert "7 heads over 2" in told("drift_attention_mass_workspace", 1, 1, 7, 2, 128, 16, 10)[0]
     assert "longest" in told("drift_attention_mass_workspace", 1, 1, 8, 2, 128, 16, -1)[0]
