@@ -787,14 +787,25 @@ __device__ __forceinline__ float half_sum(float v) {
   return v + __shfl_xor(v, 16, kWave);
 }
 
-template <typename T, bool I8, int DP>
-constexpr int kSumRows = (sizeof(T) == 4 ? 2 : 1) * DP > 256 ? 32 : 64;
 template <int DP>
 constexpr int kSets = DP > 128 ? 1 : 2;
+template <typename T, int DP>
+constexpr int kSumRows = (sizeof(T) == 4 ? 2 : 1) * DP > 256 ? 32 : 64;
+// The parts of a tile of positions: `each` tiles of rows, from `from` on; so many of them have any.
+struct Parts {
+  int from, each, count;
+};
+__device__ __forceinline__ Parts parts_of(const MassArgs& a, const Span& span, uint32_t j0, int row_tile) {
+  const uint32_t rows = (uint32_t)span.rows * (uint32_t)a.group, start = (uint32_t)span.start;
+  const int all = (int)((rows + row_tile - 1) / row_tile);
+  const int from = j0 > start ? (int)((j0 - start) * (uint32_t)a.group / row_tile) : 0;
+  const int each = j0 < (uint32_t)a.summed ? (all - from + a.parts - 1) / a.parts : all;
+  return {from, each, (all - from + each - 1) / each};
+}
 
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
-  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, KS = DP / 16, SETS = kSets<DP>, RT = kSumRows<T, I8, DP>;
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, KS = DP / 16, SETS = kSets<DP>, RT = kSumRows<T, DP>;
   constexpr int kTermBytes = RT * DP * 2, kTileBytes = TERMS * kTermBytes, kPositions = 128 * SETS;
   constexpr int kLoads = kTileBytes / 16 / 256;
   __shared__ __attribute__((aligned(16))) char tiles[2 * kTileBytes];
@@ -811,12 +822,11 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
 
   for (int64_t tile = rest % (unsigned)a.strides; tile * kPositions < length; tile += a.strides) {
     const uint32_t j0 = (uint32_t)tile * kPositions;
-    const bool parted = j0 < (uint32_t)a.summed;
-    if (!parted && part != 0) continue;
     // the tiles of rows that see some of the positions, and this part's of them
-    const int from = j0 > start ? (int)((j0 - start) * group / RT) : 0;
-    const int each = parted ? (all_tiles - from + a.parts - 1) / a.parts : all_tiles;
-    const int begin = min(from + part * each, all_tiles), end = min(begin + each, all_tiles);
+    const Parts parts = parts_of(a, span, j0, RT);
+    if (part >= parts.count) continue;
+    const bool parted = j0 < (uint32_t)a.summed;
+    const int begin = parts.from + part * parts.each, end = min(begin + parts.each, all_tiles);
 
     // ---- the rows
     u32x4 raw[kLoads];
@@ -974,14 +984,15 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_sums(MassArgs a) {
 }
 
 // Positions' sums over the parts of many rows, four a thread.
-__global__ void __launch_bounds__(64) many_parts(MassArgs a) {
+__global__ void __launch_bounds__(64) many_parts(MassArgs a, int positions, int row_tile) {
   const int kv = blockIdx.y % (unsigned)a.kv_heads, s = blockIdx.y / (unsigned)a.kv_heads;
   const Span span = span_of<false>(a.p, s);
   const int64_t j = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
   if (span.rows == 0 || j >= min(span.start + span.rows, (int64_t)a.summed)) return;
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int parts = parts_of(a, span, (uint32_t)(j / positions * positions), row_tile).count;
 #pragma unroll 4
-  for (int part = 0; part < a.parts; ++part)
+  for (int part = 0; part < parts; ++part)
     sum += *(const f32x4*)(a.partials + (((int64_t)part * a.p.sequences + s) * a.kv_heads + kv) * a.summed + j);
   const float four[4] = {sum[0], sum[1], sum[2], sum[3]};
   store_masses(a, span, j, kv, four);
@@ -1036,10 +1047,13 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     p.strides = (int)std::min(ceil_div(seen, 1024), std::max<int64_t>(kSplitBlocks / units, 1));
   } else {
     p.split = split_of(ceil_div(tokens * group, 128) * kv_heads, seen, 512, 8, 1 << 25);
+    const int64_t most_rows = (by_offsets || sequences == 1 ? tokens : 1) * group;
     const int64_t positions = dim <= 128 ? 256 : 128, tiles = ceil_div(seen, positions);
     p.strides = (int)std::min(tiles, std::max<int64_t>(kSplitBlocks / units, 1));
-    const int64_t row_tiles = ceil_div((by_offsets || sequences == 1 ? tokens : 1) * group, 64);
-    p.parts = (int)std::max<int64_t>(std::min({(int64_t)2048 / (units * tiles), ceil_div(row_tiles, 4), (int64_t)16}), 1);
+    // Rows in parts until there are some 4,096 blocks: causal rows leave later positions fewer, and chunks among
+    // single tokens leave few blocks most of the rows (us, 24 sequences of 1,811 tokens over 8 bits: by 2,048 blocks
+    // 108, 4,096 100, 8,192 114, 16,384 141; a prompt of 8,192: 694 by 2,048 and by 8,192).
+    p.parts = (int)std::max<int64_t>(std::min({4096 / (units * tiles), ceil_div(most_rows, 256), (int64_t)16}), 1);
     p.summed = p.parts > 1 ? tiles * positions : 0;
   }
   at(p.split.splits * rows * 8);
@@ -1074,7 +1088,8 @@ int launch_products(const char* entry, const T* queries, const MassArgs& a, cons
   hipLaunchKernelGGL((many_sums<T, I8, DP>), dim3((unsigned)(units * a.strides * a.parts)), block, 0, st, a);
   if (const int bad = launched(entry)) return bad;
   if (a.parts > 1) {
-    hipLaunchKernelGGL(many_parts, dim3((unsigned)ceil_div(a.summed, 256), (unsigned)units), dim3(64), 0, st, a);
+    hipLaunchKernelGGL(many_parts, dim3((unsigned)ceil_div(a.summed, 256), (unsigned)units), dim3(64), 0, st, a,
+                       128 * kSets<DP>, (kSumRows<T, DP>));
     return launched(entry);
   }
   return 0;
