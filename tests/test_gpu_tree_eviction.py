@@ -909,3 +909,156 @@ def test_a_cache_cut_to_its_heaviest(hip, kind, dtype):
         assert all(torch.equal(a, b) for a, b in zip(eager[:2], (out, kept)))
         held = [torch.equal(gathered(case, eager[2])[s], gathered(case, mass)[s]) for s in range(3)]
         assert all(held), held
+
+
+# ------------------------------------------------------------------ calls beside each other, and far ones
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("order", ["ascending", "any"])
+@pytest.mark.parametrize("count,kv,dim,page,most,start", [(24, 4, 128, 16, 300, 5), (40, 8, 64, 32, 257, 64)])
+def test_moves_of_many_lists(hip, kind, order, count, kv, dim, page, most, start):
+    """As many as keep a block each for all their chunks: in order, and (rows that come from places already
+    written) by way of the workspace."""
+    step(f"moves of many lists {kind} {order} {count} of {most}")
+    rng = np.random.default_rng(most)
+    lengths = [start + most + int(n) for n in rng.integers(1, 200, count)]
+    tables, pages = tables_for(lengths, page, 51)
+    counts = rng.integers(most - 140, most + 1, count)
+    counts[0], counts[1], counts[2] = most, 0, 128
+    kept = np.zeros((count, kv, most), np.int32)
+    for s, n in enumerate(lengths):
+        for h in range(kv):
+            row = rng.choice(n, most, replace=order == "any")  # (with the same position more than once)
+            kept[s, h] = np.sort(row) if order == "ascending" else row
+    if order == "ascending":  # from `start` on, no row comes from before its place
+        kept = np.maximum(kept, start + np.arange(most, dtype=np.int32))
+    cache, mass = cache_of(kind, pages, page, kv, dim, 52)
+    old = parts(cache, mass)
+    hip.cacheKeep(cache, dev_i32(tables), dev_i32(kept), dev_i32(counts), dev_i32([start] * count), mass=mass)
+    assert_parts(cache, mass, moved(old, tables, kept, counts, [start] * count, tables, page))
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_masses_of_steps_with_more_scores_than_are_kept(hip, kind):
+    """Page tables with room for so many positions that a step's scores are taken twice."""
+    step(f"masses of steps over wide page tables {kind}")
+    case = Case(kind, [700, 90, 0], [1, 1, 1], 2, 128, 16, seed=53)
+    case.tables = np.concatenate([case.tables, np.full((3, 400_000), -7, np.int32)], 1)
+    q = normal(54, (3, 8, 128), torch.bfloat16, 2.0).to(DEV)
+    before = masses(case, 55)
+    mass = torch.zeros_like(before)
+    hip.attentionMass(q, case.cache, case.sequences(offsets=False, longest=701), 0.1, mass, before)
+    assert_mass(case, q, 0.1, mass, before, what="wide page tables")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [1, 70])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_masses_of_scales_that_are_not_above_zero(hip, dtype, tokens, scale):
+    step(f"masses of a scale of {scale} {dtype} {tokens}")
+    case = Case("f16", [333], [tokens], 2, 64, 16, seed=56)
+    q = normal(57, (tokens, 4, 64), TYPES[dtype], 2.0).to(DEV)
+    mass = torch.zeros(case.cache.pages, 2, 16, device=DEV)
+    hip.attentionMass(q, case.cache, case.sequences(), scale, mass)
+    assert_mass(case, q, scale, mass, what=f"scale {scale}")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_a_cache_of_more_values_than_32_bits_count(hip, kind):
+    """The same sequences in a small cache and on the first and last pages of a
+    large one: the same bits."""
+    step(f"a large cache {kind}")
+    kv, dim, page, heads = 8, 128, 64, 16
+    pages = (1 << 32) // (page * kv * dim) + 100
+    case = Case(kind, [600, 500], [20, 1], kv, dim, page, seed=58)
+    small = case.cache
+    make = d.KvCache.allocate if kind == "f16" else d.QuantizedKvCache.allocate
+    large = make(pages, page, kv, dim)
+    place = torch.arange(small.pages)
+    place[1::2] += pages - small.pages  # every other page at the far end
+    far = np.where(case.tables >= 0, place.numpy()[np.clip(case.tables, 0, None)], case.tables).astype(np.int32)
+    names = ("keys", "values") + (("keyScales", "valueScales") if kind == "i8" else ())
+
+    def fill():
+        for w in names:
+            getattr(large, w)[place.to(DEV)] = getattr(small, w)
+
+    fill()
+    near_rows = case.sequences()
+    far_rows = d.Sequences(dev_i32(far), near_rows.starts, near_rows.offsets)
+    q = normal(59, (21, heads, dim), torch.bfloat16, 2.0).to(DEV)
+    sees = trees([20, 1], 60)
+    words = packed(sees, 1)
+    outs = []
+    for cache, rows in ((small, near_rows), (large, far_rows)):
+        out, mass = torch.empty_like(q), torch.zeros(cache.pages, kv, page, device=DEV)
+        hip.attentionTree(q, cache, rows, words, 0.1, out)
+        hip.attentionMass(q, cache, rows, 0.1, mass)
+        one = torch.zeros_like(mass)
+        hip.attentionMass(q[19:].contiguous(), cache, d.Sequences(rows.pageTables, dev_i32([619, 500])), 0.1, one, mass)
+        kept = torch.zeros(2, kv, 200, dtype=torch.int32, device=DEV)
+        counts = torch.zeros(2, dtype=torch.int32, device=DEV)
+        hip.heaviest(one, rows.pageTables, dev_i32([620, 501]), 4, 30, kept, counts)
+        hip.cacheKeep(cache, rows.pageTables, kept, counts, mass=one)
+        at = torch.arange(small.pages) if cache is small else place
+        outs.append([out.cpu(), kept.cpu(), counts.cpu()] + [x[at.to(DEV)].cpu() for x in (mass, one)] +
+                    [getattr(cache, w)[at.to(DEV)].cpu() for w in names])
+    for near, far_one in zip(*outs):
+        assert torch.equal(near.view(torch.uint8), far_one.view(torch.uint8))
+
+
+def test_graphs_beside_each_other(hip):
+    """Each captured call's workspace is its own: two graphs of all the calls, replayed at once on two streams with
+    eager calls on a third, give what each gives alone."""
+    step("graphs beside each other")
+    heads, kv, dim, page, runs = 8, 2, 128, 16, []
+    for n, rows in enumerate(([9, 40, 3], [70, 1, 130])):
+        case = Case("f16", [700, 350, 1200], rows, kv, dim, page, seed=61 + n)
+        q = normal(63 + n, (case.tokens, heads, dim), torch.bfloat16, 2.0).to(DEV)
+        words = packed(trees(rows, n), 5)
+        mass = torch.zeros(case.cache.pages, kv, page, device=DEV)
+        kept, counts = torch.zeros(3, kv, 150, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+        out, rest, tables = torch.empty_like(q), case.sequences(), dev_i32(case.tables)
+        lengths = dev_i32(case.starts + case.rows)
+        saved = case.cache.keys.clone(), case.cache.values.clone()
+        stream = torch.cuda.Stream()
+        ops = d.HipOps(stream)
+
+        def calls(ops=ops, case=case, q=q, words=words, mass=mass, kept=kept, counts=counts, out=out, rest=rest,
+                  tables=tables, lengths=lengths, saved=saved):
+            case.cache.keys.copy_(saved[0])
+            case.cache.values.copy_(saved[1])
+            ops.attentionTree(q, case.cache, rest, words, 0.1, out)
+            ops.attentionMass(q, case.cache, rest, 0.1, mass)
+            ops.heaviest(mass, tables, lengths, 2, 16, kept, counts)
+            ops.cacheKeep(case.cache, tables, kept, counts, mass=mass)
+
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            calls()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            calls()
+        held = [out, mass, kept, counts, case.cache.keys, case.cache.values]
+        want = [x.clone() for x in held]
+        runs.append((graph, stream, held, want, calls))  # (the calls hold what a graph reads)
+    case = Case("i8", [900], [30], kv, dim, page, seed=65)
+    q = normal(66, (30, heads, dim), torch.bfloat16, 2.0).to(DEV)
+    alone, now = (torch.zeros(case.cache.pages, kv, page, device=DEV) for _ in range(2))
+    sequence = case.sequences()
+    hip.attentionMass(q, case.cache, sequence, 0.1, alone)
+    for turn in range(4):
+        for _, _, held, _, _ in runs:
+            for x in held[:4]:
+                x.zero_()
+        torch.cuda.synchronize()
+        for graph, stream, _, _, _ in runs * 3:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        hip.attentionMass(q, case.cache, sequence, 0.1, now)
+        torch.cuda.synchronize()
+        assert torch.equal(now, alone), turn
+        for _, _, held, want, _ in runs:
+            for x, y in zip(held, want):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), turn
