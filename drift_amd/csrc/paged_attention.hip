@@ -39,13 +39,19 @@ struct AttentionArgs {
   int32_t few_slots, few_units;  // attend_few's rows of partials (0: by place), and units, of a sequence and key head
   int32_t few_rows;   // sequences of at most so many rows (tokens times group) are attend_few's, others attend_many's
   UnitColumns columns;
-  // of a tree's rows (TREE): what each sees of its sequence's new tokens, `words` words of 32 bits a token
-  const uint32_t* sees;
-  int32_t words;
 };
 
+// A tree's: what each row sees of its sequence's new tokens, `words` words of 32 bits a token. (A type of its own: with
+// these members other calls' kernels took a tenth longer.)
+struct TreeArgs : AttentionArgs {
+  const uint32_t* sees;
+  int64_t words;
+};
+template <bool TREE>
+using ArgsOf = std::conditional_t<TREE, TreeArgs, AttentionArgs>;
+
 // A tree's row's position: start - 1, and one for each of the sequence's new tokens that it sees.
-__device__ __forceinline__ int64_t tree_position(const AttentionArgs& a, const Span& span, int64_t nth) {
+__device__ __forceinline__ int64_t tree_position(const TreeArgs& a, const Span& span, int64_t nth) {
   const uint32_t* sees = a.sees + (span.first + nth) * a.words;
   int64_t position = span.start - 1;
   for (int w = 0; (int64_t)w * 32 < span.rows && w < a.words; ++w)
@@ -55,7 +61,7 @@ __device__ __forceinline__ int64_t tree_position(const AttentionArgs& a, const S
 
 // What a tree's row sees of the 64 positions from `base` on: of those before `start` the
 // ones from `low` on and the first `sinks`, of the others those whose bits it has.
-__device__ __forceinline__ uint64_t tree_sees(const AttentionArgs& a, const Span& span, int64_t nth, int64_t base,
+__device__ __forceinline__ uint64_t tree_sees(const TreeArgs& a, const Span& span, int64_t nth, int64_t base,
                                               int64_t low, int64_t sinks) {
   uint64_t seen = bits_below(span.start - base) & (~bits_below(low - base) | bits_below(sinks - base));
   const int64_t at = base - span.start;  // the first of the positions among the new tokens
@@ -76,7 +82,7 @@ __device__ __forceinline__ uint64_t tree_sees(const AttentionArgs& a, const Span
 }
 
 // The first position of a tree's row among those before `start`, but for the sinks.
-__device__ __forceinline__ int64_t tree_low(const AttentionArgs& a, const Span& span, int64_t nth) {
+__device__ __forceinline__ int64_t tree_low(const TreeArgs& a, const Span& span, int64_t nth) {
   return a.window ? min(max(tree_position(a, span, nth) - a.window + 1, (int64_t)0), span.start) : 0;
 }
 
@@ -136,7 +142,7 @@ struct RowState {
 // whatever the cache holds. WIDE: keys and values on 16-byte alignment, heads of a
 // multiple of 8 values, read in eights; else one by one, at any alignment.
 template <typename T, bool I8, bool WIDE, bool TREE>
-__device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& a, const Span& span, int64_t nth, int h,
+__device__ __forceinline__ void row_part(const T* queries, const ArgsOf<TREE>& a, const Span& span, int64_t nth, int h,
                                          int from, int step, RowScratch& r, RowState& state) {
   const int lane = threadIdx.x & (kWave - 1), kv = h / a.group;
   // the last position that may be seen
@@ -250,7 +256,7 @@ __device__ __forceinline__ void row_part(const T* queries, const AttentionArgs& 
 // One row by one wave, for the tile kernels' rows that came out as no numbers: slow,
 // and kept small, since its registers count in every kernel that calls it.
 template <typename T, bool I8, bool TREE>
-__device__ __noinline__ void attend_row_of(const T* queries, T* out, const AttentionArgs& a, const Span& span,
+__device__ __noinline__ void attend_row_of(const T* queries, T* out, const ArgsOf<TREE>& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
   RowState state;
   row_part<T, I8, false, TREE>(queries, a, span, nth, h, 0, 1, r, state);
@@ -267,9 +273,9 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const Atten
 // Copies of the arguments go by reference: the kernels' own then stay in scalar
 // registers (passed themselves, every use of theirs would read scratch memory).
 template <typename T, bool I8, bool TREE>
-__device__ __forceinline__ void attend_row(const T* queries, T* out, const AttentionArgs& a, const Span& span,
+__device__ __forceinline__ void attend_row(const T* queries, T* out, const ArgsOf<TREE>& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
-  const AttentionArgs args = a;
+  const ArgsOf<TREE> args = a;
   const Span rows = span;
   attend_row_of<T, I8, TREE>(queries, out, args, rows, nth, h, r);
 }
@@ -282,7 +288,7 @@ __device__ __forceinline__ void attend_row(const T* queries, T* out, const Atten
 constexpr int kRowWaves = 4;
 
 template <typename T, bool I8, bool WIDE, bool TREE>
-__global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* queries, T* out, AttentionArgs a) {
+__global__ void __launch_bounds__(kRowWaves * kWave) attend_rows(const T* queries, T* out, ArgsOf<TREE> a) {
   __shared__ RowScratch scratch[kRowWaves];
   __shared__ float tops[kRowWaves], totals[kRowWaves];
   __shared__ int anys[kRowWaves];
@@ -389,7 +395,7 @@ struct FewShared {
 };
 
 template <typename T, bool I8, bool TREE, int DP, int C>
-__device__ __forceinline__ void few_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
+__device__ __forceinline__ void few_block(const T* queries, T* out, const ArgsOf<TREE>& a, unsigned block,
                                           FewShared<DP, C>& shared) {
   constexpr int kWaves = kFewWaves;
   constexpr int TOK = I8 ? 64 : 32, NT = TOK / 16;  // positions a tile, and row tiles of its scores
@@ -613,13 +619,15 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
           if constexpr (I8) x *= key_scale[4 * t + e];
           score[c][t][e] = x;
         }
-      if (TREE && !whole) {
-        const uint32_t sees = okay ? (uint32_t)tree_sees(a, span, position[c], mine, low[TREE ? c : 0], a.sinks) : 0;
+      if constexpr (TREE) {
+        if (!whole) {
+          const uint32_t sees = okay ? (uint32_t)tree_sees(a, span, position[c], mine, low[TREE ? c : 0], a.sinks) : 0;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) score[c][t][e] = sees >> (4 * t + e) & 1 ? score[c][t][e] : -kInfinity;
-      } else if (!whole)
+            for (int e = 0; e < 4; ++e) score[c][t][e] = sees >> (4 * t + e) & 1 ? score[c][t][e] : -kInfinity;
+        }
+      } else if (!whole) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -629,6 +637,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
                               ((a.window == 0) | (j + (uint32_t)a.window > position[c]) | (j < (uint32_t)a.sinks));
             score[c][t][e] = seen ? score[c][t][e] : -kInfinity;
           }
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -787,7 +796,7 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const Attent
 }
 
 template <typename T, bool I8, bool TREE, int DP, int C>
-__global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, AttentionArgs a) {
+__global__ void __launch_bounds__(256, C == 1 && DP <= 128 ? 2 : 1) attend_few(const T* queries, T* out, ArgsOf<TREE> a) {
   __shared__ FewShared<DP, C> shared;
   few_block<T, I8, TREE, DP, C>(queries, out, a, blockIdx.x, shared);
 }
@@ -825,7 +834,7 @@ struct ManyTile {
 };
 
 template <typename T, bool I8, bool TREE, int DP, int WAVES>
-__device__ __forceinline__ void many_block(const T* queries, T* out, const AttentionArgs& a, unsigned block,
+__device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsOf<TREE>& a, unsigned block,
                                            unsigned blocks, char (&tiles)[2 * ManyTile<I8, DP>::kBytes]) {
   // BF16's weights have one term, 11 bits: a row's result is then within 2^-11 of its values' sizes before it is rounded
   // to 8 bits, and over many positions their roundings cancel (0.0017 off 64 bits either way, the rounding to BF16's
@@ -877,7 +886,8 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
   f16x8 query[KS][TERMS];
   const uint32_t row = row0 + min(wave_row + col, rows - 1), token = row / group;
   const uint32_t position = start + token;
-  const uint32_t row_low = TREE ? (uint32_t)tree_low(a, span, token) : 0;
+  uint32_t row_low = 0;
+  if constexpr (TREE) row_low = (uint32_t)tree_low(a, span, token);
   const T* q = queries + ((span.first + token) * a.heads + kv * a.group + (row - token * group)) * (int64_t)a.dim;
   uint32_t most = 0;
   float v[KS][8];
@@ -1383,7 +1393,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const Atten
 }
 
 template <typename T, bool I8, bool TREE, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, AttentionArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(const T* queries, T* out, ArgsOf<TREE> a) {
   __shared__ __attribute__((aligned(16))) char tiles[2 * ManyTile<I8, DP>::kBytes];
   many_block<T, I8, TREE, DP, WAVES>(queries, out, a, blockIdx.x, gridDim.x, tiles);
 }
@@ -1393,8 +1403,8 @@ __global__ void __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) attend_many(cons
 // over up to 6,000 positions, 28 heads over 4 of 128: 162 us, 226 in launches of their
 // own. The longest chunk's blocks bound it.
 template <typename T, bool I8, bool TREE, int DP>
-__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* queries, T* out, AttentionArgs few,
-                                                                     AttentionArgs many, unsigned many_blocks) {
+__global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) attend_both(const T* queries, T* out, ArgsOf<TREE> few,
+                                                                     ArgsOf<TREE> many, unsigned many_blocks) {
   constexpr size_t kMany = 2 * ManyTile<I8, DP>::kBytes, kFew = sizeof(FewShared<DP, 1>);
   __shared__ __attribute__((aligned(16))) char shared[kMany > kFew ? kMany : kFew];
   if (blockIdx.x < many_blocks)
@@ -1410,16 +1420,16 @@ template <bool FEW>
 constexpr int kJoinRows = FEW ? 16 : 32;
 
 template <typename T, bool I8, bool TREE, bool FEW, int DP>
-__global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, AttentionArgs a, int rows, int tile) {
+__device__ __forceinline__ void join_block(const T* queries, T* out, const ArgsOf<TREE>& a, unsigned block, int rows,
+                                           int tile, RowScratch (&scratch)[4]) {
   // (many rows have few splits: two fours a lane let each wave have twice the rows on the way; 2 splits of 32,672 rows
   // of 128 values 9.4 us, 11.5 by one)
   constexpr int V = FEW ? 1 : 2, N = FEW ? 8 : 4;  // fours of values a lane, splits at a time
   constexpr int L = DP / 4 / V, kRows = kJoinRows<FEW>;  // lanes a row, rows a block
-  __shared__ RowScratch scratch[4];
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), in = lane % L;
   const int parts = rows / kRows;
-  const int kv = blockIdx.x % (unsigned)a.kv_heads, part = blockIdx.x / (unsigned)a.kv_heads % (unsigned)parts;
-  const unsigned unit = blockIdx.x / (unsigned)a.kv_heads / (unsigned)parts;
+  const int kv = block % (unsigned)a.kv_heads, part = block / (unsigned)a.kv_heads % (unsigned)parts;
+  const unsigned unit = block / (unsigned)a.kv_heads / (unsigned)parts;
   int s;
   int64_t nth;
   if constexpr (FEW) s = (int)(unit % (unsigned)a.p.sequences), nth = unit / (unsigned)a.p.sequences;
@@ -1505,6 +1515,22 @@ __global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, Att
       again &= L == 64 ? 0 : ~(((1ull << (L % 64)) - 1) << (which * L));
     }
   }
+}
+
+template <typename T, bool I8, bool TREE, bool FEW, int DP>
+__global__ void __launch_bounds__(256) attend_join(const T* queries, T* out, ArgsOf<TREE> a, int rows, int tile) {
+  __shared__ RowScratch scratch[4];
+  join_block<T, I8, TREE, FEW, DP>(queries, out, a, blockIdx.x, rows, tile, scratch);
+}
+
+// Both kernels' splits in one launch, many rows' first. JOINS
+template <typename T, bool I8, bool TREE, int DP>
+__global__ void __launch_bounds__(256) attend_joins(const T* queries, T* out, ArgsOf<TREE> few, ArgsOf<TREE> many,
+                                                    int few_rows, int many_rows, unsigned many_blocks) {
+  __shared__ RowScratch scratch[4];
+  if (blockIdx.x < many_blocks)
+    join_block<T, I8, TREE, false, DP>(queries, out, many, blockIdx.x, many_rows, 64, scratch);
+  else join_block<T, I8, TREE, true, DP>(queries, out, few, blockIdx.x - many_blocks, few_rows, I8 ? 64 : 32, scratch);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1610,17 +1636,9 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
 template <typename T, bool I8, int DP>
 constexpr int kManyTiles = DP > 128 ? 1 : DP <= 64 || (sizeof(T) == 2 && !I8) ? 4 : 2;
 
-template <typename T, bool I8, bool TREE, bool FEW, int DP>
-int join(const char* entry, const T* queries, T* out, const AttentionArgs& a, int64_t units, int rows, int tile,
-         hipStream_t st) {
-  hipLaunchKernelGGL((attend_join<T, I8, TREE, FEW, DP>), dim3((unsigned)(units * a.kv_heads * (rows / kJoinRows<FEW>))), dim3(256),
-                     0, st, queries, out, a, rows, tile);
-  return launched(entry);
-}
-
 template <typename T, bool I8, bool TREE, int DP>
-int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArgs& a, const Plan& plan, hipStream_t st) {
-  AttentionArgs few = a, many = a;
+int launch_tiles(const char* entry, const T* queries, T* out, const ArgsOf<TREE>& a, const Plan& plan, hipStream_t st) {
+  ArgsOf<TREE> few = a, many = a;
   const int few_tiles = plan.few16 ? 1 : kManyTiles<T, I8, DP>, few_rows = 16 * few_tiles;
   int64_t few_units = 0, many_units = 0;
   if (plan.few.splits > 0) {
@@ -1662,15 +1680,22 @@ int launch_tiles(const char* entry, const T* queries, T* out, const AttentionArg
     }
   }
   if (const int bad = launched(entry)) return bad;
-  if (few_blocks > 0 && few.splits > 1)
-    if (const int bad = join<T, I8, TREE, true, DP>(entry, queries, out, few, few_units, few_rows, I8 ? 64 : 32, st)) return bad;
-  if (many_blocks > 0 && many.splits > 1)
-    return join<T, I8, TREE, false, DP>(entry, queries, out, many, many_units, plan.many_rows, 64, st);
-  return 0;
+  const unsigned few_joins = few_blocks > 0 && few.splits > 1 ? (unsigned)(few_units * a.kv_heads * (few_rows / kJoinRows<true>)) : 0;
+  const unsigned many_joins = many_blocks > 0 && many.splits > 1 ? (unsigned)(many_units * a.kv_heads * (plan.many_rows / kJoinRows<false>)) : 0;
+  if (few_joins > 0 && many_joins > 0)
+    hipLaunchKernelGGL((attend_joins<T, I8, TREE, DP>), dim3(many_joins + few_joins), block, 0, st, queries, out, few, many,
+                       few_rows, plan.many_rows, many_joins);
+  else if (few_joins > 0)
+    hipLaunchKernelGGL((attend_join<T, I8, TREE, true, DP>), dim3(few_joins), block, 0, st, queries, out, few, few_rows,
+                       I8 ? 64 : 32);
+  else if (many_joins > 0)
+    hipLaunchKernelGGL((attend_join<T, I8, TREE, false, DP>), dim3(many_joins), block, 0, st, queries, out, many,
+                       plan.many_rows, 64);
+  return few_joins + many_joins > 0 ? launched(entry) : 0;
 }
 
 template <typename T, bool I8, bool TREE>
-int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const Plan& plan, bool aligned, hipStream_t st) {
+int attend(const char* entry, const T* queries, T* out, ArgsOf<TREE> a, const Plan& plan, bool aligned, hipStream_t st) {
   const int64_t row_blocks = units_of(a.p, 1, 0, 1) * a.heads;
   if (row_blocks > kOneWaveBlocks) return refuse("%s: %d tokens of %d heads in one call", entry, a.p.tokens, a.heads);
   const int64_t blocks = ((int64_t)a.p.sequences * 4 * std::max(plan.few.splits, 4) +
@@ -1692,16 +1717,16 @@ int attend(const char* entry, const T* queries, T* out, AttentionArgs a, const P
 }
 
 template <typename T, bool TREE>
-int paged_attention(const char* entry, const T* queries, T* out, AttentionArgs a, int64_t longest, void* workspace,
+int paged_attention(const char* entry, const T* queries, T* out, ArgsOf<TREE> a, int64_t longest, void* workspace,
                     int64_t workspace_bytes, void* stream) {
   clear_error();
   if (const int bad = check_paging(entry, a.p, a.kv_heads, a.dim)) return bad;
   if (const int bad = check_attention(entry, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest)) return bad;
   if (a.p.tokens == 0 || a.p.sequences == 0) return 0;
   if (!queries || !out) return refuse("%s: null tensor", entry);
-  if (TREE) {
+  if constexpr (TREE) {
     if (!a.sees) return refuse("%s: null tensor", entry);
-    if (a.words <= 0) return refuse("%s: %d words of what a row sees", entry, a.words);
+    if (a.words <= 0) return refuse("%s: %d words of what a row sees", entry, (int)a.words);
     if ((reinterpret_cast<uintptr_t>(a.sees) & 3) != 0)
       return refuse("%s: what the rows see not aligned to its elements", entry);
   }
@@ -1762,10 +1787,11 @@ extern "C" int drift_tree_attention_workspace(int32_t sequences, int32_t tokens,
                              sinks, longest, true, bytes);
 }
 
-#define DRIFT_ATTENTION_ARGS(sees, words)                                                                                   \
+#define DRIFT_ATTENTION_ARGS                                                                                        \
   AttentionArgs {                                                                                                   \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr, nullptr, 0, 0, 0, {}, (const uint32_t*)sees, words \
+        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr,      \
+        nullptr, 0, 0, 0, {}                                                                                        \
   }
 
 extern "C" int drift_paged_attention_f32(const float* queries, const void* keys, const void* values,
@@ -1776,7 +1802,7 @@ extern "C" int drift_paged_attention_f32(const float* queries, const void* keys,
                                          int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                          int32_t sinks, int32_t longest, float* out, void* workspace,
                                          int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<float, false>("drift_paged_attention_f32", queries, out, DRIFT_ATTENTION_ARGS(nullptr, 0), longest, workspace,
+  return paged_attention<float, false>("drift_paged_attention_f32", queries, out, DRIFT_ATTENTION_ARGS, longest, workspace,
                                 workspace_bytes, stream);
 }
 
@@ -1788,7 +1814,7 @@ extern "C" int drift_paged_attention_bf16(const uint16_t* queries, const void* k
                                           int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                           int32_t sinks, int32_t longest, uint16_t* out, void* workspace,
                                           int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<uint16_t, false>("drift_paged_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS(nullptr, 0), longest,
+  return paged_attention<uint16_t, false>("drift_paged_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS, longest,
                                    workspace, workspace_bytes, stream);
 }
 
@@ -1800,7 +1826,7 @@ extern "C" int drift_tree_attention_f32(const float* queries, const void* keys, 
                                         int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
                                         const int32_t* sees, int32_t words, float* out, void* workspace,
                                         int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<float, true>("drift_tree_attention_f32", queries, out, DRIFT_ATTENTION_ARGS(sees, words),
+  return paged_attention<float, true>("drift_tree_attention_f32", queries, out, (TreeArgs{DRIFT_ATTENTION_ARGS, (const uint32_t*)sees, words}),
                                       longest, workspace, workspace_bytes, stream);
 }
 
@@ -1813,6 +1839,6 @@ extern "C" int drift_tree_attention_bf16(const uint16_t* queries, const void* ke
                                          int32_t sinks, int32_t longest, const int32_t* sees, int32_t words,
                                          uint16_t* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page,
                                          void* stream) {
-  return paged_attention<uint16_t, true>("drift_tree_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS(sees, words),
+  return paged_attention<uint16_t, true>("drift_tree_attention_bf16", queries, out, (TreeArgs{DRIFT_ATTENTION_ARGS, (const uint32_t*)sees, words}),
                                          longest, workspace, workspace_bytes, stream);
 }
