@@ -27,14 +27,21 @@ constexpr float kLog2E = 1.44269504088896340736f;
 typedef f32x4 Row;
 enum { kScale, kTop, kInverse };
 
-struct MassArgs {
+// What a score by itself needs (a type of its own: the call out of line that gets it by
+// reference has a copy in scratch memory, whose size costs every launch).
+struct ScoreArgs {
   Paging p;
-  int32_t heads, kv_heads, dim, group;
+  int32_t kv_heads, dim;
   float scale;
-  const void* keys;
-  const float *key_scales, *before;
-  float* mass;
   UnitColumns columns;
+  const void* keys;
+  const float* key_scales;
+};
+
+struct MassArgs : ScoreArgs {
+  int32_t heads, group;
+  const float* before;
+  float* mass;
   // the workspace: rows' statistics [splits, rows, 2] (largest score and sum), their
   // scores [rows, room] or their queries [rows, terms, padded head] and constants,
   // and positions' partial sums [parts, sequences, kv_heads, summed]
@@ -63,7 +70,7 @@ __device__ __forceinline__ const T* query_of(const T* queries, const MassArgs& a
 struct Place {
   int64_t word, key;
 };
-__device__ __forceinline__ bool place_of(const MassArgs& a, const Span& span, int64_t j, int kv, Place& place) {
+__device__ __forceinline__ bool place_of(const ScoreArgs& a, const Span& span, int64_t j, int kv, Place& place) {
   const uint32_t unit = (uint32_t)(j / 16), column = a.columns.of(unit);
   const int64_t page = span.table[column], off = j - (int64_t)column * a.p.page_size;
   if (page < 0 || page >= a.p.cache_pages) {
@@ -94,7 +101,7 @@ __device__ __forceinline__ void store_masses(const MassArgs& a, const Span& span
 
 // The score of a row and a position, by F32 products one after another.
 template <typename T, bool I8>
-__device__ __forceinline__ float score_of(const MassArgs& a, const T* query, const Place& place) {
+__device__ __forceinline__ float score_of(const ScoreArgs& a, const T* query, const Place& place) {
   float dot = 0.0f;
   for (int d = 0; d < a.dim; ++d) {
     const float k = I8 ? (float)((const int8_t*)a.keys)[place.key + d] : f16_value(((const uint16_t*)a.keys)[place.key + d]);
@@ -214,7 +221,7 @@ __device__ __forceinline__ float take_query(const T* q, const MassArgs& a, At d_
 // Scores that came out as NaN, taken again by themselves: a term of F16 may have met an
 // infinity that the whole number would have made one of.
 template <typename T, bool I8>
-__device__ __noinline__ float score_again_of(const T* query, const MassArgs& a, const Span& span, int kv, int64_t j) {
+__device__ __noinline__ float score_again_of(const T* query, const ScoreArgs& a, const Span& span, int kv, int64_t j) {
   Place place;
   if (!place_of(a, span, j, kv, place)) return -kInfinity;
   return score_of<T, I8>(a, query, place) * kLog2E;
@@ -226,7 +233,7 @@ __device__ __noinline__ float score_again_of(const T* query, const MassArgs& a, 
 template <typename T, bool I8, int N, typename At>
 __device__ __forceinline__ void scores_again(const T* query, const MassArgs& a, const Span& span, int kv, At at,
                                              float factor, float (&x)[N]) {
-  const MassArgs args = a;
+  const ScoreArgs args = a;
   const Span rows = span;
 #pragma unroll
   for (int n = 0; n < N; ++n)
@@ -1178,9 +1185,9 @@ extern "C" int drift_attention_mass_workspace(int32_t sequences, int32_t tokens,
 
 #define DRIFT_MASS_ARGS                                                                                             \
   MassArgs {                                                                                                        \
-    {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, keys, key_scales, before, mass, {}, 0, 0, nullptr, nullptr, nullptr, nullptr, \
-        nullptr, 1, 1, 1, 0, 1, 0                                                                                   \
+    {{page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page},       \
+     kv_heads, head_dim, scale, {}, keys, key_scales},                                                              \
+        heads, 0, before, mass, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, 1, 1, 1, 0, 1, 0                 \
   }
 
 extern "C" int drift_attention_mass_f32(const float* queries, const void* keys, const float* key_scales,

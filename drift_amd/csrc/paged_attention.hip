@@ -22,13 +22,28 @@ namespace drift {
 namespace {
 
 constexpr int kMaxHead = 512;
-struct AttentionArgs {
+// What a row by itself needs. Of arguments that a call out of line gets by reference the kernel
+// has a copy in scratch memory, and the size of that memory costs every launch: with 16 or 32
+// bytes a lane more than 224 a decode batch took 300 us for 248, an 8-bit chunk 116 for 106. So
+// these are apart from the rest, and a tree's from others'.
+struct RowArgs {
   Paging p;
   int32_t heads, kv_heads, dim, group;
   float scale;
   int32_t window, sinks;  // window 0: every position up to the row's own
   const void *keys, *values;
   const float *key_scales, *value_scales;
+};
+// A tree's: what each row sees of its sequence's new tokens, `words` words of 32 bits a token.
+struct TreeRowArgs : RowArgs {
+  const uint32_t* sees;
+  int64_t words;
+};
+template <bool TREE>
+using RowArgsOf = std::conditional_t<TREE, TreeRowArgs, RowArgs>;
+
+template <bool TREE>
+struct ArgsOf : RowArgsOf<TREE> {
   // the split over positions: at least `chunk` tiles a split, `splits` of them;
   // where there are several, their maxima and sums [splits, partial_rows, 3] and
   // unscaled results [splits, partial_rows, dim], a row by its place among the
@@ -41,17 +56,8 @@ struct AttentionArgs {
   UnitColumns columns;
 };
 
-// A tree's: what each row sees of its sequence's new tokens, `words` words of 32 bits a token. (A type of its own: with
-// these members other calls' kernels took a tenth longer.)
-struct TreeArgs : AttentionArgs {
-  const uint32_t* sees;
-  int64_t words;
-};
-template <bool TREE>
-using ArgsOf = std::conditional_t<TREE, TreeArgs, AttentionArgs>;
-
 // A tree's row's position: start - 1, and one for each of the sequence's new tokens that it sees.
-__device__ __forceinline__ int64_t tree_position(const TreeArgs& a, const Span& span, int64_t nth) {
+__device__ __forceinline__ int64_t tree_position(const TreeRowArgs& a, const Span& span, int64_t nth) {
   const uint32_t* sees = a.sees + (span.first + nth) * a.words;
   int64_t position = span.start - 1;
   for (int w = 0; (int64_t)w * 32 < span.rows && w < a.words; ++w)
@@ -61,7 +67,7 @@ __device__ __forceinline__ int64_t tree_position(const TreeArgs& a, const Span& 
 
 // What a tree's row sees of the 64 positions from `base` on: of those before `start` the
 // ones from `low` on and the first `sinks`, of the others those whose bits it has.
-__device__ __forceinline__ uint64_t tree_sees(const TreeArgs& a, const Span& span, int64_t nth, int64_t base,
+__device__ __forceinline__ uint64_t tree_sees(const TreeRowArgs& a, const Span& span, int64_t nth, int64_t base,
                                               int64_t low, int64_t sinks) {
   uint64_t seen = bits_below(span.start - base) & (~bits_below(low - base) | bits_below(sinks - base));
   const int64_t at = base - span.start;  // the first of the positions among the new tokens
@@ -82,7 +88,7 @@ __device__ __forceinline__ uint64_t tree_sees(const TreeArgs& a, const Span& spa
 }
 
 // The first position of a tree's row among those before `start`, but for the sinks.
-__device__ __forceinline__ int64_t tree_low(const TreeArgs& a, const Span& span, int64_t nth) {
+__device__ __forceinline__ int64_t tree_low(const TreeRowArgs& a, const Span& span, int64_t nth) {
   return a.window ? min(max(tree_position(a, span, nth) - a.window + 1, (int64_t)0), span.start) : 0;
 }
 
@@ -97,7 +103,8 @@ __device__ __forceinline__ int64_t last_position(const Span& span, uint32_t nth)
 }
 
 // Where attend_few's row `row` of a sequence and key head, at `place` among the call's, keeps its partials.
-__device__ __forceinline__ int64_t few_partial(const AttentionArgs& a, int s, int kv, uint32_t row, int64_t place) {
+template <bool TREE>
+__device__ __forceinline__ int64_t few_partial(const ArgsOf<TREE>& a, int s, int kv, uint32_t row, int64_t place) {
   return a.few_slots ? ((int64_t)s * a.kv_heads + kv) * a.few_slots + row : place;
 }
 
@@ -142,7 +149,7 @@ struct RowState {
 // whatever the cache holds. WIDE: keys and values on 16-byte alignment, heads of a
 // multiple of 8 values, read in eights; else one by one, at any alignment.
 template <typename T, bool I8, bool WIDE, bool TREE>
-__device__ __forceinline__ void row_part(const T* queries, const ArgsOf<TREE>& a, const Span& span, int64_t nth, int h,
+__device__ __forceinline__ void row_part(const T* queries, const RowArgsOf<TREE>& a, const Span& span, int64_t nth, int h,
                                          int from, int step, RowScratch& r, RowState& state) {
   const int lane = threadIdx.x & (kWave - 1), kv = h / a.group;
   // the last position that may be seen
@@ -256,7 +263,7 @@ __device__ __forceinline__ void row_part(const T* queries, const ArgsOf<TREE>& a
 // One row by one wave, for the tile kernels' rows that came out as no numbers: slow,
 // and kept small, since its registers count in every kernel that calls it.
 template <typename T, bool I8, bool TREE>
-__device__ __noinline__ void attend_row_of(const T* queries, T* out, const ArgsOf<TREE>& a, const Span& span,
+__device__ __noinline__ void attend_row_of(const T* queries, T* out, const RowArgsOf<TREE>& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
   RowState state;
   row_part<T, I8, false, TREE>(queries, a, span, nth, h, 0, 1, r, state);
@@ -273,9 +280,9 @@ __device__ __noinline__ void attend_row_of(const T* queries, T* out, const ArgsO
 // Copies of the arguments go by reference: the kernels' own then stay in scalar
 // registers (passed themselves, every use of theirs would read scratch memory).
 template <typename T, bool I8, bool TREE>
-__device__ __forceinline__ void attend_row(const T* queries, T* out, const ArgsOf<TREE>& a, const Span& span,
+__device__ __forceinline__ void attend_row(const T* queries, T* out, const RowArgsOf<TREE>& a, const Span& span,
                                            int64_t nth, int h, RowScratch& r) {
-  const ArgsOf<TREE> args = a;
+  const RowArgsOf<TREE> args = a;
   const Span rows = span;
   attend_row_of<T, I8, TREE>(queries, out, args, rows, nth, h, r);
 }
@@ -342,7 +349,8 @@ struct TileList {
   __device__ __forceinline__ int tile(int i) const { return i < sinks ? i : low + (i - sinks); }
 };
 
-__device__ __forceinline__ TileList tiles_of(const AttentionArgs& a, int64_t first, int64_t last, int size) {
+template <bool TREE>
+__device__ __forceinline__ TileList tiles_of(const ArgsOf<TREE>& a, int64_t first, int64_t last, int size) {
   TileList t;
   const int64_t low = a.window ? max(first - a.window + 1, (int64_t)0) : 0;
   t.low = (int32_t)(low / size);
@@ -352,7 +360,8 @@ __device__ __forceinline__ TileList tiles_of(const AttentionArgs& a, int64_t fir
 }
 
 // Tiles a split takes.
-__device__ __forceinline__ int split_tiles(const AttentionArgs& a, int count) {
+template <bool TREE>
+__device__ __forceinline__ int split_tiles(const ArgsOf<TREE>& a, int count) {
   return max(a.chunk, (count + a.splits - 1) / a.splits);
 }
 
@@ -1555,7 +1564,7 @@ struct Plan {
   Split few, many;  // attend_few, attend_many
   bool both;                // in one launch
   int64_t few_most;                               // rows of a sequence and key head that attend_few may have
-  int64_t few_slots, few_partials, many_partials;  // AttentionArgs::few_slots, partial_rows
+  int64_t few_slots, few_partials, many_partials;  // ArgsOf::few_slots, partial_rows
   // floats of the workspace before attend_few's partials, and before either's statistics
   int64_t few_at, few_statistics, many_statistics;
   int64_t bytes;
@@ -1717,9 +1726,11 @@ int attend(const char* entry, const T* queries, T* out, ArgsOf<TREE> a, const Pl
 }
 
 template <typename T, bool TREE>
-int paged_attention(const char* entry, const T* queries, T* out, ArgsOf<TREE> a, int64_t longest, void* workspace,
+int paged_attention(const char* entry, const T* queries, T* out, const RowArgsOf<TREE>& rows, int64_t longest, void* workspace,
                     int64_t workspace_bytes, void* stream) {
   clear_error();
+  ArgsOf<TREE> a{rows};
+  a.splits = a.chunk = 1;
   if (const int bad = check_paging(entry, a.p, a.kv_heads, a.dim)) return bad;
   if (const int bad = check_attention(entry, a.heads, a.kv_heads, a.dim, a.window, a.sinks, longest)) return bad;
   if (a.p.tokens == 0 || a.p.sequences == 0) return 0;
@@ -1787,11 +1798,10 @@ extern "C" int drift_tree_attention_workspace(int32_t sequences, int32_t tokens,
                              sinks, longest, true, bytes);
 }
 
-#define DRIFT_ATTENTION_ARGS                                                                                        \
-  AttentionArgs {                                                                                                   \
+#define DRIFT_ROW_ARGS                                                                                              \
+  RowArgs {                                                                                                         \
     {page_tables, starts, offsets, sequences, table_pages, cache_pages, page_size, start, tokens, bad_page}, heads, \
-        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales, 1, 1, 0, nullptr,      \
-        nullptr, 0, 0, 0, {}                                                                                        \
+        kv_heads, head_dim, 0, scale, window, sinks, keys, values, key_scales, value_scales                         \
   }
 
 extern "C" int drift_paged_attention_f32(const float* queries, const void* keys, const void* values,
@@ -1802,7 +1812,7 @@ extern "C" int drift_paged_attention_f32(const float* queries, const void* keys,
                                          int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                          int32_t sinks, int32_t longest, float* out, void* workspace,
                                          int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<float, false>("drift_paged_attention_f32", queries, out, DRIFT_ATTENTION_ARGS, longest, workspace,
+  return paged_attention<float, false>("drift_paged_attention_f32", queries, out, DRIFT_ROW_ARGS, longest, workspace,
                                 workspace_bytes, stream);
 }
 
@@ -1814,7 +1824,7 @@ extern "C" int drift_paged_attention_bf16(const uint16_t* queries, const void* k
                                           int32_t head_dim, int32_t page_size, float scale, int32_t window,
                                           int32_t sinks, int32_t longest, uint16_t* out, void* workspace,
                                           int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<uint16_t, false>("drift_paged_attention_bf16", queries, out, DRIFT_ATTENTION_ARGS, longest,
+  return paged_attention<uint16_t, false>("drift_paged_attention_bf16", queries, out, DRIFT_ROW_ARGS, longest,
                                    workspace, workspace_bytes, stream);
 }
 
@@ -1826,7 +1836,7 @@ extern "C" int drift_tree_attention_f32(const float* queries, const void* keys, 
                                         int32_t page_size, float scale, int32_t window, int32_t sinks, int32_t longest,
                                         const int32_t* sees, int32_t words, float* out, void* workspace,
                                         int64_t workspace_bytes, int32_t* bad_page, void* stream) {
-  return paged_attention<float, true>("drift_tree_attention_f32", queries, out, (TreeArgs{DRIFT_ATTENTION_ARGS, (const uint32_t*)sees, words}),
+  return paged_attention<float, true>("drift_tree_attention_f32", queries, out, (TreeRowArgs{DRIFT_ROW_ARGS, (const uint32_t*)sees, words}),
                                       longest, workspace, workspace_bytes, stream);
 }
 
@@ -1839,6 +1849,6 @@ extern "C" int drift_tree_attention_bf16(const uint16_t* queries, const void* ke
                                          int32_t sinks, int32_t longest, const int32_t* sees, int32_t words,
                                          uint16_t* out, void* workspace, int64_t workspace_bytes, int32_t* bad_page,
                                          void* stream) {
-  return paged_attention<uint16_t, true>("drift_tree_attention_bf16", queries, out, (TreeArgs{DRIFT_ATTENTION_ARGS, (const uint32_t*)sees, words}),
+  return paged_attention<uint16_t, true>("drift_tree_attention_bf16", queries, out, (TreeRowArgs{DRIFT_ROW_ARGS, (const uint32_t*)sees, words}),
                                          longest, workspace, workspace_bytes, stream);
 }
