@@ -275,7 +275,9 @@ __device__ __forceinline__ SplitTiles split_tiles(const MassArgs& a, uint32_t la
 // or 64 (8 bits), keys straight from memory into the operands of 16 x 16 x 32
 // products, S^T = K Q^T: the result's column (lane % 16) is a row, its rows are
 // positions, dealt out so that a lane has TOK / 4 consecutive ones. A block's four waves
-// take its split's tiles in turn.
+// take its split's tiles in turn. Memory bounds it: 64 single tokens at up to 8,000
+// positions, 32 heads over 8 of 128, 160 us for 559 MB of keys and 70 MB of scores (3.9 TB/s);
+// without the scores' stores it would be 134.
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* queries, MassArgs a) {
   constexpr int kWaves = 4;
@@ -459,7 +461,8 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
 }
 
 // The few rows' positions: a thread four of them, a block 1,024 of a sequence and key
-// head; the rows' statistics joined in LDS first, 256 at a time.
+// head; the rows' statistics joined in LDS first, 256 at a time. (19 us of that step: 70 MB
+// of scores, 3.7 TB/s.)
 template <bool I8>
 __global__ void __launch_bounds__(256) few_sums(MassArgs a) {
   constexpr int kBatch = 256;
@@ -530,6 +533,10 @@ __device__ __forceinline__ int chunk_place(int row, int chunk) {
 // Statistics of many rows: 32 a wave, 128 a block, positions in tiles of 64 that the block stages in LDS once
 // for all its rows, by 32 x 32 x 16 products, S^T = K Q^T: the result's column is a row, and its largest score and
 // sum stay in its lanes. The queries go to the workspace as the products take them, for many_sums.
+//
+// The exponentials and what goes with them bound it: a prompt of 8,192 tokens, 32 heads over 8 of 128, some 340 us, 810
+// TFLOP/s; vector instructions issue 70% of the time, the products run 38%. 64 tokens after 31,936 32 us, of which 128
+// rows a block leave most to staging.
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_statistics(const T* queries, MassArgs a) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, TOK = 64, KS = DP / 16, kThreads = 256;
@@ -781,6 +788,10 @@ __global__ void __launch_bounds__(128) many_rows(MassArgs a) {
 // rows pass through LDS in tiles that all four waves use, by the same products: a result's column is a row, and
 // each lane adds up its rows' weights for the positions in its registers, so that rows need no sums across lanes
 // until the last. A block has every `parts`-th part of the rows that see its tile of positions.
+//
+// Bound as the statistics are: the prompt's some 330 us (vector instructions 56%, products 39%; kept instead, its 4.3 GB of
+// scores would have to be written and read). With 256 positions a block each row from LDS is used
+// twice: by 128 the last 64 rows of 32,000 positions take 82 us for 79.
 //
 // A score that is NaN where its row is numbers is one of -infinity (a key's infinity met a zero term): had it
 // been NaN or infinity the row would not be. So a NaN weight counts as 0, times an inverse that is NaN where the row is.
@@ -1047,8 +1058,10 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   };
   const int64_t rows = tokens * heads, group = heads / kv_heads, units = sequences * kv_heads;
   const int64_t seen = std::max<int64_t>(std::min(longest, room), 1);
-  // Up to 16 rows a sequence and key head on average (a decode step's, or some more): their scores are kept.
-  p.few = tokens * group <= sequences * 16 && rows * room * 4 <= kMostScores;
+  // Up to 32 rows a sequence and key head on average (a decode step's, or some more): their scores are kept (us, 16
+  // sequences of 4,000 positions, 8 key heads of 128, kept / taken twice: 16 rows 50 / 76, 32 rows 71 / 81, 64 rows
+  // 123 / 83; 64 sequences of 8,000, 4 rows 179 / 413).
+  p.few = tokens * group <= sequences * 32 && rows * room * 4 <= kMostScores;
   if (p.few) {
     p.split = split_of(units, seen, 1024, 4, 16);
     p.strides = (int)std::min(ceil_div(seen, 1024), std::max<int64_t>(kSplitBlocks / units, 1));

@@ -1178,7 +1178,9 @@ class HipOps:
         for it (queries, cache, sequences and scale as attentionSequences has
         them), where the position precedes the rows added to `before` (laid
         out the same, or `mass` itself; None: 0). Other positions are left as
-        they are. Two sequences that share a page leave either's sum there."""
+        they are. Two sequences that share a page leave either's sum there, in
+        place perhaps on top of the other's: shared pages take a call a
+        sequence."""
         operation = "attentionMass"
         tokens, heads = checkAttention(operation, queries, cache, queries)
         checkMass(operation, mass, cache)

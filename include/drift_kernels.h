@@ -466,7 +466,9 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * many a copy of the queries. Other positions of mass are
  * left as they are, and so are ones on a page outside the cache, *bad_page set. The
  * same call gives the same bits every time. Two sequences that share a page leave
- * either's sum there. keys and values of drift_paged_write_*: the values are not read.
+ * either's sum there, with mass as before perhaps on top of the other's: a shared
+ * page's masses take a call a sequence. keys and values of drift_paged_write_*: the
+ * values are not read.
  *
  * drift_heaviest: the `keep` positions that each sequence and key head is to keep:
  * of a sequence of lengths[s] > keep positions the first `sinks`, the last `recent`,
