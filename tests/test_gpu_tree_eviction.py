@@ -939,6 +939,20 @@ def test_moves_of_many_lists(hip, kind, order, count, kv, dim, page, most, start
 
 
 @pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("starts,rows,group,dim", [([700, 3, 64], [7, 8, 1], 4, 128), ([0, 2000], [3, 2], 7, 64), ([95], [17], 1, 256),
+                                                  ([40, 0, 5], [32, 30, 33], 1, 80)])
+def test_masses_of_rows_past_a_unit_of_16(hip, kind, dtype, starts, rows, group, dim):
+    step(f"masses of rows past a unit {kind} {dtype} {rows} of {group} heads of {dim}")
+    case = Case(kind, starts, rows, 2, dim, 32, seed=67)
+    q = normal(68, (case.tokens, 2 * group, dim), TYPES[dtype], 2.0).to(DEV)
+    before = masses(case, 69)
+    mass = torch.zeros_like(before)
+    hip.attentionMass(q, case.cache, case.sequences(), 1 / math.sqrt(dim), mass, before)
+    assert_mass(case, q, 1 / math.sqrt(dim), mass, before, what="rows past a unit")
+
+
+@pytest.mark.parametrize("kind", CACHES)
 def test_masses_of_steps_with_more_scores_than_are_kept(hip, kind):
     """Page tables with room for so many positions that a step's scores are taken twice."""
     step(f"masses of steps over wide page tables {kind}")
