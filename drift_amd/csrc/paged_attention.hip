@@ -411,8 +411,9 @@ __device__ __forceinline__ void few_block(const T* queries, T* out, const ArgsOf
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   // Over the F16 cache weights have 22 bits for BF16 results too, since memory hides the second term (decode batch 256 us,
   // 259 with one): what is rounded to BF16 is the F32 result. In 8 bits, where the codes' conversions count and the
-  // cache's own rounding is 2^-8, they have 11 (heads of 64: 105 us, 117 with two; of 128 159 / 161).
-  constexpr int kWeightTerms = I8 ? TERMS : 2;
+  // cache's own rounding is 2^-8, they have 11 (heads of 64: 105 us, 117 with two; of 128 159 / 161); trees' have 22
+  // everywhere, as many_block says.
+  constexpr int kWeightTerms = I8 && !TREE ? TERMS : 2;
   constexpr int KS = DP / 32, DT = DP / 16;         // products along a head, value tiles
   auto& merged = shared.merged;
   auto& stats = shared.stats;
@@ -848,13 +849,15 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsO
   // BF16's weights have one term, 11 bits: a row's result is then within 2^-11 of its values' sizes before it is rounded
   // to 8 bits, and over many positions their roundings cancel (0.0017 off 64 bits either way, the rounding to BF16's
   // own). A second term costs a fifth to a third: prefill 647 us, 851 with it, window chunk 47 / 56, mixed batch
-  // 177 / 225, chunk over 8 bits 120 / 141.
-  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  // 177 / 225, chunk over 8 bits 120 / 141. Trees' weights have 22 bits: which kernel has a tree's rows depends on the
+  // call's other trees, and their results' bits must not (32 trees of 601 nodes after up to 8,000 positions 175 us, 157
+  // with one term, 16 of 811 over 8 bits 125 / 102; of BF16 results one in twelve was another than the F32 one's rounding).
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, kWeightTerms = TREE ? 2 : TERMS;
   constexpr int kThreads = 64 * WAVES;
   constexpr int kRows = WAVES * 32;  // rows a block
   constexpr int TOK = 64, KS = DP / 16, DT = DP / 32;
   constexpr int kKeyChunks = DP / 8;         // of a position
-  constexpr float kSlack = TERMS == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
+  constexpr float kSlack = kWeightTerms == 2 ? 1.0f : 8.0f, kManyLift = 15.0f - kSlack;
   constexpr int kLoads = TOK * kKeyChunks / kThreads;  // chunks a thread stages, of keys and of values
   // a tile in LDS: its keys, its values, and in 8 bits their scales, the exponents of the values' (-infinity: no scale
   // above 0) and the most and the least of them
@@ -1300,8 +1303,8 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsO
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] *= factor;
     // 16 positions at a time, the next ones' weights made between the products of these
-    Halves<TERMS> weights[2];
-    auto weigh = [&](int n, Halves<TERMS>& to) {
+    Halves<kWeightTerms> weights[2];
+    auto weigh = [&](int n, Halves<kWeightTerms>& to) {
       float value_scale[I8 ? 8 : 1];
       if constexpr (I8) {
         const float* scales = (const float*)(tile + kScalesAt) + TOK + h * 8 + n * 16;
@@ -1315,7 +1318,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsO
         total += p;
         w[e] = I8 ? p * value_scale[e] : p;
       }
-      to = halves_of<TERMS>(w);
+      to = halves_of<kWeightTerms>(w);
     };
     f16x8 values[2][DT];
     auto load_values = [&](int n, f16x8 (&to)[DT]) {
@@ -1334,13 +1337,13 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsO
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int m = 0; m < TERMS; ++m)
+        for (int m = 0; m < kWeightTerms; ++m)
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values[n % 2][d], weights[n % 2].term[m], acc[d], 0, 0, 0);
       if (n < 3) {
-        constexpr int kVector = (I8 ? 48 : 32) + (TERMS == 2 ? 24 : 0);  // about what the weights take
+        constexpr int kVector = (I8 ? 48 : 32) + (kWeightTerms == 2 ? 24 : 0);  // about what the weights take
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          __builtin_amdgcn_sched_group_barrier(kProducts, TERMS, 0);
+          __builtin_amdgcn_sched_group_barrier(kProducts, kWeightTerms, 0);
           __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
           __builtin_amdgcn_sched_group_barrier(kVectors, kVector / DT, 0);
         }

@@ -433,7 +433,9 @@ int drift_paged_attention_bf16(const uint16_t* queries, const void* keys, const 
  * P = start - 1 + the new tokens that the row sees, its depth in the tree (what the
  * window hides of the new tokens is the caller's to leave out). A row that sees nothing
  * is zeros. The workspace has drift_tree_attention_workspace's bytes. For a
- * verified chain (each token seeing those up to itself) it is drift_paged_attention_*.
+ * verified chain (each token seeing those up to itself) it is what
+ * drift_paged_attention_* computes; weights have 22 bits here in either type and over
+ * either cache, whatever the call's other trees.
  * Replaces nothing of the reference, which drafts one chain. */
 int drift_tree_attention_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,
                                    int32_t head_dim, int32_t window, int32_t sinks, int32_t longest, int64_t* bytes);

@@ -1076,3 +1076,63 @@ def test_graphs_beside_each_other(hip):
         for _, _, held, want, _ in runs:
             for x, y in zip(held, want):
                 assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), turn
+
+
+# ------------------------------------------------------------------ weights' bits
+
+def cancelling_codes(weights, dim, rng):
+    """Whole numbers [positions, dim] within 127 that almost cancel: sum_j weights[j] codes[j] is next to nothing
+    beside sum_j weights[j] |codes[j]|."""
+    codes = rng.integers(-127, 128, (len(weights), dim)).astype(np.float64)
+    rest = weights @ codes
+    for j in np.argsort(-weights):
+        to = np.clip(codes[j] - np.round(rest / weights[j]), -127, 127)
+        rest += weights[j] * (to - codes[j])
+        codes[j] = to
+    return codes
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,rows,dim", [(300, 3, 128), (300, 12, 64), (900, 70, 128), (2900, 150, 64), (500, 40, 256),
+                                            (1500, 200, 80)])
+def test_trees_weights_have_22_bits(hip, kind, dtype, start, rows, dim):
+    """Values whose weighted sum almost cancels: what is left of a row's
+    result are its weights' roundings. Rows of the same queries, +-1, that see
+    what lies before the tree; keys are whole numbers, so that scores are
+    exact but for the factor's, the scale's and the difference's roundings, 3
+    2^-24 of their size. So a row is off by 4 (3 2^-24 max|s| + 2^-20 + 2^-24
+    sqrt(n)) of its sum of p |v| and 2^-39 max p sum |v| as above, and BF16
+    results by half a step."""
+    step(f"trees' weights {kind} {dtype} {rows} rows after {start}, heads of {dim}")
+    kv, heads = 2, 4
+    case = Case(kind, [start], [rows], kv, dim, 16, seed=71)
+    rng = np.random.default_rng(start + dim)
+    j = np.arange(start)
+    page, off = torch.from_numpy(case.tables[0, j // 16].astype(np.int64)).to(DEV), torch.from_numpy(j % 16).to(DEV)
+    q = rng.choice([-1.0, 1.0], (kv, dim))
+    out, mass, lost, most = (np.zeros((kv, dim)), np.zeros((kv, dim)), np.zeros((kv, dim)), 0.0)
+    for h in range(kv):
+        keys = rng.integers(-4, 5, (start, dim)).astype(np.float64)
+        scores = keys @ q[h] / 16
+        most = max(most, float(np.abs(scores).max()))
+        p = np.exp(scores - scores.max())
+        p /= p.sum()
+        scales = np.ones(start) if kind == "f16" else (0.5 + rng.random(start, np.float32)).astype(np.float32).astype(np.float64)
+        codes = cancelling_codes(p * scales, dim, rng)
+        values = codes * scales[:, None]
+        out[h], mass[h], lost[h] = p @ values, p @ np.abs(values), p.max() * np.abs(values).sum(0)
+        if kind == "i8":
+            lost[h] = p.max() * 2 * scales.max() * 127 * start
+            case.cache.keyScales[page, h, off] = 1.0
+            case.cache.valueScales[page, h, off] = torch.from_numpy(scales.astype(np.float32)).to(DEV)
+        case.cache.keys[page, off, h] = torch.from_numpy(keys).to(DEV, case.cache.keys.dtype)
+        case.cache.values[page, h, :, off] = torch.from_numpy(codes).to(DEV, case.cache.values.dtype)
+    queries = torch.from_numpy(np.repeat(q, heads // kv, 0)).to(DEV, TYPES[dtype]).expand(rows, heads, dim).contiguous()
+    got = attend(hip, case, queries, packed([np.zeros((rows, rows), bool)], -(-rows // 32)), 1 / 16).cpu().double().numpy()
+    bar = 4 * (3 * 2.0 ** -24 * most + 2.0 ** -20 + 2.0 ** -24 * math.sqrt(start)) * mass + 2.0 ** -39 * lost
+    if dtype == "bf16":
+        bar += 2.0 ** -8 * np.abs(out)
+    worst = np.abs(got - np.repeat(out, heads // kv, 0)) / np.repeat(bar, heads // kv, 0)
+    print(f"[gpu]   worst {worst.max():.3f} of the bar, {2.0 ** -12 * (mass / bar).max():.1f} bars are 2^-12 of the sizes", flush=True)
+    assert worst.max() <= 1, worst.max()
