@@ -672,6 +672,8 @@ extern "C" int drift_cache_keep(void* keys, void* values, float* key_scales, flo
       (!key_scales && ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) & 1) != 0))
     return refuse("%s: tensors not aligned to their elements", entry);
   const bool apart = into && into != page_tables;
+  if (into && !apart && into_pages != table_pages && sequences > 1)  // (a sequence's own pages would be others')
+    return refuse("%s: into is page tables of %d pages a sequence as ones of %d", entry, table_pages, into_pages);
   const int64_t bytes = apart ? 0 : keep_bytes(sequences, most, kv_heads, head_dim, key_scales != nullptr);
   if (bytes > 0 && (!workspace || workspace_bytes < bytes || !aligned16(workspace)))
     return refuse("%s: a workspace of %lld bytes, needs %lld at a multiple of 16", entry, (long long)workspace_bytes,

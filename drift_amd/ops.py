@@ -1258,6 +1258,8 @@ class HipOps:
                              f"{cache.kvHeads} heads")
         if into is not None and checkTables(operation, into) != count:
             raise ValueError(f"{operation}: into {_shape(into)} for {count} sequences")
+        if into is not None and into.data_ptr() == pageTables.data_ptr() and into.shape != pageTables.shape and count > 1:
+            raise ValueError(f"{operation}: into {_shape(into)} is the page tables {_shape(pageTables)}")
         if mass is not None:
             checkMass(operation, mass, cache)
         checkBadPage(operation, badPage)

@@ -488,7 +488,8 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * any is written: in place (`into` NULL) lists may move rows over each other. With
  * `into`, page tables [sequences, into_pages], rows go to positions of those pages,
  * which may hold none that the lists name (else what moves there is either); the
- * pages that rows go to belong to one sequence each. Entries that are no position of
+ * pages that rows go to belong to one sequence each (`page_tables` itself, with as
+ * many pages a sequence, is in place). Entries that are no position of
  * their page table, or lie on a page outside the cache, and rows that would go to
  * one, move nothing, and a count outside 0 .. most or a start below 0 leaves its
  * sequence as it is; *bad_page is set. In place it takes the workspace (device, 16-byte

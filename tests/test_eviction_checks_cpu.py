@@ -274,3 +274,18 @@ def test_the_moves_entry_point_refuses():
     assert "in one call" in refusal(entry, *move(sequences=2 ** 30, most=2 ** 30))
     assert refusal(entry, *move(most=0)) == "code 0"
     assert refusal(entry, *move(sequences=0)) == "code 0"
+
+
+def test_moves_into_their_own_page_tables_as_others_are_refused(hip):
+    """The page tables' memory read as tables of another width would name other sequences' pages as the places that
+    rows move to in place."""
+    tables = zeros(3, 4, dtype=I32)
+    kept = zeros(3, 2, 8, dtype=I32)
+    with pytest.raises(ValueError, match=r"into \[3×2\] is the page tables \[3×4\]"):
+        hip.cacheKeep(f16_cache(), tables, kept, into=tables.view(-1)[:6].view(3, 2))
+    assert "page tables of 4 pages a sequence as ones of 2" in refusal("drift_cache_keep", *move(into=16, into_pages=2))
+    # one sequence's first pages, or the same tables, are in place: their own scratch is asked for
+    with pytest.raises(ValueError, match="device memory"):
+        hip.cacheKeep(f16_cache(), tables[:1], kept[:1], into=tables[:1, :2])
+    assert "needs" in refusal("drift_cache_keep", *move(into=16, into_pages=2, sequences=1, size=0))
+    assert "needs" in refusal("drift_cache_keep", *move(into=16, into_pages=4, size=0))

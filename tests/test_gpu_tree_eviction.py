@@ -1136,3 +1136,24 @@ def test_trees_weights_have_22_bits(hip, kind, dtype, start, rows, dim):
     worst = np.abs(got - np.repeat(out, heads // kv, 0)) / np.repeat(bar, heads // kv, 0)
     print(f"[gpu]   worst {worst.max():.3f} of the bar, {2.0 ** -12 * (mass / bar).max():.1f} bars are 2^-12 of the sizes", flush=True)
     assert worst.max() <= 1, worst.max()
+
+
+# ------------------------------------------------------------------ moves' page tables
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("most", [60, 300])
+def test_moves_into_a_sequences_first_pages(hip, kind, most):
+    """One sequence's first pages, as `into` the same memory as its page tables: in place, and rows past those pages
+    move nothing."""
+    step(f"moves into the first pages {kind} {most}")
+    tables, pages = tables_for([500], 16, 73)
+    device_tables = dev_i32(tables)
+    kept = np.random.default_rng(74).permutation(500)[:most].astype(np.int32)[None]
+    into = device_tables[:, :14]
+    assert into.data_ptr() == device_tables.data_ptr()
+    cache, mass = cache_of(kind, pages, 16, 3, 64, 75)
+    old = parts(cache, mass)
+    bad = torch.zeros(1, dtype=torch.int32, device=DEV)
+    hip.cacheKeep(cache, device_tables, dev_i32(kept), None, None, into, mass, bad)
+    assert_parts(cache, mass, moved(old, tables, kept, [most], [0], tables[:, :14], 16))
+    assert int(bad.item()) == (most > 14 * 16)
