@@ -533,13 +533,17 @@ int pieces_of(int32_t dim, bool quantized, int& piece) {
   return pieces <= 4 ? 4 : pieces <= 8 ? 8 : pieces <= 16 ? 16 : 0;
 }
 
+// Bytes of scratch of a call in place, whichever way it goes: a row each (where the tensors' alignment asks for
+// move_rows), or a thread's slots of every chunk.
 int64_t keep_bytes(int32_t sequences, int32_t most, int32_t kv_heads, int32_t dim, bool quantized) {
   const int64_t by_rows = (int64_t)sequences * most * kv_heads * scratch_row(dim, quantized);
   int piece;
   const int pieces = pieces_of(dim, quantized, piece), slots = std::max(pieces * piece / 16 + 1, quantized ? 2 : 4);
+  // a list of one chunk is read whole before it is written, and by chunks puts nothing by
+  if (pieces == 0 || most <= kKeepRows) return ceil_div(by_rows, 16) * 16;
   const int64_t by_chunks = (int64_t)sequences * kv_heads * (1 + ceil_div(dim, 64)) * ceil_div(most, kKeepRows) *
                             slots * 256 * 16;
-  return ceil_div(pieces == 0 ? by_rows : std::max(by_rows, by_chunks), 16) * 16;
+  return ceil_div(std::max(by_rows, by_chunks), 16) * 16;
 }
 
 template <typename E, int PIECE, int PIECES>

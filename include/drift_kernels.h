@@ -494,7 +494,10 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * one, move nothing, and a count outside 0 .. most or a start below 0 leaves its
  * sequence as it is; *bad_page is set. In place it takes the workspace (device, 16-byte
  * aligned) that drift_cache_keep_workspace tells, written before it is read; with
- * `into` none.
+ * `into` none. That is two to three times the bytes of the rows that the lists name, of lists up
+ * to 128 rows no more than theirs (8 heads of 128 in F16: 32 sequences' 2,048 rows 453 MB, 7
+ * rows 0.9 MB), though lists that move rows to the front alone, as drift_heaviest's do,
+ * leave most of it untouched.
  * Replaces nothing of the reference, whose cache only grows
  * (src/drift/runner/ops/KvCache.scala:5-22). */
 int drift_attention_mass_workspace(int32_t sequences, int32_t tokens, int32_t heads, int32_t kv_heads,

@@ -289,3 +289,12 @@ def test_moves_into_their_own_page_tables_as_others_are_refused(hip):
         hip.cacheKeep(f16_cache(), tables[:1], kept[:1], into=tables[:1, :2])
     assert "needs" in refusal("drift_cache_keep", *move(into=16, into_pages=2, sequences=1, size=0))
     assert "needs" in refusal("drift_cache_keep", *move(into=16, into_pages=4, size=0))
+
+
+@pytest.mark.parametrize("dim,quantized", [(128, 0), (128, 1), (96, 0), (24, 1), (512, 1), (7, 0)])
+@pytest.mark.parametrize("most", [1, 7, 128])
+def test_short_moves_ask_for_their_rows_bytes_alone(dim, quantized, most):
+    """A row's key, value, two scales and mass; a list of up to 128 rows puts no more by."""
+    code, size = told("drift_cache_keep_workspace", 32, most, 8, dim, quantized)
+    row = -(-dim * 2 * (1 if quantized else 2) // 4) * 4 + 12
+    assert code == "code 0" and size == -(-32 * most * 8 * row // 16) * 16
