@@ -1157,3 +1157,52 @@ def test_moves_into_a_sequences_first_pages(hip, kind, most):
     hip.cacheKeep(cache, device_tables, dev_i32(kept), None, None, into, mass, bad)
     assert_parts(cache, mass, moved(old, tables, kept, [most], [0], tables[:, :14], 16))
     assert int(bad.item()) == (most > 14 * 16)
+
+
+# ------------------------------------------------------------------ kernels' other forms
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("order", ["ascending", "any"])
+@pytest.mark.parametrize("dim", [8, 24, 40, 72, 200, 264])
+@pytest.mark.parametrize("most,start", [(129, 0), (300, 7)])
+def test_moves_of_heads_in_pieces_of_8_bytes(hip, kind, order, dim, most, start):
+    """Heads of other than multiples of 16 values over 8 bits, with few and many pieces a thread."""
+    step(f"moves in pieces {kind} {order} {dim} {most}")
+    rng = np.random.default_rng(dim + most)
+    lengths, kv, page = [start + most + 150, start + most + 3], 3, 16
+    tables, pages = tables_for(lengths, page, 76)
+    counts = [most, most - 2]
+    kept = np.zeros((2, kv, most), np.int32)
+    for s, n in enumerate(lengths):
+        for h in range(kv):
+            row = rng.choice(n, most, replace=order == "any")
+            kept[s, h] = np.sort(row) if order == "ascending" else row
+    cache, mass = cache_of(kind, pages, page, kv, dim, 77)
+    old = parts(cache, mass)
+    hip.cacheKeep(cache, dev_i32(tables), dev_i32(kept), dev_i32(counts), dev_i32([start] * 2), mass=mass)
+    assert_parts(cache, mass, moved(old, tables, kept, counts, [start] * 2, tables, page))
+    rooms, more = tables_for([start + most] * 2, page, 78, spare=0)
+    into = np.where(rooms >= 0, rooms + pages, rooms)
+    cache, mass = cache_of(kind, pages + more, page, kv, dim, 79)
+    old = parts(cache, mass)
+    hip.cacheKeep(cache, dev_i32(tables), dev_i32(kept), dev_i32(counts), dev_i32([start] * 2), dev_i32(into), mass)
+    assert_parts(cache, mass, moved(old, tables, kept, counts, [start] * 2, into, page))
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count,chunk,group,dim,at", [(64, 401, 4, 64, 333), (40, 143, 7, 128, 1501), (70, 517, 2, 80, 2)])
+def test_masses_of_one_long_chunk_among_single_tokens(hip, kind, dtype, count, chunk, group, dim, at):
+    """So many single tokens that the call's rows are few on average: a chunk of more rows than are added up at a
+    time keeps its scores too."""
+    step(f"masses of a chunk of {chunk} among {count} tokens {kind} {dtype} {group} heads of {dim}")
+    rows, starts = [1] * count, [(37 * i) % 90 for i in range(count)]
+    rows[count // 2], starts[count // 2] = chunk, at
+    assert sum(rows) * group <= count * 32 and chunk * group > 256
+    case = Case(kind, starts, rows, 1, dim, 16, seed=81)
+    q = normal(82, (case.tokens, group, dim), TYPES[dtype], 2.0).to(DEV)
+    before = masses(case, 83)
+    for longest in (0, 1):
+        mass = torch.zeros_like(before)
+        hip.attentionMass(q, case.cache, case.sequences(longest=longest), 1 / math.sqrt(dim), mass, before)
+        assert_mass(case, q, 1 / math.sqrt(dim), mass, before, what=f"longest {longest}")
