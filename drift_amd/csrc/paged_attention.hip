@@ -1590,9 +1590,12 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   p.few_rows = by_offsets && tokens * group > sequences * kFewRows ? 16 : kFewRows;
   // Trees have 16 to some hundred rows each, of positions that memory has to bring for all of them: in units of 16 by
   // waves two a SIMD, and past 16 rows among attend_many's, whose tiles serve 128 (us, as above / so: 8 nodes of one
-  // sequence, 32 rows, 29 / 15, 8 sequences of 12 nodes at 3,000 positions 122 / 36, 64 of 8 at 4,000 318 / 181, over 8
-  // bits 266 / 203, 16 of 20 rows over 24 heads of their own 222 / 156).
-  if (tree && each * group > kFewRows) p.few_rows = 16;
+  // sequence, 32 rows, 29 / 15, 8 sequences of 12 nodes at 3,000 positions 103 / 45, 32 of 16 at 4,000 223 / 145, 64 of 8
+  // 358 / 251, 16 of 20 rows over 24 heads of their own 259 / 207). Over 8 bits, whose second reading is half as dear and
+  // whose codes attend_many converts for rows that a tile has not, units of 16 up to kFewRows where trees have up to 40
+  // rows on average (us, among attend_many's / so: 64 of 32 rows at 4,000 281 / 238, 16 of 20 240 / 170, 4 of 32 at 1,000
+  // 41 / 21, though 8 of 32 at 4,000 51 / 58 and 16 of 35 56 / 74; with more rows 8 of 48 59 / 74, 32 of 48 at 1,000 62 / 80).
+  if (tree && each * group > kFewRows) p.few_rows = quantized && tokens * group <= sequences * 40 ? kFewRows : 16;
   p.few16 = p.few_rows == 16 || tree ? true : by_offsets ? tokens * group <= sequences * 16 : each * group <= 16;
   // Up to 768 positions a second launch takes longer than it saves (one token at 517 12.5 us, 14.2 in splits, at 767 13.5
   // and 13.8, at 1,023 15.9 and 14.3; heads of 256 over 8 bits at 500 16.4 and 17.7, at 760 20.1 and 17.7). Splits of
@@ -1620,8 +1623,9 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
     }
     p.many_rows = large && dim > 64 && dim <= 128 ? 256 : 128;
     const int64_t blocks = ceil_div(rows, p.many_rows) * kv_heads, wanted = dim > 128 || p.many_rows == 256 ? 256 : 512;
-    // (a tile of wide heads takes long enough for splits of 4: 5 trees in a window of 1,024, F32 heads of 256, 59 us in
-    // splits of 8, 47 of 4)
+    // (a tile of wide heads takes long enough for splits of 4: us, 2 heads of 256, splits of 8 / of 4, 5 trees in a window
+    // of 1,024 57 / 48, over 8 bits 71 / 51, 4 trees of 20 nodes at 700 positions 55 / 43, one of 200 at 1,500 62 / 55,
+    // 8 of 40 at 3,000 108 / 107, 2 of 100 at 8,000 and 32 of 20 at 6,000 alike)
     p.many = blocks * 4 >= wanted * 3 ? Split{1, 1} : split_of(blocks, seen, wanted, tree && dim > 128 ? 4 : 8, 1 << 25);
   }
   p.few_most = std::min(each * group, (int64_t)p.few_rows);

@@ -1206,3 +1206,20 @@ def test_masses_of_one_long_chunk_among_single_tokens(hip, kind, dtype, count, c
         mass = torch.zeros_like(before)
         hip.attentionMass(q, case.cache, case.sequences(longest=longest), 1 / math.sqrt(dim), mass, before)
         assert_mass(case, q, 1 / math.sqrt(dim), mass, before, what=f"longest {longest}")
+
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [None, d.AttentionWindow(200, 3)])
+@pytest.mark.parametrize("starts,rows,dim", [([900, 31, 0, 64, 1200, 5], [9, 16, 3, 10, 1, 12], 128),
+                                             ([400 + 7 * i for i in range(10)], [5, 4, 8, 1, 40, 6, 5, 3, 9, 0], 64),
+                                             ([2500, 100, 900], [10, 9, 8], 256)])
+def test_small_trees_together(hip, kind, dtype, window, starts, rows, dim):
+    """Trees of 17 to 64 rows a key head with few on average, one of more among them."""
+    step(f"small trees together {kind} {dtype} {window} {rows} rows, heads of {dim}")
+    case = Case(kind, starts, rows, 2, dim, 16, seed=84)
+    q = normal(85, (case.tokens, 8, dim), TYPES[dtype], 2.0).to(DEV)
+    for shape in ("random", "any"):
+        sees = trees(rows, 3, shape)
+        got = attend(hip, case, q, packed(sees, 2), 0.1, window)
+        assert_tree(case, q, 0.1, sees, got, window, what=shape)
