@@ -146,7 +146,9 @@ __global__ void __launch_bounds__(kWave) row_statistics(const T* queries, MassAr
 }
 
 // Positions' sums by one wave, a lane a position of a tile of 64; a block every `splits`-th tile of a sequence and key
-// head.
+// head. Its loads bound it, a key's value a lane at a time, again for every row: 64 single tokens at 2,000 positions, 32
+// heads over 4 of 512, 25.6 ms, a prompt of 512 tokens, 16 heads over 2 of 512, 176 ms, 2 single tokens over 4 heads of 20
+// 46 us.
 template <typename T, bool I8>
 __global__ void __launch_bounds__(kWave) position_sums(const T* queries, MassArgs a) {
   __shared__ float query[kMaxHead];
@@ -276,8 +278,8 @@ __device__ __forceinline__ SplitTiles split_tiles(const MassArgs& a, uint32_t la
 // products, S^T = K Q^T: the result's column (lane % 16) is a row, its rows are
 // positions, dealt out so that a lane has TOK / 4 consecutive ones. A block's four waves
 // take its split's tiles in turn. Memory bounds it: 64 single tokens at up to 8,000
-// positions, 32 heads over 8 of 128, 160 us for 559 MB of keys and 70 MB of scores (3.9 TB/s);
-// without the scores' stores it would be 134.
+// positions (304,719 in all), 32 heads over 8 of 128, 160 us for 624 MB of keys and 39 MB of
+// scores (4.2 TB/s); without the scores' stores it would be 134 (4.7).
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* queries, MassArgs a) {
   constexpr int kWaves = 4;
@@ -461,8 +463,9 @@ __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) few_scores(const T* que
 }
 
 // The few rows' positions: a thread four of them, a block 1,024 of a sequence and key
-// head; the rows' statistics joined in LDS first, 256 at a time. (19 us of that step: 70 MB
-// of scores, 3.7 TB/s.)
+// head; the rows' statistics joined in LDS first, 256 at a time. (19 us of that step: 39 MB of
+// scores and 20 MB of masses read and written, 3.1 TB/s, part of it out of the caches: what
+// bounds it is each block's chain, tables, statistics, then few loads a thread.)
 template <bool I8>
 __global__ void __launch_bounds__(256) few_sums(MassArgs a) {
   constexpr int kBatch = 256;
@@ -534,9 +537,9 @@ __device__ __forceinline__ int chunk_place(int row, int chunk) {
 // for all its rows, by 32 x 32 x 16 products, S^T = K Q^T: the result's column is a row, and its largest score and
 // sum stay in its lanes. The queries go to the workspace as the products take them, for many_sums.
 //
-// The exponentials and what goes with them bound it: a prompt of 8,192 tokens, 32 heads over 8 of 128, some 340 us, 810
-// TFLOP/s; vector instructions issue 70% of the time, the products run 38%. 64 tokens after 31,936 32 us, of which 128
-// rows a block leave most to staging.
+// The exponentials and what goes with them bound it: a prompt of 8,192 tokens, 32 heads over 8 of 128, 358 us at best and
+// 393 at the median of a profiled run (768 and 699 TFLOP/s); vector instructions issue 70% of the time, the products run
+// 38%. 64 tokens after 31,936 33 us, of which 128 rows a block leave most to staging.
 template <typename T, bool I8, int DP>
 __global__ void __launch_bounds__(256, DP > 128 ? 1 : 2) many_statistics(const T* queries, MassArgs a) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, TOK = 64, KS = DP / 16, kThreads = 256;
@@ -789,9 +792,10 @@ __global__ void __launch_bounds__(128) many_rows(MassArgs a) {
 // each lane adds up its rows' weights for the positions in its registers, so that rows need no sums across lanes
 // until the last. A block has every `parts`-th part of the rows that see its tile of positions.
 //
-// Bound as the statistics are: the prompt's some 330 us (vector instructions 56%, products 39%; kept instead, its 4.3 GB of
-// scores would have to be written and read). With 256 positions a block each row from LDS is used
-// twice: by 128 the last 64 rows of 32,000 positions take 82 us for 79.
+// The prompt's 337 us at best and 365 at the median (815 and 753 TFLOP/s): vector instructions issue 56% of the time, the
+// products run 39%, one after the other in each of two waves a SIMD. (Kept instead, its 4.3 GB of scores would have to be
+// written and read.) With 256 positions a block each row from LDS is used twice: by 128 the last 64 rows of 32,000
+// positions took 82 us for 79.
 //
 // A score that is NaN where its row is numbers is one of -infinity (a key's infinity met a zero term): had it
 // been NaN or infinity the row would not be. So a NaN weight counts as 0, times an inverse that is NaN where the row is.
@@ -1040,7 +1044,9 @@ struct Plan {
 };
 
 // Bytes of scores, at most, that are kept rather than taken twice: a cache's keys take eight times as much for
-// rows that share a key head by fours.
+// rows that share a key head by fours. A row has room for every position of its page table, whatever the sequences hold
+// (64 sequences of 32 heads at up to 8,000 positions in tables for 65,536: 537 MB of scratch, 164 us for 161; for 131,072
+// they are taken twice, 366 us).
 constexpr int64_t kMostScores = (int64_t)1 << 29;
 
 int64_t padded(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
@@ -1058,9 +1064,12 @@ Plan plan_of(int64_t sequences, int64_t tokens, int64_t heads, int64_t kv_heads,
   };
   const int64_t rows = tokens * heads, group = heads / kv_heads, units = sequences * kv_heads;
   const int64_t seen = std::max<int64_t>(std::min(longest, room), 1);
-  // Up to 32 rows a sequence and key head on average (a decode step's, or some more): their scores are kept (us, 16
-  // sequences of 4,000 positions, 8 key heads of 128, kept / taken twice: 16 rows 50 / 76, 32 rows 71 / 81, 64 rows
-  // 123 / 83; 64 sequences of 8,000, 4 rows 179 / 413).
+  // Up to 32 rows a sequence and key head on average (a decode step's, or some more): their scores are kept (us, kept /
+  // taken twice, 16 sequences at up to 4,000 positions, 8 key heads of 128: 8 rows each 31 / 54, 16 34 / 53, 32 47 / 53, 64
+  // (at 4,000) 123 / 83; 64 sequences 77 / 186, 96 / 184, 148 / 178, as chunks of every fourth 82 / 184, 116 / 187, 190 /
+  // 190). The average is what the host knows: where one sequence has all the rows past the others' single tokens, its
+  // units read its keys again and again, and kept scores lose from 16 on average on (64 sequences, 8 rows 117 / 190, 16
+  // 223 / 196, 32 482 / 205).
   p.few = tokens * group <= sequences * 32 && rows * room * 4 <= kMostScores;
   if (p.few) {
     p.split = split_of(units, seen, 1024, 4, 16);

@@ -39,7 +39,8 @@ constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave, kBins = 20
 // each by a histogram in LDS of the candidates that share the digits so far; two more
 // write the positions in their order, by counts of the waves before and ballots.
 // EACH: the candidates a lane keeps in registers, up to 32; 0: more, read again in each pass (us, 16 sequences of 8
-// heads, kept / read again: 1,500 positions 9 / 23, 7,000 13 / 31, 14,000 20 / 35, 30,000 42 / 67).
+// heads, kept / read again: 1,500 positions 9 / 23, 7,000 13 / 31, 14,000 20 / 35, 30,000 42 / 67). The launch takes it
+// by what the page tables have room for: 7,000 positions in tables for 32,768 20 us, for more 21 to 32.
 //
 // The passes over the orders with their additions in LDS bound it, not memory: 48 sequences of up to 16,000 positions, 8
 // heads, 31 us for 22 MB in 384 blocks, two a compute unit (vector instructions issue 36% of the time).
@@ -218,7 +219,8 @@ __device__ __forceinline__ Move move_of(const KeepArgs& a, int s, int kv, int i)
   return m;
 }
 
-// A wave a row. READ: from the cache, else from the scratch; WRITE: to the cache, else to the
+// What no chunks are made for (heads of 512 in F16, of odd sizes, tensors off 16-byte alignment): a wave a row, 1,024 of
+// 4,000 rows of 16 sequences, 4 heads of 512, in place 277 us (537 MB moved twice, 3.9 TB/s), of 20 values 61. READ: from the cache, else from the scratch; WRITE: to the cache, else to the
 // scratch, which has a row's keys, values, scales and mass one after another.
 template <typename E, bool READ, bool WRITE>
 __global__ void __launch_bounds__(256) move_rows(KeepArgs a, int64_t rows, int64_t row_bytes) {

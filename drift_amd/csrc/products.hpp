@@ -1,6 +1,9 @@
 // Shared pieces of the kernels that take scores of rows and cached positions by
 // matrix instructions: their operands' types, the 8-bit cache's codes as F16
-// numbers, F32 values as F16 terms, and the scaling of a row of queries.
+// numbers, and F32 values as F16 terms. (How a row of queries is scaled is each
+// kernel's own: those that compare products before they are scores turn a negative
+// scale's sign into the query and keep the factor above 0, attend_few, which scales
+// every product at once, needs neither.)
 #pragma once
 
 #include "paged.hpp"

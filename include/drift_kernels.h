@@ -463,9 +463,14 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * where the position precedes the sequence's rows. Rows, paging and scores are
  * drift_paged_attention_*'s, without a window, and so are the rules of the workspace,
  * whose bytes drift_attention_mass_workspace tells (`room`: table_pages * page_size,
- * at most 2147483520): of few rows a sequence it holds their scores, 4 bytes a row and
- * position of room up to 512 MiB in all (64 sequences' step, 32 heads, 8,016 positions: 66 MB), of
- * many a copy of the queries. Other positions of mass are
+ * at most 2147483520): of few rows a sequence (up to 32 a key head on average over the
+ * call) it holds their scores, 4 bytes a row and position of room up to 512 MiB in all
+ * (64 sequences' step, 32 heads, 8,016 positions: 66 MB), of many a copy of the queries.
+ * Room counts there, not what the sequences hold: where a step's page tables have room
+ * for more scores than that they are computed twice (64 sequences of 32 heads at up to 8,000
+ * positions 161 us, with room for 65,536 164 and 537 MB, for 131,072 366), and
+ * drift_heaviest reads its masses several times past 32,768 positions of room
+ * (16 sequences of 7,000: 13 us, 21 to 32). Narrow tables serve both. Other positions of mass are
  * left as they are, and so are ones on a page outside the cache, *bad_page set. The
  * same call gives the same bits every time. Two sequences that share a page leave
  * either's sum there, with mass as before perhaps on top of the other's: a shared
