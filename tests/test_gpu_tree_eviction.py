@@ -16,12 +16,14 @@ Bars, derived from the roundings on the way:
 - what is chosen and what is moved: exact.
 """
 
+import ctypes
 import math
 
 import numpy as np
 import pytest
 import torch
 
+from drift_amd import _lib
 from drift_amd import ops as d
 from tests.helpers import DEV, dev_i32, step
 from tests.test_gpu_paged_attention import CACHES, DTYPES, TYPES, Case, normal
@@ -1223,3 +1225,37 @@ def test_small_trees_together(hip, kind, dtype, window, starts, rows, dim):
         sees = trees(rows, 3, shape)
         got = attend(hip, case, q, packed(sees, 2), 0.1, window)
         assert_tree(case, q, 0.1, sees, got, window, what=shape)
+
+
+# ------------------------------------------------------------------ one sequence by the entry points' arguments
+
+@pytest.mark.parametrize("kind", CACHES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start,rows,dim", [(0, 1, 64), (517, 7, 128), (700, 90, 128), (33, 300, 64), (90, 9, 20)])
+def test_one_sequence_without_starts_and_offsets(hip, kind, dtype, start, rows, dim):
+    """The C entry points take one sequence of all rows at `start` without device arrays of either."""
+    step(f"one sequence by arguments {kind} {dtype} {rows} rows at {start}, heads of {dim}")
+    case = Case(kind, [start], [rows], 2, dim, 16, seed=86)
+    q, heads, scale = normal(87, (rows, 8, dim), TYPES[dtype], 2.0).to(DEV), 8, 0.1
+    tables, c, stream = dev_i32(case.tables), case.cache, torch.cuda.current_stream().cuda_stream
+    p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    scales = (c.keyScales, c.valueScales) if kind == "i8" else (None, None)
+    room = case.tables.shape[1] * 16
+
+    def scratch(entry, *numbers):
+        told = ctypes.c_int64()
+        _lib.call(entry, *numbers, ctypes.byref(told))
+        return torch.empty(max(told.value, 16), dtype=torch.uint8, device=DEV)
+
+    sees = trees([rows], 88)
+    words = packed(sees, -(-rows // 32))
+    out, space = torch.full_like(q, 7.0), scratch("drift_tree_attention_workspace", 1, rows, heads, 2, dim, 0, 0, room)
+    _lib.call(f"drift_tree_attention_{dtype}", p(q), p(c.keys), p(c.values), p(scales[0]), p(scales[1]), p(tables),
+              case.tables.shape[1], c.pages, None, None, 1, start, rows, heads, 2, dim, 16, scale, 0, 0, room, p(words),
+              words.shape[1], p(out), p(space), space.numel(), None, stream)
+    assert_tree(case, q, scale, sees, out, what="tree")
+    before = masses(case, 89)
+    mass, space = torch.zeros_like(before), scratch("drift_attention_mass_workspace", 1, rows, heads, 2, dim, room, room)
+    _lib.call(f"drift_attention_mass_{dtype}", p(q), p(c.keys), p(scales[0]), p(tables), case.tables.shape[1], c.pages, None,
+              None, 1, start, rows, heads, 2, dim, 16, scale, room, p(before), p(mass), p(space), space.numel(), None, stream)
+    assert_mass(case, q, scale, mass, before, what="mass")
