@@ -220,7 +220,8 @@ __device__ __forceinline__ Move move_of(const KeepArgs& a, int s, int kv, int i)
 }
 
 // What no chunks are made for (heads of 512 in F16, of odd sizes, tensors off 16-byte alignment): a wave a row, 1,024 of
-// 4,000 rows of 16 sequences, 4 heads of 512, in place 277 us (537 MB moved twice, 3.9 TB/s), of 20 values 61. READ: from the cache, else from the scratch; WRITE: to the cache, else to the
+// 4,000 rows of 16 sequences, 4 heads of 512, in place 277 us (537 MB moved twice, 3.9 TB/s), of 20 values 61.
+// READ: from the cache, else from the scratch; WRITE: to the cache, else to the
 // scratch, which has a row's keys, values, scales and mass one after another.
 template <typename E, bool READ, bool WRITE>
 __global__ void __launch_bounds__(256) move_rows(KeepArgs a, int64_t rows, int64_t row_bytes) {

@@ -850,7 +850,7 @@ __device__ __forceinline__ void many_block(const T* queries, T* out, const ArgsO
   // to 8 bits, and over many positions their roundings cancel (0.0017 off 64 bits either way, the rounding to BF16's
   // own). A second term costs a fifth to a third: prefill 647 us, 851 with it, window chunk 47 / 56, mixed batch
   // 177 / 225, chunk over 8 bits 120 / 141. Trees' weights have 22 bits: which kernel has a tree's rows depends on the
-  // call's other trees, and their results' bits must not (32 trees of 601 nodes after up to 8,000 positions 175 us, 157
+  // call's other trees, and their precision must not (32 trees of 601 nodes after up to 8,000 positions 175 us, 157
   // with one term, 16 of 811 over 8 bits 125 / 102; of BF16 results one in twelve was another than the F32 one's rounding).
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1, kWeightTerms = TREE ? 2 : TERMS;
   constexpr int kThreads = 64 * WAVES;
