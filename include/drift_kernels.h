@@ -471,8 +471,7 @@ int drift_tree_attention_bf16(const uint16_t* queries, const void* keys, const v
  * positions 161 us, with room for 65,536 164 and 537 MB, for 131,072 366), and
  * drift_heaviest reads its masses several times past 32,768 positions of room
  * (16 sequences of 7,000: 13 us, 21 to 32). Narrow tables serve both. Other positions of
- * mass are
- * left as they are, and so are ones on a page outside the cache, *bad_page set. The
+ * mass are left as they are, and so are ones on a page outside the cache, *bad_page set. The
  * same call gives the same bits every time. Two sequences that share a page leave
  * either's sum there, with mass as before perhaps on top of the other's: a shared
  * page's masses take a call a sequence. keys and values of drift_paged_write_*: the
